@@ -38,6 +38,11 @@ extern "C" {
 #define SGNN_ERR_TOO_LARGE 4        /* size beyond a stated limit */
 #define SGNN_ERR_WORKSPACE 5        /* workspace missing or too small */
 
+/* Element types of the entry points that take more than fp32 */
+#define SGNN_F32 0
+#define SGNN_BF16 1
+#define SGNN_F16 2
+
 /* SpMM algorithm selector */
 #define SGNN_SPMM_AUTO 0      /* = SGNN_SPMM_NNZ_SPLIT: safe for any degree distribution */
 #define SGNN_SPMM_ROW_SPLIT 1 /* one warp (or sub-warp) per row; deterministic; for near-uniform degrees */
@@ -436,6 +441,74 @@ int sgnn_gemm_f32_workspace_bytes(int op, int64_t M, int64_t N, int64_t K, size_
 int sgnn_gemm_f32(int op, const float *d_A, int64_t lda, const float *d_B, int64_t ldb, float *d_C, int64_t ldc,
                   int64_t M, int64_t N, int64_t K, float beta, void *d_workspace, size_t workspace_bytes,
                   void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Layer norm of the rows of a matrix, any width, fp32 / bf16 / fp16, and its gradients:
+ *     xh = (x - mean) rstd,  y = xh gamma + beta         mean, rstd = 1/sqrt(var + eps) of the row, biased variance
+ *     gx = rstd (a - mean(a) - xh mean(a xh)),  a = gy gamma
+ *     g_gamma = sum_r gy xh,  g_beta = sum_r gy
+ * Replaces the torch.nn.LayerNorm between two layers (examples/graphsage/sage.py:149-151, 192-194) where the fused
+ * epilogue above does not apply.
+ *
+ *   dtype: element type of x, y, gy, gx (SGNN_F32 / BF16 / F16); param_dtype: of gamma, beta and their gradients,
+ *   fp32 or dtype.  gamma / beta may be NULL (1 / 0).  Arithmetic and sums in fp32.
+ *   forward: d_stats fp32[n, 2] receives (mean, rstd).  With d_codes (uint8[n, ldc]) and d_params (fp32[n, 2]) not
+ *   NULL the 8-bit checkpoint of x is written in the same pass: what sgnn_checkpoint_pack_rows(x) writes.
+ *   backward: d_x, or d_codes and d_params in its place (x is then the restored checkpoint).  d_gx may be d_gy.
+ *   d_partials fp32[sgnn_layer_norm_blocks(), 2, H] scratch; the column sums are taken in a fixed order.
+ *   H <= 16384.  Rows may start anywhere (aligned rows of a multiple of 16 bytes are read fastest).
+ * ------------------------------------------------------------------------- */
+int sgnn_layer_norm_forward(int dtype, const void *d_x, int64_t ldx, int param_dtype, const void *d_gamma,
+                            const void *d_beta, float eps, void *d_y, int64_t ldy, float *d_stats, uint8_t *d_codes,
+                            int64_t ldc, float *d_params, int64_t n, int64_t H, void *stream);
+int sgnn_layer_norm_blocks(void);
+int sgnn_layer_norm_backward(int dtype, const void *d_gy, int64_t ldg, const void *d_x, int64_t ldx,
+                             const uint8_t *d_codes, int64_t ldc, const float *d_params, const float *d_stats,
+                             int param_dtype, const void *d_gamma, void *d_gx, int64_t ldgx, void *d_g_gamma,
+                             void *d_g_beta, float *d_partials, int64_t n, int64_t H, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits: per row zp = min, sc = (max - min) / 255, code = rne((x - zp) / sc), restored
+ * value zp + sc code (the boundary exchange's quantiser, super_gnn/ops/csrc/quantization_arm.cpp:79-301, at 8 bits, for
+ * rows of any width in fp32 / bf16 / fp16).  No reference counterpart: it keeps fp32 activations for the backward.
+ *   A range below 255 FLT_MIN counts as none (sc = 1, codes 0).  A row with a NaN or an infinity, or a range above
+ *   FLT_MAX, is restored as NaN.
+ *   d_codes uint8[n, ldc], d_params fp32[n, 2] = (zp, sc).
+ * sgnn_checkpoint_weight_grad: the weight gradient of y = x W^T from the codes of x,
+ *     out[m, k] = sum_r g[r, m] (zp_r + sc_r code[r, k]) + beta out[m, k]     fp32[M, ldo]
+ *   with g[n, M] of `dtype`; g sc is carried in 16 bits of significand or more, sums in fp32 and in a fixed order.
+ *   d_workspace: the bytes ..._workspace_bytes reports; not to be shared by calls that can run concurrently.
+ *   n < 2^31, M, F <= 65536.
+ * ------------------------------------------------------------------------- */
+int sgnn_checkpoint_pack_rows(int dtype, const void *d_x, int64_t ldx, uint8_t *d_codes, int64_t ldc, float *d_params,
+                              int64_t n, int64_t F, void *stream);
+int sgnn_checkpoint_unpack_rows(const uint8_t *d_codes, int64_t ldc, const float *d_params, int dtype, void *d_out,
+                                int64_t ldo, int64_t n, int64_t F, void *stream);
+int sgnn_checkpoint_weight_grad_workspace_bytes(int dtype, int64_t n, int64_t M, int64_t F, size_t *bytes);
+int sgnn_checkpoint_weight_grad(int dtype, const void *d_g, int64_t ldg, const uint8_t *d_codes, int64_t ldc,
+                                const float *d_params, int64_t n, int64_t M, int64_t F, float beta, float *d_out,
+                                int64_t ldo, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Negative log-likelihood of a linear classifier over many classes, and its gradients, in pieces of the classes: the
+ * logits [n, C] are never kept.
+ *     z = x W^T + bias,  lse[r] = log sum_c exp z[r, c],  loss = inv_count sum_{r in the loss} (lse[r] - z[r, label])
+ *     G[r, c] = inv_count (exp(z[r, c] - lse[r]) - [c == label]),  gx = G W,  gw = G^T x,  gb = sum_r G
+ * The large-C counterpart of sgnn_softmax_nll_loss, with the last linear map inside (super_gnn/layers/sageconv.py:77-87
+ * followed by examples/graphsage/sage.py:211 and examples/graphsage/train.py:41-44).
+ *
+ *   dtype: SGNN_F32 or SGNN_BF16, of x [n, ldx], w [C, ldw], gx, gw; bias [C] (may be NULL) and gb of bias_dtype (fp32
+ *   or dtype).  A row is in the loss when d_mask (uint8[n], NULL = every row) is not 0 and its label (int64) lies in
+ *   [0, C); the others are not read: their lse is 0 and their gx rows are zero, whatever x holds there.
+ *   d_loss fp32[1], d_lse fp32[n] (may be NULL); d_gx, d_gw, d_gb all NULL (loss only) or d_gx and d_gw not NULL.
+ *   Sums in a fixed order.  n < 2^31, C < 2^31, K <= 16384.
+ *   d_workspace: the bytes ..._workspace_bytes reports; not to be shared by calls that can run concurrently.
+ * ------------------------------------------------------------------------- */
+int sgnn_linear_nll_workspace_bytes(int dtype, int64_t n, int64_t K, int64_t C, int with_grad, size_t *bytes);
+int sgnn_linear_nll_loss(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, int bias_dtype,
+                         const void *d_bias, const int64_t *d_labels, const uint8_t *d_mask, float inv_count, int64_t n,
+                         int64_t K, int64_t C, float *d_loss, float *d_lse, void *d_gx, int64_t ldgx, void *d_gw,
+                         int64_t ldgw, void *d_gb, void *d_workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Minimum vertex cover of a bipartite graph (HOST arrays, set-up code): Hopcroft-Karp

@@ -53,6 +53,16 @@ SIGNATURES = {
     "sgnn_gemm_f32_workspace_bytes": (_I, [_I, _L, _L, _L, _P]),
     "sgnn_gemm_f32": (_I, [_I, _P, _L, _P, _L, _P, _L, _L, _L, _L, c_float, _P, c_size_t, _P]),
     "sgnn_dropout_mask": (_I, [c_uint64, c_float, _L, _L, _P, _P]),
+    "sgnn_layer_norm_forward": (_I, [_I, _P, _L, _I, _P, _P, c_float, _P, _L, _P, _P, _L, _P, _L, _L, _P]),
+    "sgnn_layer_norm_blocks": (_I, []),
+    "sgnn_layer_norm_backward": (_I, [_I, _P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P, _L, _P, _P, _P, _L, _L, _P]),
+    "sgnn_checkpoint_pack_rows": (_I, [_I, _P, _L, _P, _L, _P, _L, _L, _P]),
+    "sgnn_checkpoint_unpack_rows": (_I, [_P, _L, _P, _I, _P, _L, _L, _L, _P]),
+    "sgnn_checkpoint_weight_grad_workspace_bytes": (_I, [_I, _L, _L, _L, _P]),
+    "sgnn_checkpoint_weight_grad": (_I, [_I, _P, _L, _P, _L, _P, _L, _L, _L, c_float, _P, _L, _P, c_size_t, _P]),
+    "sgnn_linear_nll_workspace_bytes": (_I, [_I, _L, _L, _L, _I, _P]),
+    "sgnn_linear_nll_loss": (_I, [_I, _P, _L, _P, _L, _I, _P, _P, _P, c_float, _L, _L, _L, _P, _P, _P, _L, _P, _L, _P,
+                                  _P, c_size_t, _P]),
     "sgnn_bipartite_min_vertex_cover": (_I, [_L, _L, _P, _P, _P, _P, _P]),
     "sgnn_peer_barrier": (_I, [_P, c_int, c_int, c_uint32, _L, _P, _P]),
     "sgnn_gather_rows": (_I, [_P, _L, _P, _L, _L, _P, _L, _P]),

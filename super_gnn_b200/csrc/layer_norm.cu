@@ -1,0 +1,630 @@
+// Layer norm of the rows of a matrix and its gradients (sm_100a):
+//
+//     mean = sum_c x[c] / H,  rstd = 1 / sqrt(sum_c (x[c] - mean)^2 / H + eps),  xh = (x - mean) rstd
+//     y  = xh gamma + beta
+//     gx = rstd (a - mean(a) - xh mean(a xh)),  a = gy gamma
+//     grad_gamma[c] = sum_r gy[r, c] xh[r, c],  grad_beta[c] = sum_r gy[r, c]
+//
+// The reference calls torch.nn.LayerNorm between two layers (examples/graphsage/sage.py:149-151, 192-194).  The
+// forward can write the 8-bit checkpoint of x in the same pass, and the backward can read that checkpoint in place of
+// x: one byte an element kept between the two instead of four.
+//
+// Everything is bound by memory: the forward moves x and y once, the backward gy, x (or its codes) and gx once.  Rows
+// of up to 1024 elements belong to a warp, which holds them in registers between the reductions and the
+// outputs; longer rows to a block, which reads them again (from L1 / L2) for every step.  All sums are fp32: the variance
+// from the differences to the mean, the column sums per warp, then per block, then over the blocks, in a fixed order.
+#include "row_io.cuh"
+
+namespace sgnn {
+
+constexpr int kNormThreads = 256;
+constexpr int kNormWarps = kNormThreads / 32;
+constexpr int kNormMaxWidth = 16384;  // the block kernels keep two column sums an element in shared memory
+
+struct NormParam {
+    const void *gamma, *beta;  // nullptr: 1 and 0
+    bool f32;                  // fp32, otherwise of the activation type
+};
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+// CK: also write the 8-bit codes of x and their (zero point, scale)
+template <class T, int E, int NV, bool CK>
+__global__ void __launch_bounds__(kNormThreads)
+norm_fwd_warp_kernel(const T *__restrict__ x, int64_t ldx, NormParam par, float eps, T *__restrict__ y, int64_t ldy,
+                     float2 *__restrict__ stats, uint8_t *__restrict__ codes, int64_t ldc, float2 *__restrict__ params,
+                     int64_t n, int H)
+{
+    constexpr bool kHold = E * NV <= 8;  // gamma and beta in registers; from L1 every row where they would not fit
+    const int lane = threadIdx.x & 31;
+    const float invH = 1.0f / (float)H;
+    float ga[kHold ? NV : 1][E], be[kHold ? NV : 1][E];
+    if constexpr (kHold) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+                load_param<T, E>(par.gamma, par.f32, c, 1.f, ga[i]);
+                load_param<T, E>(par.beta, par.f32, c, 0.f, be[i]);
+            }
+        }
+    }
+    const int64_t step = (int64_t)gridDim.x * kNormWarps;
+    for (int64_t r = (int64_t)blockIdx.x * kNormWarps + (threadIdx.x >> 5); r < n; r += step) {
+        float v[NV][E];
+        float s = 0.f, mn = INFINITY, mx = -INFINITY, poison = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) load_row<T, E>(x + r * ldx + c, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((lane + 32 * i) * E < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    s += v[i][e];
+                    if (CK) {
+                        mn = fminf(mn, v[i][e]);
+                        mx = fmaxf(mx, v[i][e]);
+                        poison = __fmaf_rn(v[i][e], 0.f, poison);
+                    }
+                }
+            }
+        }
+        const float mean = all_sum(s) * invH;
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((lane + 32 * i) * E < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float d = v[i][e] - mean;
+                    q += d * d;
+                }
+            }
+        }
+        const float rstd = __frsqrt_rn(all_sum(q) * invH + eps);
+        if (lane == 0) stats[r] = make_float2(mean, rstd);
+        RowQ rq;
+        if (CK) {
+            rq = row_quantiser(redux_min(mn), redux_max(mx), all_sum(poison));
+            if (lane == 0) params[r] = make_float2(rq.mn, rq.sc);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+                if (CK) store_codes<E>(codes + r * ldc + c, v[i], rq);
+                float g[E], b[E];
+                if constexpr (!kHold) {
+                    load_param<T, E>(par.gamma, par.f32, c, 1.f, g);
+                    load_param<T, E>(par.beta, par.f32, c, 0.f, b);
+                }
+                float o[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    o[e] = (v[i][e] - mean) * rstd * (kHold ? ga[kHold ? i : 0][e] : g[e]) + (kHold ? be[kHold ? i : 0][e] : b[e]);
+                store_row<T, E>(y + r * ldy + c, o);
+            }
+        }
+    }
+}
+
+// sum over the block, the same value in every thread
+__device__ __forceinline__ float block_sum(float v, float *red)
+{
+    v = all_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < kNormWarps; ++w) t += red[w];
+    return t;
+}
+
+__device__ __forceinline__ float block_max(float v, float *red)
+{
+    v = redux_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float t = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kNormWarps; ++w) t = fmaxf(t, red[w]);
+    return t;
+}
+
+template <class T, int E, bool CK>
+__global__ void __launch_bounds__(kNormThreads)
+norm_fwd_block_kernel(const T *__restrict__ x, int64_t ldx, NormParam par, float eps, T *__restrict__ y, int64_t ldy,
+                      float2 *__restrict__ stats, uint8_t *__restrict__ codes, int64_t ldc,
+                      float2 *__restrict__ params, int64_t n, int H)
+{
+    __shared__ float red[kNormWarps];
+    const float invH = 1.0f / (float)H;
+    for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+        const T *xr = x + r * ldx;
+        float s = 0.f, mn = INFINITY, mx = -INFINITY, poison = 0.f, v[E];
+        for (int c = threadIdx.x * E; c < H; c += kNormThreads * E) {
+            load_row<T, E>(xr + c, v);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                s += v[e];
+                if (CK) mn = fminf(mn, v[e]), mx = fmaxf(mx, v[e]), poison = __fmaf_rn(v[e], 0.f, poison);
+            }
+        }
+        const float mean = block_sum(s, red) * invH;
+        float q = 0.f;
+        for (int c = threadIdx.x * E; c < H; c += kNormThreads * E) {
+            load_row<T, E>(xr + c, v);
+#pragma unroll
+            for (int e = 0; e < E; ++e) q += (v[e] - mean) * (v[e] - mean);
+        }
+        const float rstd = __frsqrt_rn(block_sum(q, red) * invH + eps);
+        RowQ rq;
+        if (CK) rq = row_quantiser(-block_max(-mn, red), block_max(mx, red), block_sum(poison, red));
+        if (threadIdx.x == 0) {
+            stats[r] = make_float2(mean, rstd);
+            if (CK) params[r] = make_float2(rq.mn, rq.sc);
+        }
+        for (int c = threadIdx.x * E; c < H; c += kNormThreads * E) {
+            float g[E], b[E];
+            load_row<T, E>(xr + c, v);
+            load_param<T, E>(par.gamma, par.f32, c, 1.f, g);
+            load_param<T, E>(par.beta, par.f32, c, 0.f, b);
+            if (CK) store_codes<E>(codes + r * ldc + c, v, rq);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = (v[e] - mean) * rstd * g[e] + b[e];
+            store_row<T, E>(y + r * ldy + c, v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// Where the backward finds xh: x itself, or the 8-bit codes of x (then xh = code (sc rstd) + (zp - mean) rstd)
+struct NormSource {
+    const void *x;
+    int64_t ldx;
+    const uint8_t *codes;
+    int64_t ldc;
+    const float2 *params;
+};
+
+struct NormAffine {
+    float mul, add;  // xh = value * mul + add, value = x or its code
+};
+
+template <bool CK>
+__device__ __forceinline__ NormAffine norm_affine(const NormSource &src, int64_t r, float2 st)
+{
+    NormAffine f;
+    if (CK) {
+        const float2 p = __ldg(src.params + r);
+        f.mul = p.y * st.y;
+        f.add = (p.x - st.x) * st.y;
+    } else {
+        f.mul = st.y;
+        f.add = -st.x;  // (x + add) * mul
+    }
+    return f;
+}
+
+template <bool CK>
+__device__ __forceinline__ float norm_hat(float v, NormAffine f)
+{
+    return CK ? __fmaf_rn(v, f.mul, f.add) : (v + f.add) * f.mul;
+}
+
+template <class T, int E, bool CK>
+__device__ __forceinline__ void load_source(const NormSource &src, int64_t r, int c, float (&v)[E])
+{
+    if constexpr (CK) load_codes<E>(src.codes + r * src.ldc + c, v);
+    else load_row<T, E>(static_cast<const T *>(src.x) + r * src.ldx + c, v);
+}
+
+// partials: [gridDim.x, 2, H], per-block column sums of (gy xh, gy)
+template <class T, int E, int NV, bool CK>
+__global__ void __launch_bounds__(kNormThreads)
+norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
+                     NormParam par, T *__restrict__ gx, int64_t ldgx, float *__restrict__ partials, int64_t n, int H)
+{
+    extern __shared__ float sums[];  // [warps, 2, H]: every lane touches its own columns only until the last step
+    constexpr bool kHold = E * NV <= 8;  // the column sums of longer rows live in shared memory
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float *mine = sums + (size_t)warp * 2 * H;
+    const float invH = 1.0f / (float)H;
+    float ga[kHold ? NV : 1][E], sg[kHold ? NV : 1][E], sb[kHold ? NV : 1][E];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (lane + 32 * i) * E;
+        if constexpr (kHold) {
+            if (c < H) load_param<T, E>(par.gamma, par.f32, c, 1.f, ga[i]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) sg[i][e] = sb[i][e] = 0.f;
+        } else if (c < H) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) mine[c + e] = mine[H + c + e] = 0.f;
+        }
+    }
+    const int64_t step = (int64_t)gridDim.x * kNormWarps;
+    for (int64_t r = (int64_t)blockIdx.x * kNormWarps + warp; r < n; r += step) {
+        float a[NV][E], xh[NV][E];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+                load_row<T, E>(gy + r * ldg + c, a[i]);
+                load_source<T, E, CK>(src, r, c, xh[i]);
+            }
+        }
+        const float2 st = __ldg(stats + r);
+        const NormAffine f = norm_affine<CK>(src, r, st);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+                float g[E];
+                if constexpr (!kHold) load_param<T, E>(par.gamma, par.f32, c, 1.f, g);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    xh[i][e] = norm_hat<CK>(xh[i][e], f);
+                    if constexpr (kHold) {
+                        sg[i][e] += a[i][e] * xh[i][e];
+                        sb[i][e] += a[i][e];
+                    } else {
+                        mine[c + e] += a[i][e] * xh[i][e];
+                        mine[H + c + e] += a[i][e];
+                    }
+                    a[i][e] *= kHold ? ga[kHold ? i : 0][e] : g[e];
+                    s1 += a[i][e];
+                    s2 += a[i][e] * xh[i][e];
+                }
+            }
+        }
+        const float m1 = all_sum(s1) * invH, m2 = all_sum(s2) * invH;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) a[i][e] = st.y * (a[i][e] - m1 - xh[i][e] * m2);
+                store_row<T, E>(gx + r * ldgx + c, a[i]);
+            }
+        }
+    }
+    if constexpr (kHold) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) mine[c + e] = sg[i][e], mine[H + c + e] = sb[i][e];
+            }
+        }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < 2 * H; k += kNormThreads) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < kNormWarps; ++w) t += sums[(size_t)w * 2 * H + k];
+        partials[(size_t)blockIdx.x * 2 * H + k] = t;
+    }
+}
+
+template <class T, int E, bool CK>
+__global__ void __launch_bounds__(kNormThreads)
+norm_bwd_block_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
+                      NormParam par, T *__restrict__ gx, int64_t ldgx, float *__restrict__ partials, int64_t n, int H)
+{
+    extern __shared__ float sums[];  // [2, H]: a column belongs to one thread
+    __shared__ float red[kNormWarps];
+    const float invH = 1.0f / (float)H;
+    for (int c = threadIdx.x * E; c < H; c += kNormThreads * E) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) sums[c + e] = sums[H + c + e] = 0.f;
+    }
+    for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+        const float2 st = __ldg(stats + r);
+        const NormAffine f = norm_affine<CK>(src, r, st);
+        float s1 = 0.f, s2 = 0.f, a[E], v[E], g[E];
+        for (int c = threadIdx.x * E; c < H; c += kNormThreads * E) {
+            load_row<T, E>(gy + r * ldg + c, a);
+            load_source<T, E, CK>(src, r, c, v);
+            load_param<T, E>(par.gamma, par.f32, c, 1.f, g);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float xh = norm_hat<CK>(v[e], f);
+                sums[c + e] += a[e] * xh;
+                sums[H + c + e] += a[e];
+                s1 += a[e] * g[e];
+                s2 += a[e] * g[e] * xh;
+            }
+        }
+        const float m1 = block_sum(s1, red) * invH, m2 = block_sum(s2, red) * invH;
+        for (int c = threadIdx.x * E; c < H; c += kNormThreads * E) {
+            load_row<T, E>(gy + r * ldg + c, a);
+            load_source<T, E, CK>(src, r, c, v);
+            load_param<T, E>(par.gamma, par.f32, c, 1.f, g);
+#pragma unroll
+            for (int e = 0; e < E; ++e) a[e] = st.y * (a[e] * g[e] - m1 - norm_hat<CK>(v[e], f) * m2);
+            store_row<T, E>(gx + r * ldgx + c, a);
+        }
+    }
+    for (int c = threadIdx.x * E; c < H; c += kNormThreads * E) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            partials[(size_t)blockIdx.x * 2 * H + c + e] = sums[c + e];
+            partials[(size_t)blockIdx.x * 2 * H + H + c + e] = sums[H + c + e];
+        }
+    }
+}
+
+// out[k] = sum over the blocks of partials[blocks, 2 H], in a fixed order: 32 columns a block, the partial rows dealt
+// over its 32 warps, whose sums are added in turn
+__global__ void __launch_bounds__(1024)
+norm_reduce_kernel(const float *__restrict__ partials, int blocks, int H, void *__restrict__ g_gamma,
+                   void *__restrict__ g_beta, int dtype)
+{
+    __shared__ float t[32][33];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int k = blockIdx.x * 32 + lane;
+    float acc = 0.f;
+    if (k < 2 * H) {
+        for (int b = w; b < blocks; b += 32) acc += partials[(size_t)b * 2 * H + k];
+    }
+    t[w][lane] = acc;
+    __syncthreads();
+    if (w != 0 || k >= 2 * H) return;
+    for (int i = 1; i < 32; ++i) acc += t[i][lane];
+    void *out = k < H ? g_gamma : g_beta;
+    const int c = k < H ? k : k - H;
+    if (dtype == SGNN_F32) static_cast<float *>(out)[c] = acc;
+    else if (dtype == SGNN_BF16) static_cast<__nv_bfloat16 *>(out)[c] = __float2bfloat16_rn(acc);
+    else static_cast<__half *>(out)[c] = __float2half_rn(acc);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct NormCall {
+    int dtype;
+    const void *x;  // forward input, or the backward's source where there are no codes
+    int64_t ldx;
+    NormParam par;
+    float eps;
+    void *y;
+    int64_t ldy;
+    float2 *stats;
+    uint8_t *codes;
+    int64_t ldc;
+    float2 *params;
+    const void *gy;
+    int64_t ldg;
+    void *gx;
+    int64_t ldgx;
+    float *partials;
+    int64_t n;
+    int H;
+    cudaStream_t stream;
+};
+
+static int norm_blocks_cap() { return sm_count() * 8; }
+
+// Blocks of a call: enough for every warp (or block) to have a row, at most what is resident at once.
+template <class K>
+static int norm_grid(K kernel, int64_t n, int rows_per_block, size_t smem, int *grid)
+{
+    if (smem > 48 * 1024)
+        SGNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    int per_sm = 0;
+    SGNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kNormThreads, smem));
+    int64_t g = (int64_t)sm_count() * (per_sm > 0 ? per_sm : 1);
+    if (g > norm_blocks_cap()) g = norm_blocks_cap();
+    const int64_t need = ceil_div(n, rows_per_block);
+    *grid = (int)(g < need ? g : need);
+    return SGNN_OK;
+}
+
+template <class T, int E, int NV, bool CK>
+static int norm_fwd_launch(const NormCall &c)
+{
+    int grid = 0;
+    if constexpr (NV > 0) {
+        int rc = norm_grid(norm_fwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, 0, &grid);
+        if (rc) return rc;
+        norm_fwd_warp_kernel<T, E, NV, CK><<<grid, kNormThreads, 0, c.stream>>>(
+            static_cast<const T *>(c.x), c.ldx, c.par, c.eps, static_cast<T *>(c.y), c.ldy, c.stats, c.codes, c.ldc,
+            c.params, c.n, c.H);
+    } else {
+        int rc = norm_grid(norm_fwd_block_kernel<T, E, CK>, c.n, 1, 0, &grid);
+        if (rc) return rc;
+        norm_fwd_block_kernel<T, E, CK><<<grid, kNormThreads, 0, c.stream>>>(
+            static_cast<const T *>(c.x), c.ldx, c.par, c.eps, static_cast<T *>(c.y), c.ldy, c.stats, c.codes, c.ldc,
+            c.params, c.n, c.H);
+    }
+    SGNN_LAUNCH_OK("layer norm forward");
+    return SGNN_OK;
+}
+
+template <class T, int E, int NV, bool CK>
+static int norm_bwd_launch(const NormCall &c, int *blocks)
+{
+    const NormSource src{c.x, c.ldx, c.codes, c.ldc, c.params};
+    if constexpr (NV > 0) {
+        const size_t smem = (size_t)kNormWarps * 2 * c.H * sizeof(float);
+        int rc = norm_grid(norm_bwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, smem, blocks);
+        if (rc) return rc;
+        norm_bwd_warp_kernel<T, E, NV, CK><<<*blocks, kNormThreads, smem, c.stream>>>(
+            static_cast<const T *>(c.gy), c.ldg, src, c.stats, c.par, static_cast<T *>(c.gx), c.ldgx, c.partials, c.n,
+            c.H);
+    } else {
+        const size_t smem = (size_t)2 * c.H * sizeof(float);
+        int rc = norm_grid(norm_bwd_block_kernel<T, E, CK>, c.n, 1, smem, blocks);
+        if (rc) return rc;
+        norm_bwd_block_kernel<T, E, CK><<<*blocks, kNormThreads, smem, c.stream>>>(
+            static_cast<const T *>(c.gy), c.ldg, src, c.stats, c.par, static_cast<T *>(c.gx), c.ldgx, c.partials, c.n,
+            c.H);
+    }
+    SGNN_LAUNCH_OK("layer norm backward");
+    return SGNN_OK;
+}
+
+// fn<T, E, NV, CK>(c, ...) with the accesses a lane needs for a row (NV = 0: the block kernel)
+#define SGNN_NORM_NV(T, E, fn, ...)                                                                                     \
+    do {                                                                                                                \
+        const int need = (int)ceil_div(c.H, 32 * E);                                                                    \
+        if constexpr (E >= 4) {                                                                                         \
+            if (need <= 1) return fn<T, E, 1, CK>(__VA_ARGS__);                                                         \
+            if (need <= 2) return fn<T, E, 2, CK>(__VA_ARGS__);                                                         \
+            if (need <= 4) return fn<T, E, 4, CK>(__VA_ARGS__);                                                         \
+            if constexpr (E == 4) {                                                                                     \
+                if (need <= 8) return fn<T, E, 8, CK>(__VA_ARGS__);                                                     \
+            }                                                                                                           \
+        } else {                                                                                                        \
+            if (need <= 8 / E) return fn<T, E, 8 / E, CK>(__VA_ARGS__);                                                 \
+            if (need <= 32 / E) return fn<T, E, 32 / E, CK>(__VA_ARGS__);                                               \
+        }                                                                                                               \
+        return fn<T, E, 0, CK>(__VA_ARGS__);                                                                            \
+    } while (0)
+
+template <bool CK>
+static int norm_fwd_dispatch(const NormCall &c)
+{
+    const size_t b = elem_bytes(c.dtype);
+    const int wide = (int)(16 / b);
+    const size_t pb = c.par.f32 ? 4 : b;
+    const RowOperand ops[] = {{c.x, c.ldx, b}, {c.y, c.ldy, b}, {c.par.gamma, 0, pb}, {c.par.beta, 0, pb},
+                              {CK ? c.codes : nullptr, c.ldc, 1}};
+    const int e = row_step(c.H, wide, ops);
+    if (c.dtype == SGNN_F32) {
+        if (e == 4) SGNN_NORM_NV(float, 4, norm_fwd_launch, c);
+        if (e == 2) SGNN_NORM_NV(float, 2, norm_fwd_launch, c);
+        SGNN_NORM_NV(float, 1, norm_fwd_launch, c);
+    }
+    if (c.dtype == SGNN_BF16) {
+        if (e == 8) SGNN_NORM_NV(__nv_bfloat16, 8, norm_fwd_launch, c);
+        if (e == 2) SGNN_NORM_NV(__nv_bfloat16, 2, norm_fwd_launch, c);
+        SGNN_NORM_NV(__nv_bfloat16, 1, norm_fwd_launch, c);
+    }
+    if (e == 8) SGNN_NORM_NV(__half, 8, norm_fwd_launch, c);
+    if (e == 2) SGNN_NORM_NV(__half, 2, norm_fwd_launch, c);
+    SGNN_NORM_NV(__half, 1, norm_fwd_launch, c);
+}
+
+template <bool CK>
+static int norm_bwd_dispatch(const NormCall &c, int *blocks)
+{
+    const size_t b = elem_bytes(c.dtype);
+    const int wide = (int)(16 / b);
+    const RowOperand ops[] = {{c.gy, c.ldg, b}, {c.gx, c.ldgx, b}, {c.par.gamma, 0, c.par.f32 ? 4 : b},
+                              {CK ? nullptr : c.x, c.ldx, b}, {CK ? c.codes : nullptr, c.ldc, 1}};
+    const int e = row_step(c.H, wide, ops);
+    if (c.dtype == SGNN_F32) {
+        if (e == 4) SGNN_NORM_NV(float, 4, norm_bwd_launch, c, blocks);
+        if (e == 2) SGNN_NORM_NV(float, 2, norm_bwd_launch, c, blocks);
+        SGNN_NORM_NV(float, 1, norm_bwd_launch, c, blocks);
+    }
+    if (c.dtype == SGNN_BF16) {
+        if (e == 8) SGNN_NORM_NV(__nv_bfloat16, 8, norm_bwd_launch, c, blocks);
+        if (e == 2) SGNN_NORM_NV(__nv_bfloat16, 2, norm_bwd_launch, c, blocks);
+        SGNN_NORM_NV(__nv_bfloat16, 1, norm_bwd_launch, c, blocks);
+    }
+    if (e == 8) SGNN_NORM_NV(__half, 8, norm_bwd_launch, c, blocks);
+    if (e == 2) SGNN_NORM_NV(__half, 2, norm_bwd_launch, c, blocks);
+    SGNN_NORM_NV(__half, 1, norm_bwd_launch, c, blocks);
+}
+#undef SGNN_NORM_NV
+
+static int norm_check(const char *who, int dtype, int param_dtype, int64_t n, int64_t H)
+{
+    SGNN_REQUIRE(elem_known(dtype) && elem_known(param_dtype), SGNN_ERR_INVALID_ARGUMENT, "%s: unknown element type", who);
+    SGNN_REQUIRE(param_dtype == dtype || param_dtype == SGNN_F32, SGNN_ERR_INVALID_ARGUMENT,
+                 "%s: gamma and beta must be fp32 or of the activation type", who);
+    SGNN_REQUIRE(n >= 0 && H > 0, SGNN_ERR_INVALID_ARGUMENT, "%s: bad size", who);
+    SGNN_REQUIRE(H <= kNormMaxWidth, SGNN_ERR_UNSUPPORTED, "%s: rows of at most %d elements (got %lld)", who,
+                 kNormMaxWidth, (long long)H);
+    SGNN_REQUIRE(n <= (1LL << 40), SGNN_ERR_TOO_LARGE, "%s: too many rows", who);
+    return SGNN_OK;
+}
+
+static bool aligned_to(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+}  // namespace sgnn
+
+using namespace sgnn;
+
+extern "C" SGNN_API int sgnn_layer_norm_forward(int dtype, const void *d_x, int64_t ldx, int param_dtype,
+                                                const void *d_gamma, const void *d_beta, float eps, void *d_y,
+                                                int64_t ldy, float *d_stats, uint8_t *d_codes, int64_t ldc,
+                                                float *d_params, int64_t n, int64_t H, void *stream)
+{
+    const char *who = "layer_norm_forward";
+    int rc = norm_check(who, dtype, param_dtype, n, H);
+    if (rc) return rc;
+    SGNN_REQUIRE(eps >= 0.f, SGNN_ERR_INVALID_ARGUMENT, "%s: eps must not be negative", who);
+    if (n == 0) return SGNN_OK;
+    SGNN_REQUIRE(d_x && d_y && d_stats, SGNN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    SGNN_REQUIRE((d_codes == nullptr) == (d_params == nullptr), SGNN_ERR_INVALID_ARGUMENT,
+                 "%s: codes and params belong together", who);
+    SGNN_REQUIRE((n == 1 || (ldx >= H && ldy >= H)) && (d_codes == nullptr || n == 1 || ldc >= H), SGNN_ERR_INVALID_ARGUMENT,
+                 "%s: leading dimension shorter than a row", who);
+    const size_t b = elem_bytes(dtype), pb = elem_bytes(param_dtype);
+    SGNN_REQUIRE(aligned_to(d_x, b) && aligned_to(d_y, b) && aligned_to(d_gamma, pb) && aligned_to(d_beta, pb) &&
+                     aligned_to(d_stats, 8) && aligned_to(d_params, 8),
+                 SGNN_ERR_INVALID_ARGUMENT, "%s: pointers must be aligned to their element (stats, params: 8 bytes)", who);
+    NormCall c{};
+    c.dtype = dtype, c.x = d_x, c.ldx = ldx, c.par = NormParam{d_gamma, d_beta, param_dtype == SGNN_F32}, c.eps = eps;
+    c.y = d_y, c.ldy = ldy, c.stats = reinterpret_cast<float2 *>(d_stats), c.codes = d_codes, c.ldc = ldc;
+    c.params = reinterpret_cast<float2 *>(d_params), c.n = n, c.H = (int)H, c.stream = (cudaStream_t)stream;
+    return d_codes ? norm_fwd_dispatch<true>(c) : norm_fwd_dispatch<false>(c);
+}
+
+extern "C" SGNN_API int sgnn_layer_norm_blocks(void) { return norm_blocks_cap(); }
+
+extern "C" SGNN_API int sgnn_layer_norm_backward(int dtype, const void *d_gy, int64_t ldg, const void *d_x, int64_t ldx,
+                                                 const uint8_t *d_codes, int64_t ldc, const float *d_params,
+                                                 const float *d_stats, int param_dtype, const void *d_gamma,
+                                                 void *d_gx, int64_t ldgx, void *d_g_gamma, void *d_g_beta,
+                                                 float *d_partials, int64_t n, int64_t H, void *stream)
+{
+    const char *who = "layer_norm_backward";
+    int rc = norm_check(who, dtype, param_dtype, n, H);
+    if (rc) return rc;
+    SGNN_REQUIRE(d_g_gamma && d_g_beta, SGNN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    const size_t b = elem_bytes(dtype), pb = elem_bytes(param_dtype);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (n == 0) {
+        SGNN_CUDA_OK(cudaMemsetAsync(d_g_gamma, 0, (size_t)H * pb, s));
+        SGNN_CUDA_OK(cudaMemsetAsync(d_g_beta, 0, (size_t)H * pb, s));
+        return SGNN_OK;
+    }
+    SGNN_REQUIRE(d_gy && d_gx && d_stats && d_partials, SGNN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    SGNN_REQUIRE((d_codes == nullptr) == (d_params == nullptr) && (d_codes == nullptr) != (d_x == nullptr),
+                 SGNN_ERR_INVALID_ARGUMENT, "%s: exactly one of x and (codes, params) must be given", who);
+    SGNN_REQUIRE(n == 1 || (ldg >= H && ldgx >= H && (d_x == nullptr || ldx >= H) && (d_codes == nullptr || ldc >= H)),
+                 SGNN_ERR_INVALID_ARGUMENT, "%s: leading dimension shorter than a row", who);
+    SGNN_REQUIRE(aligned_to(d_gy, b) && aligned_to(d_x, b) && aligned_to(d_gx, b) && aligned_to(d_gamma, pb) &&
+                     aligned_to(d_g_gamma, pb) && aligned_to(d_g_beta, pb) && aligned_to(d_stats, 8) &&
+                     aligned_to(d_params, 8) && aligned_to(d_partials, 4),
+                 SGNN_ERR_INVALID_ARGUMENT, "%s: pointers must be aligned to their element (stats, params: 8 bytes)", who);
+    NormCall c{};
+    c.dtype = dtype, c.gy = d_gy, c.ldg = ldg, c.x = d_x, c.ldx = ldx;
+    c.codes = const_cast<uint8_t *>(d_codes), c.ldc = ldc;
+    c.params = reinterpret_cast<float2 *>(const_cast<float *>(d_params));
+    c.stats = reinterpret_cast<float2 *>(const_cast<float *>(d_stats));
+    c.par = NormParam{d_gamma, nullptr, param_dtype == SGNN_F32}, c.gx = d_gx, c.ldgx = ldgx, c.partials = d_partials;
+    c.n = n, c.H = (int)H, c.stream = s;
+    int blocks = 0;
+    rc = d_codes ? norm_bwd_dispatch<true>(c, &blocks) : norm_bwd_dispatch<false>(c, &blocks);
+    if (rc) return rc;
+    norm_reduce_kernel<<<(int)ceil_div(2 * H, 32), 1024, 0, s>>>(d_partials, blocks, (int)H, d_g_gamma, d_g_beta,
+                                                                 param_dtype);
+    SGNN_LAUNCH_OK("layer norm column sums");
+    return SGNN_OK;
+}

@@ -1,0 +1,268 @@
+"""The many-class loss of a linear classifier and its gradients against the formulas in 64 bits."""
+import pytest
+import torch
+
+from super_gnn_b200 import supergnn_ops as ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+STEP = 2.0 ** -23
+
+
+def make(n, K, C, dtype, seed, bdtype=None, scale=2.0, on=0.7):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(n, K, generator=gen, device=DEV).to(dtype)
+    w = (torch.randn(C, K, generator=gen, device=DEV) * (scale / K ** 0.5)).to(dtype)
+    b = (torch.randn(C, generator=gen, device=DEV) * 0.5).to(bdtype or dtype)
+    labels = torch.randint(0, C, (n,), generator=gen, device=DEV)
+    mask = torch.rand(n, generator=gen, device=DEV) < on
+    return x, w, b, labels, mask
+
+
+class Ref:
+    """The formulas in 64 bits, and bounds.
+
+    A logit is a sum of K products of which each is off by at most a step 2^-23 of itself (fp32 operands are carried in
+    22 bits or more; bf16 products are exact), every addition by 2^-23 of the magnitudes:
+        e_z = (K + 16) 2^-23 (sum |x w| + |b|).
+    lse moves by at most max_c e_z, and the sum of C exponentials in a tree of pieces adds (300 + C / 256) 2^-23.  p is
+    then off by p (2 e_z + ...), G is rounded to the operand type (bf16: 2^-8 of it, fp32: 2^-20), and the two products are
+    sums of C (gx) and m (gw) terms."""
+
+    def __init__(self, x, w, b, labels, mask, inv):
+        n, K = x.shape
+        C = w.size(0)
+        on = (labels >= 0) & (labels < C)
+        if mask is not None:
+            on &= mask.bool()
+        self.rows = on.nonzero()[:, 0]
+        dtype = x.dtype
+        xr, w = x[self.rows].double(), w.double()
+        b = torch.zeros(C, dtype=torch.float64, device=DEV) if b is None else b.double()
+        lab = labels[self.rows]
+        z = xr @ w.t() + b
+        at = torch.arange(len(lab), device=DEV)
+        finite_b = torch.where(torch.isfinite(b), b, torch.zeros_like(b))
+        e_z = (K + 16) * STEP * (xr.abs() @ w.abs().t() + finite_b.abs())
+        lse = torch.logsumexp(z, 1)
+        e_lse = e_z.amax(1) + (300 + C / 256) * STEP + 2 * STEP * lse.abs()
+        self.lse, self.e_lse = torch.zeros(n, dtype=torch.float64, device=DEV), torch.zeros(n, dtype=torch.float64, device=DEV)
+        self.lse[self.rows], self.e_lse[self.rows] = lse, e_lse
+        terms = lse - z[at, lab]
+        self.loss = terms.sum() * inv
+        self.e_loss = abs(inv) * ((e_lse + e_z[at, lab]).sum() + (len(lab) + 8) * STEP * terms.abs().sum())
+        p = (z - lse[:, None]).exp()
+        g = p.clone()
+        g[at, lab] -= 1
+        e_g = p * (e_z + e_lse[:, None] + 8 * STEP) * 1.01 + g.abs() * (2 ** -8 if dtype == torch.bfloat16 else 2 ** -20)
+        e_g += 2.0 ** -38  # the smallest steps of a stored probability
+        m = max(1, len(lab))
+        self.gx, self.e_gx = torch.zeros(n, K, dtype=torch.float64, device=DEV), torch.zeros(n, K, dtype=torch.float64, device=DEV)
+        self.gx[self.rows] = inv * (g @ w)
+        self.e_gx[self.rows] = abs(inv) * (e_g @ w.abs() + (C + 16) * STEP * (g.abs() @ w.abs()))
+        self.gw, self.e_gw = inv * (g.t() @ xr), abs(inv) * (e_g.t() @ xr.abs() + (m + 16) * STEP * (g.abs().t() @ xr.abs()))
+        self.gb, self.e_gb = inv * g.sum(0), abs(inv) * (e_g.sum(0) + (m + 16) * STEP * g.abs().sum(0))
+
+
+def close(got, want, err):
+    off, bound = (got.double() - want).abs(), err + want.abs() * (torch.finfo(got.dtype).eps / 2) + 1e-37
+    assert torch.isfinite(got).all()
+    bad = off > bound
+    assert not bad.any(), (off[bad][:4], bound[bad][:4], int(bad.sum()), tuple(got.shape))
+
+
+def check(x, w, b, labels, mask, inv):
+    ref = Ref(x, w, b, labels, mask, inv)
+    loss, lse = ops.linear_nll_loss(x, w, b, labels, mask, inv)
+    close(loss, ref.loss.reshape(1), ref.e_loss)
+    close(lse, ref.lse, ref.e_lse)
+    off = torch.ones(len(labels), dtype=torch.bool, device=DEV)
+    off[ref.rows] = False
+    assert (lse[off] == 0).all()
+    loss2, gx, gw, gb = ops.linear_nll_loss_grad(x, w, b, labels, mask, inv)
+    assert torch.equal(loss, loss2)
+    assert gx.dtype == x.dtype and gw.dtype == w.dtype and (b is None) == (gb is None)
+    close(gx, ref.gx, ref.e_gx)
+    close(gw, ref.gw, ref.e_gw)
+    assert (gx[off] == 0).all()
+    if b is not None:
+        assert gb.dtype == b.dtype
+        close(gb, ref.gb, ref.e_gb)
+    return loss, gx, gw, gb
+
+
+@pytest.mark.parametrize("n,K,C", [(1, 1, 1), (1, 1, 2), (1, 8, 300), (2, 3, 5), (5, 64, 256), (127, 100, 257), (128, 64, 512),
+                                   (129, 65, 511), (64, 256, 4099), (300, 130, 1000), (700, 602, 333), (2100, 20, 1025),
+                                   (31, 1030, 700), (1000, 512, 3001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loss_and_gradients(n, K, C, dtype):
+    check(*make(n, K, C, dtype, n + K + C), 1.0 / n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_row_lists_and_several_pieces(dtype):
+    """More rows than a listing block looks at, and more classes than a piece holds."""
+    check(*make(5000, 16, 20_000, dtype, 3), 0.01)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masks_and_labels(dtype):
+    x, w, b, labels, mask = make(400, 40, 300, dtype, 9)
+    labels[::7] = -1
+    labels[3::11] = 300
+    check(x, w, b, labels, mask, 0.5)
+    check(x, w, b, labels, None, 0.5)
+    check(x, w, None, labels, mask.to(torch.uint8), -2.0)
+    check(x, w, b.float(), labels, mask, 0.5)
+    block = torch.zeros_like(mask)
+    block[130:140] = True  # only rows of the second tile
+    check(x, w, b, labels, block, 0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nothing_in_the_loss(dtype):
+    x, w, b, labels, mask = make(50, 40, 300, dtype, 9)
+    for lab, m in ((labels, torch.zeros_like(mask)), (torch.full_like(labels, -1), None)):
+        loss, gx, gw, gb = ops.linear_nll_loss_grad(x, w, b, lab, m, 1.0)
+        assert loss.item() == 0 and not gx.any() and not gw.any() and not gb.any()
+        assert not ops.linear_nll_loss(x, w, b, lab, m, 1.0)[1].any()
+    loss, gx, gw, gb = ops.linear_nll_loss_grad(x[:0], w, b, labels[:0], None, 1.0)
+    assert loss.item() == 0 and gx.shape == (0, 40) and not gw.any() and not gb.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_outside_the_loss_may_hold_anything(dtype):
+    x, w, b, labels, mask = make(300, 40, 500, dtype, 4)
+    clean = ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.1)
+    x = x.clone()
+    x[~mask] = float("nan")
+    x[(~mask).nonzero()[0]] = float("inf")
+    labels = torch.where(mask, labels, torch.full_like(labels, 1 << 40))
+    for a, c in zip(ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.1), clean):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_classes_that_a_bias_rules_out(dtype):
+    x, w, b, labels, mask = make(200, 40, 700, dtype, 4, bdtype=torch.float32)
+    b[256:512] = float("-inf")
+    b[5] = torch.finfo(torch.float32).min
+    labels = labels % 250 + 6  # none of them a label
+    loss, gx, gw, gb = check(x, w, b, labels, mask, 0.1)
+    assert not gw[256:512].any() and not gb[256:512].any() and not gb[5].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_logits_and_rows_of_very_different_size(dtype):
+    x, w, b, labels, mask = make(200, 64, 400, dtype, 4, scale=40.0)
+    x = (x.float() * torch.exp2(torch.randint(-6, 3, (200, 1), device=DEV).float())).to(dtype)
+    check(x, w, b, labels, mask, 0.1)
+
+
+def test_features_of_very_different_size():
+    """Columns 2^30 apart: the gradient of each column keeps its own accuracy."""
+    x, w, b, labels, mask = make(200, 64, 400, torch.float32, 4)
+    s = torch.exp2(torch.linspace(-30, 0, 64, device=DEV).round())
+    check(x * s, w / s.clamp(min=2.0 ** -10), b, labels, mask, 0.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pad,offset", [(8, 0), (1, 0), (0, 1), (5, 3)])
+def test_strides_and_alignment(dtype, pad, offset):
+    x, w, b, labels, mask = make(150, 48, 600, dtype, 4)
+    want = ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.1)
+
+    def inside(t):
+        wide = torch.full((t.size(0), t.size(1) + pad + offset), float("nan"), dtype=dtype, device=DEV)
+        wide[:, offset:offset + t.size(1)] = t
+        return wide[:, offset:offset + t.size(1)]
+
+    for xx, ww in ((inside(x), w), (x, inside(w)), (x.t().contiguous().t(), w.t().contiguous().t())):
+        for a, c in zip(ops.linear_nll_loss_grad(xx, ww, b, labels, mask, 0.1), want):
+            assert torch.equal(a, c)
+
+
+def test_broadcast_input():
+    _, w, b, labels, _ = make(20, 48, 300, torch.float32, 4)
+    row = torch.randn(1, 48, device=DEV)
+    check(row.expand(20, 48), w, b, labels, None, 0.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_repeatable(dtype):
+    args = make(1500, 130, 3000, dtype, 4)
+    first = ops.linear_nll_loss_grad(*args, 0.01)
+    for _ in range(3):
+        for a, c in zip(ops.linear_nll_loss_grad(*args, 0.01), first):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_and_on_another_stream(dtype):
+    """A captured call sees the inputs of the replay, next to calls of another size on another stream."""
+    x, w, b, labels, mask = make(260, 72, 900, dtype, 4)
+    other = make(90, 40, 400, dtype, 5)
+    want_other = ops.linear_nll_loss_grad(*other, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.1)
+    for seed in (6, 7):
+        new = make(260, 72, 900, dtype, seed)
+        for t, v in zip((x, w, b, labels, mask), new):
+            t.copy_(v)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            others = [ops.linear_nll_loss_grad(*other, 0.1) for _ in range(3)]
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ops.linear_nll_loss_grad(*new, 0.1)
+        for a, c in zip(got, want):
+            assert torch.equal(a, c)
+        for o in others:
+            for a, c in zip(o, want_other):
+                assert torch.equal(a, c)
+
+
+def test_gradient_against_differences():
+    x, w, b, labels, mask = make(12, 10, 40, torch.float32, 4)
+    _, *grads = ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.25)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    base = [x.double(), w.double(), b.double()]
+
+    def value(xx, ww, bb):
+        logp = torch.log_softmax(xx @ ww.t() + bb, 1)
+        return float(-(logp.gather(1, labels[:, None])[:, 0] * mask).sum() * 0.25)
+
+    for at, grad in enumerate(grads):
+        v = torch.randn(base[at].shape, generator=gen, device=DEV, dtype=torch.float64)
+        up, down = list(base), list(base)
+        up[at], down[at] = base[at] + 1e-5 * v, base[at] - 1e-5 * v
+        want = (value(*up) - value(*down)) / 2e-5
+        # truncation 1e-10 of the third derivative, fp32 gradients
+        assert abs(float((grad.double() * v).sum()) - want) <= 1e-5 * float((grad.double() * v).abs().sum())
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, w, b, l, m: ops.linear_nll_loss(x.half(), w.half(), None, l, m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w.bfloat16(), b, l, m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w[:, :-1], b, l, m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w, b[:-1], l, m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w, b.double(), l, m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w, b, l.int(), m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w, b, l[:-1], m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w, b, l, m[:-1], 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w, b, l, m.float(), 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w, b, l, m, float("nan")),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x.cpu(), w, b, l, m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss(x, w[:0], None, l, m, 1.0),
+    lambda x, w, b, l, m: ops.linear_nll_loss_grad(torch.empty(8, 16385, device=DEV), torch.empty(9, 16385, device=DEV), None,
+                                                   l, m, 1.0),
+])
+def test_refusals(call):
+    with pytest.raises(RuntimeError):
+        call(*make(8, 16, 300, torch.float32, 1))
