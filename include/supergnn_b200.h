@@ -501,7 +501,8 @@ int sgnn_checkpoint_weight_grad(int dtype, const void *d_g, int64_t ldg, const u
  *   or dtype).  A row is in the loss when d_mask (uint8[n], NULL = every row) is not 0 and its label (int64) lies in
  *   [0, C); the others are not read: their lse is 0 and their gx rows are zero, whatever x holds there.
  *   d_loss fp32[1], d_lse fp32[n] (may be NULL); d_gx, d_gw, d_gb all NULL (loss only) or d_gx and d_gw not NULL.
- *   Sums in a fixed order.  n < 2^31, C < 2^31, K <= 16384.
+ *   Sums in a fixed order.  n, C <= 2^30, K <= 16384.
+ *   A kernel whose wait was not answered within two seconds gives up; the loss and gx are then NaN.
  *   d_workspace: the bytes ..._workspace_bytes reports; not to be shared by calls that can run concurrently.
  * ------------------------------------------------------------------------- */
 int sgnn_linear_nll_workspace_bytes(int dtype, int64_t n, int64_t K, int64_t C, int with_grad, size_t *bytes);
