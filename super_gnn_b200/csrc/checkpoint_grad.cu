@@ -1,73 +1,402 @@
 // Weight gradient of a linear map whose input was kept as 8-bit codes (sm_100a):
 //
 //     gW[m, k] = sum_r g[r, m] (zp_r + sc_r code[r, k])  (+ beta gW[m, k])
+//              = sum_r (g[r, m] sc_r) code[r, k]  +  sum_r g[r, m] zp_r
 //
-// The rows are split over the blocks; the partial products are added in a fixed order.
+// The first sum runs on the tensor cores: a code is exact in bf16, and g sc is carried as two bf16 terms (16 bits and
+// more of significand, 2^-17 of a value at most, next to codes that are half a step of 255 off), so a tile takes two
+// products where two fp32 operands would take six.  The second does not depend on k: a few fp32 multiply-adds beside the
+// conversion of g.  The activations are never restored in memory: one byte an element is read.
+//
+// A block owns 128 x 256 results and a range of the rows.  Per 32 rows TMA brings 128 columns of g and 256 of the codes
+// into shared memory as they are (where an operand is not aligned for it, the threads load it themselves);
+// eight warps convert them into the swizzled operands, both "MN-major" (the rows of g and of the codes are the reduction),
+// which keeps the order of the matrices; one thread issues the products.  Tensor memory rounds every addition
+// towards zero, which over thousands of rows would shrink the result by 1e-5 of itself, so after 512 rows the sums move on
+// into fp32 registers (the other half of the tensor memory takes over meanwhile).  The partial results of the row ranges
+// are added in a fixed order.
 #include "row_io.cuh"
-#include "tile_product.cuh"
+#include "umma.cuh"
 
 namespace sgnn {
 
-template <class T>
-struct GradOperand {  // A(m, r) = g[r, m]
-    const T *g;
-    int64_t ldg;
-    int M;
-    __device__ float operator()(int64_t m, int64_t r) const { return m < M ? to_f32<T>(g[r * ldg + m]) : 0.f; }
-};
+constexpr int kGM = 128, kGN = 256, kGRows = 32;  // results of a block, rows a step
+constexpr int kGWorkers = 8;                      // warps that convert and add up
+constexpr int kGThreads = (kGWorkers + 2) * 32;
+constexpr int kGRaw = 3, kGStages = 4;            // buffers of operands as they come, and converted
+constexpr int kGPromote = 16;                     // steps between two moves into registers
+constexpr int kGPlane = kGM * kGRows * 2, kGCodes = kGN * kGRows * 2;
+constexpr int kGStageBytes = 2 * kGPlane + kGCodes;
 
-struct CodeOperand {  // B(k, r) = zp_r + sc_r code[r, k]
-    const uint8_t *codes;
+struct GradCall {
+    CUtensorMap g, codes;
+    const void *g_ptr;
+    int64_t ldg;
+    const uint8_t *code_ptr;
     int64_t ldc;
     const float2 *params;
-    int F;
-    __device__ float operator()(int64_t k, int64_t r) const
-    {
-        return k < F ? __fmaf_rn((float)codes[r * ldc + k], params[r].y, params[r].x) : 0.f;
-    }
-};
-
-struct PartialStore {
-    float *out;
+    int64_t n;
     int M, F;
-    __device__ void operator()(int64_t m, int64_t n, const float (&acc)[4][4], int split) const
-    {
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j)
-                if (m + i < M && n + j < F) out[((int64_t)split * M + m + i) * F + n + j] = acc[i][j];
-    }
+    int tiles_m, tiles_n, steps, per_split;  // steps of kGRows rows, of all and of a split
+    float *partials;                         // [splits, M, ld]
+    int64_t ld;
+    int *failed;
 };
 
-__global__ void weight_grad_join_kernel(const float *__restrict__ partials, int splits, int M, int F, float beta,
-                                        float *__restrict__ out, int64_t ldo)
-{
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (int64_t)M * F) return;
-    float acc = 0.f;
-    for (int s = 0; s < splits; ++s) acc += partials[(int64_t)s * M * F + i];
-    float *o = out + (i / F) * ldo + i % F;
-    *o = beta == 0.f ? acc : acc + beta * *o;
-}
+template <class T>
+constexpr int grad_raw_bytes() { return kGRows * (kGM * (int)sizeof(T) + kGN); }
+template <class T, bool TMA>
+constexpr int grad_shared_bytes() { return kGStages * kGStageBytes + (TMA ? kGRaw * grad_raw_bytes<T>() : 16 * kGM * 4) + 256; }
 
-static int weight_grad_splits(int64_t n, int64_t M, int64_t F)
+// Eight codes -> eight bf16 values, exact.  A code c in the low byte below 0x43 reads as 128 + c for c < 128 and as 2 c from
+// there on; c is the smaller of that minus 128 and half of it.
+__device__ __forceinline__ uint4 code_values(uint2 c)
 {
-    const int64_t tiles = ceil_div(M, kTile) * ceil_div(F, kTile), most = ceil_div(n, 256);
-    int64_t s = ceil_div(4 * sm_count(), tiles);
-    s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s);
+    uint4 out;
+    __nv_bfloat162 *o = reinterpret_cast<__nv_bfloat162 *>(&out);
+    const uint32_t w[4] = {__byte_perm(c.x, 0x43434343u, 0x4140), __byte_perm(c.x, 0x43434343u, 0x4342),
+                           __byte_perm(c.y, 0x43434343u, 0x4140), __byte_perm(c.y, 0x43434343u, 0x4342)};
+    const __nv_bfloat162 less = __floats2bfloat162_rn(-128.0f, -128.0f), half = __floats2bfloat162_rn(0.5f, 0.5f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(w + i);
+        o[i] = __hmin2(__hadd2(v, less), __hmul2(v, half));
+    }
+    return out;
 }
 
 template <class T>
-static int weight_grad_run(const void *g, int64_t ldg, const uint8_t *codes, int64_t ldc, const float2 *params, int64_t n,
-                           int M, int F, float beta, float *out, int64_t ldo, float *partials, cudaStream_t s)
+__device__ __forceinline__ void unpack8(const uint4 *p, float (&v)[8])
 {
-    const int splits = weight_grad_splits(n, M, F);
-    const dim3 grid((unsigned)ceil_div(F, kTile), (unsigned)ceil_div(M, kTile), (unsigned)splits);
-    tile_product_kernel<<<grid, kTileThreads, 0, s>>>(GradOperand<T>{static_cast<const T *>(g), ldg, M},
-                                                      CodeOperand{codes, ldc, params, F}, PartialStore{partials, M, F}, n,
-                                                      ceil_div(n, splits));
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 a = *p;
+        const T *e = reinterpret_cast<const T *>(&a);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+    }
+}
+
+template <class T, bool TMA>
+__global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_constant__ GradCall c)
+{
+    extern __shared__ __align__(1024) uint8_t base[];
+    uint8_t *raw = base + kGStages * kGStageBytes;
+    constexpr int kRawBytes = grad_raw_bytes<T>(), kRawArea = TMA ? kGRaw * kRawBytes : 16 * kGM * 4;
+    uint64_t *raw_full = reinterpret_cast<uint64_t *>(raw + kRawArea), *raw_empty = raw_full + kGRaw;
+    uint64_t *full = raw_empty + kGRaw, *empty = full + kGStages, *acc_full = empty + kGStages, *acc_empty = acc_full + 2;
+    uint64_t *drained = acc_empty + 2;
+    uint32_t *slot = reinterpret_cast<uint32_t *>(drained + 1);
+    volatile int *gone = reinterpret_cast<volatile int *>(slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if ((smem_addr(base) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
+        if (threadIdx.x == 0) atomicExch(c.failed, 1);
+        return;
+    }
+    const int tile = blockIdx.x % (c.tiles_m * c.tiles_n), split = blockIdx.x / (c.tiles_m * c.tiles_n);
+    const int m0 = tile % c.tiles_m * kGM, n0 = tile / c.tiles_m * kGN;
+    const int first = split * c.per_split;
+    const int count = (first + c.per_split < c.steps ? c.per_split : c.steps - first);  // at least one: see weight_grad_plan
+    const int rounds = (count + kGPromote - 1) / kGPromote;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kGRaw; ++s) bar_init(raw_full + s, 1), bar_init(raw_empty + s, kGWorkers);
+        for (int s = 0; s < kGStages; ++s) bar_init(full + s, kGWorkers), bar_init(empty + s, 1);
+        for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, kGWorkers);
+        bar_init(drained, 1);
+        *gone = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kGWorkers + 1) tmem_alloc(slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+
+    if (warp == kGWorkers) {
+        // ---- loads ----
+        if (TMA && lane == 0) {
+            tma_prefetch(&c.g);
+            tma_prefetch(&c.codes);
+            int s = 0, done = 0;
+            unsigned phase = 0;
+            for (; done < count; ++done) {
+                if (!bar_wait(raw_empty + s, phase ^ 1, gone)) break;
+                uint8_t *at = raw + s * kRawBytes;
+                const int r0 = (first + done) * kGRows;
+                bar_expect(raw_full + s, kRawBytes);
+                tma_load(at, &c.g, m0, r0, 0, raw_full + s);
+                tma_load(at + kGRows * kGM * sizeof(T), &c.codes, n0, r0, 0, raw_full + s);
+                if (++s == kGRaw) s = 0, phase ^= 1;
+            }
+            if (done < count) {
+                for (int b = 0; b < kGRaw && b < done; ++b) bar_drain(raw_full + b, ((done - 1 - b) / kGRaw) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == kGWorkers + 1) {
+        // ---- products ----
+        if (lane == 0) {
+            const int left = c.F - n0, n = left < kGN ? (left + 15) / 16 * 16 : kGN;
+            const uint32_t idesc = umma_idesc(true, true, true, n);
+            int s = 0;
+            unsigned phase = 0;
+            bool ok = true;
+            for (int k = 0; k < count; ++k) {
+                const int round = k / kGPromote, acc = round & 1;
+                if (k % kGPromote == 0) {
+                    ok = bar_wait(acc_empty + acc, ((round >> 1) & 1) ^ 1, gone);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                ok = bar_wait(full + s, phase, gone);
+                if (!ok) break;
+                tc_fence_after();
+                const uint8_t *at = base + s * kGStageBytes;
+                const uint64_t a0 = umma_desc(at, kGRows * 128, 1024), a1 = umma_desc(at + kGPlane, kGRows * 128, 1024);
+                const uint64_t b = umma_desc(at + 2 * kGPlane, kGRows * 128, 1024);
+                const uint32_t d = tmem + acc * kGN;
+#pragma unroll
+                for (int j = 0; j < kGRows / 16; ++j) {  // sixteen rows: two groups of eight
+                    const uint64_t step = 2048u * j >> 4;
+                    umma(d, a0 + step, b + step, idesc, k % kGPromote > 0 || j > 0);
+                    umma(d, a1 + step, b + step, idesc, true);
+                }
+                tc_commit(empty + s);
+                if (k % kGPromote == kGPromote - 1 || k == count - 1) tc_commit(acc_full + acc);
+                if (++s == kGStages) s = 0, phase ^= 1;
+            }
+            if (!ok) {
+                tc_commit(drained);
+                bar_drain(drained, 0);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- conversion, and the sums ----
+        const int tid = threadIdx.x;
+        const int q = tid & 15, ra = tid >> 4;   // of g: eight columns, rows ra and ra + 16
+        const int mq = m0 + q * 8, nq = n0 + lane * 8;  // of the codes: eight columns, rows warp, warp + 8, ...
+        const int quarter = warp & 3, half = warp >> 2;
+        float sum[128];
+#pragma unroll
+        for (int e = 0; e < 128; ++e) sum[e] = 0.f;
+        float zero[8] = {};  // sum of g zp over this thread's rows
+        int s = 0, t = 0, taken = 0;
+        unsigned phase = 0, raw_phase = 0;
+        bool ok = true;
+        // operands of a step that come without TMA, one step ahead
+        float gv[2][8];
+        uint2 cv[4];
+        float2 pv[2];
+        const auto fetch = [&](int k) {
+            const int64_t r0 = (int64_t)(first + k) * kGRows;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t r = r0 + ra + 16 * i;
+                pv[i] = r < c.n ? __ldg(c.params + r) : make_float2(0.f, 0.f);
+                if constexpr (!TMA) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        gv[i][e] = r < c.n && mq + e < c.M ? to_f32<T>(static_cast<const T *>(c.g_ptr)[r * c.ldg + mq + e]) : 0.f;
+                }
+            }
+            if constexpr (!TMA) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = r0 + warp + 8 * i;
+                    uint8_t b[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) b[e] = r < c.n && nq + e < c.F ? c.code_ptr[r * c.ldc + nq + e] : (uint8_t)0;
+                    cv[i].x = b[0] | b[1] << 8 | b[2] << 16 | (uint32_t)b[3] << 24;
+                    cv[i].y = b[4] | b[5] << 8 | b[6] << 16 | (uint32_t)b[7] << 24;
+                }
+            }
+        };
+        // moves the sums of a round into registers
+        const auto promote = [&](int round) {
+            const int acc = round & 1;
+            if (!bar_wait(acc_full + acc, (round >> 1) & 1, gone)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v[32];
+                tmem_load32(tmem + acc * kGN + half * 128 + 32 * j + ((uint32_t)quarter << 21), v);
+                tmem_load_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sum[32 * j + e] += v[e];
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(acc_empty + acc);
+            return true;
+        };
+        fetch(0);
+        for (int k = 0; k < count && ok; ++k) {
+            const uint8_t *in = raw + s * kRawBytes;
+            if (TMA) {
+                ok = bar_wait(raw_full + s, raw_phase, gone);
+                if (!ok) break;
+            }
+            ok = bar_wait(empty + t, phase ^ 1, gone);
+            if (!ok) break;
+            uint8_t *at = base + t * kGStageBytes;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = ra + 16 * i;
+                float v[8];
+                if constexpr (TMA) {
+                    unpack8<T>(reinterpret_cast<const uint4 *>(in + (r * kGM + q * 8) * sizeof(T)), v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = gv[i][e];
+                }
+                const float sc = pv[i].y, zp = pv[i].x;
+                uint4 hi, lo;
+                uint32_t *ph = reinterpret_cast<uint32_t *>(&hi), *pl = reinterpret_cast<uint32_t *>(&lo);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    zero[2 * e] = __fmaf_rn(v[2 * e], zp, zero[2 * e]);
+                    zero[2 * e + 1] = __fmaf_rn(v[2 * e + 1], zp, zero[2 * e + 1]);
+                    const float x = v[2 * e] * sc, y = v[2 * e + 1] * sc;
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                    const float2 hf = __bfloat1622float2(h);
+                    const __nv_bfloat162 l = __floats2bfloat162_rn(x - hf.x, y - hf.y);
+                    ph[e] = *reinterpret_cast<const uint32_t *>(&h);
+                    pl[e] = *reinterpret_cast<const uint32_t *>(&l);
+                }
+                uint8_t *o = at + (q >> 3) * (kGRows * 128) + r * 128 + ((q & 7) ^ (r & 7)) * 16;
+                *reinterpret_cast<uint4 *>(o) = hi;
+                *reinterpret_cast<uint4 *>(o + kGPlane) = lo;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = warp + 8 * i;
+                const uint2 code = TMA ? *reinterpret_cast<const uint2 *>(in + kGRows * kGM * sizeof(T) + r * kGN + lane * 8) : cv[i];
+                *reinterpret_cast<uint4 *>(at + 2 * kGPlane + (lane >> 3) * (kGRows * 128) + r * 128 + ((lane & 7) ^ (r & 7)) * 16) = code_values(code);
+            }
+            if (k + 1 < count) fetch(k + 1);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) {
+                bar_arrive(full + t);
+                if (TMA) bar_arrive(raw_empty + s);
+            }
+            if (++t == kGStages) t = 0, phase ^= 1;
+            if (++s == kGRaw) s = 0, raw_phase ^= 1;
+            // half a round later its products are done, and the next round's still have work in front of them
+            if (k % kGPromote == kGPromote / 2 && k > kGPromote) ok = promote(taken++);
+        }
+        while (ok && taken < rounds) ok = promote(taken++);
+        // the zero points' share of every column, over the sixteen row groups
+        float *share = reinterpret_cast<float *>(raw);  // [16][128]: every buffer of operands has been read
+        asm volatile("bar.sync 1, %0;" ::"n"(kGWorkers * 32) : "memory");
+#pragma unroll
+        for (int e = 0; e < 8; ++e) share[ra * kGM + q * 8 + e] = zero[e];
+        asm volatile("bar.sync 1, %0;" ::"n"(kGWorkers * 32) : "memory");
+        const int m = quarter * 32 + lane;
+        float own = 0.f;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) own += share[g * kGM + m];
+        if (m0 + m < c.M) {
+            float *o = c.partials + ((int64_t)split * c.M + m0 + m) * c.ld + n0 + half * 128;
+#pragma unroll
+            for (int e = 0; e < 128; e += 4) {  // ld is F rounded up to 4
+                if (n0 + half * 128 + e < c.F)
+                    *reinterpret_cast<float4 *>(o + e) = make_float4(sum[e] + own, sum[e + 1] + own, sum[e + 2] + own, sum[e + 3] + own);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (threadIdx.x == 0 && *gone) atomicExch(c.failed, 1);
+    if (warp == kGWorkers + 1) tmem_free(tmem, 512);
+}
+
+// out = sum of the partial results, in their order, + beta out: 32 columns a block row, the splits dealt over eight warps
+__global__ void __launch_bounds__(256)
+weight_grad_join_kernel(const float *__restrict__ partials, int splits, int M, int F, int64_t ld, float beta,
+                        const int *__restrict__ failed, float *__restrict__ out, int64_t ldo)
+{
+    __shared__ float red[8][33];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int64_t f = (int64_t)blockIdx.x * 32 + lane;
+    const bool bad = splits > 0 && *failed != 0;
+    for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+        float acc = 0.f;
+        if (f < F) {
+#pragma unroll 4
+            for (int s = g; s < splits; s += 8) acc += partials[((int64_t)s * M + m) * ld + f];
+        }
+        __syncthreads();
+        red[g][lane] = acc;
+        __syncthreads();
+        if (g == 0 && f < F) {
+            for (int w = 1; w < 8; ++w) acc += red[w][lane];
+            float *o = out + m * ldo + f;
+            if (bad) acc = __int_as_float(0x7fffffff);
+            *o = beta == 0.f ? acc : acc + beta * *o;
+        }
+    }
+}
+
+struct GradPlan {
+    int tiles_m, tiles_n, steps, per_split, splits;
+    int64_t ld;
+    size_t bytes;
+};
+
+// As many row ranges as fill the SMs once, each with at least one move into registers' worth of rows where there are that
+// many; every range has rows.
+static GradPlan weight_grad_plan(int64_t n, int64_t M, int64_t F)
+{
+    GradPlan p{};
+    p.tiles_m = (int)ceil_div(M, kGM), p.tiles_n = (int)ceil_div(F, kGN);
+    p.steps = (int)ceil_div(n, kGRows);
+    int64_t s = sm_count() / ((int64_t)p.tiles_m * p.tiles_n);
+    const int64_t most = ceil_div(p.steps, kGPromote);
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    p.per_split = (int)ceil_div(p.steps, s);
+    p.splits = (int)ceil_div(p.steps, p.per_split);
+    p.ld = ceil_div(F, 4) * 4;
+    p.bytes = 256 + (size_t)p.splits * M * p.ld * sizeof(float);
+    return p;
+}
+
+template <class T, bool TMA>
+static int weight_grad_launch(const GradCall &c, const GradPlan &p, cudaStream_t s)
+{
+    constexpr int smem = grad_shared_bytes<T, TMA>();
+    SGNN_CUDA_OK(cudaFuncSetAttribute(weight_grad_kernel<T, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    weight_grad_kernel<T, TMA><<<(unsigned)(p.tiles_m * p.tiles_n * p.splits), kGThreads, smem, s>>>(c);
     SGNN_LAUNCH_OK("checkpoint_weight_grad");
-    weight_grad_join_kernel<<<(unsigned)ceil_div((int64_t)M * F, 256), 256, 0, s>>>(partials, splits, M, F, beta, out, ldo);
+    return SGNN_OK;
+}
+
+template <class T>
+static int weight_grad_run(const void *g, int64_t ldg, const uint8_t *codes, int64_t ldc, const float2 *params, int64_t n, int M,
+                           int F, float beta, float *out, int64_t ldo, void *ws, const GradPlan &p, cudaStream_t s)
+{
+    GradCall c{};
+    c.g_ptr = g, c.ldg = ldg, c.code_ptr = codes, c.ldc = ldc, c.params = params, c.n = n, c.M = M, c.F = F;
+    c.tiles_m = p.tiles_m, c.tiles_n = p.tiles_n, c.steps = p.steps, c.per_split = p.per_split, c.ld = p.ld;
+    c.failed = static_cast<int *>(ws), c.partials = reinterpret_cast<float *>(static_cast<char *>(ws) + 256);
+    SGNN_CUDA_OK(cudaMemsetAsync(c.failed, 0, 4, s));
+    int rc;
+    if (n > 1 && aligned16(g) && ldg * sizeof(T) % 16 == 0 && aligned16(codes) && ldc % 16 == 0) {
+        if ((rc = raw_tensor_map(&c.g, g, sizeof(T), M, n, ldg, kGM, kGRows))) return rc;
+        if ((rc = raw_tensor_map(&c.codes, codes, 1, F, n, ldc, kGN, kGRows))) return rc;
+        rc = weight_grad_launch<T, true>(c, p, s);
+    } else {
+        rc = weight_grad_launch<T, false>(c, p, s);
+    }
+    if (rc) return rc;
+    const dim3 grid((unsigned)ceil_div(F, 32), (unsigned)(M < 65535 ? M : 65535));
+    weight_grad_join_kernel<<<grid, 256, 0, s>>>(c.partials, p.splits, M, F, p.ld, beta, c.failed, out, ldo);
     SGNN_LAUNCH_OK("checkpoint_weight_grad join");
     return SGNN_OK;
 }
@@ -90,7 +419,7 @@ extern "C" SGNN_API int sgnn_checkpoint_weight_grad_workspace_bytes(int dtype, i
     int rc = weight_grad_check(who, dtype, n, M, F);
     if (rc) return rc;
     SGNN_REQUIRE(bytes != nullptr, SGNN_ERR_INVALID_ARGUMENT, "%s: null result pointer", who);
-    *bytes = n == 0 ? 0 : (size_t)weight_grad_splits(n, M, F) * M * F * sizeof(float);
+    *bytes = n == 0 ? 0 : weight_grad_plan(n, M, F).bytes;
     return SGNN_OK;
 }
 
@@ -106,7 +435,8 @@ extern "C" SGNN_API int sgnn_checkpoint_weight_grad(int dtype, const void *d_g, 
     SGNN_REQUIRE(d_out != nullptr && ldo >= F, SGNN_ERR_INVALID_ARGUMENT, "%s: bad output", who);
     cudaStream_t s = (cudaStream_t)stream;
     if (n == 0) {
-        weight_grad_join_kernel<<<(unsigned)ceil_div(M * F, 256), 256, 0, s>>>(nullptr, 0, (int)M, (int)F, beta, d_out, ldo);
+        const dim3 grid((unsigned)ceil_div(F, 32), (unsigned)(M < 65535 ? M : 65535));
+        weight_grad_join_kernel<<<grid, 256, 0, s>>>(nullptr, 0, (int)M, (int)F, F, beta, nullptr, d_out, ldo);
         SGNN_LAUNCH_OK("checkpoint_weight_grad join");
         return SGNN_OK;
     }
@@ -114,16 +444,12 @@ extern "C" SGNN_API int sgnn_checkpoint_weight_grad(int dtype, const void *d_g, 
     SGNN_REQUIRE(n == 1 || (ldg >= M && ldc >= F), SGNN_ERR_INVALID_ARGUMENT, "%s: leading dimension shorter than a row", who);
     SGNN_REQUIRE(reinterpret_cast<uintptr_t>(d_g) % elem_bytes(dtype) == 0 && reinterpret_cast<uintptr_t>(d_params) % 8 == 0,
                  SGNN_ERR_INVALID_ARGUMENT, "%s: pointers must be aligned to their element (params: 8 bytes)", who);
-    size_t need = 0;
-    rc = sgnn_checkpoint_weight_grad_workspace_bytes(dtype, n, M, F, &need);
-    if (rc) return rc;
-    SGNN_REQUIRE(d_workspace != nullptr && workspace_bytes >= need, SGNN_ERR_WORKSPACE,
-                 "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+    const GradPlan p = weight_grad_plan(n, M, F);
+    SGNN_REQUIRE(d_workspace != nullptr && workspace_bytes >= p.bytes && reinterpret_cast<uintptr_t>(d_workspace) % 256 == 0,
+                 SGNN_ERR_WORKSPACE, "%s: 256-byte aligned workspace of %zu bytes needed, %zu given", who, p.bytes, workspace_bytes);
     const float2 *params = reinterpret_cast<const float2 *>(d_params);
-    float *partials = static_cast<float *>(d_workspace);
-    if (dtype == SGNN_F32)
-        return weight_grad_run<float>(d_g, ldg, d_codes, ldc, params, n, (int)M, (int)F, beta, d_out, ldo, partials, s);
-    if (dtype == SGNN_BF16)
-        return weight_grad_run<__nv_bfloat16>(d_g, ldg, d_codes, ldc, params, n, (int)M, (int)F, beta, d_out, ldo, partials, s);
-    return weight_grad_run<__half>(d_g, ldg, d_codes, ldc, params, n, (int)M, (int)F, beta, d_out, ldo, partials, s);
+    const int m = (int)M, f = (int)F;
+    if (dtype == SGNN_F32) return weight_grad_run<float>(d_g, ldg, d_codes, ldc, params, n, m, f, beta, d_out, ldo, d_workspace, p, s);
+    if (dtype == SGNN_BF16) return weight_grad_run<__nv_bfloat16>(d_g, ldg, d_codes, ldc, params, n, m, f, beta, d_out, ldo, d_workspace, p, s);
+    return weight_grad_run<__half>(d_g, ldg, d_codes, ldc, params, n, m, f, beta, d_out, ldo, d_workspace, p, s);
 }

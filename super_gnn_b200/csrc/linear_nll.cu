@@ -8,9 +8,8 @@
 //
 // The rows in the loss are listed first (in order) and copied together, so that a row outside the mask costs nothing and
 // whatever it holds is not read.  The products run on the tensor cores (nll_product.cuh): 8 m C K operations for m rows,
-// of which 2 m C K compute the logits again, the price of not keeping them.  Rows go in chunks of up to 32768, classes in
-// pieces, so that G (16 bits an element, rows of the chunk x classes of the piece) stays in the L2 cache between the
-// kernel that writes it and the two products that read it.
+// of which 2 m C K compute the logits again, the price of not keeping them.  Rows go in chunks and classes in pieces,
+// and only G of one chunk and one piece exists at a time, 16 bits an element.
 //
 // bf16 operands enter the products as they are; G is rounded to bf16, as it is between two bf16 layers.  fp32 operands are
 // split into two fp16 planes, v 2^e = v0 + v1 with 2^e bringing the largest value of the row below 2^15: 22 bits of every
@@ -42,38 +41,6 @@ nll_count_kernel(const int64_t *__restrict__ labels, const uint8_t *__restrict__
     if (threadIdx.x == 0) counts[blockIdx.x] = c;
 }
 
-// rows[0 .. m) = the rows in the loss, ascending; *total = m
-__global__ void __launch_bounds__(kListThreads)
-nll_list_kernel(const int64_t *__restrict__ labels, const uint8_t *__restrict__ mask, int64_t n, int64_t C,
-                const int *__restrict__ counts, int *__restrict__ rows, int *__restrict__ total)
-{
-    __shared__ int part[kListThreads / 32], before[kListThreads / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = 0;
-    for (int b = threadIdx.x; b < blockIdx.x; b += kListThreads) s += counts[b];
-    s = __reduce_add_sync(FULL, s);
-    if (lane == 0) part[warp] = s;
-    __syncthreads();
-    int at = 0;
-    for (int w = 0; w < kListThreads / 32; ++w) at += part[w];
-    for (int i = 0; i < kListRows / kListThreads; ++i) {
-        const int64_t r = (int64_t)blockIdx.x * kListRows + i * kListThreads + threadIdx.x;
-        const bool on = in_loss(labels, mask, r, n, C);
-        const unsigned vote = __ballot_sync(FULL, on);
-        __syncthreads();
-        if (lane == 0) before[warp] = __popc(vote);
-        __syncthreads();
-        int pos = at + __popc(vote & ((1u << lane) - 1u));
-        for (int w = 0; w < kListThreads / 32; ++w) {
-            if (w < warp) pos += before[w];
-            at += before[w];
-        }
-        if (on) rows[pos] = (int)r;
-    }
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *total = at;
-}
-
-
 struct NllBias {
     const void *b;
     bool f32;
@@ -86,27 +53,61 @@ __device__ __forceinline__ float bias_at(NllBias b, int64_t c)
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// bias log2(e) of the classes, -inf up to the end of the last tile: classes that are not there have probability 0 (their
-// rows of W read as zeros, scaled by 1)
-template <class T>
-__global__ void nll_bias_kernel(NllBias bias, int64_t C, int64_t padded, float *__restrict__ bias2, float *__restrict__ w_down,
-                                int *__restrict__ failed)
-{
-    const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (c == 0) *failed = 0;
-    if (c < padded) bias2[c] = c < C ? bias_at<T>(bias, c) * kLog2e : -INFINITY;
-    if (c >= C && c < padded && w_down != nullptr) w_down[c] = 1.0f;
-}
+// The first `blocks` blocks list the rows in the loss: rows[0 .. m) ascending, *total = m (`counts`: rows in the loss of
+// every listing block before).  The others set what the later kernels start from: bias log2(e) of the classes, -inf up to
+// the end of the last tile (classes that are not there have probability 0; their rows of W read as zeros, scaled by 1),
+// lse = 0 of all rows, and the counters.
+struct NllStart {
+    const int64_t *labels;
+    const uint8_t *mask;
+    int64_t n, C, padded;  // padded: classes of whole tiles
+    const int *counts;
+    int *rows, *total;
+    int blocks;
+    NllBias bias;
+    float *bias2, *w_down, *lse;
+    int *failed, *joined;
+};
 
-// 2^e that brings `largest` into [2^14, 2^15), and 2^-e; 1 for nothing but zeros and for what is not finite
-__device__ __forceinline__ void plane_scale(float largest, float &up, float &down)
+template <class T>
+__global__ void __launch_bounds__(kListThreads) nll_start_kernel(const NllStart a)
 {
-    up = down = 1.0f;
-    if (!(largest > 0.f) || !(largest <= FLT_MAX)) return;
-    int e = 14 - ((int)(__float_as_uint(largest) >> 23) - 127);
-    e = e < -126 ? -126 : e > 126 ? 126 : e;
-    up = __uint_as_float((unsigned)(e + 127) << 23);
-    down = __uint_as_float((unsigned)(127 - e) << 23);
+    if ((int)blockIdx.x >= a.blocks) {
+        const int64_t first = (int64_t)(blockIdx.x - a.blocks) * kListThreads + threadIdx.x;
+        const int64_t step = (int64_t)(gridDim.x - a.blocks) * kListThreads;
+        if (first == 0) *a.failed = 0, *a.joined = 0;
+        for (int64_t c = first; c < a.padded; c += step) {
+            a.bias2[c] = c < a.C ? bias_at<T>(a.bias, c) * kLog2e : -INFINITY;
+            if (c >= a.C && a.w_down != nullptr) a.w_down[c] = 1.0f;
+        }
+        if (a.lse != nullptr)
+            for (int64_t i = first; i < a.n; i += step) a.lse[i] = 0.f;
+        return;
+    }
+    __shared__ int part[kListThreads / 32], before[kListThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int s = 0;
+    for (int b = threadIdx.x; b < (int)blockIdx.x; b += kListThreads) s += a.counts[b];
+    s = __reduce_add_sync(FULL, s);
+    if (lane == 0) part[warp] = s;
+    __syncthreads();
+    int at = 0;
+    for (int w = 0; w < kListThreads / 32; ++w) at += part[w];
+    for (int i = 0; i < kListRows / kListThreads; ++i) {
+        const int64_t r = (int64_t)blockIdx.x * kListRows + i * kListThreads + threadIdx.x;
+        const bool on = in_loss(a.labels, a.mask, r, a.n, a.C);
+        const unsigned vote = __ballot_sync(FULL, on);
+        __syncthreads();
+        if (lane == 0) before[warp] = __popc(vote);
+        __syncthreads();
+        int pos = at + __popc(vote & ((1u << lane) - 1u));
+        for (int w = 0; w < kListThreads / 32; ++w) {
+            if (w < warp) pos += before[w];
+            at += before[w];
+        }
+        if (on) a.rows[pos] = (int)r;
+    }
+    if ((int)blockIdx.x == a.blocks - 1 && threadIdx.x == 0) *a.total = at;
 }
 
 // Where the rows of a matrix come from: row i is src[rows[i]] for i < *total, or src[i] for i < count
@@ -144,15 +145,17 @@ __device__ __forceinline__ void store_split(const Planes &pl, int64_t at, float 
     reinterpret_cast<__half *>(pl.p)[at + pl.stride] = __float2half_rn(s - __half2float(h));
 }
 
-// largest |value| of every column, as bits (a NaN or an infinity stays above every number)
-__global__ void __launch_bounds__(256) nll_column_max_kernel(RowSource s, unsigned *__restrict__ largest)
+// largest |value| of every column of x (z = 0) and W (z = 1), as bits: a NaN or an infinity stays above every number
+__global__ void __launch_bounds__(256) nll_column_max_kernel(RowSource x, RowSource w, unsigned *__restrict__ largest)
 {
     __shared__ unsigned part[8][32];
+    const RowSource s = blockIdx.z == 0 ? x : w;
     const int k = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
-    const int64_t n = source_rows(s);
+    const int64_t n = source_rows(s), step = (int64_t)gridDim.y * 8;
     unsigned m = 0;
     if (k < s.K) {
-        for (int64_t i = (int64_t)blockIdx.y * 8 + g; i < n; i += (int64_t)gridDim.y * 8) {
+#pragma unroll 4
+        for (int64_t i = (int64_t)blockIdx.y * 8 + g; i < n; i += step) {
             const unsigned b = __float_as_uint(static_cast<const float *>(s.src)[source_row(s, i) * s.ld + k]) & 0x7fffffffu;
             m = b > m ? b : m;
         }
@@ -160,30 +163,34 @@ __global__ void __launch_bounds__(256) nll_column_max_kernel(RowSource s, unsign
     part[g][threadIdx.x & 31] = m;
     __syncthreads();
     if (g == 0 && k < s.K) {
-        for (int w = 1; w < 8; ++w) m = part[w][threadIdx.x] > m ? part[w][threadIdx.x] : m;
-        atomicMax(largest + k, m);
+        for (int w8 = 1; w8 < 8; ++w8) m = part[w8][threadIdx.x] > m ? part[w8][threadIdx.x] : m;
+        atomicMax(largest + (blockIdx.z == 0 ? 0 : s.K) + k, m);
     }
 }
 
-__global__ void nll_column_scale_kernel(const unsigned *__restrict__ largest, int K, float *__restrict__ up, float *__restrict__ down)
-{
-    const int k = blockIdx.x * blockDim.x + threadIdx.x;
-    if (k < K) plane_scale(__uint_as_float(largest[k]), up[k], down[k]);
-}
+// One side of the operands: where it comes from, its planes scaled by row and (fp32 with gradients) by column
+struct TakeSide {
+    RowSource src;
+    Planes row, col;
+    const unsigned *largest;  // of the columns
+    float *row_down;
+    int blocks;
+};
 
-// Rows together, one warp a row, and zero rows up to a whole tile behind the listed ones.  fp32 (SPLIT): planes scaled by
-// row and, where col.p is given, planes scaled by column.
+// Rows together, one warp a row, zero rows up to a whole tile behind the listed ones; the first blocks take x, the rest W.
 template <class T, bool SPLIT>
-__global__ void __launch_bounds__(256)
-nll_take_kernel(RowSource s, Planes row, Planes col, const float *__restrict__ col_up, float *__restrict__ row_down, Picked pick)
+__global__ void __launch_bounds__(256) nll_take_kernel(const TakeSide xs, const TakeSide ws, const Picked pick)
 {
-    const int lane = threadIdx.x & 31;
+    const bool is_x = (int)blockIdx.x < xs.blocks;
+    const TakeSide &t = is_x ? xs : ws;
+    const RowSource &s = t.src;
+    const int lane = threadIdx.x & 31, block = is_x ? blockIdx.x : blockIdx.x - xs.blocks;
     const int64_t n = source_rows(s), end = s.total ? (n + kPM - 1) / kPM * kPM : n;
-    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += (int64_t)gridDim.x * 8) {
+    for (int64_t i = (int64_t)block * 8 + (threadIdx.x >> 5); i < end; i += (int64_t)t.blocks * 8) {
         const bool there = i < n;
         const int64_t r = there ? source_row(s, i) : 0;
         const T *x = static_cast<const T *>(s.src) + r * s.ld;
-        if (pick.label != nullptr && there) {
+        if (is_x && there) {
             const int64_t label = pick.labels[r];
             const T *w = static_cast<const T *>(pick.w) + label * pick.ldw;
             float z = 0.f;
@@ -204,94 +211,135 @@ nll_take_kernel(RowSource s, Planes row, Planes col, const float *__restrict__ c
             }
             largest = warp_max(largest);
             if (all_sum(poison) == 0.f) plane_scale(largest, up, down);
-            if (lane == 0) row_down[i] = down;
+            if (lane == 0) t.row_down[i] = down;
         }
-        for (int k = lane; k < row.ld; k += 32) {
+        for (int k = lane; k < t.row.ld; k += 32) {
             const bool in = there && k < s.K;
-            const int64_t at = i * row.ld + k;
+            const int64_t at = i * t.row.ld + k;
             if (SPLIT) {
                 const float v = in ? to_f32<T>(x[k]) : 0.f;
-                store_split(row, at, v, up);
-                if (col.p) store_split(col, at, v, k < s.K ? __ldg(col_up + k) : 1.f);
+                store_split(t.row, at, v, up);
+                if (t.col.p) {
+                    float cup = 1.f, cdown;
+                    if (k < s.K) plane_scale(__uint_as_float(__ldg(t.largest + k)), cup, cdown);
+                    store_split(t.col, at, v, cup);
+                }
             } else {
-                row.p[at] = in ? reinterpret_cast<const uint16_t *>(x)[k] : (uint16_t)0;
+                t.row.p[at] = in ? reinterpret_cast<const uint16_t *>(x)[k] : (uint16_t)0;
             }
         }
     }
 }
 
-// lse of the rows of a chunk from the parts of their tiles, and the sum of their losses a block
-__global__ void __launch_bounds__(256)
-nll_join_kernel(const float2 *__restrict__ stats, int parts, int row0, int row_cap, const int *__restrict__ rows,
-                const int *__restrict__ total, const float *__restrict__ picked2, float *__restrict__ lse2,
-                float *__restrict__ lse_out, float *__restrict__ loss_part)
+__device__ __forceinline__ void join_stats(float &mx, float &sum, float2 v)
 {
-    __shared__ float2 red[8][32];
+    const float top = fmaxf(mx, v.x), ref = top == -INFINITY ? 0.f : top;
+    sum = sum * exp2_fast(mx - ref) + v.y * exp2_fast(v.x - ref);
+    mx = top;
+}
+
+// lse of the rows of a chunk from the parts of their tiles: 32 rows a block, the parts dealt over its 32 warps.  The sum of
+// their losses goes to loss_part; the block that comes last of all chunks adds those up, in their order.
+struct NllJoin {
+    const float2 *stats;
+    int parts, row0, row_cap;
+    const int *rows, *total;
+    const float *picked2;
+    float *lse2, *lse_out, *loss_part;  // loss_part: of this chunk
+    const float *all_parts;
+    int all_count;
+    float inv_count;
+    int *joined;
+    const int *failed;
+    float *loss;
+};
+
+__global__ void __launch_bounds__(1024) nll_join_kernel(const NllJoin a)
+{
+    __shared__ float2 red[32][33];
+    __shared__ bool last;
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
     const int i = blockIdx.x * 32 + lane;  // of the chunk
-    const bool on = i < row_cap && row0 + i < *total;
+    const bool on = i < a.row_cap && a.row0 + i < *a.total;
     float mx = -INFINITY, sum = 0.f;
     if (on) {
-        for (int p = g; p < parts; p += 8) {
-            const float2 v = stats[(int64_t)p * row_cap + i];
-            const float top = fmaxf(mx, v.x), ref = top == -INFINITY ? 0.f : top;
-            sum = sum * exp2f(mx - ref) + v.y * exp2f(v.x - ref);
-            mx = top;
-        }
+#pragma unroll 4
+        for (int p = g; p < a.parts; p += 32) join_stats(mx, sum, a.stats[(int64_t)p * a.row_cap + i]);
     }
     red[g][lane] = make_float2(mx, sum);
     __syncthreads();
-    if (g != 0) return;
-    for (int w = 1; w < 8; ++w) {
-        const float2 v = red[w][lane];
-        const float top = fmaxf(mx, v.x), ref = top == -INFINITY ? 0.f : top;
-        sum = sum * exp2f(mx - ref) + v.y * exp2f(v.x - ref);
-        mx = top;
+    // warp g joins row g: in a tree, the same for every number of parts
+    const float2 mine = red[lane][g];
+    mx = mine.x, sum = mine.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float2 other = make_float2(__shfl_xor_sync(FULL, mx, o), __shfl_xor_sync(FULL, sum, o));
+        join_stats(mx, sum, other);
     }
-    float loss = 0.f;
-    if (on) {
-        const float l = mx + log2f(sum);
-        lse2[i] = l;
-        if (lse_out) lse_out[rows[row0 + i]] = l * kLn2;
-        loss = (l - picked2[i]) * kLn2;
-    }
-    loss = all_sum(loss);
-    if (lane == 0) loss_part[blockIdx.x] = loss;
-}
-
-__global__ void __launch_bounds__(1024)
-nll_loss_kernel(const float *__restrict__ parts, int count, float inv_count, const int *__restrict__ failed, float *__restrict__ loss)
-{
-    __shared__ float red[32];
-    float s = 0.f;
-    for (int i = threadIdx.x; i < count; i += 1024) s += parts[i];
-    s = all_sum(s);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        s = all_sum(red[threadIdx.x]);
-        if (threadIdx.x == 0) *loss = *failed ? __int_as_float(0x7fffffff) : s * inv_count;
+    if (lane == 0) red[0][g] = make_float2(mx, sum);
+    __syncthreads();
+    if (g == 0) {
+        const float2 v = red[0][lane];
+        float loss = 0.f;
+        if (on) {
+            const float l = v.x + log2f(v.y);
+            a.lse2[i] = l;
+            if (a.lse_out) a.lse_out[a.rows[a.row0 + i]] = l * kLn2;
+            loss = (l - a.picked2[i]) * kLn2;
+        }
+        loss = all_sum(loss);
+        if (lane == 0) {
+            a.loss_part[blockIdx.x] = loss;
+            __threadfence();
+            last = atomicAdd(a.joined, 1) == a.all_count - 1;
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    float s = 0.f;
+    for (int p = threadIdx.x; p < a.all_count; p += 1024) s += __ldcg(a.all_parts + p);
+    s = all_sum(s);
+    if (lane == 0) red[1][g].x = s;
+    __syncthreads();
+    if (g == 0) {
+        s = all_sum(red[1][lane].x);
+        if (lane == 0) *a.loss = *a.failed ? __int_as_float(0x7fffffff) : s * a.inv_count;
     }
 }
 
-// gx of the listed rows of a chunk: the partial sums of the splits, scaled back; NaN when a wait gave up before
+// gx of the listed rows of a chunk: the partial sums of the splits, scaled back; NaN when a wait gave up before.  One row
+// and 32 columns a block of 32 x 8 threads with many splits (dealt over the eight), a warp a row otherwise.
 template <class T>
 __global__ void __launch_bounds__(256)
 nll_rows_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_split, int splits, int row0, int row_cap,
-                    const int *__restrict__ rows, const int *__restrict__ total, float scale, const float *__restrict__ col_down,
-                    const int *__restrict__ failed, T *__restrict__ gx, int64_t ldgx, int K, float *__restrict__ loss)
+                    const int *__restrict__ rows, const int *__restrict__ total, float scale, const unsigned *__restrict__ largest,
+                    const int *__restrict__ failed, T *__restrict__ gx, int64_t ldgx, int K, float *__restrict__ loss, bool dealt)
 {
-    const int lane = threadIdx.x & 31;
+    __shared__ float red[8][33];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
     const bool bad = *failed != 0;
-    if (bad && blockIdx.x == 0 && threadIdx.x == 0) *loss = __int_as_float(0x7fffffff);
-    for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < row_cap && row0 + i < *total; i += gridDim.x * 8) {
+    if (bad && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *loss = __int_as_float(0x7fffffff);
+    const int left = *total - row0, count = left < row_cap ? left : row_cap;
+    for (int i = dealt ? blockIdx.x : blockIdx.x * 8 + g; i < count; i += dealt ? gridDim.x : gridDim.x * 8) {
         T *out = gx + (int64_t)rows[row0 + i] * ldgx;
-        for (int k = lane; k < K; k += 32) {
+        for (int k = (dealt ? blockIdx.y * 32 : 0) + lane; k < K || dealt; k += 32) {
             float v = 0.f;
-            for (int s = 0; s < splits; ++s) v += acc[s * acc_split + (int64_t)i * acc_ld + k];
-            v *= scale;
-            if (col_down) v *= col_down[k];
-            out[k] = from_f32<T>(bad ? __int_as_float(0x7fffffff) : v);
+            if (k < K) {
+#pragma unroll 4
+                for (int s = dealt ? g : 0; s < splits; s += dealt ? 8 : 1) v += acc[s * acc_split + (int64_t)i * acc_ld + k];
+            }
+            if (dealt) {
+                __syncthreads();
+                red[g][lane] = v;
+                __syncthreads();
+                for (int w = 1; w < 8; ++w) v = (w == 1 ? red[0][lane] : v) + red[w][lane];
+            }
+            float up, down = 1.f;
+            if (largest != nullptr && k < K) plane_scale(__uint_as_float(largest[k]), up, down);
+            if (k < K && (!dealt || g == 0)) out[k] = from_f32<T>(bad ? __int_as_float(0x7fffffff) : v * scale * down);
+            if (dealt) break;
         }
     }
 }
@@ -300,21 +348,21 @@ nll_rows_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_s
 template <class T>
 __global__ void __launch_bounds__(256)
 nll_weight_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_split, const float *__restrict__ bias_acc,
-                      int64_t bias_split, int splits, int64_t C, int K, float scale, const float *__restrict__ col_down,
-                      T *__restrict__ gw, int64_t ldgw, bool gb_f32, void *__restrict__ gb)
+                      int splits, int64_t C, int K, float scale, const unsigned *__restrict__ largest, T *__restrict__ gw,
+                      int64_t ldgw, bool gb_f32, void *__restrict__ gb)
 {
     const int lane = threadIdx.x & 31;
     for (int64_t c = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); c < C; c += (int64_t)gridDim.x * 8) {
+#pragma unroll 4
         for (int k = lane; k < K; k += 32) {
-            float v = 0.f;
+            float v = 0.f, up, down = 1.f;
             for (int s = 0; s < splits; ++s) v += acc[s * acc_split + c * acc_ld + k];
-            v *= scale;
-            if (col_down) v *= col_down[k];
-            gw[c * ldgw + k] = from_f32<T>(v);
+            if (largest != nullptr) plane_scale(__uint_as_float(__ldg(largest + k)), up, down);
+            gw[c * ldgw + k] = from_f32<T>(v * scale * down);
         }
         if (lane == 0 && gb != nullptr) {
             float v = 0.f;
-            for (int s = 0; s < splits; ++s) v += bias_acc[s * bias_split + c];
+            for (int s = 0; s < splits; ++s) v += bias_acc[s * C + c];
             if (gb_f32) static_cast<float *>(gb)[c] = v * scale;
             else static_cast<T *>(gb)[c] = from_f32<T>(v * scale);
         }
@@ -324,40 +372,74 @@ nll_weight_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr int64_t kNllRowCap = 32768;             // rows of a chunk
-constexpr int64_t kNllPieceBytes = 64ll << 20;    // of G: half of the L2 cache
+// G of a chunk and a piece, elements of 16 bits (336 MB).  Measured for 16k rows, 64k classes, 512 features in bf16, the
+// products alone: 5.0 ms with 20 M elements, 4.5 with 45 M, 4.29 with 90 M, 4.26 with 180 M, 4.13 with 360 M: fewer and longer
+// launches win over a G that stays in the L2 cache.
+constexpr int64_t kNllPieceElements = 160ll << 20;
 
 static int64_t round_up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
 
-// Splits of a reduction of `blocks` steps for `tiles` result tiles: the fewest that keep nine of ten SMs busy (or the
-// best there is), each with at least four steps.
-static int nll_splits(int64_t tiles, int64_t blocks)
+// Time of the products of one kind on all SMs, in ns: `tiles` results of `blocks` reduction steps each, split s ways, and
+// the partial sums (`result` bytes a split) that then have to be written.  A step is 0.4 us at the rate the products reach.
+static double nll_product_ns(int64_t tiles, int64_t blocks, int64_t s, int products, double result)
 {
-    const int64_t sms = sm_count();
-    int64_t most = blocks / 4, best = 1;
-    if (most > 148) most = 148;
-    double best_use = 0;
-    for (int64_t s = 1; s <= most; ++s) {
-        const int64_t units = tiles * s;
-        const double use = (double)units / (double)(round_up(units, sms));
-        if (use > best_use + 1e-9) best = s, best_use = use;
-        if (use >= 0.9) break;
+    return (double)ceil_div(tiles * s, sm_count()) * (double)ceil_div(blocks, s) * 400.0 * products + (double)s * result / 4000.0;
+}
+
+static int nll_splits(int64_t tiles, int64_t blocks, int products, double result, double *ns)
+{
+    int64_t most = blocks / 4 < 148 ? blocks / 4 : 148, best = 1;
+    *ns = nll_product_ns(tiles, blocks, 1, products, result);
+    for (int64_t s = 2; s <= most && tiles * s <= 8 * sm_count(); ++s) {
+        const double t = nll_product_ns(tiles, blocks, s, products, result);
+        if (t < *ns) *ns = t, best = s;
     }
     return (int)best;
 }
 
 struct NllPlan {
     int planes;
-    int64_t blocks, padded, row_cap, chunks, cls_padded, piece, pieces, ld, acc_ld;
+    int64_t blocks, padded, row_cap, chunks, cls_padded, piece, ld, acc_ld;
     int row_splits, weight_splits;
-    bool copy_w, weights_direct;
-    size_t counts, rows, total, failed, label, picked2, lse2, loss_part, bias2, stats;
-    size_t x_row, x_col, w_row, w_col, x_down, w_down, x_largest, w_largest, x_up, x_cdown, w_up, w_cdown;
+    bool copy_w, direct;
+    size_t counts, rows, total, failed, joined, label, picked2, lse2, loss_part, bias2, stats;
+    size_t x_row, x_col, w_row, w_col, x_down, w_down, largest;
     size_t grad, acc_x, acc_w, bias_acc, bytes;
 };
 
-// `copy_w`: bf16 weights whose rows TMA cannot read where they are.  The size query allows for the copy.
-static NllPlan nll_plan(int dtype, int64_t n, int64_t K, int64_t C, bool grad, bool copy_w)
+// Rows in chunks, classes in pieces, reductions in splits: of the chunk sizes up to 128 tiles the one whose modelled time is
+// least.  Few long chunks add up gw less often, short ones leave longer pieces and add up gx less often, and the tiles of
+// the two products should fill whole rounds of the SMs.
+static void nll_divide(NllPlan &p, int64_t K, int64_t C, bool may_direct)
+{
+    const int64_t tiles = p.padded / kPM, tiles_k = ceil_div(K, kPN), cls_tiles = p.cls_padded / kPN;
+    const int products = p.planes == 2 ? 3 : 1;
+    const int64_t area = kNllPieceElements / p.planes / (kPM * kPN);  // tiles of G
+    double best = 0;
+    for (int64_t t = tiles < 128 ? tiles : 128; t >= 1; --t) {
+        const int64_t chunks = ceil_div(tiles, t);
+        if (t != ceil_div(tiles, chunks)) continue;  // not the even division into that many chunks
+        int64_t piece = area / t < 1 ? 1 : area / t < cls_tiles ? area / t : cls_tiles;
+        const int64_t pieces = ceil_div(cls_tiles, piece);
+        piece = ceil_div(cls_tiles, pieces);
+        double rows_ns, weights_ns;
+        const double x_bytes = (double)t * kPM * K * 4, w_bytes = (double)piece * kPN * K * 4;
+        const int rs = nll_splits(t * tiles_k, piece * (kPN / kPK), products, pieces > 1 ? 2 * x_bytes : x_bytes, &rows_ns);
+        const int ws = nll_splits(2 * piece * tiles_k, t * (kPM / kPK), products, chunks > 1 ? 2 * w_bytes : w_bytes, &weights_ns);
+        const bool direct = may_direct && chunks == 1 && ws == 1;
+        const double logits_ns = (double)ceil_div(t * piece, sm_count()) * (double)ceil_div(K, kPK) * 400.0 * products;
+        const double ns = (double)(chunks * pieces) * (rows_ns + weights_ns + logits_ns + 9000.0) +
+                          (direct ? 0.0 : (double)ws * C * K * 4 / 4000.0) + (double)chunks * rs * x_bytes / 4000.0;
+        if (best == 0 || ns < best) {
+            best = ns;
+            p.row_cap = t * kPM, p.chunks = chunks, p.piece = piece * kPN, p.row_splits = rs, p.weight_splits = ws, p.direct = direct;
+        }
+        if (tiles <= 8) break;  // a small call: one chunk, and no search
+    }
+}
+
+// `copy_w`: bf16 weights whose rows TMA cannot read where they are.  `may_direct`: gw's rows can be written by TMA.
+static NllPlan nll_plan(int dtype, int64_t n, int64_t K, int64_t C, bool grad, bool copy_w, bool may_direct)
 {
     NllPlan p{};
     const bool f32 = dtype == SGNN_F32;
@@ -365,19 +447,10 @@ static NllPlan nll_plan(int dtype, int64_t n, int64_t K, int64_t C, bool grad, b
     p.copy_w = f32 || copy_w;
     p.blocks = ceil_div(n, kListRows);
     p.padded = round_up(n, kPM);
-    p.row_cap = p.padded < kNllRowCap ? p.padded : kNllRowCap;
-    p.chunks = ceil_div(p.padded, p.row_cap);
     p.cls_padded = round_up(C, kPN);
-    p.piece = kNllPieceBytes / (2 * p.planes * p.row_cap) / kPN * kPN;
-    if (p.piece < kPN) p.piece = kPN;
-    if (p.piece > p.cls_padded) p.piece = p.cls_padded;
-    p.pieces = ceil_div(p.cls_padded, p.piece);
     p.ld = round_up(K, 8);
     p.acc_ld = round_up(K, 32);
-    const int64_t tiles_k = ceil_div(K, kPN);
-    p.row_splits = nll_splits(p.row_cap / kPM * tiles_k, p.piece / kPK);
-    p.weight_splits = nll_splits(p.piece / kPM * tiles_k, p.row_cap / kPK);
-    p.weights_direct = p.chunks == 1 && p.weight_splits == 1;
+    nll_divide(p, K, C, may_direct);
     size_t at = 0;
     const auto take = [&at](size_t bytes) {
         const size_t here = at;
@@ -385,24 +458,20 @@ static NllPlan nll_plan(int dtype, int64_t n, int64_t K, int64_t C, bool grad, b
         return here;
     };
     const size_t mat_x = (size_t)p.planes * p.padded * p.ld * 2, mat_w = (size_t)p.planes * C * p.ld * 2;
-    p.counts = take(p.blocks * 4), p.rows = take(n * 4), p.total = take(4), p.failed = take(4);
+    p.counts = take(p.blocks * 4), p.rows = take(n * 4), p.total = take(4), p.failed = take(4), p.joined = take(4);
     p.label = take(p.padded * 4), p.picked2 = take(p.padded * 4), p.lse2 = take(p.row_cap * 4);
-    p.loss_part = take(ceil_div(p.padded, 32) * 4), p.bias2 = take(p.cls_padded * 4);
+    p.loss_part = take(p.chunks * p.row_cap / 32 * 4), p.bias2 = take(p.cls_padded * 4);
     p.stats = take((size_t)p.cls_padded / 128 * p.row_cap * 8);
     p.x_row = take(mat_x), p.w_row = take(p.copy_w ? mat_w : 0);
     if (f32) {
         p.x_down = take(p.padded * 4), p.w_down = take(p.cls_padded * 4);
-        if (grad) {
-            p.x_col = take(mat_x), p.w_col = take(mat_w);
-            p.x_largest = take(2 * K * 4), p.w_largest = p.x_largest + K * 4;  // one clear for both
-            p.x_up = take(K * 4), p.x_cdown = take(K * 4), p.w_up = take(K * 4), p.w_cdown = take(K * 4);
-        }
+        if (grad) p.x_col = take(mat_x), p.w_col = take(mat_w), p.largest = take(2 * K * 4);
     }
     if (grad) {
         p.grad = take((size_t)p.planes * p.row_cap * p.piece * 2);
         p.acc_x = take((size_t)p.row_splits * p.row_cap * p.acc_ld * 4);
-        p.acc_w = take(p.weights_direct ? 0 : (size_t)p.weight_splits * C * p.acc_ld * 4);
-        p.bias_acc = take(p.weights_direct ? 0 : (size_t)p.weight_splits * C * 4);
+        p.acc_w = take(p.direct ? 0 : (size_t)p.weight_splits * C * p.acc_ld * 4);
+        p.bias_acc = take(p.direct ? 0 : (size_t)p.weight_splits * C * 4);
     }
     p.bytes = at;
     return p;
@@ -433,11 +502,15 @@ static bool nll_must_copy_weights(int dtype, const void *w, int64_t ldw, int64_t
 {
     return dtype == SGNN_BF16 && !(aligned16(w) && ldw % 8 == 0 && C > 1);
 }
+static bool nll_may_direct(int dtype, const void *gw, int64_t ldgw)
+{
+    return aligned16(gw) && ldgw * (int64_t)elem_bytes(dtype) % 16 == 0;
+}
 
 template <int KIND, int PLANES>
 static int nll_product(const ProductCall &c, int64_t units, cudaStream_t s)
 {
-    constexpr int smem = ProductShared<PLANES>::kBytes;
+    constexpr int smem = product_shared_bytes<KIND, PLANES>();
     SGNN_CUDA_OK(cudaFuncSetAttribute(nll_product_kernel<KIND, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const int64_t grid = units < sm_count() ? units : sm_count();
     nll_product_kernel<KIND, PLANES><<<(unsigned)grid, kPThreads, smem, s>>>(c);
@@ -446,118 +519,114 @@ static int nll_product(const ProductCall &c, int64_t units, cudaStream_t s)
 }
 
 template <class T, int PLANES>
-static int nll_run(const NllCall &c)
+static int nll_run(const NllCall &c, const NllPlan &p)
 {
     constexpr bool f32 = PLANES == 2;
     const bool grad = c.gx != nullptr;
-    const NllPlan p = nll_plan(c.dtype, c.n, c.K, c.C, grad, nll_must_copy_weights(c.dtype, c.w, c.ldw, c.C));
     const auto ints = [&](size_t at) { return reinterpret_cast<int *>(c.ws + at); };
     const auto floats = [&](size_t at) { return reinterpret_cast<float *>(c.ws + at); };
     const auto halves = [&](size_t at) { return reinterpret_cast<uint16_t *>(c.ws + at); };
+    const int64_t wide = 16 * sm_count();
+    const auto blocks = [wide](int64_t warps) { return (unsigned)(ceil_div(warps, 8) < wide ? ceil_div(warps, 8) : wide); };
     cudaStream_t s = c.s;
     int rc;
 
-    // the rows in the loss
-    if (p.blocks > 1)
+    // the rows in the loss, and what later kernels start from
+    if (p.blocks > 1) {
         nll_count_kernel<<<(unsigned)p.blocks, kListThreads, 0, s>>>(c.labels, c.mask, c.n, c.C, ints(p.counts));
-    nll_list_kernel<<<(unsigned)p.blocks, kListThreads, 0, s>>>(c.labels, c.mask, c.n, c.C, ints(p.counts), ints(p.rows), ints(p.total));
-    nll_bias_kernel<T><<<(unsigned)ceil_div(p.cls_padded, 256), 256, 0, s>>>(c.bias, c.C, p.cls_padded, floats(p.bias2),
-                                                                              f32 ? floats(p.w_down) : nullptr, ints(p.failed));
-    if (c.lse) SGNN_CUDA_OK(cudaMemsetAsync(c.lse, 0, c.n * 4, s));
+        SGNN_LAUNCH_OK("linear_nll count");
+    }
+    const NllStart start{c.labels, c.mask, c.n, c.C, p.cls_padded, ints(p.counts), ints(p.rows), ints(p.total), (int)p.blocks, c.bias,
+                         floats(p.bias2), f32 ? floats(p.w_down) : nullptr, c.lse, ints(p.failed), ints(p.joined)};
+    nll_start_kernel<T><<<(unsigned)p.blocks + blocks(ceil_div(p.cls_padded + (c.lse ? c.n : 0), 32)), kListThreads, 0, s>>>(start);
     if (grad) SGNN_CUDA_OK(cudaMemset2DAsync(c.gx, c.ldgx * sizeof(T), 0, c.K * sizeof(T), c.n, s));
 
     // the operands as the products read them
-    const RowSource xs{c.x, c.ldx, ints(p.rows), ints(p.total), 0, (int)c.K}, wsrc{c.w, c.ldw, nullptr, nullptr, c.C, (int)c.K};
-    const Planes x_row{halves(p.x_row), p.ld, p.padded * p.ld}, w_row{halves(p.w_row), p.ld, c.C * p.ld};
     const bool cols = f32 && grad;
-    const Planes x_col{cols ? halves(p.x_col) : nullptr, p.ld, p.padded * p.ld}, w_col{cols ? halves(p.w_col) : nullptr, p.ld, c.C * p.ld};
+    unsigned *largest = cols ? reinterpret_cast<unsigned *>(c.ws + p.largest) : nullptr;
+    TakeSide xs{RowSource{c.x, c.ldx, ints(p.rows), ints(p.total), 0, (int)c.K},
+                Planes{halves(p.x_row), p.ld, p.padded * p.ld},
+                Planes{cols ? halves(p.x_col) : nullptr, p.ld, p.padded * p.ld},
+                largest, f32 ? floats(p.x_down) : nullptr, (int)blocks(p.padded)};
+    TakeSide ws{RowSource{c.w, c.ldw, nullptr, nullptr, c.C, (int)c.K},
+                Planes{halves(p.w_row), p.ld, c.C * p.ld},
+                Planes{cols ? halves(p.w_col) : nullptr, p.ld, c.C * p.ld},
+                cols ? largest + c.K : nullptr, f32 ? floats(p.w_down) : nullptr, p.copy_w ? (int)blocks(c.C) : 0};
     if (cols) {
-        SGNN_CUDA_OK(cudaMemsetAsync(c.ws + p.x_largest, 0, 2 * c.K * 4, s));
-        const int64_t tall = 4 * sm_count();
-        const dim3 gx((unsigned)ceil_div(c.K, 32), (unsigned)(ceil_div(c.n, 64) < tall ? ceil_div(c.n, 64) : tall));
-        const dim3 gw((unsigned)ceil_div(c.K, 32), (unsigned)(ceil_div(c.C, 64) < tall ? ceil_div(c.C, 64) : tall));
-        unsigned *xl = reinterpret_cast<unsigned *>(c.ws + p.x_largest), *wl = reinterpret_cast<unsigned *>(c.ws + p.w_largest);
-        nll_column_max_kernel<<<gx, 256, 0, s>>>(xs, xl);
-        nll_column_max_kernel<<<gw, 256, 0, s>>>(wsrc, wl);
-        nll_column_scale_kernel<<<(unsigned)ceil_div(c.K, 256), 256, 0, s>>>(xl, (int)c.K, floats(p.x_up), floats(p.x_cdown));
-        nll_column_scale_kernel<<<(unsigned)ceil_div(c.K, 256), 256, 0, s>>>(wl, (int)c.K, floats(p.w_up), floats(p.w_cdown));
+        SGNN_CUDA_OK(cudaMemsetAsync(largest, 0, 2 * c.K * 4, s));
+        const int64_t rows = c.n > c.C ? c.n : c.C, tall = ceil_div(rows, 64) < 2 * sm_count() ? ceil_div(rows, 64) : 2 * sm_count();
+        nll_column_max_kernel<<<dim3((unsigned)ceil_div(c.K, 32), (unsigned)tall, 2), 256, 0, s>>>(xs.src, ws.src, largest);
     }
-    const int64_t wide = 16 * sm_count();
-    const Picked pick{c.labels, c.w, c.ldw, c.bias, ints(p.label), floats(p.picked2)};
-    nll_take_kernel<T, f32><<<(unsigned)(p.padded / 8 < wide ? p.padded / 8 : wide), 256, 0, s>>>(
-        xs, x_row, x_col, cols ? floats(p.x_up) : nullptr, f32 ? floats(p.x_down) : nullptr, pick);
-    if (p.copy_w)
-        nll_take_kernel<T, f32><<<(unsigned)(ceil_div(c.C, 8) < wide ? ceil_div(c.C, 8) : wide), 256, 0, s>>>(
-            wsrc, w_row, w_col, cols ? floats(p.w_up) : nullptr, f32 ? floats(p.w_down) : nullptr, Picked{});
+    nll_take_kernel<T, f32><<<(unsigned)(xs.blocks + ws.blocks), 256, 0, s>>>(
+        xs, ws, Picked{c.labels, c.w, c.ldw, c.bias, ints(p.label), floats(p.picked2)});
     SGNN_LAUNCH_OK("linear_nll operands");
 
     // tensor maps: x and W along k (rows of a tile at once) and across it (64 steps of the reduction at once), G likewise
-    ProductCall lc{}, rc_{}, wc{};
-    const void *wp = p.copy_w ? (const void *)w_row.p : c.w;
-    const int64_t wld = p.copy_w ? p.ld : c.ldw, wst = p.copy_w ? w_row.stride : c.C * c.ldw;
-    if ((rc = umma_tensor_map(&lc.a, x_row.p, !f32, c.K, p.padded, p.ld, PLANES, x_row.stride, kPM))) return rc;
+    ProductCall lc{}, xc{}, wc{};
+    const void *wp = p.copy_w ? (const void *)ws.row.p : c.w;
+    const int64_t wld = p.copy_w ? p.ld : c.ldw, wst = p.copy_w ? ws.row.stride : c.C * c.ldw;
+    if ((rc = umma_tensor_map(&lc.a, xs.row.p, !f32, c.K, p.padded, p.ld, PLANES, xs.row.stride, kPM))) return rc;
     if ((rc = umma_tensor_map(&lc.b, wp, !f32, c.K, c.C, wld, PLANES, wst, kPN))) return rc;
     lc.total = ints(p.total), lc.failed = ints(p.failed), lc.feats = (int)c.K, lc.splits = 1, lc.bf16 = !f32;
-    lc.bias2 = floats(p.bias2), lc.row_scale = f32 ? floats(p.x_down) : nullptr, lc.cls_scale = f32 ? floats(p.w_down) : nullptr;
+    lc.bias2 = floats(p.bias2), lc.row_scale = xs.row_down, lc.cls_scale = ws.row_down, lc.classes = c.C;
     lc.stats = reinterpret_cast<float2 *>(c.ws + p.stats), lc.row_cap = (int)p.row_cap, lc.lse2 = floats(p.lse2);
     lc.scale = c.inv_count * (f32 ? 1.0f / kGradScale : 1.0f);
+    const int64_t x_split = p.row_cap * p.acc_ld, w_split = c.C * p.acc_ld;
     if (grad) {
-        lc.grad = halves(p.grad), lc.grad_ld = p.piece;
-        rc_ = lc, wc = lc;
+        xc = lc, wc = lc;
+        uint16_t *g = halves(p.grad);
         const int64_t plane = p.row_cap * p.piece;
-        if ((rc = umma_tensor_map(&rc_.a, lc.grad, !f32, p.piece, p.row_cap, p.piece, PLANES, plane, kPM))) return rc;
-        if ((rc = umma_tensor_map(&rc_.b, f32 ? (const void *)w_col.p : wp, !f32, c.K, c.C, wld, PLANES, wst, kPK))) return rc;
-        if ((rc = umma_tensor_map(&wc.a, lc.grad, !f32, p.piece, p.row_cap, p.piece, PLANES, plane, kPK))) return rc;
-        if ((rc = umma_tensor_map(&wc.b, f32 ? x_col.p : x_row.p, !f32, c.K, p.padded, p.ld, PLANES, x_row.stride, kPK))) return rc;
-        rc_.splits = p.row_splits, rc_.out = floats(p.acc_x), rc_.out_ld = p.acc_ld, rc_.out_split = p.row_cap * p.acc_ld;
-        wc.splits = p.weight_splits, wc.out_ld = p.acc_ld, wc.out_split = c.C * p.acc_ld, wc.bias_split = c.C;
-        wc.col_scale = f32 ? floats(p.x_cdown) : nullptr;
-        if (p.weights_direct)
-            wc.gw = c.gw, wc.gw_ld = c.ldgw, wc.gb = c.gb, wc.gw_f32 = f32, wc.gb_f32 = c.bias.f32;
+        if ((rc = umma_store_map(&lc.o, g, f32 ? StoreType::kF16 : StoreType::kBf16, p.piece, p.row_cap, p.piece, PLANES, plane, f32 ? 32 : 64))) return rc;
+        if ((rc = umma_tensor_map(&xc.a, g, !f32, p.piece, p.row_cap, p.piece, PLANES, plane, kPM))) return rc;
+        if ((rc = umma_tensor_map(&xc.b, f32 ? (const void *)ws.col.p : wp, !f32, c.K, c.C, wld, PLANES, wst, kPK))) return rc;
+        if ((rc = umma_store_map(&xc.o, floats(p.acc_x), StoreType::kF32, p.acc_ld, p.row_cap, p.acc_ld, p.row_splits, x_split, 32))) return rc;
+        if ((rc = umma_tensor_map(&wc.a, g, !f32, p.piece, p.row_cap, p.piece, PLANES, plane, kPK))) return rc;
+        if ((rc = umma_tensor_map(&wc.b, f32 ? xs.col.p : xs.row.p, !f32, c.K, p.padded, p.ld, PLANES, xs.row.stride, kPK))) return rc;
+        xc.splits = p.row_splits, wc.splits = p.weight_splits;
+        wc.direct = p.direct, wc.direct_bf16 = !f32, wc.gb_f32 = c.bias.f32, wc.col_largest = largest;
+        if (p.direct) {
+            wc.gb = c.gb;
+            rc = umma_store_map(&wc.o, c.gw, f32 ? StoreType::kF32 : StoreType::kBf16, c.K, c.C, c.ldgw, 1, c.C * c.ldgw, f32 ? 32 : 64);
+        } else {
+            wc.bias_out = floats(p.bias_acc);
+            rc = umma_store_map(&wc.o, floats(p.acc_w), StoreType::kF32, p.acc_ld, c.C, p.acc_ld, p.weight_splits, w_split, 32);
+        }
+        if (rc) return rc;
     }
-    const int64_t tiles_k = ceil_div(c.K, kPN), loss_blocks = ceil_div(p.row_cap, 32);
+    const int64_t tiles_k = ceil_div(c.K, kPN), join_blocks = p.row_cap / 32, tiles_m = p.row_cap / kPM;
     for (int64_t q = 0; q < p.chunks; ++q) {
         const int row0 = (int)(q * p.row_cap);
-        for (ProductCall *k : {&lc, &rc_, &wc}) k->row0 = row0;
+        for (ProductCall *k : {&lc, &xc, &wc}) k->row0 = row0;
         lc.label = ints(p.label) + row0, lc.picked2 = floats(p.picked2) + row0;
         lc.cls0 = 0, lc.cls_count = (int)c.C;
-        const int64_t tiles_m = p.row_cap / kPM;
         if ((rc = nll_product<kLogitStats, PLANES>(lc, tiles_m * ceil_div(c.C, kPN), s))) return rc;
-        const int64_t left = p.padded - row0 < p.row_cap ? p.padded - row0 : p.row_cap;
-        nll_join_kernel<<<(unsigned)ceil_div(left, 32), 256, 0, s>>>(lc.stats, (int)(p.cls_padded / 128), row0, (int)p.row_cap,
-                                                                     ints(p.rows), ints(p.total), lc.picked2, floats(p.lse2), c.lse,
-                                                                     floats(p.loss_part) + q * loss_blocks);
+        const NllJoin join{lc.stats, (int)(p.cls_padded / 128), row0, (int)p.row_cap, ints(p.rows), ints(p.total), lc.picked2,
+                           floats(p.lse2), c.lse, floats(p.loss_part) + q * join_blocks, floats(p.loss_part),
+                           (int)(p.chunks * join_blocks), c.inv_count, ints(p.joined), ints(p.failed), c.loss};
+        nll_join_kernel<<<(unsigned)join_blocks, 1024, 0, s>>>(join);
         SGNN_LAUNCH_OK("linear_nll join");
         if (!grad) continue;
         for (int64_t first = 0; first < c.C; first += p.piece) {
             const int64_t count = c.C - first < p.piece ? c.C - first : p.piece;
-            for (ProductCall *k : {&lc, &rc_, &wc}) k->cls0 = (int)first, k->cls_count = (int)count;
+            for (ProductCall *k : {&lc, &xc, &wc}) k->cls0 = (int)first, k->cls_count = (int)count;
             if ((rc = nll_product<kLogitGrad, PLANES>(lc, tiles_m * ceil_div(count, kPN), s))) return rc;
-            rc_.add = first > 0;
-            if ((rc = nll_product<kRowGrad, PLANES>(rc_, tiles_m * tiles_k * p.row_splits, s))) return rc;
+            xc.add = first > 0;
+            if ((rc = nll_product<kRowGrad, PLANES>(xc, tiles_m * tiles_k * p.row_splits, s))) return rc;
             wc.add = q > 0;
-            if (!p.weights_direct) wc.out = floats(p.acc_w) + first * p.acc_ld, wc.bias_out = floats(p.bias_acc) + first;
             if ((rc = nll_product<kWeightGrad, PLANES>(wc, ceil_div(count, kPM) * tiles_k * p.weight_splits, s))) return rc;
         }
-        if (q + 1 < p.chunks) {
-            nll_rows_out_kernel<T><<<(unsigned)(left / 8 < wide ? left / 8 : wide), 256, 0, s>>>(
-                floats(p.acc_x), p.acc_ld, rc_.out_split, p.row_splits, row0, (int)p.row_cap, ints(p.rows), ints(p.total), lc.scale,
-                f32 ? floats(p.w_cdown) : nullptr, ints(p.failed), static_cast<T *>(c.gx), c.ldgx, (int)c.K, c.loss);
-        }
+        const bool dealt = p.row_splits >= 8;
+        const dim3 out_grid = dealt ? dim3((unsigned)(p.row_cap < wide ? p.row_cap : wide), (unsigned)ceil_div(c.K, 32)) : dim3(blocks(p.row_cap));
+        nll_rows_out_kernel<T><<<out_grid, 256, 0, s>>>(floats(p.acc_x), p.acc_ld, x_split, p.row_splits, row0, (int)p.row_cap, ints(p.rows),
+                                                        ints(p.total), lc.scale, cols ? largest + c.K : nullptr, ints(p.failed),
+                                                        static_cast<T *>(c.gx), c.ldgx, (int)c.K, c.loss, dealt);
+        SGNN_LAUNCH_OK("linear_nll row gradients");
     }
-    nll_loss_kernel<<<1, 1024, 0, s>>>(floats(p.loss_part), (int)ceil_div(p.padded, 32), c.inv_count, ints(p.failed), c.loss);
-    if (grad) {
-        const int row0 = (int)((p.chunks - 1) * p.row_cap);
-        const int64_t left = p.padded - row0;
-        nll_rows_out_kernel<T><<<(unsigned)(left / 8 < wide ? left / 8 : wide), 256, 0, s>>>(
-            floats(p.acc_x), p.acc_ld, rc_.out_split, p.row_splits, row0, (int)p.row_cap, ints(p.rows), ints(p.total), lc.scale,
-            f32 ? floats(p.w_cdown) : nullptr, ints(p.failed), static_cast<T *>(c.gx), c.ldgx, (int)c.K, c.loss);
-        if (!p.weights_direct)
-            nll_weight_out_kernel<T><<<(unsigned)(ceil_div(c.C, 8) < wide ? ceil_div(c.C, 8) : wide), 256, 0, s>>>(
-                floats(p.acc_w), p.acc_ld, wc.out_split, floats(p.bias_acc), wc.bias_split, p.weight_splits, c.C, (int)c.K, lc.scale,
-                f32 ? floats(p.x_cdown) : nullptr, static_cast<T *>(c.gw), c.ldgw, c.bias.f32, c.gb);
+    if (grad && !p.direct) {
+        nll_weight_out_kernel<T><<<blocks(c.C), 256, 0, s>>>(floats(p.acc_w), p.acc_ld, w_split, floats(p.bias_acc), p.weight_splits, c.C,
+                                                             (int)c.K, lc.scale, largest, static_cast<T *>(c.gw), c.ldgw, c.bias.f32, c.gb);
+        SGNN_LAUNCH_OK("linear_nll weight gradients");
     }
-    SGNN_LAUNCH_OK("linear_nll_loss");
     return SGNN_OK;
 }
 
@@ -579,7 +648,12 @@ extern "C" SGNN_API int sgnn_linear_nll_workspace_bytes(int dtype, int64_t n, in
     int rc = nll_check(who, dtype, n, K, C);
     if (rc) return rc;
     SGNN_REQUIRE(bytes != nullptr, SGNN_ERR_INVALID_ARGUMENT, "%s: null result pointer", who);
-    *bytes = n == 0 ? 0 : nll_plan(dtype, n, K, C, with_grad != 0, true).bytes;
+    *bytes = 0;
+    if (n > 0) {  // enough for every layout of the weights: a copy of them, gw written directly or not
+        const size_t added = nll_plan(dtype, n, K, C, with_grad != 0, true, false).bytes;
+        const size_t direct = nll_plan(dtype, n, K, C, with_grad != 0, true, true).bytes;
+        *bytes = added > direct ? added : direct;
+    }
     return SGNN_OK;
 }
 
@@ -610,12 +684,11 @@ extern "C" SGNN_API int sgnn_linear_nll_loss(int dtype, const void *d_x, int64_t
     }
     SGNN_REQUIRE(d_x && d_w && d_labels, SGNN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
     SGNN_REQUIRE((n == 1 || ldx >= K) && (C == 1 || ldw >= K), SGNN_ERR_INVALID_ARGUMENT, "%s: leading dimension shorter than a row", who);
-    size_t need = 0;
-    rc = sgnn_linear_nll_workspace_bytes(dtype, n, K, C, d_gx != nullptr, &need);
-    if (rc) return rc;
-    SGNN_REQUIRE(d_workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(d_workspace) % 256 == 0,
-                 SGNN_ERR_WORKSPACE, "%s: 256-byte aligned workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+    const NllPlan p = nll_plan(dtype, n, K, C, d_gx != nullptr, nll_must_copy_weights(dtype, d_w, ldw, C),
+                               nll_may_direct(dtype, d_gw, ldgw));
+    SGNN_REQUIRE(d_workspace != nullptr && workspace_bytes >= p.bytes && reinterpret_cast<uintptr_t>(d_workspace) % 256 == 0,
+                 SGNN_ERR_WORKSPACE, "%s: 256-byte aligned workspace of %zu bytes needed, %zu given", who, p.bytes, workspace_bytes);
     const NllCall c{dtype, d_x, ldx, d_w, ldw, NllBias{d_bias, bias_dtype == SGNN_F32}, d_labels, d_mask, inv_count, n, K, C, d_loss,
                     d_lse, d_gx, ldgx, d_gw, ldgw, d_gb, static_cast<char *>(d_workspace), s};
-    return dtype == SGNN_F32 ? nll_run<float, 2>(c) : nll_run<__nv_bfloat16, 1>(c);
+    return dtype == SGNN_F32 ? nll_run<float, 2>(c, p) : nll_run<__nv_bfloat16, 1>(c, p);
 }

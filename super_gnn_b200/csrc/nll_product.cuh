@@ -24,7 +24,7 @@ constexpr int kPAccCols = 512;  // all of the tensor memory: two results, or one
 enum ProductKind { kLogitStats, kLogitGrad, kRowGrad, kWeightGrad };
 
 struct ProductCall {
-    CUtensorMap a, b;
+    CUtensorMap a, b, o;  // operands, result
     const int *total;     // rows in the loss
     int *failed;          // set when a wait gave up
     int row0, row_cap;    // this chunk of them
@@ -34,27 +34,21 @@ struct ProductCall {
     bool bf16;
     // logits
     const float *bias2;      // [classes rounded up to 256]: bias log2(e), -inf beyond the last class
-    const float *row_scale;  // fp32: 2^-e of the rows of x (all of them) and of W; nullptr: 1
+    const float *row_scale;  // fp32: 2^-e of the rows of x (all of them) and of W
     const float *cls_scale;
     float2 *stats;           // [2 x class tiles, row_cap]: (maximum, sum of 2^(t - maximum)), in units of log2
     const float *lse2;       // [row_cap]
     const float *picked2;    // [row_cap] the label's logit
     const int *label;        // [row_cap]
-    uint16_t *grad;          // [planes, row_cap, grad_ld]
-    int64_t grad_ld;
-    // gradients
-    float *out;           // rows: [splits, row_cap, out_ld]; weights: [splits, classes, out_ld] at the piece's first class
-    int64_t out_ld, out_split;
-    bool add;
-    // weights, when nothing is left to add: the result itself
-    void *gw;
-    int64_t gw_ld;
-    void *gb;
-    bool gw_f32, gb_f32;
-    const float *col_scale;  // fp32: 2^-e of the columns of x
+    // gradients of rows: o = [splits, row_cap, K rounded up to 32] fp32
+    bool add;                // onto what the pieces (chunks) before have left there
+    // gradients of weights: o = [splits, C, K rounded up to 32] fp32, or the result itself where nothing is left to add
+    bool direct, direct_bf16, gb_f32;
+    const unsigned *col_largest;  // fp32: the columns of x are scaled by it
     float scale;
-    float *bias_out;  // [splits, classes] at the piece's first class
-    int64_t bias_split;
+    void *gb;
+    float *bias_out;         // [splits, C] when not direct
+    int64_t classes;
 };
 
 template <int PLANES>
@@ -62,9 +56,19 @@ struct ProductShared {
     static constexpr int kStages = 4 / PLANES;
     static constexpr int kA = kPM * kPK * 2, kB = kPN * kPK * 2;
     static constexpr int kStageBytes = PLANES * (kA + kB);
-    static constexpr int kOnes = 16 * kPK * 2;
-    static constexpr int kBytes = kStages * kStageBytes + kOnes + 2 * kPN * 8 + 256 + 1024;
+    static constexpr int kBox = 4096;  // result box of a warp: 32 rows of 128 bytes
+    static constexpr int kOnes = 256;
 };
+
+template <int KIND, int PLANES>
+constexpr int product_shared_bytes()
+{
+    using S = ProductShared<PLANES>;
+    const int ring = S::kStages * S::kStageBytes;
+    if (KIND == kLogitStats) return ring + 2 * kPN * 8 + 256;
+    if (KIND == kLogitGrad) return ring + kPEpilogueWarps * S::kBox + kPN * 8 + 256;
+    return ring + kPEpilogueWarps * S::kBox + S::kOnes + 256;
+}
 
 // sizes of the product of this chunk and piece, from the number of rows in the loss
 struct ProductUnits {
@@ -120,6 +124,17 @@ __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi)
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+// 2^e that brings `largest` into [2^14, 2^15), and 2^-e; 1 for nothing but zeros and for what is not finite
+__device__ __forceinline__ void plane_scale(float largest, float &up, float &down)
+{
+    up = down = 1.0f;
+    if (!(largest > 0.f) || !(largest <= 3.402823466e+38f)) return;
+    int e = 14 - ((int)(__float_as_uint(largest) >> 23) - 127);
+    e = e < -126 ? -126 : e > 126 ? 126 : e;
+    up = __uint_as_float((unsigned)(e + 127) << 23);
+    down = __uint_as_float((unsigned)(127 - e) << 23);
+}
+
 constexpr float kGradScale = 32768.0f;  // fp16 planes of G: |G| <= 1 fills the range, 2^-40 is the smallest step
 
 template <int KIND, int PLANES>
@@ -129,11 +144,13 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     constexpr bool kLogits = KIND == kLogitStats || KIND == kLogitGrad;
     constexpr bool kAmn = KIND == kWeightGrad, kBmn = !kLogits;
     constexpr int kAcc = KIND == kWeightGrad ? 1 : 2;  // results in flight
-    extern __shared__ uint8_t raw[];
-    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
-    uint8_t *ones = base + S::kStages * S::kStageBytes;
-    float2 *column = reinterpret_cast<float2 *>(ones + S::kOnes);  // [2][256]: (bias, scale) of the classes of a tile
-    uint64_t *full = reinterpret_cast<uint64_t *>(column + 2 * kPN);
+    extern __shared__ __align__(1024) uint8_t base[];
+    uint8_t *boxes = base + S::kStages * S::kStageBytes;
+    uint8_t *ones = boxes + (KIND == kLogitStats ? 0 : kPEpilogueWarps * S::kBox);
+    float *column = reinterpret_cast<float *>(ones);  // logits: bias, then scale, of the classes of a tile
+    constexpr int kColumns = KIND == kLogitStats ? 2 : 1;  // tiles whose classes are held at once
+    uint8_t *behind = ones + (kLogits ? kColumns * kPN * 8 : S::kOnes);
+    uint64_t *full = reinterpret_cast<uint64_t *>(behind);
     uint64_t *empty = full + S::kStages, *acc_full = empty + S::kStages, *acc_empty = acc_full + 2;
     uint64_t *drained = acc_empty + 2;
     uint32_t *slot = reinterpret_cast<uint32_t *>(drained + 1);
@@ -141,6 +158,10 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ProductUnits u = product_units<KIND>(c);
     if ((int)blockIdx.x >= u.units) return;
+    if ((smem_addr(base) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
+        if (threadIdx.x == 0) atomicExch(c.failed, 1);
+        return;
+    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) bar_init(full + s, 1), bar_init(empty + s, 1);
@@ -152,7 +173,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     if (KIND == kWeightGrad) {
         const uint32_t one = c.bf16 ? 0x3F803F80u : 0x3C003C00u;
         for (int i = threadIdx.x; i < S::kOnes / 4; i += kPThreads) reinterpret_cast<uint32_t *>(ones)[i] = one;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        async_fence();
     }
     if (warp == kPEpilogueWarps + 1) tmem_alloc(slot, kPAccCols);
     tc_fence_before();
@@ -235,7 +256,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         da[p] = umma_desc(at + p * S::kA, a_run, 1024);
                         db[p] = umma_desc(at + PLANES * S::kA + p * S::kB, b_run, 1024);
                     }
-                    const uint64_t dones = umma_desc(ones, 16, 1024);
+                    const uint64_t dones = umma_desc_same(ones);
 #pragma unroll
                     for (int j = 0; j < kPK / 16; ++j) {
                         // sixteen steps of the reduction: 32 bytes along a row, or two groups of eight rows
@@ -266,21 +287,25 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
         __syncwarp();
     } else {
         // ---- results ----
-        const int quarter = warp & 3, half = warp >> 2;
-        const int tid = threadIdx.x;
+        const int quarter = warp & 3, half = warp >> 2, tid = threadIdx.x;
+        uint8_t *box = boxes + warp * S::kBox;
+        uint8_t *box_row = box + lane * 128;
         int acc = 0;
         unsigned acc_phase = 0;
         for (int i = blockIdx.x; i < u.units; i += gridDim.x) {
             const ProductUnit t = product_unit(u, i);
             const int row = t.m0 + quarter * 32 + lane;  // of the product
-            float2 *col = column + acc * kPN;
+            float *bias_col = column + (kColumns == 2 ? acc : 0) * 2 * kPN, *scale_col = bias_col + kPN;
             if (kLogits) {
                 const int cls = c.cls0 + t.n0 + tid;  // the arrays cover whole tiles
-                col[tid] = make_float2(__ldg(c.bias2 + cls), c.cls_scale ? __ldg(c.cls_scale + cls) : 1.0f);
+                const float b = __ldg(c.bias2 + cls);
+                if (kColumns == 1) asm volatile("bar.sync 1, %0;" ::"n"(kPEpilogueWarps * 32) : "memory");
+                bias_col[tid] = b;
+                if (PLANES == 2) scale_col[tid] = __ldg(c.cls_scale + cls);
                 asm volatile("bar.sync 1, %0;" ::"n"(kPEpilogueWarps * 32) : "memory");
             }
             float scale = 1.4426950408889634f, lse2 = 0.f;
-            if (kLogits && c.row_scale) scale *= __ldg(c.row_scale + c.row0 + (row < u.m ? row : 0));
+            if (kLogits && PLANES == 2) scale *= __ldg(c.row_scale + c.row0 + (row < u.m ? row : 0));
             if (KIND == kLogitGrad && row < u.m) lse2 = __ldg(c.lse2 + row);
             if (!bar_wait(acc_full + acc, acc_phase, gone)) {  // the others may stand at the barrier above: keep coming to it
                 if (++acc == kAcc) acc = 0, acc_phase ^= 1;
@@ -290,79 +315,117 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
             const uint32_t d = tmem + acc * kPN + half * 128 + ((uint32_t)quarter << 21);
             const bool there = t.count > 0;  // an empty range of the reduction: zeros
             float v[32];
+            // logits in units of log2, 32 columns at a time
+            const auto logits = [&](int j) {
+                tmem_load32(d + 32 * j, v);
+                tmem_load_wait();
+                const float4 *b4 = reinterpret_cast<const float4 *>(bias_col + half * 128 + 32 * j);
+                const float4 *s4 = reinterpret_cast<const float4 *>(scale_col + half * 128 + 32 * j);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 b = b4[q];
+                    if (PLANES == 2) {
+                        const float4 w = s4[q];
+                        v[4 * q] *= w.x, v[4 * q + 1] *= w.y, v[4 * q + 2] *= w.z, v[4 * q + 3] *= w.w;
+                    }
+                    v[4 * q] = __fmaf_rn(v[4 * q], scale, b.x), v[4 * q + 1] = __fmaf_rn(v[4 * q + 1], scale, b.y);
+                    v[4 * q + 2] = __fmaf_rn(v[4 * q + 2], scale, b.z), v[4 * q + 3] = __fmaf_rn(v[4 * q + 3], scale, b.w);
+                }
+            };
+            // the box is free again / filled: hand it on
+            const auto box_free = [&]() {
+                if (lane == 0) store_wait_read();
+                __syncwarp();
+            };
+            const auto box_done = [&]() {
+                async_fence();
+                __syncwarp();
+            };
             if constexpr (KIND == kLogitStats) {
                 float mx = -INFINITY, sum = 0.f;
 #pragma unroll 1
                 for (int j = 0; j < 4; ++j) {
-                    tmem_load32(d + 32 * j, v);
-                    tmem_load_wait();
-                    const float2 *cj = col + half * 128 + 32 * j;
+                    logits(j);
                     float top = mx;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float2 b = cj[e];
-                        v[e] = __fmaf_rn(v[e] * b.y, scale, b.x);
-                        top = fmaxf(top, v[e]);
-                    }
+                    for (int e = 0; e < 32; ++e) top = fmaxf(top, v[e]);
                     const float ref = top == -INFINITY ? 0.f : top;
                     sum *= exp2_fast(mx - ref);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) sum += exp2_fast(v[e] - ref);
                     mx = top;
                 }
-                if (row < u.m)
-                    c.stats[(int64_t)(t.n0 / 128 + half) * c.row_cap + row] = make_float2(mx, sum);
+                if (row < u.m) c.stats[(int64_t)(t.n0 / 128 + half) * c.row_cap + row] = make_float2(mx, sum);
             } else if constexpr (KIND == kLogitGrad) {
                 const int label = row < u.m ? c.label[row] - c.cls0 - t.n0 - half * 128 : -1;
-                const bool mine = label >= 0 && label < 128;
-                uint16_t *g = c.grad + (int64_t)row * c.grad_ld + t.n0 + half * 128;
-                const int64_t plane = (int64_t)c.row_cap * c.grad_ld;
+                const float own = label >= 0 && label < 128
+                                      ? (exp2_fast(__ldg(c.picked2 + row) - lse2) - 1.0f) * (PLANES == 2 ? kGradScale : 1.0f)
+                                      : 0.f;  // G of the label's class
+                const int x0 = t.n0 + half * 128, y0 = t.m0 + quarter * 32;
 #pragma unroll 1
                 for (int j = 0; j < 4; ++j) {
-                    tmem_load32(d + 32 * j, v);
-                    tmem_load_wait();
-                    const float2 *cj = col + half * 128 + 32 * j;
+                    logits(j);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float2 b = cj[e];
-                        v[e] = row < u.m ? exp2_fast(__fmaf_rn(v[e] * b.y, scale, b.x) - lse2) : 0.f;
+                        v[e] = row < u.m ? exp2_fast(v[e] - lse2) : 0.f;
                         if (PLANES == 2) v[e] *= kGradScale;
                     }
+                    const int at = label - 32 * j;  // 0 .. 31: in these columns
+                    if (PLANES == 1) {  // 64 columns a box: 128 bytes a row, two turns
+                        if ((j & 1) == 0) box_free();
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint4 w;
-                        uint32_t *pw = reinterpret_cast<uint32_t *>(&w);
-                        if (PLANES == 1) {
+                        for (int q = 0; q < 4; ++q) {
+                            uint4 w;
+                            uint32_t *pw = reinterpret_cast<uint32_t *>(&w);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) pw[e] = pack16<__nv_bfloat16>(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
-                            *reinterpret_cast<uint4 *>(g + 32 * j + 8 * q) = w;
-                        } else {
-                            uint4 w1;
-                            uint32_t *pw1 = reinterpret_cast<uint32_t *>(&w1);
+                            const int place = ((j & 1) * 4 + q) ^ (lane & 7);
+                            *reinterpret_cast<uint4 *>(box_row + place * 16) = w;
+                        }
+                        if (at >= 0 && at < 32) {
+                            const int place = ((j & 1) * 4 + at / 8) ^ (lane & 7);
+                            *reinterpret_cast<__nv_bfloat16 *>(box_row + place * 16 + at % 8 * 2) = __float2bfloat16_rn(own);
+                        }
+                        if (j & 1) {
+                            box_done();
+                            if (lane == 0) {
+                                tma_store(&c.o, box, x0 + 32 * (j - 1), y0, 0);
+                                store_commit();
+                            }
+                        }
+                    } else {  // 32 columns of both planes: 64 bytes a row each
+                        box_free();
+                        uint8_t *r0 = box + lane * 64, *r1 = r0 + 2048;
+                        const int turn = (lane >> 1) & 3;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint4 w0, w1;
+                            uint32_t *p0 = reinterpret_cast<uint32_t *>(&w0), *p1 = reinterpret_cast<uint32_t *>(&w1);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float x0 = v[8 * q + 2 * e], x1 = v[8 * q + 2 * e + 1];
-                                pw[e] = pack16<__half>(x0, x1);
-                                const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(pw + e));
-                                pw1[e] = pack16<__half>(x0 - r.x, x1 - r.y);
+                                const float g0 = v[8 * q + 2 * e], g1 = v[8 * q + 2 * e + 1];
+                                p0[e] = pack16<__half>(g0, g1);
+                                const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(p0 + e));
+                                p1[e] = pack16<__half>(g0 - r.x, g1 - r.y);
                             }
-                            *reinterpret_cast<uint4 *>(g + 32 * j + 8 * q) = w;
-                            *reinterpret_cast<uint4 *>(g + plane + 32 * j + 8 * q) = w1;
+                            *reinterpret_cast<uint4 *>(r0 + (q ^ turn) * 16) = w0;
+                            *reinterpret_cast<uint4 *>(r1 + (q ^ turn) * 16) = w1;
+                        }
+                        if (at >= 0 && at < 32) {
+                            const int off = ((at / 8) ^ turn) * 16 + at % 8 * 2;
+                            const __half h = __float2half_rn(own);
+                            *reinterpret_cast<__half *>(r0 + off) = h;
+                            *reinterpret_cast<__half *>(r1 + off) = __float2half_rn(own - __half2float(h));
+                        }
+                        box_done();
+                        if (lane == 0) {
+                            tma_store(&c.o, box, x0 + 32 * j, y0, 0);
+                            tma_store(&c.o, box + 2048, x0 + 32 * j, y0, 1);
+                            store_commit();
                         }
                     }
                 }
-                if (mine) {  // the label's class: the same thread wrote it just now without the -1
-                    const float p = (exp2_fast(c.picked2[row] - lse2) - 1.0f) * (PLANES == 2 ? kGradScale : 1.0f);
-                    if (PLANES == 1) {
-                        reinterpret_cast<__nv_bfloat16 *>(g)[label] = __float2bfloat16_rn(p);
-                    } else {
-                        const __half p0 = __float2half_rn(p);
-                        reinterpret_cast<__half *>(g)[label] = p0;
-                        reinterpret_cast<__half *>(g + plane)[label] = __float2half_rn(p - __half2float(p0));
-                    }
-                }
             } else {
-                const bool last = KIND == kWeightGrad && c.gw != nullptr;
                 if (KIND == kWeightGrad && t.n0 == 0 && half == 0 && (c.gb != nullptr || c.bias_out != nullptr)) {
                     uint32_t one;
                     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];"
@@ -372,7 +435,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                     const float s = there ? __uint_as_float(one) : 0.f;
                     if (row < u.m) {
                         if (c.bias_out) {
-                            float *o = c.bias_out + t.split * c.bias_split + row;
+                            float *o = c.bias_out + t.split * c.classes + c.cls0 + row;
                             *o = c.add ? *o + s : s;
                         } else if (c.gb_f32) {
                             static_cast<float *>(c.gb)[c.cls0 + row] = s * c.scale;
@@ -381,6 +444,8 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         }
                     }
                 }
+                const bool direct = KIND == kWeightGrad && c.direct, wide = direct && c.direct_bf16;
+                const int y0 = t.m0 + quarter * 32 + (KIND == kWeightGrad ? c.cls0 : 0);
 #pragma unroll 1
                 for (int j = 0; j < 4; ++j) {
                     const int k0 = t.n0 + half * 128 + 32 * j;
@@ -391,57 +456,42 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = 0.f;
                     }
-                    if (row < u.m && !last) {  // partial sums: rows of out_ld floats, a multiple of 32
-                        float4 *o = reinterpret_cast<float4 *>(c.out + t.split * c.out_split + (int64_t)row * c.out_ld + k0);
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            float4 w = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                            if (c.add) {
-                                const float4 old = o[q];
-                                w.x += old.x, w.y += old.y, w.z += old.z, w.w += old.w;
-                            }
-                            o[q] = w;
-                        }
-                    } else if (row < u.m) {
+                    if (direct) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] *= c.scale;
-                        if (c.col_scale) {
+                        if (PLANES == 2) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (k0 + e < u.n) v[e] *= __ldg(c.col_scale + k0 + e);
-                        }
-                        const int64_t at = (int64_t)(c.cls0 + row) * c.gw_ld + k0;
-                        const bool whole = k0 + 32 <= u.n;
-                        if (c.gw_f32) {
-                            float *o = static_cast<float *>(c.gw) + at;
-                            if (whole && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
-#pragma unroll
-                                for (int q = 0; q < 8; ++q)
-                                    reinterpret_cast<float4 *>(o)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (k0 + e < u.n) o[e] = v[e];
-                            }
-                        } else {
-                            __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(c.gw) + at;
-                            if (whole && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    uint4 w;
-                                    uint32_t *pw = reinterpret_cast<uint32_t *>(&w);
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) pw[e] = pack16<__nv_bfloat16>(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
-                                    reinterpret_cast<uint4 *>(o)[q] = w;
-                                }
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (k0 + e < u.n) o[e] = __float2bfloat16_rn(v[e]);
+                            for (int e = 0; e < 32; ++e) {
+                                float up, down;
+                                plane_scale(__uint_as_float(k0 + e < u.n ? __ldg(c.col_largest + k0 + e) : 0u), up, down);
+                                v[e] *= down;
                             }
                         }
                     }
-                    __syncwarp();
+                    if (!wide || (j & 1) == 0) box_free();
+                    if (!wide) {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            *reinterpret_cast<float4 *>(box_row + (q ^ (lane & 7)) * 16) =
+                                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint4 w;
+                            uint32_t *pw = reinterpret_cast<uint32_t *>(&w);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) pw[e] = pack16<__nv_bfloat16>(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
+                            *reinterpret_cast<uint4 *>(box_row + (((j & 1) * 4 + q) ^ (lane & 7)) * 16) = w;
+                        }
+                        if ((j & 1) == 0 && k0 + 32 < u.n) continue;  // 64 columns a box
+                    }
+                    box_done();
+                    if (lane == 0 && (KIND != kWeightGrad || y0 < c.classes)) {
+                        const int x0 = wide ? t.n0 + half * 128 + 64 * (j >> 1) : k0;
+                        if (c.add) tma_add(&c.o, box, x0, y0, t.split);
+                        else tma_store(&c.o, box, x0, y0, t.split);
+                        store_commit();
+                    }
                 }
             }
             tc_fence_before();
@@ -449,6 +499,8 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
             if (lane == 0) bar_arrive(acc_empty + acc);
             if (++acc == kAcc) acc = 0, acc_phase ^= 1;
         }
+        if (KIND != kLogitStats && lane == 0) store_wait_all();
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();

@@ -18,6 +18,14 @@ namespace sgnn {
 int umma_tensor_map(CUtensorMap *map, const void *base, bool bf16, int64_t cols, int64_t rows, int64_t ld, int planes,
                     int64_t plane_stride, int box_rows);
 
+// A matrix of elements of 1, 2 or 4 bytes as boxes of `box_cols` x `box_rows` that lie in shared memory row after row
+int raw_tensor_map(CUtensorMap *map, const void *base, int elem_bytes, int64_t cols, int64_t rows, int64_t ld, int box_cols, int box_rows);
+
+// Results that leave a warp as 32 rows of `box_cols` columns (128 or 64 bytes a row, swizzled as wide)
+enum class StoreType { kF32, kBf16, kF16 };
+int umma_store_map(CUtensorMap *map, void *base, StoreType type, int64_t cols, int64_t rows, int64_t ld, int planes,
+                   int64_t plane_stride, int box_cols);
+
 #ifdef __CUDACC__
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -86,6 +94,25 @@ __device__ __forceinline__ void tma_prefetch(const CUtensorMap *map)
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
+// A box in shared memory to global memory, or added to what is there; boxes are cut off at the extents.  The issuing
+// thread waits with store_wait_read before the box is written again and with store_wait_all before it leaves.
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, const void *src, int x, int y, int z)
+{
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(smem_addr(src))
+                 : "memory");
+}
+__device__ __forceinline__ void tma_add(const CUtensorMap *map, const void *src, int x, int y, int z)
+{
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x),
+                 "r"(y), "r"(z), "r"(smem_addr(src))
+                 : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 __device__ __forceinline__ void tmem_alloc(uint32_t *slot, int cols)
 {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols) : "memory");
@@ -113,6 +140,12 @@ __device__ __forceinline__ uint64_t umma_desc(const void *p, unsigned run_bytes,
 {
     return (uint64_t)((smem_addr(p) & 0x3FFFFu) >> 4) | ((uint64_t)(run_bytes >> 4) << 16) | ((uint64_t)(group_bytes >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
+}
+
+// A 16-byte run that every row of an operand reads (16 rows x 16 steps, no swizzle, all strides zero)
+__device__ __forceinline__ uint64_t umma_desc_same(const void *p)
+{
+    return (uint64_t)((smem_addr(p) & 0x3FFFFu) >> 4) | (1ull << 46);
 }
 
 // 128 x n product of 16-bit operands with fp32 sums
