@@ -13,7 +13,7 @@
 // eight warps convert them into the swizzled operands, both "MN-major" (the rows of g and of the codes are the reduction),
 // which keeps the order of the matrices; one thread issues the products.  Tensor memory rounds every addition
 // towards zero, which over thousands of rows would shrink the result by 1e-5 of itself, so after 512 rows the sums move on
-// into fp32 registers (the other half of the tensor memory takes over meanwhile).  The partial results of the row ranges
+// into the fp32 registers of eight other warps (the other half of the tensor memory takes over meanwhile).  The partial results of the row ranges
 // are added in a fixed order.
 #include "row_io.cuh"
 #include "umma.cuh"
@@ -21,15 +21,16 @@
 namespace sgnn {
 
 constexpr int kGM = 128, kGN = 256, kGRows = 32;  // results of a block, rows a step
-constexpr int kGWorkers = 8;                      // warps that convert and add up
-constexpr int kGThreads = (kGWorkers + 2) * 32;
+constexpr int kGKeepers = 8;                      // warps that hold the sums
+constexpr int kGWorkers = 8;                      // warps that convert
+constexpr int kGThreads = (kGKeepers + kGWorkers + 4) * 32;  // and a group of four: one feeds, one issues the products
 constexpr int kGRaw = 3, kGStages = 4;            // buffers of operands as they come, and converted
 constexpr int kGPromote = 16;                     // steps between two moves into registers
 constexpr int kGPlane = kGM * kGRows * 2, kGCodes = kGN * kGRows * 2;
 constexpr int kGStageBytes = 2 * kGPlane + kGCodes;
 
 struct GradCall {
-    CUtensorMap g, codes;
+    CUtensorMap g, codes, zs;  // zs: params as one long row
     const void *g_ptr;
     int64_t ldg;
     const uint8_t *code_ptr;
@@ -43,10 +44,18 @@ struct GradCall {
     int *failed;
 };
 
-template <class T>
-constexpr int grad_raw_bytes() { return kGRows * (kGM * (int)sizeof(T) + kGN); }
-template <class T, bool TMA>
-constexpr int grad_shared_bytes() { return kGStages * kGStageBytes + (TMA ? kGRaw * grad_raw_bytes<T>() : 16 * kGM * 4) + 256; }
+// What TMA brings: neither g nor the codes (and parameters), the codes, both.  The threads load the rest themselves.
+enum GradFeed { kFeedNone, kFeedCodes, kFeedBoth };
+template <class T, int FEED>
+constexpr int grad_raw_bytes() { return FEED == kFeedNone ? 0 : kGRows * ((FEED == kFeedBoth ? kGM * (int)sizeof(T) : 0) + kGN + 8); }
+template <class T, int FEED>
+constexpr int grad_raw_area()
+{
+    const int ring = kGRaw * grad_raw_bytes<T, FEED>(), share = kGRows / 2 * kGM * 4;  // the shares of the zero points go there last
+    return ring > share ? ring : share;
+}
+template <class T, int FEED>
+constexpr int grad_shared_bytes() { return kGStages * kGStageBytes + grad_raw_area<T, FEED>() + 256; }
 
 // Eight codes -> eight bf16 values, exact.  A code c in the low byte below 0x43 reads as 128 + c for c < 128 and as 2 c from
 // there on; c is the smaller of that minus 128 and half of it.
@@ -65,6 +74,31 @@ __device__ __forceinline__ uint4 code_values(uint2 c)
     return out;
 }
 
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// eight values times sc as two bf16 terms each, hi + lo
+__device__ __forceinline__ void two_terms(const float (&v)[8], float sc, uint4 &hi, uint4 &lo)
+{
+    uint32_t *ph = reinterpret_cast<uint32_t *>(&hi), *pl = reinterpret_cast<uint32_t *>(&lo);
+    const unsigned long long sc2 = pk2(sc, sc);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned long long x2 = mul2(pk2(v[2 * e], v[2 * e + 1]), sc2);
+        float x, y;
+        unpk2(x2, x, y);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        ph[e] = *reinterpret_cast<const uint32_t *>(&h);
+        unpk2(sub2(x2, pk2(__uint_as_float(ph[e] << 16), __uint_as_float(ph[e] & 0xFFFF0000u))), x, y);
+        const __nv_bfloat162 l = __floats2bfloat162_rn(x, y);
+        pl[e] = *reinterpret_cast<const uint32_t *>(&l);
+    }
+}
+
 template <class T>
 __device__ __forceinline__ void unpack8(const uint4 *p, float (&v)[8])
 {
@@ -79,12 +113,13 @@ __device__ __forceinline__ void unpack8(const uint4 *p, float (&v)[8])
     }
 }
 
-template <class T, bool TMA>
+template <class T, int FEED>
 __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_constant__ GradCall c)
 {
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *raw = base + kGStages * kGStageBytes;
-    constexpr int kRawBytes = grad_raw_bytes<T>(), kRawArea = TMA ? kGRaw * kRawBytes : 16 * kGM * 4;
+    constexpr int kRawBytes = grad_raw_bytes<T, FEED>(), kRawArea = grad_raw_area<T, FEED>();
+    constexpr int kRawG = FEED == kFeedBoth ? kGRows * kGM * (int)sizeof(T) : 0;  // g first, then the codes, then the parameters
     uint64_t *raw_full = reinterpret_cast<uint64_t *>(raw + kRawArea), *raw_empty = raw_full + kGRaw;
     uint64_t *full = raw_empty + kGRaw, *empty = full + kGStages, *acc_full = empty + kGStages, *acc_empty = acc_full + 2;
     uint64_t *drained = acc_empty + 2;
@@ -104,31 +139,39 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     if (threadIdx.x == 0) {
         for (int s = 0; s < kGRaw; ++s) bar_init(raw_full + s, 1), bar_init(raw_empty + s, kGWorkers);
         for (int s = 0; s < kGStages; ++s) bar_init(full + s, kGWorkers), bar_init(empty + s, 1);
-        for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, kGWorkers);
+        for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, kGKeepers);
         bar_init(drained, 1);
         *gone = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kGWorkers + 1) tmem_alloc(slot, 512);
+    if (warp == kGKeepers + kGWorkers + 1) tmem_alloc(slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
 
-    if (warp == kGWorkers) {
+    // Registers follow the work: the 20 warps are launched with 96 each, 8 x 152 + 8 x 64 + 4 x 48 = 20 x 96.
+    if (warp < kGKeepers) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    else if (warp < kGKeepers + kGWorkers) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+
+    if (warp == kGKeepers + kGWorkers) {
         // ---- loads ----
-        if (TMA && lane == 0) {
-            tma_prefetch(&c.g);
+        if (FEED != kFeedNone && lane == 0) {
+            if (FEED == kFeedBoth) tma_prefetch(&c.g);
             tma_prefetch(&c.codes);
+            tma_prefetch(&c.zs);
             int s = 0, done = 0;
             unsigned phase = 0;
+#pragma unroll 1
             for (; done < count; ++done) {
                 if (!bar_wait(raw_empty + s, phase ^ 1, gone)) break;
                 uint8_t *at = raw + s * kRawBytes;
                 const int r0 = (first + done) * kGRows;
                 bar_expect(raw_full + s, kRawBytes);
-                tma_load(at, &c.g, m0, r0, 0, raw_full + s);
-                tma_load(at + kGRows * kGM * sizeof(T), &c.codes, n0, r0, 0, raw_full + s);
+                if (FEED == kFeedBoth) tma_load(at, &c.g, m0, r0, 0, raw_full + s);
+                tma_load(at + kRawG, &c.codes, n0, r0, 0, raw_full + s);
+                tma_load(at + kRawG + kGRows * kGN, &c.zs, 2 * r0, 0, 0, raw_full + s);
                 if (++s == kGRaw) s = 0, phase ^= 1;
             }
             if (done < count) {
@@ -136,7 +179,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             }
         }
         __syncwarp();
-    } else if (warp == kGWorkers + 1) {
+    } else if (warp == kGKeepers + kGWorkers + 1) {
         // ---- products ----
         if (lane == 0) {
             const int left = c.F - n0, n = left < kGN ? (left + 15) / 16 * 16 : kGN;
@@ -144,6 +187,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             int s = 0;
             unsigned phase = 0;
             bool ok = true;
+#pragma unroll 1
             for (int k = 0; k < count; ++k) {
                 const int round = k / kGPromote, acc = round & 1;
                 if (k % kGPromote == 0) {
@@ -174,132 +218,35 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             }
         }
         __syncwarp();
-    } else {
-        // ---- conversion, and the sums ----
-        const int tid = threadIdx.x;
-        const int q = tid & 15, ra = tid >> 4;   // of g: eight columns, rows ra and ra + 16
-        const int mq = m0 + q * 8, nq = n0 + lane * 8;  // of the codes: eight columns, rows warp, warp + 8, ...
-        const int quarter = warp & 3, half = warp >> 2;
+    } else if (warp < kGKeepers) {
+        // ---- the sums ----
+        const int quarter = warp & 3, half = warp >> 2;  // 32 rows, 128 columns of the results
         float sum[128];
 #pragma unroll
         for (int e = 0; e < 128; ++e) sum[e] = 0.f;
-        float zero[8] = {};  // sum of g zp over this thread's rows
-        int s = 0, t = 0, taken = 0;
-        unsigned phase = 0, raw_phase = 0;
-        bool ok = true;
-        // operands of a step that come without TMA, one step ahead
-        float gv[2][8];
-        uint2 cv[4];
-        float2 pv[2];
-        const auto fetch = [&](int k) {
-            const int64_t r0 = (int64_t)(first + k) * kGRows;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t r = r0 + ra + 16 * i;
-                pv[i] = r < c.n ? __ldg(c.params + r) : make_float2(0.f, 0.f);
-                if constexpr (!TMA) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        gv[i][e] = r < c.n && mq + e < c.M ? to_f32<T>(static_cast<const T *>(c.g_ptr)[r * c.ldg + mq + e]) : 0.f;
-                }
-            }
-            if constexpr (!TMA) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t r = r0 + warp + 8 * i;
-                    uint8_t b[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) b[e] = r < c.n && nq + e < c.F ? c.code_ptr[r * c.ldc + nq + e] : (uint8_t)0;
-                    cv[i].x = b[0] | b[1] << 8 | b[2] << 16 | (uint32_t)b[3] << 24;
-                    cv[i].y = b[4] | b[5] << 8 | b[6] << 16 | (uint32_t)b[7] << 24;
-                }
-            }
-        };
-        // moves the sums of a round into registers
-        const auto promote = [&](int round) {
+#pragma unroll 1
+        for (int round = 0; round < rounds; ++round) {
             const int acc = round & 1;
-            if (!bar_wait(acc_full + acc, (round >> 1) & 1, gone)) return false;
+            if (!bar_wait(acc_full + acc, (round >> 1) & 1, gone)) break;
             tc_fence_after();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float v[32];
-                tmem_load32(tmem + acc * kGN + half * 128 + 32 * j + ((uint32_t)quarter << 21), v);
+            for (int j = 0; j < 8; ++j) {
+                float v[16];
+                tmem_load16(tmem + acc * kGN + half * 128 + 16 * j + ((uint32_t)quarter << 21), v);
                 tmem_load_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) sum[32 * j + e] += v[e];
+                for (int e = 0; e < 16; ++e) sum[16 * j + e] += v[e];
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(acc_empty + acc);
-            return true;
-        };
-        fetch(0);
-        for (int k = 0; k < count && ok; ++k) {
-            const uint8_t *in = raw + s * kRawBytes;
-            if (TMA) {
-                ok = bar_wait(raw_full + s, raw_phase, gone);
-                if (!ok) break;
-            }
-            ok = bar_wait(empty + t, phase ^ 1, gone);
-            if (!ok) break;
-            uint8_t *at = base + t * kGStageBytes;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = ra + 16 * i;
-                float v[8];
-                if constexpr (TMA) {
-                    unpack8<T>(reinterpret_cast<const uint4 *>(in + (r * kGM + q * 8) * sizeof(T)), v);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = gv[i][e];
-                }
-                const float sc = pv[i].y, zp = pv[i].x;
-                uint4 hi, lo;
-                uint32_t *ph = reinterpret_cast<uint32_t *>(&hi), *pl = reinterpret_cast<uint32_t *>(&lo);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    zero[2 * e] = __fmaf_rn(v[2 * e], zp, zero[2 * e]);
-                    zero[2 * e + 1] = __fmaf_rn(v[2 * e + 1], zp, zero[2 * e + 1]);
-                    const float x = v[2 * e] * sc, y = v[2 * e + 1] * sc;
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-                    const float2 hf = __bfloat1622float2(h);
-                    const __nv_bfloat162 l = __floats2bfloat162_rn(x - hf.x, y - hf.y);
-                    ph[e] = *reinterpret_cast<const uint32_t *>(&h);
-                    pl[e] = *reinterpret_cast<const uint32_t *>(&l);
-                }
-                uint8_t *o = at + (q >> 3) * (kGRows * 128) + r * 128 + ((q & 7) ^ (r & 7)) * 16;
-                *reinterpret_cast<uint4 *>(o) = hi;
-                *reinterpret_cast<uint4 *>(o + kGPlane) = lo;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = warp + 8 * i;
-                const uint2 code = TMA ? *reinterpret_cast<const uint2 *>(in + kGRows * kGM * sizeof(T) + r * kGN + lane * 8) : cv[i];
-                *reinterpret_cast<uint4 *>(at + 2 * kGPlane + (lane >> 3) * (kGRows * 128) + r * 128 + ((lane & 7) ^ (r & 7)) * 16) = code_values(code);
-            }
-            if (k + 1 < count) fetch(k + 1);
-            async_fence();
-            __syncwarp();
-            if (lane == 0) {
-                bar_arrive(full + t);
-                if (TMA) bar_arrive(raw_empty + s);
-            }
-            if (++t == kGStages) t = 0, phase ^= 1;
-            if (++s == kGRaw) s = 0, raw_phase ^= 1;
-            // half a round later its products are done, and the next round's still have work in front of them
-            if (k % kGPromote == kGPromote / 2 && k > kGPromote) ok = promote(taken++);
         }
-        while (ok && taken < rounds) ok = promote(taken++);
-        // the zero points' share of every column, over the sixteen row groups
-        float *share = reinterpret_cast<float *>(raw);  // [16][128]: every buffer of operands has been read
-        asm volatile("bar.sync 1, %0;" ::"n"(kGWorkers * 32) : "memory");
-#pragma unroll
-        for (int e = 0; e < 8; ++e) share[ra * kGM + q * 8 + e] = zero[e];
-        asm volatile("bar.sync 1, %0;" ::"n"(kGWorkers * 32) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
+        const float *share = reinterpret_cast<const float *>(raw);
         const int m = quarter * 32 + lane;
         float own = 0.f;
 #pragma unroll
-        for (int g = 0; g < 16; ++g) own += share[g * kGM + m];
+        for (int g = 0; g < kGRows / 2; ++g) own += share[g * kGM + m];
         if (m0 + m < c.M) {
             float *o = c.partials + ((int64_t)split * c.M + m0 + m) * c.ld + n0 + half * 128;
 #pragma unroll
@@ -308,12 +255,103 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                     *reinterpret_cast<float4 *>(o + e) = make_float4(sum[e] + own, sum[e + 1] + own, sum[e + 2] + own, sum[e + 3] + own);
             }
         }
+    } else if (warp < kGKeepers + kGWorkers) {
+        // ---- conversion ----
+        const int tid = threadIdx.x - kGKeepers * 32, w = warp - kGKeepers;
+        const int q = tid & 15, ra = tid >> 4;          // of g: eight columns, rows ra and ra + 16
+        const int mq = m0 + q * 8, nq = n0 + lane * 8;  // of the codes: eight columns, rows w, w + 8, ...
+        unsigned long long zero[4] = {};  // sum of g zp over this thread's rows, two columns each
+        int s = 0, t = 0;
+        unsigned phase = 0, raw_phase = 0;
+        // operands of a step that come without TMA, one step ahead
+        float gv[2][8];
+        uint2 cv[4];
+        float2 pv[2];
+        const auto fetch = [&](int k) {
+            const int64_t r0 = (int64_t)(first + k) * kGRows;
+            if constexpr (FEED != kFeedBoth) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int64_t r = r0 + ra + 16 * i;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        gv[i][e] = r < c.n && mq + e < c.M ? to_f32<T>(static_cast<const T *>(c.g_ptr)[r * c.ldg + mq + e]) : 0.f;
+                }
+            }
+            if constexpr (FEED == kFeedNone) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int64_t r = r0 + ra + 16 * i;
+                    pv[i] = r < c.n ? __ldg(c.params + r) : make_float2(0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = r0 + w + 8 * i;
+                    uint8_t b[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) b[e] = r < c.n && nq + e < c.F ? c.code_ptr[r * c.ldc + nq + e] : (uint8_t)0;
+                    cv[i].x = b[0] | b[1] << 8 | b[2] << 16 | (uint32_t)b[3] << 24;
+                    cv[i].y = b[4] | b[5] << 8 | b[6] << 16 | (uint32_t)b[7] << 24;
+                }
+            }
+        };
+        fetch(0);
+#pragma unroll 1
+        for (int k = 0; k < count; ++k) {
+            const uint8_t *in = raw + s * kRawBytes;
+            if (FEED != kFeedNone && !bar_wait(raw_full + s, raw_phase, gone)) break;
+            if (!bar_wait(empty + t, phase ^ 1, gone)) break;
+            uint8_t *at = base + t * kGStageBytes;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = ra + 16 * i;
+                float v[8];
+                float2 par;
+                if constexpr (FEED == kFeedNone) par = pv[i];
+                else par = *reinterpret_cast<const float2 *>(in + kRawG + kGRows * kGN + r * 8);
+                if constexpr (FEED == kFeedBoth) {
+                    unpack8<T>(reinterpret_cast<const uint4 *>(in + (r * kGM + q * 8) * sizeof(T)), v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = gv[i][e];
+                }
+                const unsigned long long zp2 = pk2(par.x, par.x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) zero[e] = fma2(pk2(v[2 * e], v[2 * e + 1]), zp2, zero[e]);
+                uint4 hi, lo;
+                two_terms(v, par.y, hi, lo);
+                uint8_t *o = at + (q >> 3) * (kGRows * 128) + r * 128 + ((q & 7) ^ (r & 7)) * 16;
+                *reinterpret_cast<uint4 *>(o) = hi;
+                *reinterpret_cast<uint4 *>(o + kGPlane) = lo;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = w + 8 * i;
+                const uint2 code = FEED == kFeedNone ? cv[i] : *reinterpret_cast<const uint2 *>(in + kRawG + r * kGN + lane * 8);
+                *reinterpret_cast<uint4 *>(at + 2 * kGPlane + (lane >> 3) * (kGRows * 128) + r * 128 + ((lane & 7) ^ (r & 7)) * 16) = code_values(code);
+            }
+            if (FEED != kFeedBoth && k + 1 < count) fetch(k + 1);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) {
+                bar_arrive(full + t);
+                if (FEED != kFeedNone) bar_arrive(raw_empty + s);
+            }
+            if (++t == kGStages) t = 0, phase ^= 1;
+            if (++s == kGRaw) s = 0, raw_phase ^= 1;
+        }
+        // the zero points' share of every column, [16][128]: every buffer of operands as they come has been read by then
+        asm volatile("bar.sync 2, %0;" ::"n"(kGWorkers * 32) : "memory");
+        float *share = reinterpret_cast<float *>(raw);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) unpk2(zero[e], share[ra * kGM + q * 8 + 2 * e], share[ra * kGM + q * 8 + 2 * e + 1]);
+        asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (threadIdx.x == 0 && *gone) atomicExch(c.failed, 1);
-    if (warp == kGWorkers + 1) tmem_free(tmem, 512);
+    if (warp == kGKeepers + kGWorkers + 1) tmem_free(tmem, 512);
 }
 
 // out = sum of the partial results, in their order, + beta out: 32 columns a block row, the splits dealt over eight warps
@@ -367,12 +405,12 @@ static GradPlan weight_grad_plan(int64_t n, int64_t M, int64_t F)
     return p;
 }
 
-template <class T, bool TMA>
+template <class T, int FEED>
 static int weight_grad_launch(const GradCall &c, const GradPlan &p, cudaStream_t s)
 {
-    constexpr int smem = grad_shared_bytes<T, TMA>();
-    SGNN_CUDA_OK(cudaFuncSetAttribute(weight_grad_kernel<T, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    weight_grad_kernel<T, TMA><<<(unsigned)(p.tiles_m * p.tiles_n * p.splits), kGThreads, smem, s>>>(c);
+    constexpr int smem = grad_shared_bytes<T, FEED>();
+    SGNN_CUDA_OK(cudaFuncSetAttribute(weight_grad_kernel<T, FEED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    weight_grad_kernel<T, FEED><<<(unsigned)(p.tiles_m * p.tiles_n * p.splits), kGThreads, smem, s>>>(c);
     SGNN_LAUNCH_OK("checkpoint_weight_grad");
     return SGNN_OK;
 }
@@ -387,12 +425,19 @@ static int weight_grad_run(const void *g, int64_t ldg, const uint8_t *codes, int
     c.failed = static_cast<int *>(ws), c.partials = reinterpret_cast<float *>(static_cast<char *>(ws) + 256);
     SGNN_CUDA_OK(cudaMemsetAsync(c.failed, 0, 4, s));
     int rc;
-    if (n > 1 && aligned16(g) && ldg * sizeof(T) % 16 == 0 && aligned16(codes) && ldc % 16 == 0) {
-        if ((rc = raw_tensor_map(&c.g, g, sizeof(T), M, n, ldg, kGM, kGRows))) return rc;
+    const bool codes_fed = n > 1 && n <= (1ll << 29) && aligned16(codes) && ldc % 16 == 0 && aligned16(params);
+    const bool g_fed = codes_fed && aligned16(g) && ldg * sizeof(T) % 16 == 0;
+    if (codes_fed) {
+        if ((rc = raw_tensor_map(&c.zs, params, 4, 2 * n, 1, ceil_div(n, 2) * 4, 2 * kGRows, 1))) return rc;
         if ((rc = raw_tensor_map(&c.codes, codes, 1, F, n, ldc, kGN, kGRows))) return rc;
-        rc = weight_grad_launch<T, true>(c, p, s);
+    }
+    if (g_fed) {
+        if ((rc = raw_tensor_map(&c.g, g, sizeof(T), M, n, ldg, kGM, kGRows))) return rc;
+        rc = weight_grad_launch<T, kFeedBoth>(c, p, s);
+    } else if (codes_fed) {
+        rc = weight_grad_launch<T, kFeedCodes>(c, p, s);
     } else {
-        rc = weight_grad_launch<T, false>(c, p, s);
+        rc = weight_grad_launch<T, kFeedNone>(c, p, s);
     }
     if (rc) return rc;
     const dim3 grid((unsigned)ceil_div(F, 32), (unsigned)(M < 65535 ? M : 65535));
