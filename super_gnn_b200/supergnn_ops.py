@@ -985,49 +985,95 @@ def softmax_nll_loss(logits, bias, labels, mask, inv_count: float, grad=None):
 # ---------------------------------------------------------------------------
 # layer norm, 8-bit activation checkpoints, many-class loss
 # ---------------------------------------------------------------------------
+# The smallest of these calls take microseconds on the device, so the wrappers below test first and build messages only
+# for what failed, and ask for the device and its stream the cheap way.
 _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # torch.cuda.current_stream without the object
 
 
-def _element(t, name, allowed=(torch.float32, torch.bfloat16, torch.float16)) -> int:
-    _need(t.dtype in allowed, f"{name} must be one of {', '.join(str(a) for a in allowed)}, got {t.dtype}")
-    return _ELEMENT[t.dtype]
+def _stream_on(dev) -> int:
+    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+class _NoSwitch:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def _on(dev):
+    """Context in which ``dev`` is the current device."""
+    return _NO_SWITCH if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _matrix(t, name, allowed=_ELEMENT) -> int:
+    """Checks a 2-d CUDA tensor with at least one column; its element code."""
+    code = allowed.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 else None
+    if code is None or t.size(1) == 0:
+        _cuda(t, name, None, 2)
+        _need(t.dtype in allowed, f"{name} must be one of {', '.join(str(a) for a in allowed)}, got {t.dtype}")
+        _need(False, f"{name} must have at least one column")
+    return code
 
 
 def _row_major(t):
     """``t`` with contiguous rows that do not overlap; anything else (a transposed or an expanded tensor, such as the
     gradient of a sum) is copied."""
+    if t.is_contiguous():
+        return t
     n, width = t.shape
     return t if (width <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= width) else t.contiguous()
 
 
-def _params_of(x, named, width):
-    """Element code of the parameter vectors ``named`` = [(tensor or None, name), ...] of ``width`` entries."""
-    code, dtype = 0, None
-    for t, name in named:
-        if t is None:
-            continue
+def _vector(t, name, dtype, width, dev) -> int:
+    """Checks a contiguous parameter vector (or None) that is fp32 or ``dtype``; its element code."""
+    if t is None:
+        return 0
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 1 and t.numel() == width and t.is_contiguous()
+            and (t.dtype == dtype or t.dtype == torch.float32) and t.device == dev):
         _cuda(t, name, None, 1)
         _need(t.numel() == width and t.is_contiguous(), f"{name} must be a contiguous [{width}] tensor")
-        _need(t.dtype in (torch.float32, x.dtype), f"{name} must be float32 or {x.dtype}, got {t.dtype}")
-        _need(dtype in (None, t.dtype), f"{' and '.join(nm for _, nm in named)} must have one type")
-        dtype, code = t.dtype, _ELEMENT[t.dtype]
-    return code
+        _need(t.dtype in (torch.float32, dtype), f"{name} must be float32 or {dtype}, got {t.dtype}")
+        _need(False, "all tensors must be on the same CUDA device")
+    return _ELEMENT[t.dtype]
 
 
 def _new_codes(n, width, device):
     """Codes and parameters of an 8-bit checkpoint; the rows are padded to 16 bytes."""
     pitch = -(-width // 16) * 16
-    return (torch.empty((n, pitch), dtype=torch.uint8, device=device)[:, :width],
-            torch.empty((n, 2), dtype=torch.float32, device=device))
+    codes = torch.empty((n, pitch), dtype=torch.uint8, device=device)
+    return (codes if pitch == width else codes[:, :width]), torch.empty((n, 2), dtype=torch.float32, device=device)
+
+
+def _pairs(t, name, n, dev):
+    """Checks a contiguous fp32 [n, 2] tensor."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.dim() == 2 and t.size(0) == n
+            and t.size(1) == 2 and t.is_contiguous() and t.device == dev):
+        _cuda(t, name, torch.float32, 2)
+        _need(tuple(t.shape) == (n, 2) and t.is_contiguous(), f"{name} must be a contiguous [{n}, 2] tensor")
+        _need(False, "all tensors must be on the same CUDA device")
+
+
+_CODES = {torch.uint8: 0}
 
 
 def _checkpoint_args(codes, params):
-    _cuda(codes, "codes", torch.uint8, 2)
-    _cuda(params, "params", torch.float32, 2)
-    n, width = codes.shape
-    _need(width > 0, "codes must have at least one column")
-    _need(tuple(params.shape) == (n, 2) and params.is_contiguous(), "params must be a contiguous [rows, 2] tensor")
+    _matrix(codes, "codes", _CODES)
+    _pairs(params, "params", codes.size(0), codes.device)
     return _row_major(codes)
+
+
+def _result(out, name, n, width, dtype, dev):
+    """Checks a caller's result: [n, width] of ``dtype`` with contiguous rows that do not overlap."""
+    _cuda(out, name, dtype, 2)
+    _need(tuple(out.shape) == (n, width) and (width <= 1 or out.stride(1) == 1) and (n <= 1 or out.stride(0) >= width),
+          f"{name} must be [{n}, {width}] with contiguous rows")
+    _need(out.device == dev, "all tensors must be on the same CUDA device")
 
 
 def layer_norm_forward(x, gamma=None, beta=None, eps: float = 1e-5, checkpoint: bool = False, out=None):
@@ -1035,57 +1081,62 @@ def layer_norm_forward(x, gamma=None, beta=None, eps: float = 1e-5, checkpoint: 
     and beta fp32 or of x's type, or None).  Returns ``(y, stats)`` with ``stats`` [n, 2] = (mean, reciprocal standard
     deviation) in fp32, and with ``checkpoint`` ``(y, stats, codes, params)``: the 8-bit checkpoint of ``x``, written in
     the same pass (see :func:`checkpoint_pack_rows`)."""
-    _cuda(x, "x", None, 2)
-    code = _element(x, "x")
+    code = _matrix(x, "x")
     n, H = x.shape
-    _need(H > 0, "x must have at least one column")
-    pcode = _params_of(x, [(gamma, "gamma"), (beta, "beta")], H)
-    if out is None:
-        out = torch.empty((n, H), dtype=x.dtype, device=x.device)
-    _cuda(out, "out", x.dtype, 2)
-    _need(tuple(out.shape) == (n, H) and (H <= 1 or out.stride(1) == 1) and (n <= 1 or out.stride(0) >= H),
-          "out must be [n, H] with contiguous rows")
-    _same_device(x, gamma, beta, out)
+    dev, dtype = x.device, x.dtype
+    pcode = _vector(gamma, "gamma", dtype, H, dev)
+    bcode = _vector(beta, "beta", dtype, H, dev)
+    if gamma is None:
+        pcode = bcode
+    elif beta is not None and pcode != bcode:
+        raise RuntimeError("gamma and beta must have one type")
     x = _row_major(x)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device)
-    codes, params = _new_codes(n, H, x.device) if checkpoint else (None, None)
-    with torch.cuda.device(x.device), _Logged("layer_norm_fwd", x.device, n=n, H=H):
-        rc = _cabi.lib().sgnn_layer_norm_forward(code, _ptr(x), x.stride(0), pcode, _ptr(gamma), _ptr(beta), float(eps),
-                                                 _ptr(out), out.stride(0), _ptr(stats), _ptr(codes),
-                                                 codes.stride(0) if checkpoint else 0, _ptr(params), n, H, _stream(x))
-    _cabi.check(rc, "layer_norm_forward")
+    if out is None:
+        out = torch.empty_like(x) if x.is_contiguous() else torch.empty((n, H), dtype=dtype, device=dev)
+    else:
+        _result(out, "out", n, H, dtype, dev)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=dev)
+    codes, params = _new_codes(n, H, dev) if checkpoint else (None, None)
+    with _on(dev), _Logged("layer_norm_fwd", dev, n=n, H=H):
+        rc = _cabi.lib().sgnn_layer_norm_forward(code, x.data_ptr(), x.stride(0), pcode, _ptr(gamma), _ptr(beta), eps,
+                                                 out.data_ptr(), out.stride(0), stats.data_ptr(), _ptr(codes),
+                                                 codes.stride(0) if checkpoint else 0, _ptr(params), n, H, _stream_on(dev))
+    if rc:
+        _cabi.check(rc, "layer_norm_forward")
     return (out, stats, codes, params) if checkpoint else (out, stats)
 
 
 def _layer_norm_backward(gy, x, codes, params, stats, gamma, in_place):
-    code = _element(gy, "gy")
+    code = _matrix(gy, "gy")
     n, H = gy.shape
-    _need(H > 0, "gy must have at least one column")
-    pcode = _params_of(gy, [(gamma, "gamma")], H)
-    _cuda(stats, "stats", torch.float32, 2)
-    _need(tuple(stats.shape) == (n, 2) and stats.is_contiguous(), "stats must be a contiguous [n, 2] tensor")
-    _same_device(gy, x, codes, params, stats, gamma)
+    dev, dtype = gy.device, gy.dtype
+    pcode = _vector(gamma, "gamma", dtype, H, dev)
+    _pairs(stats, "stats", n, dev)
+    if (codes if x is None else x).device != dev:
+        raise RuntimeError("all tensors must be on the same CUDA device")
     rows = _row_major(gy)
     _need(not in_place or rows is gy, "in_place needs gy with contiguous rows")
     gy = rows
-    gx = gy if in_place else torch.empty((n, H), dtype=gy.dtype, device=gy.device)
-    g_gamma = torch.empty(H, dtype=torch.float32 if gamma is None else gamma.dtype, device=gy.device)
-    g_beta = torch.empty_like(g_gamma)
+    gx = gy if in_place else torch.empty((n, H), dtype=dtype, device=dev)
+    grads = torch.empty((2, H), dtype=torch.float32 if gamma is None else gamma.dtype, device=dev)
+    g_gamma, g_beta = grads[0], grads[1]
     lib = _cabi.lib()
-    with torch.cuda.device(gy.device), _Logged("layer_norm_bwd", gy.device, n=n, H=H):
-        partials = torch.empty((int(lib.sgnn_layer_norm_blocks()), 2, H), dtype=torch.float32, device=gy.device)
-        rc = lib.sgnn_layer_norm_backward(code, _ptr(gy), gy.stride(0), _ptr(x), x.stride(0) if x is not None else 0,
+    with _on(dev), _Logged("layer_norm_bwd", dev, n=n, H=H):
+        partials = torch.empty((lib.sgnn_layer_norm_blocks(), 2, H), dtype=torch.float32, device=dev)
+        rc = lib.sgnn_layer_norm_backward(code, gy.data_ptr(), gy.stride(0), _ptr(x), x.stride(0) if x is not None else 0,
                                           _ptr(codes), codes.stride(0) if codes is not None else 0, _ptr(params),
-                                          _ptr(stats), pcode, _ptr(gamma), _ptr(gx), gx.stride(0), _ptr(g_gamma),
-                                          _ptr(g_beta), _ptr(partials), n, H, _stream(gy))
-    _cabi.check(rc, "layer_norm_backward")
+                                          stats.data_ptr(), pcode, _ptr(gamma), gx.data_ptr(), gx.stride(0),
+                                          g_gamma.data_ptr(), g_beta.data_ptr(), partials.data_ptr(), n, H,
+                                          _stream_on(dev))
+    if rc:
+        _cabi.check(rc, "layer_norm_backward")
     return gx, g_gamma, g_beta
 
 
 def layer_norm_backward(gy, x, stats, gamma=None, in_place: bool = False):
     """Gradients of :func:`layer_norm_forward` from the same ``x`` and its ``stats``: ``(gx, g_gamma, g_beta)``, the
     last two in gamma's type.  ``in_place``: ``gx`` overwrites ``gy``."""
-    _cuda(gy, "gy", None, 2)
+    _matrix(gy, "gy")
     _cuda(x, "x", gy.dtype, 2)
     _need(gy.shape == x.shape, "gy and x must have the same shape")
     return _layer_norm_backward(gy, _row_major(x), None, None, stats, gamma, in_place)
@@ -1093,7 +1144,7 @@ def layer_norm_backward(gy, x, stats, gamma=None, in_place: bool = False):
 
 def layer_norm_backward_checkpoint(gy, codes, params, stats, gamma=None, in_place: bool = False):
     """:func:`layer_norm_backward` with the 8-bit checkpoint of ``x`` in the place of ``x``."""
-    _cuda(gy, "gy", None, 2)
+    _matrix(gy, "gy")
     codes = _checkpoint_args(codes, params)
     _need(gy.shape == codes.shape, "gy and codes must have the same shape")
     return _layer_norm_backward(gy, None, codes, params, stats, gamma, in_place)
@@ -1103,97 +1154,108 @@ def checkpoint_pack_rows(x):
     """8-bit checkpoint of the rows of ``x`` [n, F] (fp32, bf16 or fp16): ``(codes, params)``, uint8 [n, F] and fp32
     [n, 2] = (zero_point, scale) with ``scale = (max - min) / 255`` and ``code = rne((x - min) / scale)`` for each row.
     A row that holds a NaN or an infinity, or whose range is above the largest fp32, is restored as NaN."""
-    _cuda(x, "x", None, 2)
-    code = _element(x, "x")
+    code = _matrix(x, "x")
     n, F = x.shape
-    _need(F > 0, "x must have at least one column")
+    dev = x.device
     x = _row_major(x)
-    codes, params = _new_codes(n, F, x.device)
-    with torch.cuda.device(x.device), _Logged("checkpoint_pack", x.device, n=n, F=F):
-        rc = _cabi.lib().sgnn_checkpoint_pack_rows(code, _ptr(x), x.stride(0), _ptr(codes), codes.stride(0), _ptr(params),
-                                                   n, F, _stream(x))
-    _cabi.check(rc, "checkpoint_pack_rows")
+    codes, params = _new_codes(n, F, dev)
+    with _on(dev), _Logged("checkpoint_pack", dev, n=n, F=F):
+        rc = _cabi.lib().sgnn_checkpoint_pack_rows(code, x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0),
+                                                   params.data_ptr(), n, F, _stream_on(dev))
+    if rc:
+        _cabi.check(rc, "checkpoint_pack_rows")
     return codes, params
 
 
 def checkpoint_unpack_rows(codes, params, dtype=torch.float32):
     """The values ``zero_point + scale * code`` that a checkpoint stands for, as a [n, F] tensor of ``dtype``."""
     codes = _checkpoint_args(codes, params)
-    _same_device(codes, params)
-    _need(dtype in _ELEMENT, f"dtype must be one of {', '.join(str(a) for a in _ELEMENT)}, got {dtype}")
+    code = _ELEMENT.get(dtype)
+    if code is None:
+        raise RuntimeError(f"dtype must be one of {', '.join(str(a) for a in _ELEMENT)}, got {dtype}")
     n, F = codes.shape
-    out = torch.empty((n, F), dtype=dtype, device=codes.device)
-    with torch.cuda.device(out.device), _Logged("checkpoint_unpack", out.device, n=n, F=F):
-        rc = _cabi.lib().sgnn_checkpoint_unpack_rows(_ptr(codes), codes.stride(0), _ptr(params), _ELEMENT[dtype],
-                                                     _ptr(out), out.stride(0), n, F, _stream(out))
-    _cabi.check(rc, "checkpoint_unpack_rows")
+    dev = codes.device
+    out = torch.empty((n, F), dtype=dtype, device=dev)
+    with _on(dev), _Logged("checkpoint_unpack", dev, n=n, F=F):
+        rc = _cabi.lib().sgnn_checkpoint_unpack_rows(codes.data_ptr(), codes.stride(0), params.data_ptr(), code,
+                                                     out.data_ptr(), out.stride(0), n, F, _stream_on(dev))
+    if rc:
+        _cabi.check(rc, "checkpoint_unpack_rows")
     return out
 
 
 def checkpoint_weight_grad(g, codes, params, out=None, beta: float = 0.0):
     """``out = g.T @ x (+ beta * out)`` with ``x`` [n, F] given by its 8-bit checkpoint and ``g`` [n, M] in fp32, bf16
     or fp16: the weight gradient of a linear map, fp32 [M, F], straight from the codes."""
-    _cuda(g, "g", None, 2)
-    code = _element(g, "g")
+    code = _matrix(g, "g")
     codes = _checkpoint_args(codes, params)
     n, F = codes.shape
-    _need(g.size(0) == n and g.size(1) > 0, "g must be [n, M] with the checkpoint's n")
-    M = g.size(1)
+    M, dev = g.size(1), g.device
+    if g.size(0) != n or codes.device != dev:
+        _need(g.size(0) == n, "g must be [n, M] with the checkpoint's n")
+        _need(False, "all tensors must be on the same CUDA device")
     if out is None:
         _need(beta == 0.0, "checkpoint_weight_grad: beta needs an existing out")
-        out = torch.empty((M, F), dtype=torch.float32, device=g.device)
-    _cuda(out, "out", torch.float32, 2)
-    _need(tuple(out.shape) == (M, F) and (F <= 1 or out.stride(1) == 1) and (M <= 1 or out.stride(0) >= F),
-          "out must be [M, F] with contiguous rows")
-    _same_device(g, codes, params, out)
+        out = torch.empty((M, F), dtype=torch.float32, device=dev)
+    else:
+        _result(out, "out", M, F, torch.float32, dev)
     g = _row_major(g)
     lib = _cabi.lib()
-    with torch.cuda.device(g.device), _Logged("checkpoint_weight_grad", g.device, n=n, M=M, F=F):
+    with _on(dev), _Logged("checkpoint_weight_grad", dev, n=n, M=M, F=F):
         need = ctypes.c_size_t(0)
         _cabi.check(lib.sgnn_checkpoint_weight_grad_workspace_bytes(code, n, M, F, ctypes.byref(need)),
                     "checkpoint_weight_grad")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=g.device)
-        rc = lib.sgnn_checkpoint_weight_grad(code, _ptr(g), g.stride(0), _ptr(codes), codes.stride(0), _ptr(params), n, M,
-                                             F, float(beta), _ptr(out), max(out.stride(0), F), _ptr(ws), ws.numel(),
-                                             _stream(g))
-    _cabi.check(rc, "checkpoint_weight_grad")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        rc = lib.sgnn_checkpoint_weight_grad(code, g.data_ptr(), g.stride(0), codes.data_ptr(), codes.stride(0),
+                                             params.data_ptr(), n, M, F, beta, out.data_ptr(), max(out.stride(0), F),
+                                             ws.data_ptr(), need.value, _stream_on(dev))
+    if rc:
+        _cabi.check(rc, "checkpoint_weight_grad")
     return out
 
 
+_NLL_ELEMENT = {torch.float32: 0, torch.bfloat16: 1}
+
+
 def _linear_nll(x, weight, bias, labels, mask, inv_count, with_grad: bool):
-    _cuda(x, "x", None, 2)
-    code = _element(x, "x", (torch.float32, torch.bfloat16))
-    _cuda(weight, "weight", x.dtype, 2)
+    code = _matrix(x, "x", _NLL_ELEMENT)
     n, K = x.shape
+    dev, dtype = x.device, x.dtype
+    _cuda(weight, "weight", dtype, 2)
     C = weight.size(0)
-    _need(K > 0 and C > 0 and weight.size(1) == K, "weight must be [C, K] with x's K")
-    bcode = _params_of(x, [(bias, "bias")], C)
+    if C == 0 or weight.size(1) != K or weight.device != dev:
+        _need(weight.device == dev, "all tensors must be on the same CUDA device")
+        _need(False, f"weight must be [C, {K}] like x")
+    bcode = _vector(bias, "bias", dtype, C, dev)
     _cuda(labels, "labels", torch.int64, 1)
-    _need(labels.numel() == n and labels.is_contiguous(), "labels must be a contiguous int64 [n] tensor")
+    if labels.numel() != n or not labels.is_contiguous() or labels.device != dev:
+        _need(labels.device == dev, "all tensors must be on the same CUDA device")
+        _need(False, "labels must be a contiguous int64 [n] tensor")
     if mask is not None:
         _cuda(mask, "mask", None, 1)
-        _need(mask.dtype in (torch.bool, torch.uint8) and mask.numel() == n and mask.is_contiguous(),
-              "mask must be a contiguous bool / uint8 [n] tensor")
-    _same_device(x, weight, bias, labels, mask)
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != n or not mask.is_contiguous() or mask.device != dev:
+            _need(mask.device == dev, "all tensors must be on the same CUDA device")
+            _need(False, "mask must be a contiguous bool / uint8 [n] tensor")
     x, weight = _row_major(x), _row_major(weight)
-    dev = x.device
     loss = torch.empty(1, dtype=torch.float32, device=dev)
     lse = gx = gw = gb = None
     if with_grad:
-        gx = torch.empty((n, K), dtype=x.dtype, device=dev)
-        gw = torch.empty((C, K), dtype=x.dtype, device=dev)
+        gx = torch.empty((n, K), dtype=dtype, device=dev)
+        gw = torch.empty((C, K), dtype=dtype, device=dev)
         gb = torch.empty(C, dtype=bias.dtype, device=dev) if bias is not None else None
     else:
         lse = torch.empty(n, dtype=torch.float32, device=dev)
     lib = _cabi.lib()
-    with torch.cuda.device(dev), _Logged("linear_nll_grad" if with_grad else "linear_nll", dev, n=n, K=K, C=C):
+    with _on(dev), _Logged("linear_nll_grad" if with_grad else "linear_nll", dev, n=n, K=K, C=C):
         need = ctypes.c_size_t(0)
-        _cabi.check(lib.sgnn_linear_nll_workspace_bytes(code, n, K, C, int(with_grad), ctypes.byref(need)), "linear_nll_loss")
+        _cabi.check(lib.sgnn_linear_nll_workspace_bytes(code, n, K, C, with_grad, ctypes.byref(need)), "linear_nll_loss")
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        rc = lib.sgnn_linear_nll_loss(code, _ptr(x), x.stride(0), _ptr(weight), weight.stride(0), bcode, _ptr(bias),
-                                      _ptr(labels), _ptr(mask), float(inv_count), n, K, C, _ptr(loss), _ptr(lse),
-                                      _ptr(gx), K, _ptr(gw), K, _ptr(gb), _ptr(ws), ws.numel(), _stream(x))
-    _cabi.check(rc, "linear_nll_loss")
+        rc = lib.sgnn_linear_nll_loss(code, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), bcode,
+                                      _ptr(bias), labels.data_ptr(), _ptr(mask), inv_count, n, K, C, loss.data_ptr(),
+                                      _ptr(lse), _ptr(gx), K, _ptr(gw), K, _ptr(gb), ws.data_ptr(), need.value,
+                                      _stream_on(dev))
+    if rc:
+        _cabi.check(rc, "linear_nll_loss")
     return loss, lse, gx, gw, gb
 
 
