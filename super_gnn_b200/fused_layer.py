@@ -13,6 +13,10 @@ elementwise / normalisation ops run as one kernel each way, and the backward agg
 the self-path gradient in place.  Saved for the backward: the aggregated input, the GEMM output
 h and two numbers per row (mean, reciprocal standard deviation); the normalised values, the
 sign of the output and the dropout mask are recomputed from those.
+
+With ``checkpoint_bits=8`` the nodes keep their activations as 8-bit checkpoints (``ops.checkpoint_pack_rows``), a quarter
+of the memory: the weight gradients are taken straight from the codes and h is restored for its kernel.  The forward
+results do not change; an input that the caller holds anyway (the features) is kept as it is.
 """
 from __future__ import annotations
 
@@ -38,6 +42,18 @@ _AX = {}
 _OWN_GRADS = set()
 
 
+def _keep(x, bits):
+    """What the backward keeps of an activation: itself, or its 8-bit checkpoint (codes, params)."""
+    return [x] if bits == 32 else list(ops.checkpoint_pack_rows(x))
+
+
+def _kept_grad(g, kept, out=None, beta=0.0):
+    """``g^T x (+ beta out)`` for what :func:`_keep` kept of ``x``."""
+    if len(kept) == 1:
+        return ops.gemm_tn(g, kept[0], out=out, beta=beta)
+    return ops.checkpoint_weight_grad(g, kept[0], kept[1], out=out, beta=beta)
+
+
 def reset_layer_buffers():
     _AX.clear()
     _OWN_GRADS.clear()
@@ -55,6 +71,7 @@ def _concat_buffer(x):
     buf = _AX.get(x.data_ptr())
     if (buf is not None and tuple(buf.shape) == (n, 2 * K) and x.stride() == (2 * K, 1) and buf.device == x.device
             and x.data_ptr() == buf.data_ptr() + 4 * K):
+        del _AX[x.data_ptr()]  # its one reader has it: from here on it lives as long as someone keeps it
         return buf
     return None
 
@@ -67,8 +84,9 @@ class FusedSAGELayer(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_neigh, w_self, bias, gamma, beta, graph, layer, num_bits, is_pre_delay, training, p, eps,
-                seed, mask, feeds_fused_layer=False):
+                seed, mask, feeds_fused_layer=False, checkpoint_bits=32):
         n, K = x.shape
+        bits = checkpoint_bits
         H = w_neigh.size(0)
         actx = _AggCtx()
         ax = _concat_buffer(x)  # [agg | x], or None
@@ -82,11 +100,13 @@ class FusedSAGELayer(torch.autograd.Function):
         if ax is not None:
             w_cat = torch.cat([w_neigh, w_self], dim=1)  # [H, 2K]
             h = ops.gemm_nt(ax, w_cat)
-            keep = [ax, w_cat]
+            # in 8 bits each half has its own range
+            keep = [w_cat] + ([ax] if bits == 32 else _keep(agg, bits) + _keep(x, bits))
         else:
             h = ops.gemm_nt(agg, w_neigh)
             ops.gemm_nt(x, w_self, out=h, beta=1.0)
-            keep = [x, agg, w_neigh, w_self]
+            ctx.x_bits = bits if ctx.needs_input_grad[0] else 32  # the features stay with the caller anyway
+            keep = [w_neigh, w_self] + _keep(x, ctx.x_bits) + _keep(agg, bits)
         if feeds_fused_layer:
             nxt = x.new_empty((n, 2 * H))  # the next layer's [agg | x] buffer: this layer's output is its right half
             y, stats = ops.sage_epilogue_forward(h, bias, gamma, beta, p, training, seed, eps, mask, out=nxt[:, H:])
@@ -96,18 +116,22 @@ class FusedSAGELayer(torch.autograd.Function):
         ctx.actx, ctx.graph = actx, graph
         ctx.cfg = (training, p, seed)
         ctx.has_mask = mask is not None
-        ctx.K, ctx.concat = K, ax is not None
-        saved = [h, stats, bias, gamma, beta] + keep + ([mask] if mask is not None else [])
+        ctx.K, ctx.concat, ctx.bits = K, ax is not None, bits
+        saved = [stats, bias, gamma, beta] + ([mask] if mask is not None else []) + _keep(h, bits) + keep
         ctx.save_for_backward(*saved)
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        saved = ctx.saved_tensors
-        h, stats, bias, gamma, beta = saved[:5]
-        mask = saved[-1] if ctx.has_mask else None
+        stats, bias, gamma, beta, *saved = ctx.saved_tensors
+        mask = saved.pop(0) if ctx.has_mask else None
         training, p, seed = ctx.cfg
-        K = ctx.K
+        K, bits = ctx.K, ctx.bits
+        if bits == 32:
+            h, *saved = saved
+        else:
+            codes, params, *saved = saved
+            h = ops.checkpoint_unpack_rows(codes, params)
         gy = gy if gy.stride(-1) == 1 else gy.contiguous()
         mine = gy.data_ptr() in _OWN_GRADS and gy.stride(0) % 4 == 0  # produced by the layer above for this one alone
         _OWN_GRADS.discard(gy.data_ptr())
@@ -115,8 +139,13 @@ class FusedSAGELayer(torch.autograd.Function):
                                                                  mask, in_place=mine)
         gx = None
         if ctx.concat:
-            ax, w_cat = saved[5:7]
-            gw = ops.gemm_tn(gh, ax)  # [H, 2K] = [grad W_neigh | grad W_self]
+            w_cat, *kept = saved
+            if bits == 32:
+                gw = ops.gemm_tn(gh, kept[0])  # [H, 2K] = [grad W_neigh | grad W_self]
+            else:
+                gw = gh.new_empty((gh.size(1), 2 * K))
+                _kept_grad(gh, kept[:2], out=gw[:, :K])
+                _kept_grad(gh, kept[2:], out=gw[:, K:])
             gw_neigh, gw_self = gw[:, :K], gw[:, K:]
             if ctx.needs_input_grad[0]:
                 # [gh W_neigh | gh W_self] in one GEMM; the backward aggregation reads the left half and adds onto
@@ -126,16 +155,17 @@ class FusedSAGELayer(torch.autograd.Function):
                     g_cat[:, :K].div_(ctx.graph.in_degrees)
                 gx = aggregate_backward(ctx.actx, g_cat[:, :K], out=g_cat[:, K:], accumulate=True)
         else:
-            x, agg, w_neigh, w_self = saved[5:9]
-            gw_neigh = ops.gemm_tn(gh, agg)
-            gw_self = ops.gemm_tn(gh, x)
+            w_neigh, w_self, *kept = saved
+            half = 1 if ctx.x_bits == 32 else 2
+            gw_neigh = _kept_grad(gh, kept[half:])
+            gw_self = _kept_grad(gh, kept[:half])
             if ctx.needs_input_grad[0]:
                 g_agg = ops.gemm_nt(gh, w_neigh.t().contiguous())
                 if not getattr(ctx.graph, "fold_mean", False):
                     g_agg.div_(ctx.graph.in_degrees)
                 gx = ops.gemm_nt(gh, w_self.t().contiguous())
                 gx = aggregate_backward(ctx.actx, g_agg, out=gx, accumulate=True)
-        return (_own(gx), gw_neigh, gw_self, g_bias, g_gamma, g_beta) + (None,) * 10
+        return (_own(gx), gw_neigh, gw_self, g_bias, g_gamma, g_beta) + (None,) * 11
 
 
 def _pad_rows(w, rows):
@@ -180,8 +210,8 @@ def _narrow_local_forward(x, w_neigh, w_self, graph, layer, num_bits, is_pre_del
 
 
 def _narrow_local_backward(ctx, G, x, agg_remote, w_cat):
-    """G = [. | g] with the gradient of the logits in the right half (padding columns zero): returns
-    (grad_x, grad_W_neigh, grad_W_self); the exchanged rows are those of A_remote^T (g W_neigh), as in the
+    """G = [. | g] with the gradient of the logits in the right half (padding columns zero), x and agg_remote as
+    kept: returns (grad_x, grad_W_neigh, grad_W_self); the exchanged rows are those of A_remote^T (g W_neigh), as in the
     reference."""
     C, Cp = ctx.dims
     graph = ctx.graph
@@ -196,8 +226,8 @@ def _narrow_local_backward(ctx, G, x, agg_remote, w_cat):
         return ops.gemm_nt(G, w_cat.t().contiguous(), out=g_agg)
 
     gx = _own(aggregate_backward(ctx.actx, g_agg, local_work=local_work))
-    gw = ops.gemm_tn(G, x)  # rows [0, Cp): local share of grad W_neigh; rows [Cp, 2 Cp): grad W_self
-    ops.gemm_tn(g_right, agg_remote, out=gw[:Cp], beta=1.0)  # + g^T (remote share of the aggregation)
+    gw = _kept_grad(G, x)  # rows [0, Cp): local share of grad W_neigh; rows [Cp, 2 Cp): grad W_self
+    _kept_grad(g_right, agg_remote, out=gw[:Cp], beta=1.0)  # + g^T (remote share of the aggregation)
     return gx, gw[:C], gw[Cp:Cp + C]
 
 
@@ -216,10 +246,11 @@ class FusedSAGEOutputLayer(torch.autograd.Function):
     narrow_local = True
 
     @staticmethod
-    def forward(ctx, x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training):
+    def forward(ctx, x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training, checkpoint_bits=32):
         C, K = w_neigh.shape
         Cp = (C + 3) // 4 * 4
         actx = _AggCtx()
+        bits = ctx.bits = checkpoint_bits
         ctx.actx, ctx.graph = actx, graph
         ctx.has_bias = bias is not None
         ctx.dims = (C, Cp)
@@ -228,7 +259,7 @@ class FusedSAGEOutputLayer(torch.autograd.Function):
             ctx.actx, w_cat, agg_remote, logits, _ = _narrow_local_forward(x, w_neigh, w_self, graph, layer, num_bits,
                                                                            is_pre_delay, training)
             out = logits + bias if bias is not None else logits.contiguous()
-            ctx.save_for_backward(x, agg_remote, w_cat)
+            ctx.save_for_backward(w_cat, *_keep(x, bits), *_keep(agg_remote, bits))
             return out
         agg = aggregate_forward(actx, graph, x, layer, num_bits, is_pre_delay, training)
         if not getattr(graph, "fold_mean", False):
@@ -237,29 +268,32 @@ class FusedSAGEOutputLayer(torch.autograd.Function):
         out = ops.gemm_nt(agg, wn)
         ops.gemm_nt(x, ws, out=out, beta=1.0)
         out = out[:, :C] + bias if bias is not None else out[:, :C].contiguous()
-        ctx.save_for_backward(x, agg, wn, ws)
+        ctx.save_for_backward(wn, ws, *_keep(x, bits), *_keep(agg, bits))
         return out
 
     @staticmethod
     def backward(ctx, g):
         C, Cp = ctx.dims
         g_bias = g.sum(0) if ctx.has_bias else None
+        half = 1 if ctx.bits == 32 else 2
         if ctx.hybrid:
-            x, agg_remote, w_cat = ctx.saved_tensors
+            w_cat, *kept = ctx.saved_tensors
+            x, agg_remote = kept[:half], kept[half:]
             G = g.new_empty((g.size(0), 2 * Cp))  # [A_local^T (g / in_degrees) | g], zero in the padding columns
             G[:, Cp:Cp + C] = g
             if Cp > C:
                 G[:, Cp + C:] = 0
             gx, gw_neigh, gw_self = _narrow_local_backward(ctx, G, x, agg_remote, w_cat)
-            return (gx, gw_neigh, gw_self, g_bias) + (None,) * 5
-        x, agg, wn, ws = ctx.saved_tensors
+            return (gx, gw_neigh, gw_self, g_bias) + (None,) * 6
+        wn, ws, *kept = ctx.saved_tensors
+        x, agg = kept[:half], kept[half:]
         if Cp != C:
             gp = g.new_zeros((g.size(0), Cp))
             gp[:, :C] = g
         else:
             gp = g.contiguous()
-        gw_neigh = ops.gemm_tn(gp, agg)[:C]
-        gw_self = ops.gemm_tn(gp, x)[:C]
+        gw_neigh = _kept_grad(gp, agg)[:C]
+        gw_self = _kept_grad(gp, x)[:C]
         gx = None
         if ctx.needs_input_grad[0]:
             g_agg = ops.gemm_nt(gp, wn.t().contiguous())
@@ -267,7 +301,7 @@ class FusedSAGEOutputLayer(torch.autograd.Function):
                 g_agg.div_(ctx.graph.in_degrees)
             gx = ops.gemm_nt(gp, ws.t().contiguous())
             gx = _own(aggregate_backward(ctx.actx, g_agg, out=gx, accumulate=True))
-        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 5
+        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 6
 
 
 def _project_first_forward(x, w_neigh, w_self, graph, layer, num_bits, is_pre_delay, training):
@@ -291,14 +325,14 @@ def _project_first_forward(x, w_neigh, w_self, graph, layer, num_bits, is_pre_de
 
 
 def _project_first_backward(ctx, G, x, w_cat, need_gx: bool):
-    """G = [. | g] with the gradient of the logits in the right half (padding columns zero): fills the left half
-    with A^T (g / in_degrees) and returns (grad_x, grad_W_neigh, grad_W_self)."""
+    """G = [. | g] with the gradient of the logits in the right half (padding columns zero), x as kept: fills the
+    left half with A^T (g / in_degrees) and returns (grad_x, grad_W_neigh, grad_W_self)."""
     C, Cp = ctx.dims
     g_in = G[:, Cp:]
     if not getattr(ctx.graph, "fold_mean", False):
         g_in = g_in / ctx.graph.in_degrees
     aggregate_backward(ctx.actx, g_in, out=G[:, :Cp], accumulate=False)
-    gw = ops.gemm_tn(G, x)  # [2 Cp, K]: rows of grad W_neigh, then of grad W_self
+    gw = _kept_grad(G, x)  # [2 Cp, K]: rows of grad W_neigh, then of grad W_self
     gx = _own(ops.gemm_nt(G, w_cat.t().contiguous())) if need_gx else None
     return gx, gw[:C], gw[Cp:Cp + C]
 
@@ -322,18 +356,18 @@ class FusedSAGEOutputLayerProjectFirst(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training):
+    def forward(ctx, x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training, checkpoint_bits=32):
         actx, w_cat, logits, ctx.dims = _project_first_forward(x, w_neigh, w_self, graph, layer, num_bits,
                                                                is_pre_delay, training)
         out = logits + bias if bias is not None else logits.contiguous()
         ctx.actx, ctx.graph = actx, graph
         ctx.has_bias = bias is not None
-        ctx.save_for_backward(x, w_cat)
+        ctx.save_for_backward(w_cat, *_keep(x, checkpoint_bits))
         return out
 
     @staticmethod
     def backward(ctx, g):
-        x, w_cat = ctx.saved_tensors
+        w_cat, *x = ctx.saved_tensors
         C, Cp = ctx.dims
         G = g.new_empty((g.size(0), 2 * Cp))  # [A^T (g / in_degrees) | g], zero in the padding columns
         G[:, Cp:Cp + C] = g
@@ -341,7 +375,7 @@ class FusedSAGEOutputLayerProjectFirst(torch.autograd.Function):
             G[:, Cp + C:] = 0
         g_bias = g.sum(0) if ctx.has_bias else None
         gx, gw_neigh, gw_self = _project_first_backward(ctx, G, x, w_cat, ctx.needs_input_grad[0])
-        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 5
+        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 6
 
 
 class FusedSAGELossProjectFirst(torch.autograd.Function):
@@ -357,7 +391,7 @@ class FusedSAGELossProjectFirst(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training, labels, mask,
-                inv_count, unit_grad):
+                inv_count, unit_grad, checkpoint_bits=32):
         actx, w_cat, logits, ctx.dims = _project_first_forward(x, w_neigh, w_self, graph, layer, num_bits,
                                                                is_pre_delay, training)
         C, Cp = ctx.dims
@@ -366,18 +400,18 @@ class FusedSAGELossProjectFirst(torch.autograd.Function):
         ctx.actx, ctx.graph = actx, graph
         ctx.has_bias = bias is not None
         ctx.unit_grad = bool(unit_grad)
-        ctx.save_for_backward(x, w_cat, G)
+        ctx.save_for_backward(w_cat, G, *_keep(x, checkpoint_bits))
         return loss.reshape(())
 
     @staticmethod
     def backward(ctx, g_loss):
-        x, w_cat, G = ctx.saved_tensors
+        w_cat, G, *x = ctx.saved_tensors
         C, Cp = ctx.dims
         if not ctx.unit_grad:
             G[:, Cp:].mul_(g_loss)
         g_bias = G[:, Cp:Cp + C].sum(0) if ctx.has_bias else None
         gx, gw_neigh, gw_self = _project_first_backward(ctx, G, x, w_cat, ctx.needs_input_grad[0])
-        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 9
+        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 10
 
 
 class FusedSAGELossNarrowLocal(torch.autograd.Function):
@@ -386,7 +420,7 @@ class FusedSAGELossNarrowLocal(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training, labels, mask,
-                inv_count, unit_grad):
+                inv_count, unit_grad, checkpoint_bits=32):
         ctx.actx, w_cat, agg_remote, logits, ctx.dims = _narrow_local_forward(x, w_neigh, w_self, graph, layer,
                                                                               num_bits, is_pre_delay, training)
         C, Cp = ctx.dims
@@ -395,15 +429,75 @@ class FusedSAGELossNarrowLocal(torch.autograd.Function):
         ctx.graph = graph
         ctx.has_bias = bias is not None
         ctx.unit_grad = bool(unit_grad)
-        ctx.save_for_backward(x, agg_remote, w_cat, G)
+        ctx.bits = checkpoint_bits
+        ctx.save_for_backward(w_cat, G, *_keep(x, checkpoint_bits), *_keep(agg_remote, checkpoint_bits))
         return loss.reshape(())
 
     @staticmethod
     def backward(ctx, g_loss):
-        x, agg_remote, w_cat, G = ctx.saved_tensors
+        w_cat, G, *kept = ctx.saved_tensors
+        half = 1 if ctx.bits == 32 else 2
+        x, agg_remote = kept[:half], kept[half:]
         C, Cp = ctx.dims
         if not ctx.unit_grad:
             G[:, Cp:].mul_(g_loss)
         g_bias = G[:, Cp:Cp + C].sum(0) if ctx.has_bias else None
         gx, gw_neigh, gw_self = _narrow_local_backward(ctx, G, x, agg_remote, w_cat)
-        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 9
+        return (gx, gw_neigh, gw_self, g_bias) + (None,) * 10
+
+
+class FusedSAGELossManyClasses(torch.autograd.Function):
+    """The last layer and the training loss for any number of classes, without the logits in memory:
+
+        loss = nll_loss(log_softmax([Aggregator(x) / in_degrees | x] [W_neigh | W_self]^T + bias)[mask], labels[mask],
+                        reduction="sum") * inv_count
+
+    (super_gnn/layers/sageconv.py:62-89, examples/graphsage/sage.py:211, examples/graphsage/train.py:41-44).  The boundary
+    exchange is the reference's: rows of x at the configured bit width.  The gradients come with the loss
+    (``ops.linear_nll_loss_grad``) and are held until the backward pass, which sends the aggregated half's through the
+    graph.  ``unit_grad``: see :class:`FusedSAGELossProjectFirst`."""
+
+    @staticmethod
+    def forward(ctx, x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training, labels, mask,
+                inv_count, unit_grad):
+        ctx.actx, ax, w_cat = _many_classes_input(x, w_neigh, w_self, graph, layer, num_bits, is_pre_delay, training)
+        loss, gax, gw, gb = ops.linear_nll_loss_grad(ax, w_cat, bias, labels, mask, inv_count)
+        ctx.graph, ctx.unit_grad = graph, bool(unit_grad)
+        ctx.save_for_backward(gax, gw, gb)
+        return loss.reshape(())
+
+    @staticmethod
+    def backward(ctx, g_loss):
+        gax, gw, gb = ctx.saved_tensors
+        if not ctx.unit_grad:
+            gax, gw, gb = gax * g_loss, gw * g_loss, gb * g_loss if gb is not None else None
+        K = gax.size(1) // 2
+        gx = None
+        if ctx.needs_input_grad[0]:
+            g_agg = gax[:, :K]
+            if not getattr(ctx.graph, "fold_mean", False):
+                g_agg = g_agg / ctx.graph.in_degrees
+            # the loss is the only reader of gax: its right half becomes grad_x (a second backward pass starts from a copy)
+            out = gax[:, K:] if not ctx.unit_grad else gax[:, K:].clone()
+            gx = _own(aggregate_backward(ctx.actx, g_agg, out=out, accumulate=True))
+        return (gx, gw[:, :K], gw[:, K:], gb) + (None,) * 9
+
+
+def _many_classes_input(x, w_neigh, w_self, graph, layer, num_bits, is_pre_delay, training):
+    """(aggregation context, [Aggregator(x) / in_degrees | x], [W_neigh | W_self])"""
+    n, K = x.shape
+    ax = _concat_buffer(x)
+    if ax is None:
+        ax = x.new_empty((n, 2 * K))
+        ax[:, K:] = x
+    actx = _AggCtx()
+    aggregate_forward(actx, graph, ax[:, K:], layer, num_bits, is_pre_delay, training, out=ax[:, :K])
+    if not getattr(graph, "fold_mean", False):
+        ax[:, :K].div_(graph.in_degrees)
+    return actx, ax, torch.cat([w_neigh, w_self], dim=1)
+
+
+def many_classes_loss(x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, labels, mask, inv_count):
+    """The loss of :class:`FusedSAGELossManyClasses` alone, for validation: nothing is kept for a backward pass."""
+    _, ax, w_cat = _many_classes_input(x, w_neigh, w_self, graph, layer, num_bits, is_pre_delay, False)
+    return ops.linear_nll_loss(ax, w_cat, bias, labels, mask, inv_count)[0].reshape(())

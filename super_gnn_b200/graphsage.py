@@ -12,14 +12,16 @@ import torch.distributed as dist
 import torch.nn.functional as F
 from torch.nn import LayerNorm
 
-from .fused_layer import (FusedSAGELayer, FusedSAGELossNarrowLocal, FusedSAGELossProjectFirst, FusedSAGEOutputLayer,
-                          FusedSAGEOutputLayerProjectFirst, narrow_local_applies, reset_layer_buffers)
+from .fused_layer import (FusedSAGELayer, FusedSAGELossManyClasses, FusedSAGELossNarrowLocal, FusedSAGELossProjectFirst,
+                          FusedSAGEOutputLayer, FusedSAGEOutputLayerProjectFirst, many_classes_loss, narrow_local_applies,
+                          reset_layer_buffers)
 from .layers import DistSAGEConvGrad
+from .layers.functional import check_bits, layer_norm
 
 
 class DistSAGE(torch.nn.Module):
     def __init__(self, in_channels, hidden_channels, out_channels, num_layers=3, dropout=0.5, num_bits=32,
-                 is_pre_delay=False, norm_type="LayerNorm"):
+                 is_pre_delay=False, norm_type="LayerNorm", checkpoint_bits=32, chunked_loss=False):
         super().__init__()
         self.convs = torch.nn.ModuleList()
         self.norms = torch.nn.ModuleList()
@@ -32,6 +34,13 @@ class DistSAGE(torch.nn.Module):
             raise ValueError("only norm_type=None or 'LayerNorm' is provided on this path")
         self.dropout = dropout
         self.norm_type = norm_type
+        # 8: on the GPU the layers keep their activations for the backward pass in 8 bits (a quarter of the memory)
+        self.checkpoint_bits = check_bits(checkpoint_bits)
+        for conv in self.convs:
+            conv.checkpoint_bits = self.checkpoint_bits
+        # the training loss of the last layer in pieces of the classes, without the logits in memory (any number of
+        # classes; the boundary exchange stays the reference's)
+        self.chunked_loss = bool(chunked_loss)
         # optional fixed dropout masks (one per hidden layer) for runs that must be
         # reproducible against a CPU reference; None = native dropout
         self.dropout_masks = None
@@ -74,8 +83,10 @@ class DistSAGE(torch.nn.Module):
     def can_fuse_loss(self, nodes_feats, graph=None) -> bool:
         """True when ``forward(..., loss_mask=, loss_inv_count=)`` returns the training loss from a fused node: fused
         CUDA path, at most 256 classes, and a last layer that either projects before it aggregates or (given the
-        graph) aggregates only the remote edges at the input width."""
+        graph) aggregates only the remote edges at the input width; or ``chunked_loss``, for any number of classes."""
         last = self.convs[-1]
+        if self.chunked_loss:
+            return nodes_feats.is_cuda and nodes_feats.dtype == torch.float32 and last.normalize
         if not (self._fused_ok(nodes_feats) and self._layer_fusable(last, hidden=False) and last.out_channels <= 256):
             return False
         return self._project_first(last) or (fuse_loss_narrow_local and graph is not None
@@ -86,6 +97,8 @@ class DistSAGE(torch.nn.Module):
         """Log-probabilities per node (examples/graphsage/sage.py:179-211).  With ``loss_mask`` and
         ``loss_inv_count`` (and ``can_fuse_loss``) the summed negative log-likelihood of ``labels`` over the masked
         nodes times ``loss_inv_count`` is returned instead, computed together with the last layer."""
+        chunked = (self.chunked_loss and loss_mask is not None and loss_inv_count is not None
+                   and self.can_fuse_loss(nodes_feats, graph))
         if self._fused_ok(nodes_feats):
             reset_layer_buffers()
             for i, conv in enumerate(self.convs[:-1]):
@@ -101,9 +114,12 @@ class DistSAGE(torch.nn.Module):
                                                    conv.lin_self.weight, conv.bias, norm.weight, norm.bias, graph, i,
                                                    conv.num_bits, conv.is_pre_delay, self.training, float(self.dropout),
                                                    float(norm.eps), seed, mask,
-                                                   i + 1 < len(self.convs) - 1
-                                                   and self._layer_fusable(self.convs[i + 1], hidden=True))
+                                                   (i + 1 < len(self.convs) - 1
+                                                    and self._layer_fusable(self.convs[i + 1], hidden=True))
+                                                   or (i + 1 == len(self.convs) - 1 and chunked), self.checkpoint_bits)
             last = self.convs[-1]
+            if chunked:
+                return self._chunked_loss(graph, nodes_feats, labels, loss_mask, loss_inv_count, loss_unit_grad)
             if not self._layer_fusable(last, hidden=False):
                 nodes_feats = last(graph, nodes_feats, len(self.convs) - 1)
                 return F.log_softmax(nodes_feats, dim=1)
@@ -112,14 +128,17 @@ class DistSAGE(torch.nn.Module):
                 return node.apply(nodes_feats, last.lin_neigh.weight,
                                   last.lin_self.weight, last.bias, graph, len(self.convs) - 1,
                                   last.num_bits, last.is_pre_delay, self.training, labels,
-                                  loss_mask, float(loss_inv_count), bool(loss_unit_grad))
+                                  loss_mask, float(loss_inv_count), bool(loss_unit_grad), self.checkpoint_bits)
             node = FusedSAGEOutputLayerProjectFirst if self._project_first(last) else FusedSAGEOutputLayer
             nodes_feats = node.apply(nodes_feats, last.lin_neigh.weight,
                                      last.lin_self.weight, last.bias, graph, len(self.convs) - 1,
-                                     last.num_bits, last.is_pre_delay, self.training)
+                                     last.num_bits, last.is_pre_delay, self.training, self.checkpoint_bits)
             return F.log_softmax(nodes_feats, dim=1)
         for i in range(len(self.convs) - 1):
             nodes_feats = self._unfused_hidden(graph, nodes_feats, i)
+        if chunked:
+            reset_layer_buffers()
+            return self._chunked_loss(graph, nodes_feats, labels, loss_mask, loss_inv_count, loss_unit_grad)
         nodes_feats = self.convs[-1](graph, nodes_feats, len(self.convs) - 1)
         return F.log_softmax(nodes_feats, dim=1)
 
@@ -131,8 +150,19 @@ class DistSAGE(torch.nn.Module):
         else:
             nodes_feats = F.dropout(nodes_feats, p=self.dropout, training=self.training)
         if self.norm_type is not None:
-            nodes_feats = self.norms[i](nodes_feats)
+            norm = self.norms[i]
+            if self.checkpoint_bits == 8 and nodes_feats.is_cuda:
+                nodes_feats = layer_norm(nodes_feats, norm.weight, norm.bias, norm.eps, self.checkpoint_bits)
+            else:
+                nodes_feats = norm(nodes_feats)
         return F.relu(nodes_feats)
+
+    def _chunked_loss(self, graph, x, labels, mask, inv_count, unit_grad):
+        last, layer = self.convs[-1], len(self.convs) - 1
+        args = (x, last.lin_neigh.weight, last.lin_self.weight, last.bias, graph, layer, last.num_bits, last.is_pre_delay)
+        if not torch.is_grad_enabled():
+            return many_classes_loss(*args, labels, mask, float(inv_count))
+        return FusedSAGELossManyClasses.apply(*args, self.training, labels, mask, float(inv_count), bool(unit_grad))
 
 
 def allreduce_hook(process_group, bucket):
@@ -144,7 +174,8 @@ def allreduce_hook(process_group, bucket):
 def create_model_and_optimizer(config: dict, device=None):
     model = DistSAGE(config["in_channels"], config["hidden_channels"], config["out_channels"],
                      config.get("num_layers", 3), config.get("dropout", 0.5), config.get("num_bits", 32),
-                     config.get("is_pre_delay", False), config.get("norm_type", "LayerNorm"))
+                     config.get("is_pre_delay", False), config.get("norm_type", "LayerNorm"),
+                     config.get("checkpoint_bits", 32), config.get("chunked_loss", False))
     model.reset_parameters()
     if device is not None:
         model = model.to(device)

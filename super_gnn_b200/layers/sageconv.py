@@ -10,6 +10,7 @@ from torch.nn import Linear, Parameter
 
 from ..aggregator import Aggregator
 from ..time_recorder import TimeRecorder
+from .functional import linear
 
 
 class DistSAGEConvGrad(torch.nn.Module):
@@ -22,6 +23,7 @@ class DistSAGEConvGrad(torch.nn.Module):
         self.normalize = normalize
         self.num_bits = num_bits
         self.is_pre_delay = is_pre_delay
+        self.checkpoint_bits = 32  # 8: the inputs of the two linear maps are kept in 8 bits for the backward pass
         self.lin_neigh = Linear(in_channels, out_channels, bias=False)
         self.lin_self = Linear(in_channels, out_channels, bias=False)
         if bias:
@@ -44,8 +46,12 @@ class DistSAGEConvGrad(torch.nn.Module):
             if self.normalize and not getattr(graph, "fold_mean", False):
                 out /= graph.in_degrees  # otherwise the Aggregator has already applied 1 / in_degree
         with TimeRecorder.ctx.time_block("nn_operation", is_record=False):
-            out = self.lin_neigh(out)
-            out += self.lin_self(local_nodes_feat)
+            if self.checkpoint_bits == 32 or not out.is_cuda:
+                out = self.lin_neigh(out)
+                out += self.lin_self(local_nodes_feat)
+            else:
+                out = linear(out, self.lin_neigh.weight, self.checkpoint_bits)
+                out += linear(local_nodes_feat, self.lin_self.weight, self.checkpoint_bits)
         with TimeRecorder.ctx.time_block("add_bias", is_record=False):
             if self.bias is not None:
                 out += self.bias
