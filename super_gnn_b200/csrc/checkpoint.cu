@@ -110,25 +110,26 @@ struct CkptCall {
 };
 
 template <class K>
-static int ckpt_grid(K kernel, int64_t n, int rows_per_block, int *grid)
+static int ckpt_grid(K kernel, int64_t n, int rows_per_block, ResidentCache &cache, int *grid)
 {
-    int per_sm = 0;
-    SGNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kCkptThreads, 0));
-    const int64_t g = (int64_t)sm_count() * (per_sm > 0 ? per_sm : 1), need = ceil_div(n, rows_per_block);
+    int g = 0;
+    int rc = resident_blocks(kernel, kCkptThreads, 0, 0, cache, &g);
+    const int64_t need = ceil_div(n, rows_per_block);
     *grid = (int)(g < need ? g : need);
-    return SGNN_OK;
+    return rc;
 }
 
 template <class T, int E, int NV>
 static int pack_launch(const CkptCall &c)
 {
+    static ResidentCache cache;
     int grid = 0, rc;
     if constexpr (NV > 0) {
-        if ((rc = ckpt_grid(checkpoint_pack_warp_kernel<T, E, NV>, c.n, kCkptWarps, &grid))) return rc;
+        if ((rc = ckpt_grid(checkpoint_pack_warp_kernel<T, E, NV>, c.n, kCkptWarps, cache, &grid))) return rc;
         checkpoint_pack_warp_kernel<T, E, NV><<<grid, kCkptThreads, 0, c.stream>>>(static_cast<const T *>(c.x), c.ldx,
                                                                                    c.codes, c.ldc, c.params, c.n, c.F);
     } else {
-        if ((rc = ckpt_grid(checkpoint_pack_block_kernel<T, E>, c.n, 1, &grid))) return rc;
+        if ((rc = ckpt_grid(checkpoint_pack_block_kernel<T, E>, c.n, 1, cache, &grid))) return rc;
         checkpoint_pack_block_kernel<T, E><<<grid, kCkptThreads, 0, c.stream>>>(static_cast<const T *>(c.x), c.ldx,
                                                                                 c.codes, c.ldc, c.params, c.n, c.F);
     }
@@ -157,8 +158,9 @@ static int pack_width(const CkptCall &c)
 template <class T, int E>
 static int unpack_launch(const CkptCall &c)
 {
+    static ResidentCache cache;
     int grid = 0;
-    int rc = ckpt_grid(checkpoint_unpack_kernel<T, E>, c.n, kCkptWarps, &grid);
+    int rc = ckpt_grid(checkpoint_unpack_kernel<T, E>, c.n, kCkptWarps, cache, &grid);
     if (rc) return rc;
     checkpoint_unpack_kernel<T, E><<<grid, kCkptThreads, 0, c.stream>>>(c.codes, c.ldc, c.params, static_cast<T *>(c.x),
                                                                         c.ldx, c.n, c.F);

@@ -409,7 +409,9 @@ template <class T, int FEED>
 static int weight_grad_launch(const GradCall &c, const GradPlan &p, cudaStream_t s)
 {
     constexpr int smem = grad_shared_bytes<T, FEED>();
-    SGNN_CUDA_OK(cudaFuncSetAttribute(weight_grad_kernel<T, FEED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static ResidentCache cache;  // one block an SM; asked for the shared memory's attribute
+    int resident = 0, rc = resident_blocks(weight_grad_kernel<T, FEED>, kGThreads, smem, smem, cache, &resident);
+    if (rc) return rc;
     weight_grad_kernel<T, FEED><<<(unsigned)(p.tiles_m * p.tiles_n * p.splits), kGThreads, smem, s>>>(c);
     SGNN_LAUNCH_OK("checkpoint_weight_grad");
     return SGNN_OK;

@@ -49,6 +49,32 @@ int sm_count();
 // ---- device side ----------------------------------------------------------
 #ifdef __CUDACC__
 
+// Blocks of `threads` threads and `smem` bytes that fit the SMs of the current device at once.  `smem_cap`: the largest
+// dynamic shared memory the kernel is ever launched with (its attribute is set once a device); a call whose `smem` varies
+// asks again.  Queries cost microseconds, as much as the smallest kernels: `cache` (one a kernel) keeps the answers of
+// the first devices, the same whoever writes them.
+struct ResidentCache {
+    int blocks[16] = {}, smem[16] = {};
+};
+template <class K>
+int resident_blocks(K kernel, int threads, size_t smem, size_t smem_cap, ResidentCache &cache, int *blocks)
+{
+    int dev = 0;
+    SGNN_CUDA_OK(cudaGetDevice(&dev));
+    const bool known = dev < 16 && cache.blocks[dev] > 0 && cache.smem[dev] == (int)smem + 1;
+    if (known) {
+        *blocks = cache.blocks[dev];
+        return SGNN_OK;
+    }
+    if (smem_cap > 48 * 1024)
+        SGNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_cap));
+    int per_sm = 0;
+    SGNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    *blocks = sm_count() * (per_sm > 0 ? per_sm : 1);
+    if (dev < 16 && smem_cap == smem) cache.smem[dev] = (int)smem + 1, cache.blocks[dev] = *blocks;
+    return SGNN_OK;
+}
+
 constexpr unsigned FULL = 0xffffffffu;
 
 // Streaming (read-once) loads: keep them out of L1 so the gathered rows keep it.

@@ -418,13 +418,11 @@ static int norm_blocks_cap() { return sm_count() * 8; }
 
 // Blocks of a call: enough for every warp (or block) to have a row, at most what is resident at once.
 template <class K>
-static int norm_grid(K kernel, int64_t n, int rows_per_block, size_t smem, int *grid)
+static int norm_grid(K kernel, int64_t n, int rows_per_block, size_t smem, size_t smem_cap, ResidentCache &cache, int *grid)
 {
-    if (smem > 48 * 1024)
-        SGNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    int per_sm = 0;
-    SGNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kNormThreads, smem));
-    int64_t g = (int64_t)sm_count() * (per_sm > 0 ? per_sm : 1);
+    int g = 0;
+    int rc = resident_blocks(kernel, kNormThreads, smem, smem_cap, cache, &g);
+    if (rc) return rc;
     if (g > norm_blocks_cap()) g = norm_blocks_cap();
     const int64_t need = ceil_div(n, rows_per_block);
     *grid = (int)(g < need ? g : need);
@@ -434,15 +432,16 @@ static int norm_grid(K kernel, int64_t n, int rows_per_block, size_t smem, int *
 template <class T, int E, int NV, bool CK>
 static int norm_fwd_launch(const NormCall &c)
 {
+    static ResidentCache cache;
     int grid = 0;
     if constexpr (NV > 0) {
-        int rc = norm_grid(norm_fwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, 0, &grid);
+        int rc = norm_grid(norm_fwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, 0, 0, cache, &grid);
         if (rc) return rc;
         norm_fwd_warp_kernel<T, E, NV, CK><<<grid, kNormThreads, 0, c.stream>>>(
             static_cast<const T *>(c.x), c.ldx, c.par, c.eps, static_cast<T *>(c.y), c.ldy, c.stats, c.codes, c.ldc,
             c.params, c.n, c.H);
     } else {
-        int rc = norm_grid(norm_fwd_block_kernel<T, E, CK>, c.n, 1, 0, &grid);
+        int rc = norm_grid(norm_fwd_block_kernel<T, E, CK>, c.n, 1, 0, 0, cache, &grid);
         if (rc) return rc;
         norm_fwd_block_kernel<T, E, CK><<<grid, kNormThreads, 0, c.stream>>>(
             static_cast<const T *>(c.x), c.ldx, c.par, c.eps, static_cast<T *>(c.y), c.ldy, c.stats, c.codes, c.ldc,
@@ -455,17 +454,20 @@ static int norm_fwd_launch(const NormCall &c)
 template <class T, int E, int NV, bool CK>
 static int norm_bwd_launch(const NormCall &c, int *blocks)
 {
+    static ResidentCache cache;
     const NormSource src{c.x, c.ldx, c.codes, c.ldc, c.params};
     if constexpr (NV > 0) {
+        // room for the widest row of this kernel, whatever the row: the answer about residency then stays the same
+        constexpr size_t most = (size_t)kNormWarps * 2 * 32 * E * NV * sizeof(float);
         const size_t smem = (size_t)kNormWarps * 2 * c.H * sizeof(float);
-        int rc = norm_grid(norm_bwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, smem, blocks);
+        int rc = norm_grid(norm_bwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, E * NV <= 8 ? most : smem, most, cache, blocks);
         if (rc) return rc;
         norm_bwd_warp_kernel<T, E, NV, CK><<<*blocks, kNormThreads, smem, c.stream>>>(
             static_cast<const T *>(c.gy), c.ldg, src, c.stats, c.par, static_cast<T *>(c.gx), c.ldgx, c.partials, c.n,
             c.H);
     } else {
         const size_t smem = (size_t)2 * c.H * sizeof(float);
-        int rc = norm_grid(norm_bwd_block_kernel<T, E, CK>, c.n, 1, smem, blocks);
+        int rc = norm_grid(norm_bwd_block_kernel<T, E, CK>, c.n, 1, smem, 2 * kNormMaxWidth * sizeof(float), cache, blocks);
         if (rc) return rc;
         norm_bwd_block_kernel<T, E, CK><<<*blocks, kNormThreads, smem, c.stream>>>(
             static_cast<const T *>(c.gy), c.ldg, src, c.stats, c.par, static_cast<T *>(c.gx), c.ldgx, c.partials, c.n,

@@ -56,7 +56,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // The first `blocks` blocks list the rows in the loss: rows[0 .. m) ascending, *total = m (`counts`: rows in the loss of
 // every listing block before).  The others set what the later kernels start from: bias log2(e) of the classes, -inf up to
 // the end of the last tile (classes that are not there have probability 0; their rows of W read as zeros, scaled by 1),
-// lse = 0 of all rows, and the counters.
+// lse = 0 and gx = 0 of all rows, and the counters.
 struct NllStart {
     const int64_t *labels;
     const uint8_t *mask;
@@ -67,6 +67,10 @@ struct NllStart {
     NllBias bias;
     float *bias2, *w_down, *lse;
     int *failed, *joined;
+    unsigned *largest;  // 2 K of them, or nullptr
+    int K;
+    void *gx;
+    int64_t ldgx;
 };
 
 template <class T>
@@ -82,6 +86,19 @@ __global__ void __launch_bounds__(kListThreads) nll_start_kernel(const NllStart 
         }
         if (a.lse != nullptr)
             for (int64_t i = first; i < a.n; i += step) a.lse[i] = 0.f;
+        if (a.largest != nullptr)
+            for (int64_t k = first; k < 2 * a.K; k += step) a.largest[k] = 0u;
+        if (a.gx != nullptr) {
+            T *gx = static_cast<T *>(a.gx);
+            const int64_t all = a.n * a.K;
+            if (a.ldgx == a.K && (reinterpret_cast<uintptr_t>(gx) & 15) == 0) {
+                constexpr int64_t per = 16 / sizeof(T);
+                for (int64_t i = first; i < all / per; i += step) reinterpret_cast<uint4 *>(gx)[i] = make_uint4(0, 0, 0, 0);
+                if (first < all % per) gx[all / per * per + first] = from_f32<T>(0.f);
+            } else {
+                for (int64_t i = first; i < all; i += step) gx[i / a.K * a.ldgx + i % a.K] = from_f32<T>(0.f);
+            }
+        }
         return;
     }
     __shared__ int part[kListThreads / 32], before[kListThreads / 32];
@@ -511,8 +528,10 @@ template <int KIND, int PLANES>
 static int nll_product(const ProductCall &c, int64_t units, cudaStream_t s)
 {
     constexpr int smem = product_shared_bytes<KIND, PLANES>();
-    SGNN_CUDA_OK(cudaFuncSetAttribute(nll_product_kernel<KIND, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const int64_t grid = units < sm_count() ? units : sm_count();
+    static ResidentCache cache;
+    int resident = 0, rc = resident_blocks(nll_product_kernel<KIND, PLANES>, kPThreads, smem, smem, cache, &resident);
+    if (rc) return rc;
+    const int64_t grid = units < resident ? units : resident;
     nll_product_kernel<KIND, PLANES><<<(unsigned)grid, kPThreads, smem, s>>>(c);
     SGNN_LAUNCH_OK("linear_nll product");
     return SGNN_OK;
@@ -536,14 +555,15 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         nll_count_kernel<<<(unsigned)p.blocks, kListThreads, 0, s>>>(c.labels, c.mask, c.n, c.C, ints(p.counts));
         SGNN_LAUNCH_OK("linear_nll count");
     }
-    const NllStart start{c.labels, c.mask, c.n, c.C, p.cls_padded, ints(p.counts), ints(p.rows), ints(p.total), (int)p.blocks, c.bias,
-                         floats(p.bias2), f32 ? floats(p.w_down) : nullptr, c.lse, ints(p.failed), ints(p.joined)};
-    nll_start_kernel<T><<<(unsigned)p.blocks + blocks(ceil_div(p.cls_padded + (c.lse ? c.n : 0), 32)), kListThreads, 0, s>>>(start);
-    if (grad) SGNN_CUDA_OK(cudaMemset2DAsync(c.gx, c.ldgx * sizeof(T), 0, c.K * sizeof(T), c.n, s));
-
-    // the operands as the products read them
     const bool cols = f32 && grad;
     unsigned *largest = cols ? reinterpret_cast<unsigned *>(c.ws + p.largest) : nullptr;
+    const NllStart start{c.labels, c.mask, c.n, c.C, p.cls_padded, ints(p.counts), ints(p.rows), ints(p.total), (int)p.blocks, c.bias,
+                         floats(p.bias2), f32 ? floats(p.w_down) : nullptr, c.lse, ints(p.failed), ints(p.joined), largest, (int)c.K,
+                         grad ? c.gx : nullptr, c.ldgx};
+    const int64_t cleared = p.cls_padded + (c.lse ? c.n : 0) + (grad ? c.n * c.K / 8 : 0);
+    nll_start_kernel<T><<<(unsigned)p.blocks + blocks(ceil_div(cleared, 32)), kListThreads, 0, s>>>(start);
+
+    // the operands as the products read them
     TakeSide xs{RowSource{c.x, c.ldx, ints(p.rows), ints(p.total), 0, (int)c.K},
                 Planes{halves(p.x_row), p.ld, p.padded * p.ld},
                 Planes{cols ? halves(p.x_col) : nullptr, p.ld, p.padded * p.ld},
@@ -553,7 +573,6 @@ static int nll_run(const NllCall &c, const NllPlan &p)
                 Planes{cols ? halves(p.w_col) : nullptr, p.ld, c.C * p.ld},
                 cols ? largest + c.K : nullptr, f32 ? floats(p.w_down) : nullptr, p.copy_w ? (int)blocks(c.C) : 0};
     if (cols) {
-        SGNN_CUDA_OK(cudaMemsetAsync(largest, 0, 2 * c.K * 4, s));
         const int64_t rows = c.n > c.C ? c.n : c.C, tall = ceil_div(rows, 64) < 2 * sm_count() ? ceil_div(rows, 64) : 2 * sm_count();
         nll_column_max_kernel<<<dim3((unsigned)ceil_div(c.K, 32), (unsigned)tall, 2), 256, 0, s>>>(xs.src, ws.src, largest);
     }

@@ -1107,7 +1107,7 @@ def layer_norm_forward(x, gamma=None, beta=None, eps: float = 1e-5, checkpoint: 
 
 
 def _layer_norm_backward(gy, x, codes, params, stats, gamma, in_place):
-    code = _matrix(gy, "gy")
+    code = _ELEMENT[gy.dtype]
     n, H = gy.shape
     dev, dtype = gy.device, gy.dtype
     pcode = _vector(gamma, "gamma", dtype, H, dev)
@@ -1117,12 +1117,12 @@ def _layer_norm_backward(gy, x, codes, params, stats, gamma, in_place):
     rows = _row_major(gy)
     _need(not in_place or rows is gy, "in_place needs gy with contiguous rows")
     gy = rows
-    gx = gy if in_place else torch.empty((n, H), dtype=dtype, device=dev)
-    grads = torch.empty((2, H), dtype=torch.float32 if gamma is None else gamma.dtype, device=dev)
-    g_gamma, g_beta = grads[0], grads[1]
+    gx = gy if in_place else torch.empty_like(gy) if gy.is_contiguous() else torch.empty((n, H), dtype=dtype, device=dev)
+    g_gamma = torch.empty(H, dtype=torch.float32, device=dev) if gamma is None else torch.empty_like(gamma)
+    g_beta = torch.empty_like(g_gamma)
     lib = _cabi.lib()
     with _on(dev), _Logged("layer_norm_bwd", dev, n=n, H=H):
-        partials = torch.empty((lib.sgnn_layer_norm_blocks(), 2, H), dtype=torch.float32, device=dev)
+        partials = torch.empty(lib.sgnn_layer_norm_blocks() * 2 * H, dtype=torch.float32, device=dev)
         rc = lib.sgnn_layer_norm_backward(code, gy.data_ptr(), gy.stride(0), _ptr(x), x.stride(0) if x is not None else 0,
                                           _ptr(codes), codes.stride(0) if codes is not None else 0, _ptr(params),
                                           stats.data_ptr(), pcode, _ptr(gamma), gx.data_ptr(), gx.stride(0),
