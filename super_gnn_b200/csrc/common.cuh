@@ -50,9 +50,9 @@ int sm_count();
 #ifdef __CUDACC__
 
 // Blocks of `threads` threads and `smem` bytes that fit the SMs of the current device at once.  `smem_cap`: the largest
-// dynamic shared memory the kernel is ever launched with (its attribute is set once a device); a call whose `smem` varies
-// asks again.  Queries cost microseconds, as much as the smallest kernels: `cache` (one a kernel) keeps the answers of
-// the first devices, the same whoever writes them.
+// dynamic shared memory the kernel is ever launched with, what its attribute is set to.  Queries cost microseconds, as
+// much as the smallest kernels: `cache` (one a kernel) keeps the last answer of each of the first devices.  Calls that race
+// may at worst launch with another call's number of blocks, which is good for any size of grid.
 struct ResidentCache {
     int blocks[16] = {}, smem[16] = {};
 };
@@ -71,7 +71,7 @@ int resident_blocks(K kernel, int threads, size_t smem, size_t smem_cap, Residen
     int per_sm = 0;
     SGNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
     *blocks = sm_count() * (per_sm > 0 ? per_sm : 1);
-    if (dev < 16 && smem_cap == smem) cache.smem[dev] = (int)smem + 1, cache.blocks[dev] = *blocks;
+    if (dev < 16) cache.blocks[dev] = *blocks, cache.smem[dev] = (int)smem + 1;
     return SGNN_OK;
 }
 

@@ -14,6 +14,7 @@
 // outputs; longer rows to a block, which reads them again (from L1 / L2) for every step.  All sums are fp32: the variance
 // from the differences to the mean, the column sums per warp, then per block, then over the blocks, in a fixed order.
 #include "row_io.cuh"
+#include "umma.cuh"
 
 namespace sgnn {
 
@@ -110,6 +111,258 @@ norm_fwd_warp_kernel(const T *__restrict__ x, int64_t ldx, NormParam par, float 
             }
         }
     }
+}
+
+// ---------------------------------------------------------------------------
+// Packed rows that do not start on 16-byte boundaries (602 bf16 columns, say).  Eight rows together do: they are one run of
+// memory of a multiple of 16 bytes, which a bulk copy brings into shared memory whatever the width.  A block walks over
+// batches of eight rows, a row a warp, through a ring of such buffers: the copies of the next batches run while one is
+// computed, and the results go back from the buffer they were computed in.  With loads of one or two elements a thread instead,
+// 100003 x 602 in bf16 took 117 us forward and 303 us backward (too few bytes on their way, and 146 registers).
+// ---------------------------------------------------------------------------
+constexpr int kStagedMax = 4;             // buffers of the ring
+constexpr size_t kStagedCap = 160 * 1024;  // shared memory of a block: two buffers of two operands of 1024 floats are 131 KB
+
+struct StagedRing {
+    uint8_t *base;  // buffer s at base + s * stride; the second operand of the backward `second` bytes behind
+    size_t stride, second;
+    int depth;
+};
+
+// 8 H sizeof(T) bytes from each of one or two operands into buffer s; the last batch of a matrix may be short and is copied
+// by the threads.
+template <class T>
+__device__ __forceinline__ void staged_load(const StagedRing &ring, int s, const T *p, const T *q, int64_t batch, int64_t full, int64_t n,
+                                            int H, uint64_t *bar)
+{
+    if (batch >= full || threadIdx.x != 0) return;
+    const unsigned bytes = (unsigned)(kNormWarps * H * sizeof(T));
+    uint8_t *at = ring.base + s * ring.stride;
+    bar_expect(bar, q ? 2 * bytes : bytes);
+    bulk_load(at, p + batch * kNormWarps * H, bytes, bar);
+    if (q) bulk_load(at + ring.second, q + batch * kNormWarps * H, bytes, bar);
+}
+template <class T>
+__device__ __forceinline__ void staged_copy_in(T *dst, const T *src, int64_t batch, int64_t n, int H)
+{
+    const int64_t first = batch * kNormWarps * H, count = n * H - first;
+    for (int64_t i = threadIdx.x; i < count; i += kNormThreads) dst[i] = src[first + i];
+}
+template <class T>
+__device__ __forceinline__ void staged_copy_out(T *dst, const T *src, int64_t batch, int64_t n, int H)
+{
+    const int64_t first = batch * kNormWarps * H, count = n * H - first;
+    for (int64_t i = threadIdx.x; i < count; i += kNormThreads) dst[first + i] = src[i];
+}
+
+template <class T, int E>
+__device__ __forceinline__ void shared_get(const T *p, float (&v)[E])
+{
+    union {
+        typename Word<E * sizeof(T)>::type w;
+        T e[E];
+    } u;
+    u.w = *reinterpret_cast<const typename Word<E * sizeof(T)>::type *>(p);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = to_f32<T>(u.e[i]);
+}
+template <class T, int E>
+__device__ __forceinline__ void shared_put(T *p, const float (&v)[E])
+{
+    union {
+        typename Word<E * sizeof(T)>::type w;
+        T e[E];
+    } u;
+#pragma unroll
+    for (int i = 0; i < E; ++i) u.e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<typename Word<E * sizeof(T)>::type *>(p) = u.w;
+}
+
+// One walk over the batches of a block: `row(data, other, r)` computes a row of this warp in place of `data`.
+// Every wait is for a copy this block has issued.  *gone: a copy did not come within the bound; no result is written from then
+// on, and a NaN in the statistics or the column sums says so.
+template <class T, class Row>
+__device__ __forceinline__ void staged_walk(const StagedRing &ring, const T *p, const T *q, T *out, int64_t n, int H, uint64_t *full_bar,
+                                            volatile int *gone, Row row)
+{
+    const int64_t batches = (n + kNormWarps - 1) / kNormWarps, full = n / kNormWarps;
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ring.depth; ++s) bar_init(full_bar + s, 1);
+        *gone = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    for (int s = 0; s < ring.depth; ++s)
+        if ((int64_t)blockIdx.x + (int64_t)s * gridDim.x < batches)
+            staged_load(ring, s, p, q, (int64_t)blockIdx.x + (int64_t)s * gridDim.x, full, n, H, full_bar + s);
+    int s = 0;
+    unsigned phase = 0;
+    for (int64_t b = blockIdx.x; b < batches; b += gridDim.x) {
+        T *data = reinterpret_cast<T *>(ring.base + s * ring.stride);
+        T *other = reinterpret_cast<T *>(ring.base + s * ring.stride + ring.second);
+        if (b < full) {
+            bar_wait(full_bar + s, phase, gone);
+        } else {
+            staged_copy_in(data, p, b, n, H);
+            if (q) staged_copy_in(other, q, b, n, H);
+            __syncthreads();
+        }
+        const int64_t r = b * kNormWarps + warp;
+        if (r < n) row(data + (size_t)warp * H, other + (size_t)warp * H, r);
+        async_fence();
+        __syncthreads();
+        if (*gone) break;  // the same for every thread: read after the barrier, written before it
+        if (b >= full) {
+            staged_copy_out(out, data, b, n, H);  // the last batch of all
+        } else if (threadIdx.x == 0) {
+            bulk_store(out + b * kNormWarps * H, data, (unsigned)(kNormWarps * H * sizeof(T)));
+            store_commit();
+        }
+        // refill the buffer before this one: its store was issued a batch ago
+        const int64_t next = b + (int64_t)(ring.depth - 1) * gridDim.x;
+        if (b != blockIdx.x && next < batches) {
+            const int before = s == 0 ? ring.depth - 1 : s - 1;
+            if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            staged_load(ring, before, p, q, next, full, n, H, full_bar + before);
+        }
+        if (++s == ring.depth) s = 0, phase ^= 1;
+    }
+    if (threadIdx.x == 0) {
+        store_wait_all();
+        if (*gone)
+            for (int i = 0; i < ring.depth; ++i) bar_drain(full_bar + i, phase);
+    }
+}
+
+template <class T, int E, int NV>
+__global__ void __launch_bounds__(kNormThreads)
+norm_fwd_staged_kernel(const T *__restrict__ x, NormParam par, float eps, T *__restrict__ y, float2 *__restrict__ stats, int64_t n, int H,
+                       size_t stride, int depth)
+{
+    extern __shared__ __align__(128) uint8_t area[];
+    __shared__ uint64_t bars[kStagedMax];
+    __shared__ int gone;
+    float *ga = reinterpret_cast<float *>(area), *be = ga + H;
+    for (int c = threadIdx.x; c < H; c += kNormThreads) {
+        float g[1], b[1];
+        load_param<T, 1>(par.gamma, par.f32, c, 1.f, g);
+        load_param<T, 1>(par.beta, par.f32, c, 0.f, b);
+        ga[c] = g[0], be[c] = b[0];
+    }
+    const StagedRing ring{area + ((size_t)2 * H * sizeof(float) + 127) / 128 * 128, stride, 0, depth};
+    const int lane = threadIdx.x & 31;
+    const float invH = 1.0f / (float)H;
+    staged_walk<T>(ring, x, static_cast<const T *>(nullptr), y, n, H, bars, &gone, [&](T *data, T *, int64_t r) {
+        float v[NV][E];
+        float s = 0.f, q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+                shared_get<T, E>(data + c, v[i]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s += v[i][e];
+            }
+        }
+        const float mean = all_sum(s) * invH;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((lane + 32 * i) * E < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[i][e] -= mean, q += v[i][e] * v[i][e];
+            }
+        }
+        const float rstd = __frsqrt_rn(all_sum(q) * invH + eps);
+        if (lane == 0) stats[r] = make_float2(mean, rstd);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[i][e] = v[i][e] * rstd * ga[c + e] + be[c + e];
+                shared_put<T, E>(data + c, v[i]);
+            }
+        }
+    });
+    if (threadIdx.x == 0 && gone) stats[blockIdx.x % n] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
+}
+
+template <class T, int E, int NV>
+__global__ void __launch_bounds__(kNormThreads)
+norm_bwd_staged_kernel(const T *__restrict__ gy, const T *__restrict__ x, const float2 *__restrict__ stats, NormParam par,
+                       T *__restrict__ gx, float *__restrict__ partials, int64_t n, int H, size_t stride, size_t second, int depth)
+{
+    extern __shared__ __align__(128) uint8_t area[];
+    __shared__ uint64_t bars[kStagedMax];
+    __shared__ int gone;
+    float *ga = reinterpret_cast<float *>(area);
+    for (int c = threadIdx.x; c < H; c += kNormThreads) {
+        float g[1];
+        load_param<T, 1>(par.gamma, par.f32, c, 1.f, g);
+        ga[c] = g[0];
+    }
+    const StagedRing ring{area + ((size_t)H * sizeof(float) + 127) / 128 * 128, stride, second, depth};
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float invH = 1.0f / (float)H;
+    float sg[NV][E], sb[NV][E];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) sg[i][e] = sb[i][e] = 0.f;
+    staged_walk<T>(ring, gy, x, gx, n, H, bars, &gone, [&](T *data, T *other, int64_t r) {
+        float a[NV][E], xh[NV][E];
+        const float2 st = __ldg(stats + r);
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+                shared_get<T, E>(data + c, a[i]);
+                shared_get<T, E>(other + c, xh[i]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    xh[i][e] = (xh[i][e] - st.x) * st.y;
+                    sg[i][e] += a[i][e] * xh[i][e];
+                    sb[i][e] += a[i][e];
+                    a[i][e] *= ga[c + e];
+                    s1 += a[i][e];
+                    s2 += a[i][e] * xh[i][e];
+                }
+            }
+        }
+        const float m1 = all_sum(s1) * invH, m2 = all_sum(s2) * invH;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + 32 * i) * E;
+            if (c < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) a[i][e] = st.y * (a[i][e] - m1 - xh[i][e] * m2);
+                shared_put<T, E>(data + c, a[i]);
+            }
+        }
+    });
+    __syncthreads();
+    // the block's column sums: the buffers are free (the last store from them has been waited for)
+    float *sums = reinterpret_cast<float *>(ring.base);
+    const float bad = gone ? __int_as_float(0x7fffffff) : 0.f;
+    for (int w = 0; w < kNormWarps; ++w) {  // one warp after the other
+        if (warp == w) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (lane + 32 * i) * E;
+                if (c < H) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        sums[c + e] = (w ? sums[c + e] : bad) + sg[i][e];
+                        sums[H + c + e] = (w ? sums[H + c + e] : bad) + sb[i][e];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    for (int k = threadIdx.x; k < 2 * H; k += kNormThreads) partials[(size_t)blockIdx.x * 2 * H + k] = sums[k];
 }
 
 // sum over the block, the same value in every thread
@@ -477,6 +730,76 @@ static int norm_bwd_launch(const NormCall &c, int *blocks)
     return SGNN_OK;
 }
 
+// Staged rows: packed operands on 16-byte boundaries, rows of a warp's length; where narrow accesses were the alternative.
+// The ring has as many buffers as leave room for two blocks an SM, at least two, at most four.
+static bool norm_can_stage(const NormCall &c, size_t bytes)
+{
+    const bool fwd = c.y != nullptr;
+    const auto packed = [&](const void *p, int64_t ld) { return ld == c.H && aligned16(p); };
+    return c.n >= kNormWarps && c.H <= 1024 && c.H * bytes >= 128 && packed(c.x, c.ldx) &&
+           (fwd ? packed(c.y, c.ldy) : packed(c.gy, c.ldg) && packed(c.gx, c.ldgx));
+}
+struct NormStage {
+    size_t stride, second, smem;
+    int depth;
+};
+static NormStage norm_stage(const NormCall &c, size_t bytes, int operands, int vectors)
+{
+    NormStage g{};
+    const size_t one = ((size_t)kNormWarps * c.H * bytes + 127) / 128 * 128;
+    const size_t head = ((size_t)vectors * c.H * sizeof(float) + 127) / 128 * 128;
+    g.second = operands == 2 ? one : 0;
+    g.stride = one * operands;
+    g.depth = (int)((110 * 1024 - head) / g.stride);
+    g.depth = g.depth < 2 ? 2 : g.depth > kStagedMax ? kStagedMax : g.depth;
+    size_t ring = g.stride * g.depth;
+    const size_t sums = 2 * (size_t)c.H * sizeof(float);
+    if (ring < sums) ring = sums;
+    g.smem = head + ring;
+    return g;
+}
+
+template <class T, int E, int NV>
+static int norm_fwd_staged(const NormCall &c)
+{
+    static ResidentCache cache;
+    const NormStage g = norm_stage(c, sizeof(T), 1, 2);
+    int grid = 0;
+    int rc = norm_grid(norm_fwd_staged_kernel<T, E, NV>, c.n, kNormWarps, g.smem, kStagedCap, cache, &grid);
+    if (rc) return rc;
+    norm_fwd_staged_kernel<T, E, NV><<<grid, kNormThreads, g.smem, c.stream>>>(static_cast<const T *>(c.x), c.par, c.eps,
+                                                                             static_cast<T *>(c.y), c.stats, c.n, c.H, g.stride, g.depth);
+    SGNN_LAUNCH_OK("layer norm forward");
+    return SGNN_OK;
+}
+template <class T, int E, int NV>
+static int norm_bwd_staged(const NormCall &c, int *blocks)
+{
+    static ResidentCache cache;
+    const NormStage g = norm_stage(c, sizeof(T), 2, 1);
+    int rc = norm_grid(norm_bwd_staged_kernel<T, E, NV>, c.n, kNormWarps, g.smem, kStagedCap, cache, blocks);
+    if (rc) return rc;
+    norm_bwd_staged_kernel<T, E, NV><<<*blocks, kNormThreads, g.smem, c.stream>>>(
+        static_cast<const T *>(c.gy), static_cast<const T *>(c.x), c.stats, c.par, static_cast<T *>(c.gx), c.partials, c.n, c.H, g.stride,
+        g.second, g.depth);
+    SGNN_LAUNCH_OK("layer norm backward");
+    return SGNN_OK;
+}
+// 8, 16 or 32 elements a lane, two at a time where 16-bit rows of even length allow it
+#define SGNN_NORM_STAGED(T, fn, ...)                                                                                    \
+    do {                                                                                                                \
+        if constexpr (sizeof(T) == 2) {                                                                                 \
+            if (c.H % 2 == 0) {                                                                                         \
+                if (c.H <= 256) return fn<T, 2, 4>(c, ##__VA_ARGS__);                                                   \
+                if (c.H <= 640) return fn<T, 2, 10>(c, ##__VA_ARGS__);                                                  \
+                return fn<T, 2, 16>(c, ##__VA_ARGS__);                                                                  \
+            }                                                                                                           \
+        }                                                                                                               \
+        if (c.H <= 256) return fn<T, 1, 8>(c, ##__VA_ARGS__);                                                           \
+        if (c.H <= 640) return fn<T, 1, 20>(c, ##__VA_ARGS__);                                                          \
+        return fn<T, 1, 32>(c, ##__VA_ARGS__);                                                                          \
+    } while (0)
+
 // fn<T, E, NV, CK>(c, ...) with the accesses a lane needs for a row (NV = 0: the block kernel)
 #define SGNN_NORM_NV(T, E, fn, ...)                                                                                     \
     do {                                                                                                                \
@@ -504,6 +827,11 @@ static int norm_fwd_dispatch(const NormCall &c)
     const RowOperand ops[] = {{c.x, c.ldx, b}, {c.y, c.ldy, b}, {c.par.gamma, 0, pb}, {c.par.beta, 0, pb},
                               {CK ? c.codes : nullptr, c.ldc, 1}};
     const int e = row_step(c.H, wide, ops);
+    if (!CK && e != wide && norm_can_stage(c, b)) {
+        if (c.dtype == SGNN_F32) SGNN_NORM_STAGED(float, norm_fwd_staged);
+        if (c.dtype == SGNN_BF16) SGNN_NORM_STAGED(__nv_bfloat16, norm_fwd_staged);
+        SGNN_NORM_STAGED(__half, norm_fwd_staged);
+    }
     if (c.dtype == SGNN_F32) {
         if (e == 4) SGNN_NORM_NV(float, 4, norm_fwd_launch, c);
         if (e == 2) SGNN_NORM_NV(float, 2, norm_fwd_launch, c);
@@ -527,6 +855,11 @@ static int norm_bwd_dispatch(const NormCall &c, int *blocks)
     const RowOperand ops[] = {{c.gy, c.ldg, b}, {c.gx, c.ldgx, b}, {c.par.gamma, 0, c.par.f32 ? 4 : b},
                               {CK ? nullptr : c.x, c.ldx, b}, {CK ? c.codes : nullptr, c.ldc, 1}};
     const int e = row_step(c.H, wide, ops);
+    if (!CK && e != wide && norm_can_stage(c, b)) {
+        if (c.dtype == SGNN_F32) SGNN_NORM_STAGED(float, norm_bwd_staged, blocks);
+        if (c.dtype == SGNN_BF16) SGNN_NORM_STAGED(__nv_bfloat16, norm_bwd_staged, blocks);
+        SGNN_NORM_STAGED(__half, norm_bwd_staged, blocks);
+    }
     if (c.dtype == SGNN_F32) {
         if (e == 4) SGNN_NORM_NV(float, 4, norm_bwd_launch, c, blocks);
         if (e == 2) SGNN_NORM_NV(float, 2, norm_bwd_launch, c, blocks);
@@ -542,6 +875,7 @@ static int norm_bwd_dispatch(const NormCall &c, int *blocks)
     SGNN_NORM_NV(__half, 1, norm_bwd_launch, c, blocks);
 }
 #undef SGNN_NORM_NV
+#undef SGNN_NORM_STAGED
 
 static int norm_check(const char *who, int dtype, int param_dtype, int64_t n, int64_t H)
 {
