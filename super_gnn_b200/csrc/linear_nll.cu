@@ -255,8 +255,10 @@ __device__ __forceinline__ void join_stats(float &mx, float &sum, float2 v)
     mx = top;
 }
 
-// lse of the rows of a chunk from the parts of their tiles: 32 rows a block, the parts dealt over its 32 warps.  The sum of
-// their losses goes to loss_part; the block that comes last of all chunks adds those up, in their order.
+// lse of the rows of a chunk from the parts of their tiles: eight rows a block, the parts dealt over 128 groups of eight
+// threads.  The sum of their losses goes to loss_part; the block that comes last of all chunks adds those up, in their order.
+constexpr int kJoinRows = 8;
+
 struct NllJoin {
     const float2 *stats;
     int parts, row0, row_cap;
@@ -273,44 +275,46 @@ struct NllJoin {
 
 __global__ void __launch_bounds__(1024) nll_join_kernel(const NllJoin a)
 {
-    __shared__ float2 red[32][33];
+    __shared__ float2 red[32][kJoinRows];
+    __shared__ float total[32];
     __shared__ bool last;
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int i = blockIdx.x * 32 + lane;  // of the chunk
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, row = threadIdx.x % kJoinRows;
+    const int i = blockIdx.x * kJoinRows + row;  // of the chunk
     const bool on = i < a.row_cap && a.row0 + i < *a.total;
     float mx = -INFINITY, sum = 0.f;
     if (on) {
 #pragma unroll 4
-        for (int p = g; p < a.parts; p += 32) join_stats(mx, sum, a.stats[(int64_t)p * a.row_cap + i]);
+        for (int p = threadIdx.x / kJoinRows; p < a.parts; p += 1024 / kJoinRows) join_stats(mx, sum, a.stats[(int64_t)p * a.row_cap + i]);
     }
-    red[g][lane] = make_float2(mx, sum);
-    __syncthreads();
-    // warp g joins row g: in a tree, the same for every number of parts
-    const float2 mine = red[lane][g];
-    mx = mine.x, sum = mine.y;
+    // the four groups of a warp, then the 32 warps, in trees: the same for every number of parts
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float2 other = make_float2(__shfl_xor_sync(FULL, mx, o), __shfl_xor_sync(FULL, sum, o));
-        join_stats(mx, sum, other);
+    for (int o = 16; o >= kJoinRows; o >>= 1) join_stats(mx, sum, make_float2(__shfl_xor_sync(FULL, mx, o), __shfl_xor_sync(FULL, sum, o)));
+    if (lane < kJoinRows) red[g][row] = make_float2(mx, sum);
+    __syncthreads();
+    if (g < kJoinRows) {  // warp g: row g of the block
+        const float2 mine = red[lane][g];
+        mx = mine.x, sum = mine.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) join_stats(mx, sum, make_float2(__shfl_xor_sync(FULL, mx, o), __shfl_xor_sync(FULL, sum, o)));
+        const int r = blockIdx.x * kJoinRows + g;
+        if (lane == 0) {
+            float loss = 0.f;
+            if (r < a.row_cap && a.row0 + r < *a.total) {
+                const float l = mx + log2f(sum);
+                a.lse2[r] = l;
+                if (a.lse_out) a.lse_out[a.rows[a.row0 + r]] = l * kLn2;
+                loss = (l - a.picked2[r]) * kLn2;
+            }
+            total[g] = loss;
+        }
     }
     __syncthreads();
-    if (lane == 0) red[0][g] = make_float2(mx, sum);
-    __syncthreads();
-    if (g == 0) {
-        const float2 v = red[0][lane];
+    if (threadIdx.x == 0) {
         float loss = 0.f;
-        if (on) {
-            const float l = v.x + log2f(v.y);
-            a.lse2[i] = l;
-            if (a.lse_out) a.lse_out[a.rows[a.row0 + i]] = l * kLn2;
-            loss = (l - a.picked2[i]) * kLn2;
-        }
-        loss = all_sum(loss);
-        if (lane == 0) {
-            a.loss_part[blockIdx.x] = loss;
-            __threadfence();
-            last = atomicAdd(a.joined, 1) == a.all_count - 1;
-        }
+        for (int r = 0; r < kJoinRows; ++r) loss += total[r];
+        a.loss_part[blockIdx.x] = loss;
+        __threadfence();
+        last = atomicAdd(a.joined, 1) == a.all_count - 1;
     }
     __syncthreads();
     if (!last) return;
@@ -318,10 +322,10 @@ __global__ void __launch_bounds__(1024) nll_join_kernel(const NllJoin a)
     float s = 0.f;
     for (int p = threadIdx.x; p < a.all_count; p += 1024) s += __ldcg(a.all_parts + p);
     s = all_sum(s);
-    if (lane == 0) red[1][g].x = s;
+    if (lane == 0) total[g] = s;
     __syncthreads();
     if (g == 0) {
-        s = all_sum(red[1][lane].x);
+        s = all_sum(total[lane]);
         if (lane == 0) *a.loss = *a.failed ? __int_as_float(0x7fffffff) : s * a.inv_count;
     }
 }
@@ -361,12 +365,38 @@ nll_rows_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_s
     }
 }
 
-// gw and gb from the partial sums of the splits (and of all chunks)
+// gb of a piece from the sums over 32 rows of a chunk, onto those of the chunks before (acc); the last chunk writes the result.
+// 32 classes a block, the sums dealt over its 32 warps.
+template <class T>
+__global__ void __launch_bounds__(1024)
+nll_bias_out_kernel(const float *__restrict__ part, int64_t ld, int row0, int row_cap, const int *__restrict__ total, int count, float scale,
+                    float *__restrict__ acc, bool first, bool last, bool f32, void *__restrict__ gb)
+{
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    int rows = *total - row0;
+    rows = rows < 0 ? 0 : rows < row_cap ? rows : row_cap;
+    const int groups = (rows + kPM - 1) / kPM * (kPM / 32);  // whole tiles have been written
+    float s = 0.f;
+    if (c < count) {
+#pragma unroll 4
+        for (int i = g; i < groups; i += 32) s += part[(int64_t)i * ld + c];
+    }
+    red[g][lane] = s;
+    __syncthreads();
+    if (g != 0 || c >= count) return;
+    for (int w = 1; w < 32; ++w) s += red[w][lane];
+    if (!first) s += acc[c];
+    if (!last) acc[c] = s;
+    else if (f32) static_cast<float *>(gb)[c] = s * scale;
+    else static_cast<T *>(gb)[c] = from_f32<T>(s * scale);
+}
+
+// gw from the partial sums of the splits (and of all chunks)
 template <class T>
 __global__ void __launch_bounds__(256)
-nll_weight_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_split, const float *__restrict__ bias_acc,
-                      int splits, int64_t C, int K, float scale, const unsigned *__restrict__ largest, T *__restrict__ gw,
-                      int64_t ldgw, bool gb_f32, void *__restrict__ gb)
+nll_weight_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_split, int splits, int64_t C, int K, float scale,
+                      const unsigned *__restrict__ largest, T *__restrict__ gw, int64_t ldgw)
 {
     const int lane = threadIdx.x & 31;
     for (int64_t c = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); c < C; c += (int64_t)gridDim.x * 8) {
@@ -376,12 +406,6 @@ nll_weight_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc
             for (int s = 0; s < splits; ++s) v += acc[s * acc_split + c * acc_ld + k];
             if (largest != nullptr) plane_scale(__uint_as_float(__ldg(largest + k)), up, down);
             gw[c * ldgw + k] = from_f32<T>(v * scale * down);
-        }
-        if (lane == 0 && gb != nullptr) {
-            float v = 0.f;
-            for (int s = 0; s < splits; ++s) v += bias_acc[s * C + c];
-            if (gb_f32) static_cast<float *>(gb)[c] = v * scale;
-            else static_cast<T *>(gb)[c] = from_f32<T>(v * scale);
         }
     }
 }
@@ -421,7 +445,7 @@ struct NllPlan {
     bool copy_w, direct;
     size_t counts, rows, total, failed, joined, label, picked2, lse2, loss_part, bias2, stats;
     size_t x_row, x_col, w_row, w_col, x_down, w_down, largest;
-    size_t grad, acc_x, acc_w, bias_acc, bytes;
+    size_t grad, acc_x, acc_w, bias_part, bias_acc, bytes;
 };
 
 // Rows in chunks, classes in pieces, reductions in splits: of the chunk sizes up to 128 tiles the one whose modelled time is
@@ -477,7 +501,7 @@ static NllPlan nll_plan(int dtype, int64_t n, int64_t K, int64_t C, bool grad, b
     const size_t mat_x = (size_t)p.planes * p.padded * p.ld * 2, mat_w = (size_t)p.planes * C * p.ld * 2;
     p.counts = take(p.blocks * 4), p.rows = take(n * 4), p.total = take(4), p.failed = take(4), p.joined = take(4);
     p.label = take(p.padded * 4), p.picked2 = take(p.padded * 4), p.lse2 = take(p.row_cap * 4);
-    p.loss_part = take(p.chunks * p.row_cap / 32 * 4), p.bias2 = take(p.cls_padded * 4);
+    p.loss_part = take(p.chunks * p.row_cap / kJoinRows * 4), p.bias2 = take(p.cls_padded * 4);
     p.stats = take((size_t)p.cls_padded / 128 * p.row_cap * 8);
     p.x_row = take(mat_x), p.w_row = take(p.copy_w ? mat_w : 0);
     if (f32) {
@@ -488,7 +512,8 @@ static NllPlan nll_plan(int dtype, int64_t n, int64_t K, int64_t C, bool grad, b
         p.grad = take((size_t)p.planes * p.row_cap * p.piece * 2);
         p.acc_x = take((size_t)p.row_splits * p.row_cap * p.acc_ld * 4);
         p.acc_w = take(p.direct ? 0 : (size_t)p.weight_splits * C * p.acc_ld * 4);
-        p.bias_acc = take(p.direct ? 0 : (size_t)p.weight_splits * C * 4);
+        p.bias_part = take((size_t)p.row_cap / 32 * p.piece * 4);
+        p.bias_acc = take(p.chunks > 1 ? (size_t)C * 4 : 0);
     }
     p.bytes = at;
     return p;
@@ -592,6 +617,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
     lc.scale = c.inv_count * (f32 ? 1.0f / kGradScale : 1.0f);
     const int64_t x_split = p.row_cap * p.acc_ld, w_split = c.C * p.acc_ld;
     if (grad) {
+        lc.bias_part = c.gb ? floats(p.bias_part) : nullptr, lc.grad_ld = p.piece;
         xc = lc, wc = lc;
         uint16_t *g = halves(p.grad);
         const int64_t plane = p.row_cap * p.piece;
@@ -602,17 +628,15 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         if ((rc = umma_tensor_map(&wc.a, g, !f32, p.piece, p.row_cap, p.piece, PLANES, plane, kPK))) return rc;
         if ((rc = umma_tensor_map(&wc.b, f32 ? xs.col.p : xs.row.p, !f32, c.K, p.padded, p.ld, PLANES, xs.row.stride, kPK))) return rc;
         xc.splits = p.row_splits, wc.splits = p.weight_splits;
-        wc.direct = p.direct, wc.direct_bf16 = !f32, wc.gb_f32 = c.bias.f32, wc.col_largest = largest;
+        wc.direct = p.direct, wc.direct_bf16 = !f32, wc.col_largest = largest;
         if (p.direct) {
-            wc.gb = c.gb;
             rc = umma_store_map(&wc.o, c.gw, f32 ? StoreType::kF32 : StoreType::kBf16, c.K, c.C, c.ldgw, 1, c.C * c.ldgw, f32 ? 32 : 64);
         } else {
-            wc.bias_out = floats(p.bias_acc);
             rc = umma_store_map(&wc.o, floats(p.acc_w), StoreType::kF32, p.acc_ld, c.C, p.acc_ld, p.weight_splits, w_split, 32);
         }
         if (rc) return rc;
     }
-    const int64_t tiles_k = ceil_div(c.K, kPN), join_blocks = p.row_cap / 32, tiles_m = p.row_cap / kPM;
+    const int64_t tiles_k = ceil_div(c.K, kPN), join_blocks = p.row_cap / kJoinRows, tiles_m = p.row_cap / kPM;
     for (int64_t q = 0; q < p.chunks; ++q) {
         const int row0 = (int)(q * p.row_cap);
         for (ProductCall *k : {&lc, &xc, &wc}) k->row0 = row0;
@@ -633,6 +657,13 @@ static int nll_run(const NllCall &c, const NllPlan &p)
             if ((rc = nll_product<kRowGrad, PLANES>(xc, tiles_m * tiles_k * p.row_splits, s))) return rc;
             wc.add = q > 0;
             if ((rc = nll_product<kWeightGrad, PLANES>(wc, ceil_div(count, kPM) * tiles_k * p.weight_splits, s))) return rc;
+            if (c.gb) {
+                char *gb = static_cast<char *>(c.gb) + first * (c.bias.f32 ? 4 : sizeof(T));
+                nll_bias_out_kernel<T><<<(unsigned)ceil_div(count, 32), 1024, 0, s>>>(
+                    lc.bias_part, p.piece, row0, (int)p.row_cap, ints(p.total), (int)count, lc.scale,
+                    p.chunks > 1 ? floats(p.bias_acc) + first : nullptr, q == 0, q + 1 == p.chunks, c.bias.f32, gb);
+                SGNN_LAUNCH_OK("linear_nll bias gradient");
+            }
         }
         const bool dealt = p.row_splits >= 8;
         const dim3 out_grid = dealt ? dim3((unsigned)(p.row_cap < wide ? p.row_cap : wide), (unsigned)ceil_div(c.K, 32)) : dim3(blocks(p.row_cap));
@@ -642,8 +673,8 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         SGNN_LAUNCH_OK("linear_nll row gradients");
     }
     if (grad && !p.direct) {
-        nll_weight_out_kernel<T><<<blocks(c.C), 256, 0, s>>>(floats(p.acc_w), p.acc_ld, w_split, floats(p.bias_acc), p.weight_splits, c.C,
-                                                             (int)c.K, lc.scale, largest, static_cast<T *>(c.gw), c.ldgw, c.bias.f32, c.gb);
+        nll_weight_out_kernel<T><<<blocks(c.C), 256, 0, s>>>(floats(p.acc_w), p.acc_ld, w_split, p.weight_splits, c.C, (int)c.K, lc.scale,
+                                                             largest, static_cast<T *>(c.gw), c.ldgw);
         SGNN_LAUNCH_OK("linear_nll weight gradients");
     }
     return SGNN_OK;

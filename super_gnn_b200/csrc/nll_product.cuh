@@ -9,8 +9,10 @@
 // the outputs.  The operands lie as their matrices do: x and W are read along k by the first product and across it by the
 // other two, G along the classes by the second and across by the third, so that nothing is ever transposed in memory.
 //
-// fp32 operands come as two fp16 planes (v 2^e = v0 + v1, 22 bits; see split planes in linear_nll.cu) and three products
-// v0 w0 + v0 w1 + v1 w0 a tile; bf16 operands as one plane and one product.
+// fp32 operands come as two fp16 planes (v 2^e = v0 + v1, 22 bits; see linear_nll.cu) and three products
+// v0 w0 + v0 w1 + v1 w0 a tile; bf16 operands as one plane and one product.  Tensor memory rounds every addition towards zero, a
+// relative 2^-25 on average, so in the two gradients, whose reductions are long, the cross products of the planes, 2^-11 of
+// the others, have sums of their own, and the main sums a third of the additions.
 #pragma once
 #include "umma.cuh"
 
@@ -19,7 +21,7 @@ namespace sgnn {
 constexpr int kPM = 128, kPN = 256, kPK = 64;  // tile of a product, step of its reduction
 constexpr int kPEpilogueWarps = 8;
 constexpr int kPThreads = (kPEpilogueWarps + 2) * 32;
-constexpr int kPAccCols = 512;  // all of the tensor memory: two results, or one and the sums of the bias gradient
+constexpr int kPAccCols = 512;  // all of the tensor memory: two results, or one and its cross products
 
 enum ProductKind { kLogitStats, kLogitGrad, kRowGrad, kWeightGrad };
 
@@ -40,14 +42,14 @@ struct ProductCall {
     const float *lse2;       // [row_cap]
     const float *picked2;    // [row_cap] the label's logit
     const int *label;        // [row_cap]
+    float *bias_part;        // [row_cap / 32, grad_ld]: sums of G over 32 rows, or nullptr
+    int64_t grad_ld;
     // gradients of rows: o = [splits, row_cap, K rounded up to 32] fp32
     bool add;                // onto what the pieces (chunks) before have left there
     // gradients of weights: o = [splits, C, K rounded up to 32] fp32, or the result itself where nothing is left to add
-    bool direct, direct_bf16, gb_f32;
+    bool direct, direct_bf16;
     const unsigned *col_largest;  // fp32: the columns of x are scaled by it
     float scale;
-    void *gb;
-    float *bias_out;         // [splits, C] when not direct
     int64_t classes;
 };
 
@@ -57,7 +59,6 @@ struct ProductShared {
     static constexpr int kA = kPM * kPK * 2, kB = kPN * kPK * 2;
     static constexpr int kStageBytes = PLANES * (kA + kB);
     static constexpr int kBox = 4096;  // result box of a warp: 32 rows of 128 bytes
-    static constexpr int kOnes = 256;
 };
 
 template <int KIND, int PLANES>
@@ -67,7 +68,7 @@ constexpr int product_shared_bytes()
     const int ring = S::kStages * S::kStageBytes;
     if (KIND == kLogitStats) return ring + 2 * kPN * 8 + 256;
     if (KIND == kLogitGrad) return ring + kPEpilogueWarps * S::kBox + kPN * 8 + 256;
-    return ring + kPEpilogueWarps * S::kBox + S::kOnes + 256;
+    return ring + kPEpilogueWarps * S::kBox + 256;
 }
 
 // sizes of the product of this chunk and piece, from the number of rows in the loss
@@ -143,13 +144,14 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     using S = ProductShared<PLANES>;
     constexpr bool kLogits = KIND == kLogitStats || KIND == kLogitGrad;
     constexpr bool kAmn = KIND == kWeightGrad, kBmn = !kLogits;
-    constexpr int kAcc = KIND == kWeightGrad ? 1 : 2;  // results in flight
+    constexpr bool kCross = !kLogits && PLANES == 2;  // cross products have their own sums, in the other half of the tensor memory
+    constexpr int kAcc = kCross ? 1 : 2;              // results in flight
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *boxes = base + S::kStages * S::kStageBytes;
-    uint8_t *ones = boxes + (KIND == kLogitStats ? 0 : kPEpilogueWarps * S::kBox);
-    float *column = reinterpret_cast<float *>(ones);  // logits: bias, then scale, of the classes of a tile
+    uint8_t *after = boxes + (KIND == kLogitStats ? 0 : kPEpilogueWarps * S::kBox);
+    float *column = reinterpret_cast<float *>(after);  // logits: bias, then scale, of the classes of a tile
     constexpr int kColumns = KIND == kLogitStats ? 2 : 1;  // tiles whose classes are held at once
-    uint8_t *behind = ones + (kLogits ? kColumns * kPN * 8 : S::kOnes);
+    uint8_t *behind = after + (kLogits ? kColumns * kPN * 8 : 0);
     uint64_t *full = reinterpret_cast<uint64_t *>(behind);
     uint64_t *empty = full + S::kStages, *acc_full = empty + S::kStages, *acc_empty = acc_full + 2;
     uint64_t *drained = acc_empty + 2;
@@ -169,11 +171,6 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
         bar_init(drained, 1);
         *gone = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (KIND == kWeightGrad) {
-        const uint32_t one = c.bf16 ? 0x3F803F80u : 0x3C003C00u;
-        for (int i = threadIdx.x; i < S::kOnes / 4; i += kPThreads) reinterpret_cast<uint32_t *>(ones)[i] = one;
-        async_fence();
     }
     if (warp == kPEpilogueWarps + 1) tmem_alloc(slot, kPAccCols);
     tc_fence_before();
@@ -238,7 +235,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                 const ProductUnit t = product_unit(u, i);
                 const int left = u.n - t.n0;
                 const int n = kBmn ? (left < kPN ? (left + 15) / 16 * 16 : kPN) : kPN;
-                const uint32_t idesc = umma_idesc(c.bf16, kAmn, kBmn, n), idesc_ones = umma_idesc(c.bf16, kAmn, false, 16);
+                const uint32_t idesc = umma_idesc(c.bf16, kAmn, kBmn, n);
                 ok = bar_wait(acc_empty + acc, acc_phase ^ 1, gone);
                 if (!ok) break;
                 tc_fence_after();
@@ -256,7 +253,6 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         da[p] = umma_desc(at + p * S::kA, a_run, 1024);
                         db[p] = umma_desc(at + PLANES * S::kA + p * S::kB, b_run, 1024);
                     }
-                    const uint64_t dones = umma_desc_same(ones);
 #pragma unroll
                     for (int j = 0; j < kPK / 16; ++j) {
                         // sixteen steps of the reduction: 32 bytes along a row, or two groups of eight rows
@@ -264,12 +260,9 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         const bool more = k > 0 || j > 0;
                         umma(d, da[0] + sa, db[0] + sb, idesc, more);
                         if (PLANES == 2) {
-                            umma(d, da[0] + sa, db[PLANES - 1] + sb, idesc, true);
-                            umma(d, da[PLANES - 1] + sa, db[0] + sb, idesc, true);
-                        }
-                        if (KIND == kWeightGrad && t.n0 == 0) {
-                            umma(tmem + kPN, da[0] + sa, dones, idesc_ones, more);
-                            if (PLANES == 2) umma(tmem + kPN, da[PLANES - 1] + sa, dones, idesc_ones, true);
+                            const uint32_t dx = kCross ? tmem + kPN : d;
+                            umma(dx, da[0] + sa, db[PLANES - 1] + sb, idesc, !kCross || more);
+                            umma(dx, da[PLANES - 1] + sa, db[0] + sb, idesc, true);
                         }
                     }
                     tc_commit(empty + stage);
@@ -371,6 +364,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         if (PLANES == 2) v[e] *= kGradScale;
                     }
                     const int at = label - 32 * j;  // 0 .. 31: in these columns
+                    float *part = c.bias_part + (int64_t)(y0 >> 5) * c.grad_ld + x0;
                     if (PLANES == 1) {  // 64 columns a box: 128 bytes a row, two turns
                         if ((j & 1) == 0) box_free();
 #pragma unroll
@@ -392,8 +386,19 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                                 tma_store(&c.o, box, x0 + 32 * (j - 1), y0, 0);
                                 store_commit();
                             }
+                            if (c.bias_part != nullptr) {  // two columns a lane, down the rows of the box
+                                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                                for (int r = 0; r < 32; ++r) {
+                                    const uint32_t two = *reinterpret_cast<const uint32_t *>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                                    sum.x += __uint_as_float(two << 16), sum.y += __uint_as_float(two & 0xFFFF0000u);
+                                }
+                                *reinterpret_cast<float2 *>(part + 32 * (j - 1) + 2 * lane) = sum;
+                            }
                         }
                     } else {  // 32 columns of both planes: 64 bytes a row each
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = e == at ? own : v[e];
                         box_free();
                         uint8_t *r0 = box + lane * 64, *r1 = r0 + 2048;
                         const int turn = (lane >> 1) & 3;
@@ -411,39 +416,28 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                             *reinterpret_cast<uint4 *>(r0 + (q ^ turn) * 16) = w0;
                             *reinterpret_cast<uint4 *>(r1 + (q ^ turn) * 16) = w1;
                         }
-                        if (at >= 0 && at < 32) {
-                            const int off = ((at / 8) ^ turn) * 16 + at % 8 * 2;
-                            const __half h = __float2half_rn(own);
-                            *reinterpret_cast<__half *>(r0 + off) = h;
-                            *reinterpret_cast<__half *>(r1 + off) = __float2half_rn(own - __half2float(h));
-                        }
                         box_done();
                         if (lane == 0) {
                             tma_store(&c.o, box, x0 + 32 * j, y0, 0);
                             tma_store(&c.o, box + 2048, x0 + 32 * j, y0, 1);
                             store_commit();
                         }
-                    }
-                }
-            } else {
-                if (KIND == kWeightGrad && t.n0 == 0 && half == 0 && (c.gb != nullptr || c.bias_out != nullptr)) {
-                    uint32_t one;
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];"
-                                 : "=r"(one)
-                                 : "r"(tmem + kPN + ((uint32_t)quarter << 21)));
-                    tmem_load_wait();
-                    const float s = there ? __uint_as_float(one) : 0.f;
-                    if (row < u.m) {
-                        if (c.bias_out) {
-                            float *o = c.bias_out + t.split * c.classes + c.cls0 + row;
-                            *o = c.add ? *o + s : s;
-                        } else if (c.gb_f32) {
-                            static_cast<float *>(c.gb)[c.cls0 + row] = s * c.scale;
-                        } else {
-                            static_cast<__nv_bfloat16 *>(c.gb)[c.cls0 + row] = __float2bfloat16_rn(s * c.scale);
+                        if (c.bias_part != nullptr) {
+                            // 32 rows x 32 columns: every exchange halves the columns a lane carries; lane l ends with column l
+#pragma unroll
+                            for (int o = 16; o > 0; o >>= 1) {
+                                const bool upper = (lane & o) != 0;
+#pragma unroll
+                                for (int e = 0; e < o; ++e) {
+                                    const float keep = upper ? v[e + o] : v[e], give = upper ? v[e] : v[e + o];
+                                    v[e] = keep + __shfl_xor_sync(FULL, give, o);
+                                }
+                            }
+                            part[32 * j + lane] = v[0];
                         }
                     }
                 }
+            } else {
                 const bool direct = KIND == kWeightGrad && c.direct, wide = direct && c.direct_bf16;
                 const int y0 = t.m0 + quarter * 32 + (KIND == kWeightGrad ? c.cls0 : 0);
 #pragma unroll 1
@@ -452,6 +446,13 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                     if (k0 >= u.n) break;
                     tmem_load32(d + 32 * j, v);
                     tmem_load_wait();
+                    if (kCross) {
+                        float x[32];
+                        tmem_load32(d + kPN + 32 * j, x);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] += x[e];
+                    }
                     if (!there) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = 0.f;

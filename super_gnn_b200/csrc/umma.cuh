@@ -154,12 +154,6 @@ __device__ __forceinline__ uint64_t umma_desc(const void *p, unsigned run_bytes,
            (1ull << 46) | (2ull << 61);
 }
 
-// A 16-byte run that every row of an operand reads (16 rows x 16 steps, no swizzle, all strides zero)
-__device__ __forceinline__ uint64_t umma_desc_same(const void *p)
-{
-    return (uint64_t)((smem_addr(p) & 0x3FFFFu) >> 4) | (1ull << 46);
-}
-
 // 128 x n product of 16-bit operands with fp32 sums
 __device__ __forceinline__ uint32_t umma_idesc(bool bf16, bool a_mn, bool b_mn, int n)
 {
