@@ -49,6 +49,23 @@ int sm_count();
 // ---- device side ----------------------------------------------------------
 #ifdef __CUDACC__
 
+// Launch of one of a chain of kernels on a stream: its blocks may start while the kernel before them still runs and have to
+// come to wait_for_kernels_before() ahead of their first access to global memory; let_next_kernel_start() allows the kernel
+// behind the same.  Hides what a small kernel spends on being launched and set up (a microsecond or two).
+template <class... P, class... A>
+cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args)
+{
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+__device__ __forceinline__ void wait_for_kernels_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Blocks of `threads` threads and `smem` bytes that fit the SMs of the current device at once.  `smem_cap`: the largest
 // dynamic shared memory the kernel is ever launched with, what its attribute is set to.  Queries cost microseconds, as
 // much as the smallest kernels: `cache` (one a kernel) keeps the last answer of each of the first devices.  Calls that race

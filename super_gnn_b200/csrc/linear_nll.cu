@@ -35,10 +35,20 @@ __device__ __forceinline__ bool in_loss(const int64_t *labels, const uint8_t *ma
 __global__ void __launch_bounds__(kListThreads)
 nll_count_kernel(const int64_t *__restrict__ labels, const uint8_t *__restrict__ mask, int64_t n, int64_t C, int *__restrict__ counts)
 {
+    __shared__ int part[kListThreads / 32];
+    let_next_kernel_start();
+    wait_for_kernels_before();
     int c = 0;
+#pragma unroll
     for (int i = 0; i < kListRows / kListThreads; ++i)
-        c += __syncthreads_count(in_loss(labels, mask, (int64_t)blockIdx.x * kListRows + i * kListThreads + threadIdx.x, n, C));
-    if (threadIdx.x == 0) counts[blockIdx.x] = c;
+        c += in_loss(labels, mask, (int64_t)blockIdx.x * kListRows + i * kListThreads + threadIdx.x, n, C) ? 1 : 0;
+    c = __reduce_add_sync(FULL, c);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kListThreads / 32; ++w) c += part[w];
+        counts[blockIdx.x] = c;
+    }
 }
 
 struct NllBias {
@@ -76,6 +86,8 @@ struct NllStart {
 template <class T>
 __global__ void __launch_bounds__(kListThreads) nll_start_kernel(const NllStart a)
 {
+    let_next_kernel_start();
+    wait_for_kernels_before();
     if ((int)blockIdx.x >= a.blocks) {
         const int64_t first = (int64_t)(blockIdx.x - a.blocks) * kListThreads + threadIdx.x;
         const int64_t step = (int64_t)(gridDim.x - a.blocks) * kListThreads;
@@ -110,9 +122,13 @@ __global__ void __launch_bounds__(kListThreads) nll_start_kernel(const NllStart 
     __syncthreads();
     int at = 0;
     for (int w = 0; w < kListThreads / 32; ++w) at += part[w];
+    unsigned ons = 0;
+#pragma unroll
+    for (int i = 0; i < kListRows / kListThreads; ++i)
+        ons |= in_loss(a.labels, a.mask, (int64_t)blockIdx.x * kListRows + i * kListThreads + threadIdx.x, a.n, a.C) ? 1u << i : 0u;
     for (int i = 0; i < kListRows / kListThreads; ++i) {
         const int64_t r = (int64_t)blockIdx.x * kListRows + i * kListThreads + threadIdx.x;
-        const bool on = in_loss(a.labels, a.mask, r, a.n, a.C);
+        const bool on = (ons >> i & 1u) != 0;
         const unsigned vote = __ballot_sync(FULL, on);
         __syncthreads();
         if (lane == 0) before[warp] = __popc(vote);
@@ -166,6 +182,8 @@ __device__ __forceinline__ void store_split(const Planes &pl, int64_t at, float 
 __global__ void __launch_bounds__(256) nll_column_max_kernel(RowSource x, RowSource w, unsigned *__restrict__ largest)
 {
     __shared__ unsigned part[8][32];
+    let_next_kernel_start();
+    wait_for_kernels_before();
     const RowSource s = blockIdx.z == 0 ? x : w;
     const int k = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
     const int64_t n = source_rows(s), step = (int64_t)gridDim.y * 8;
@@ -198,6 +216,8 @@ struct TakeSide {
 template <class T, bool SPLIT>
 __global__ void __launch_bounds__(256) nll_take_kernel(const TakeSide xs, const TakeSide ws, const Picked pick)
 {
+    let_next_kernel_start();
+    wait_for_kernels_before();
     const bool is_x = (int)blockIdx.x < xs.blocks;
     const TakeSide &t = is_x ? xs : ws;
     const RowSource &s = t.src;
@@ -278,6 +298,8 @@ __global__ void __launch_bounds__(1024) nll_join_kernel(const NllJoin a)
     __shared__ float2 red[32][kJoinRows];
     __shared__ float total[32];
     __shared__ bool last;
+    let_next_kernel_start();
+    wait_for_kernels_before();
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, row = threadIdx.x % kJoinRows;
     const int i = blockIdx.x * kJoinRows + row;  // of the chunk
     const bool on = i < a.row_cap && a.row0 + i < *a.total;
@@ -339,6 +361,8 @@ nll_rows_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_s
                     const int *__restrict__ failed, T *__restrict__ gx, int64_t ldgx, int K, float *__restrict__ loss, bool dealt)
 {
     __shared__ float red[8][33];
+    let_next_kernel_start();
+    wait_for_kernels_before();
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
     const bool bad = *failed != 0;
     if (bad && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *loss = __int_as_float(0x7fffffff);
@@ -366,26 +390,31 @@ nll_rows_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_s
 }
 
 // gb of a piece from the sums over 32 rows of a chunk, onto those of the chunks before (acc); the last chunk writes the result.
-// 32 classes a block, the sums dealt over its 32 warps.
+// 32 classes a block, the sums dealt over its 32 warps; with few rows a thread adds up a class alone.
 template <class T>
 __global__ void __launch_bounds__(1024)
 nll_bias_out_kernel(const float *__restrict__ part, int64_t ld, int row0, int row_cap, const int *__restrict__ total, int count, float scale,
-                    float *__restrict__ acc, bool first, bool last, bool f32, void *__restrict__ gb)
+                    float *__restrict__ acc, bool first, bool last, bool f32, void *__restrict__ gb, bool dealt)
 {
     __shared__ float red[32][33];
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    let_next_kernel_start();
+    wait_for_kernels_before();
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = dealt ? blockIdx.x * 32 + lane : blockIdx.x * 1024 + threadIdx.x;
     int rows = *total - row0;
     rows = rows < 0 ? 0 : rows < row_cap ? rows : row_cap;
     const int groups = (rows + kPM - 1) / kPM * (kPM / 32);  // whole tiles have been written
     float s = 0.f;
     if (c < count) {
 #pragma unroll 4
-        for (int i = g; i < groups; i += 32) s += part[(int64_t)i * ld + c];
+        for (int i = dealt ? g : 0; i < groups; i += dealt ? 32 : 1) s += part[(int64_t)i * ld + c];
     }
-    red[g][lane] = s;
-    __syncthreads();
-    if (g != 0 || c >= count) return;
-    for (int w = 1; w < 32; ++w) s += red[w][lane];
+    if (dealt) {
+        red[g][lane] = s;
+        __syncthreads();
+        if (g != 0) return;
+        for (int w = 1; w < 32; ++w) s += red[w][lane];
+    }
+    if (c >= count) return;
     if (!first) s += acc[c];
     if (!last) acc[c] = s;
     else if (f32) static_cast<float *>(gb)[c] = s * scale;
@@ -398,6 +427,8 @@ __global__ void __launch_bounds__(256)
 nll_weight_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_split, int splits, int64_t C, int K, float scale,
                       const unsigned *__restrict__ largest, T *__restrict__ gw, int64_t ldgw)
 {
+    let_next_kernel_start();
+    wait_for_kernels_before();
     const int lane = threadIdx.x & 31;
     for (int64_t c = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); c < C; c += (int64_t)gridDim.x * 8) {
 #pragma unroll 4
@@ -557,8 +588,7 @@ static int nll_product(const ProductCall &c, int64_t units, cudaStream_t s)
     int resident = 0, rc = resident_blocks(nll_product_kernel<KIND, PLANES>, kPThreads, smem, smem, cache, &resident);
     if (rc) return rc;
     const int64_t grid = units < resident ? units : resident;
-    nll_product_kernel<KIND, PLANES><<<(unsigned)grid, kPThreads, smem, s>>>(c);
-    SGNN_LAUNCH_OK("linear_nll product");
+    SGNN_CUDA_OK(launch_chained(nll_product_kernel<KIND, PLANES>, dim3((unsigned)grid), kPThreads, smem, s, c));
     return SGNN_OK;
 }
 
@@ -577,8 +607,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
 
     // the rows in the loss, and what later kernels start from
     if (p.blocks > 1) {
-        nll_count_kernel<<<(unsigned)p.blocks, kListThreads, 0, s>>>(c.labels, c.mask, c.n, c.C, ints(p.counts));
-        SGNN_LAUNCH_OK("linear_nll count");
+        SGNN_CUDA_OK(launch_chained(nll_count_kernel, dim3((unsigned)p.blocks), kListThreads, 0, s, c.labels, c.mask, c.n, c.C, ints(p.counts)));
     }
     const bool cols = f32 && grad;
     unsigned *largest = cols ? reinterpret_cast<unsigned *>(c.ws + p.largest) : nullptr;
@@ -586,7 +615,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
                          floats(p.bias2), f32 ? floats(p.w_down) : nullptr, c.lse, ints(p.failed), ints(p.joined), largest, (int)c.K,
                          grad ? c.gx : nullptr, c.ldgx};
     const int64_t cleared = p.cls_padded + (c.lse ? c.n : 0) + (grad ? c.n * c.K / 8 : 0);
-    nll_start_kernel<T><<<(unsigned)p.blocks + blocks(ceil_div(cleared, 32)), kListThreads, 0, s>>>(start);
+    SGNN_CUDA_OK(launch_chained(nll_start_kernel<T>, dim3((unsigned)p.blocks + blocks(ceil_div(cleared, 32))), kListThreads, 0, s, start));
 
     // the operands as the products read them
     TakeSide xs{RowSource{c.x, c.ldx, ints(p.rows), ints(p.total), 0, (int)c.K},
@@ -599,11 +628,10 @@ static int nll_run(const NllCall &c, const NllPlan &p)
                 cols ? largest + c.K : nullptr, f32 ? floats(p.w_down) : nullptr, p.copy_w ? (int)blocks(c.C) : 0};
     if (cols) {
         const int64_t rows = c.n > c.C ? c.n : c.C, tall = ceil_div(rows, 64) < 2 * sm_count() ? ceil_div(rows, 64) : 2 * sm_count();
-        nll_column_max_kernel<<<dim3((unsigned)ceil_div(c.K, 32), (unsigned)tall, 2), 256, 0, s>>>(xs.src, ws.src, largest);
+        SGNN_CUDA_OK(launch_chained(nll_column_max_kernel, dim3((unsigned)ceil_div(c.K, 32), (unsigned)tall, 2), 256, 0, s, xs.src, ws.src, largest));
     }
-    nll_take_kernel<T, f32><<<(unsigned)(xs.blocks + ws.blocks), 256, 0, s>>>(
-        xs, ws, Picked{c.labels, c.w, c.ldw, c.bias, ints(p.label), floats(p.picked2)});
-    SGNN_LAUNCH_OK("linear_nll operands");
+    SGNN_CUDA_OK(launch_chained(nll_take_kernel<T, f32>, dim3((unsigned)(xs.blocks + ws.blocks)), 256, 0, s, xs, ws,
+                                Picked{c.labels, c.w, c.ldw, c.bias, ints(p.label), floats(p.picked2)}));
 
     // tensor maps: x and W along k (rows of a tile at once) and across it (64 steps of the reduction at once), G likewise
     ProductCall lc{}, xc{}, wc{};
@@ -646,8 +674,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         const NllJoin join{lc.stats, (int)(p.cls_padded / 128), row0, (int)p.row_cap, ints(p.rows), ints(p.total), lc.picked2,
                            floats(p.lse2), c.lse, floats(p.loss_part) + q * join_blocks, floats(p.loss_part),
                            (int)(p.chunks * join_blocks), c.inv_count, ints(p.joined), ints(p.failed), c.loss};
-        nll_join_kernel<<<(unsigned)join_blocks, 1024, 0, s>>>(join);
-        SGNN_LAUNCH_OK("linear_nll join");
+        SGNN_CUDA_OK(launch_chained(nll_join_kernel, dim3((unsigned)join_blocks), 1024, 0, s, join));
         if (!grad) continue;
         for (int64_t first = 0; first < c.C; first += p.piece) {
             const int64_t count = c.C - first < p.piece ? c.C - first : p.piece;
@@ -659,23 +686,22 @@ static int nll_run(const NllCall &c, const NllPlan &p)
             if ((rc = nll_product<kWeightGrad, PLANES>(wc, ceil_div(count, kPM) * tiles_k * p.weight_splits, s))) return rc;
             if (c.gb) {
                 char *gb = static_cast<char *>(c.gb) + first * (c.bias.f32 ? 4 : sizeof(T));
-                nll_bias_out_kernel<T><<<(unsigned)ceil_div(count, 32), 1024, 0, s>>>(
-                    lc.bias_part, p.piece, row0, (int)p.row_cap, ints(p.total), (int)count, lc.scale,
-                    p.chunks > 1 ? floats(p.bias_acc) + first : nullptr, q == 0, q + 1 == p.chunks, c.bias.f32, gb);
-                SGNN_LAUNCH_OK("linear_nll bias gradient");
+                const bool deal = p.row_cap / 32 > 32;
+                SGNN_CUDA_OK(launch_chained(nll_bias_out_kernel<T>, dim3((unsigned)ceil_div(count, deal ? 32 : 1024)), 1024, 0, s,
+                                            lc.bias_part, p.piece, row0, (int)p.row_cap, ints(p.total), (int)count, lc.scale,
+                                            p.chunks > 1 ? floats(p.bias_acc) + first : nullptr, q == 0, q + 1 == p.chunks,
+                                            c.bias.f32, gb, deal));
             }
         }
         const bool dealt = p.row_splits >= 8;
         const dim3 out_grid = dealt ? dim3((unsigned)(p.row_cap < wide ? p.row_cap : wide), (unsigned)ceil_div(c.K, 32)) : dim3(blocks(p.row_cap));
-        nll_rows_out_kernel<T><<<out_grid, 256, 0, s>>>(floats(p.acc_x), p.acc_ld, x_split, p.row_splits, row0, (int)p.row_cap, ints(p.rows),
-                                                        ints(p.total), lc.scale, cols ? largest + c.K : nullptr, ints(p.failed),
-                                                        static_cast<T *>(c.gx), c.ldgx, (int)c.K, c.loss, dealt);
-        SGNN_LAUNCH_OK("linear_nll row gradients");
+        SGNN_CUDA_OK(launch_chained(nll_rows_out_kernel<T>, out_grid, 256, 0, s, floats(p.acc_x), p.acc_ld, x_split, p.row_splits, row0,
+                                    (int)p.row_cap, ints(p.rows), ints(p.total), lc.scale, cols ? largest + c.K : nullptr, ints(p.failed),
+                                    static_cast<T *>(c.gx), c.ldgx, (int)c.K, c.loss, dealt));
     }
     if (grad && !p.direct) {
-        nll_weight_out_kernel<T><<<blocks(c.C), 256, 0, s>>>(floats(p.acc_w), p.acc_ld, w_split, p.weight_splits, c.C, (int)c.K, lc.scale,
-                                                             largest, static_cast<T *>(c.gw), c.ldgw);
-        SGNN_LAUNCH_OK("linear_nll weight gradients");
+        SGNN_CUDA_OK(launch_chained(nll_weight_out_kernel<T>, dim3(blocks(c.C)), 256, 0, s, floats(p.acc_w), p.acc_ld, w_split,
+                                    p.weight_splits, c.C, (int)c.K, lc.scale, largest, static_cast<T *>(c.gw), c.ldgw));
     }
     return SGNN_OK;
 }

@@ -158,9 +158,9 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     uint32_t *slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int *gone = reinterpret_cast<volatile int *>(slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const ProductUnits u = product_units<KIND>(c);
-    if ((int)blockIdx.x >= u.units) return;
+    let_next_kernel_start();
     if ((smem_addr(base) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
+        wait_for_kernels_before();
         if (threadIdx.x == 0) atomicExch(c.failed, 1);
         return;
     }
@@ -177,6 +177,8 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
+    wait_for_kernels_before();
+    const ProductUnits u = product_units<KIND>(c);
 
     if (warp == kPEpilogueWarps) {
         // ---- loads ----

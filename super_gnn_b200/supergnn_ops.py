@@ -10,6 +10,7 @@ C ABI (``include/supergnn_b200.h``) and the call returns without synchronising.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -1011,6 +1012,14 @@ def _on(dev):
     return _NO_SWITCH if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query: str, device: int, *sizes) -> int:
+    """Bytes a call of these sizes needs on this device: a function of its arguments, asked of the library once."""
+    need = ctypes.c_size_t(0)
+    _cabi.check(getattr(_cabi.lib(), query)(*sizes, ctypes.byref(need)), query)
+    return need.value
+
+
 def _matrix(t, name, allowed=_ELEMENT) -> int:
     """Checks a 2-d CUDA tensor with at least one column; its element code."""
     code = allowed.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 else None
@@ -1202,13 +1211,11 @@ def checkpoint_weight_grad(g, codes, params, out=None, beta: float = 0.0):
     g = _row_major(g)
     lib = _cabi.lib()
     with _on(dev), _Logged("checkpoint_weight_grad", dev, n=n, M=M, F=F):
-        need = ctypes.c_size_t(0)
-        _cabi.check(lib.sgnn_checkpoint_weight_grad_workspace_bytes(code, n, M, F, ctypes.byref(need)),
-                    "checkpoint_weight_grad")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        need = _workspace_bytes("sgnn_checkpoint_weight_grad_workspace_bytes", dev.index, code, n, M, F)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = lib.sgnn_checkpoint_weight_grad(code, g.data_ptr(), g.stride(0), codes.data_ptr(), codes.stride(0),
                                              params.data_ptr(), n, M, F, beta, out.data_ptr(), max(out.stride(0), F),
-                                             ws.data_ptr(), need.value, _stream_on(dev))
+                                             ws.data_ptr(), need, _stream_on(dev))
     if rc:
         _cabi.check(rc, "checkpoint_weight_grad")
     return out
@@ -1247,12 +1254,11 @@ def _linear_nll(x, weight, bias, labels, mask, inv_count, with_grad: bool):
         lse = torch.empty(n, dtype=torch.float32, device=dev)
     lib = _cabi.lib()
     with _on(dev), _Logged("linear_nll_grad" if with_grad else "linear_nll", dev, n=n, K=K, C=C):
-        need = ctypes.c_size_t(0)
-        _cabi.check(lib.sgnn_linear_nll_workspace_bytes(code, n, K, C, with_grad, ctypes.byref(need)), "linear_nll_loss")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        need = _workspace_bytes("sgnn_linear_nll_workspace_bytes", dev.index, code, n, K, C, with_grad)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = lib.sgnn_linear_nll_loss(code, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), bcode,
                                       _ptr(bias), labels.data_ptr(), _ptr(mask), inv_count, n, K, C, loss.data_ptr(),
-                                      _ptr(lse), _ptr(gx), K, _ptr(gw), K, _ptr(gb), ws.data_ptr(), need.value,
+                                      _ptr(lse), _ptr(gx), K, _ptr(gw), K, _ptr(gb), ws.data_ptr(), need,
                                       _stream_on(dev))
     if rc:
         _cabi.check(rc, "linear_nll_loss")
