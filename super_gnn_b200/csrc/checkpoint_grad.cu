@@ -9,12 +9,13 @@
 // conversion of g.  The activations are never restored in memory: one byte an element is read.
 //
 // A block owns 128 x 256 results and a range of the rows.  Per 32 rows TMA brings 128 columns of g and 256 of the codes
-// into shared memory as they are (where an operand is not aligned for it, the threads load it themselves);
-// eight warps convert them into the swizzled operands, both "MN-major" (the rows of g and of the codes are the reduction),
-// which keeps the order of the matrices; one thread issues the products.  Tensor memory rounds every addition
-// towards zero, which over thousands of rows would shrink the result by 1e-5 of itself, so after 512 rows the sums move on
-// into the fp32 registers of eight other warps (the other half of the tensor memory takes over meanwhile).  The partial results of the row ranges
-// are added in a fixed order.
+// into shared memory as they are (where an operand is not aligned for it, the threads load it themselves); eight warps
+// convert them: the terms of g go to tensor memory, a thread for each of its 128 lanes, the codes back to shared memory as the
+// swizzled "MN-major" operand that keeps the order of their rows; one thread issues the products.  What bounds the kernel is the
+// bandwidth of shared memory (128 bytes a clock: 105 KB a step; 129 KB with the terms of g there as well).
+// Tensor memory rounds every addition towards zero, which over thousands of rows would shrink the result by 1e-5 of itself, so
+// after 512 rows the sums move on into the fp32 registers of eight other warps.  The partial results of the row ranges are added
+// in a fixed order.
 #include "row_io.cuh"
 #include "umma.cuh"
 
@@ -24,10 +25,10 @@ constexpr int kGM = 128, kGN = 256, kGRows = 32;  // results of a block, rows a 
 constexpr int kGKeepers = 8;                      // warps that hold the sums
 constexpr int kGWorkers = 8;                      // warps that convert
 constexpr int kGThreads = (kGKeepers + kGWorkers + 4) * 32;  // and a group of four: one feeds, one issues the products
-constexpr int kGRaw = 3, kGStages = 4;            // buffers of operands as they come, and converted
+constexpr int kGRaw = 5, kGStages = 4;            // buffers of operands as they come, and converted
 constexpr int kGPromote = 16;                     // steps between two moves into registers
-constexpr int kGPlane = kGM * kGRows * 2, kGCodes = kGN * kGRows * 2;
-constexpr int kGStageBytes = 2 * kGPlane + kGCodes;
+constexpr int kGStageBytes = kGN * kGRows * 2;    // the codes of a step; the two terms of g take 32 columns of tensor memory
+constexpr int kGTerms = kGN;                      // where those columns begin, behind the sums
 
 struct GradCall {
     CUtensorMap g, codes, zs;  // zs: params as one long row
@@ -51,7 +52,7 @@ constexpr int grad_raw_bytes() { return FEED == kFeedNone ? 0 : kGRows * ((FEED 
 template <class T, int FEED>
 constexpr int grad_raw_area()
 {
-    const int ring = kGRaw * grad_raw_bytes<T, FEED>(), share = kGRows / 2 * kGM * 4;  // the shares of the zero points go there last
+    const int ring = kGRaw * grad_raw_bytes<T, FEED>(), share = 2 * kGM * 4;  // the shares of the zero points go there last
     return ring > share ? ring : share;
 }
 template <class T, int FEED>
@@ -81,36 +82,17 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
     return r;
 }
 
-// eight values times sc as two bf16 terms each, hi + lo
-__device__ __forceinline__ void two_terms(const float (&v)[8], float sc, uint4 &hi, uint4 &lo)
+// two values times their scales as two bf16 terms each, hi + lo
+__device__ __forceinline__ void two_terms(float v0, float v1, float sc0, float sc1, uint32_t &hi, uint32_t &lo)
 {
-    uint32_t *ph = reinterpret_cast<uint32_t *>(&hi), *pl = reinterpret_cast<uint32_t *>(&lo);
-    const unsigned long long sc2 = pk2(sc, sc);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const unsigned long long x2 = mul2(pk2(v[2 * e], v[2 * e + 1]), sc2);
-        float x, y;
-        unpk2(x2, x, y);
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        ph[e] = *reinterpret_cast<const uint32_t *>(&h);
-        unpk2(sub2(x2, pk2(__uint_as_float(ph[e] << 16), __uint_as_float(ph[e] & 0xFFFF0000u))), x, y);
-        const __nv_bfloat162 l = __floats2bfloat162_rn(x, y);
-        pl[e] = *reinterpret_cast<const uint32_t *>(&l);
-    }
-}
-
-template <class T>
-__device__ __forceinline__ void unpack8(const uint4 *p, float (&v)[8])
-{
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-        const uint4 a = *p;
-        const T *e = reinterpret_cast<const T *>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
-    }
+    const unsigned long long x2 = mul2(pk2(v0, v1), pk2(sc0, sc1));
+    float x, y;
+    unpk2(x2, x, y);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    unpk2(sub2(x2, pk2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u))), x, y);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(x, y);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
 template <class T, int FEED>
@@ -121,11 +103,11 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     constexpr int kRawBytes = grad_raw_bytes<T, FEED>(), kRawArea = grad_raw_area<T, FEED>();
     constexpr int kRawG = FEED == kFeedBoth ? kGRows * kGM * (int)sizeof(T) : 0;  // g first, then the codes, then the parameters
     uint64_t *raw_full = reinterpret_cast<uint64_t *>(raw + kRawArea), *raw_empty = raw_full + kGRaw;
-    uint64_t *full = raw_empty + kGRaw, *empty = full + kGStages, *acc_full = empty + kGStages, *acc_empty = acc_full + 2;
-    uint64_t *drained = acc_empty + 2;
+    uint64_t *full = raw_empty + kGRaw, *empty = full + kGStages, *acc_full = empty + kGStages, *acc_empty = acc_full + 1;
+    uint64_t *drained = acc_empty + 1;
     uint32_t *slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int *gone = reinterpret_cast<volatile int *>(slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the same for a warp, and known to be
     if ((smem_addr(base) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
         if (threadIdx.x == 0) atomicExch(c.failed, 1);
         return;
@@ -139,7 +121,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     if (threadIdx.x == 0) {
         for (int s = 0; s < kGRaw; ++s) bar_init(raw_full + s, 1), bar_init(raw_empty + s, kGWorkers);
         for (int s = 0; s < kGStages; ++s) bar_init(full + s, kGWorkers), bar_init(empty + s, 1);
-        for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, kGKeepers);
+        bar_init(acc_full, 1), bar_init(acc_empty, kGKeepers);
         bar_init(drained, 1);
         *gone = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -151,102 +133,95 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     const uint32_t tmem = *slot;
 
     // Registers follow the work: the 20 warps are launched with 96 each, 8 x 152 + 8 x 64 + 4 x 48 = 20 x 96.
-    if (warp < kGKeepers) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
-    else if (warp < kGKeepers + kGWorkers) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-
-    if (warp == kGKeepers + kGWorkers) {
-        // ---- loads ----
-        if (FEED != kFeedNone && lane == 0) {
-            if (FEED == kFeedBoth) tma_prefetch(&c.g);
-            tma_prefetch(&c.codes);
-            tma_prefetch(&c.zs);
-            int s = 0, done = 0;
-            unsigned phase = 0;
+    if (warp >= kGKeepers + kGWorkers) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == kGKeepers + kGWorkers) {
+            // ---- loads ----
+            if (FEED != kFeedNone && lane == 0) {
+                if (FEED == kFeedBoth) tma_prefetch(&c.g);
+                tma_prefetch(&c.codes);
+                tma_prefetch(&c.zs);
+                int s = 0, done = 0;
+                unsigned phase = 0;
 #pragma unroll 1
-            for (; done < count; ++done) {
-                if (!bar_wait(raw_empty + s, phase ^ 1, gone)) break;
-                uint8_t *at = raw + s * kRawBytes;
-                const int r0 = (first + done) * kGRows;
-                bar_expect(raw_full + s, kRawBytes);
-                if (FEED == kFeedBoth) tma_load(at, &c.g, m0, r0, 0, raw_full + s);
-                tma_load(at + kRawG, &c.codes, n0, r0, 0, raw_full + s);
-                tma_load(at + kRawG + kGRows * kGN, &c.zs, 2 * r0, 0, 0, raw_full + s);
-                if (++s == kGRaw) s = 0, phase ^= 1;
+                for (; done < count; ++done) {
+                    if (!bar_wait(raw_empty + s, phase ^ 1, gone)) break;
+                    uint8_t *at = raw + s * kRawBytes;
+                    const int r0 = (first + done) * kGRows;
+                    bar_expect(raw_full + s, kRawBytes);
+                    if (FEED == kFeedBoth) tma_load(at, &c.g, m0, r0, 0, raw_full + s);
+                    tma_load(at + kRawG, &c.codes, n0, r0, 0, raw_full + s);
+                    tma_load(at + kRawG + kGRows * kGN, &c.zs, 2 * r0, 0, 0, raw_full + s);
+                    if (++s == kGRaw) s = 0, phase ^= 1;
+                }
+                if (done < count) {
+                    for (int b = 0; b < kGRaw && b < done; ++b) bar_drain(raw_full + b, ((done - 1 - b) / kGRaw) & 1);
+                }
             }
-            if (done < count) {
-                for (int b = 0; b < kGRaw && b < done; ++b) bar_drain(raw_full + b, ((done - 1 - b) / kGRaw) & 1);
-            }
-        }
-        __syncwarp();
-    } else if (warp == kGKeepers + kGWorkers + 1) {
-        // ---- products ----
-        if (lane == 0) {
-            const int left = c.F - n0, n = left < kGN ? (left + 15) / 16 * 16 : kGN;
-            const uint32_t idesc = umma_idesc(true, true, true, n);
-            int s = 0;
-            unsigned phase = 0;
-            bool ok = true;
+            __syncwarp();
+        } else if (warp == kGKeepers + kGWorkers + 1) {
+            // ---- products ----
+            if (lane == 0) {
+                const int left = c.F - n0, n = left < kGN ? (left + 15) / 16 * 16 : kGN;
+                const uint32_t idesc = umma_idesc(true, false, true, n);
+                int s = 0;
+                unsigned phase = 0;
+                bool ok = true;
 #pragma unroll 1
-            for (int k = 0; k < count; ++k) {
-                const int round = k / kGPromote, acc = round & 1;
-                if (k % kGPromote == 0) {
-                    ok = bar_wait(acc_empty + acc, ((round >> 1) & 1) ^ 1, gone);
+                for (int k = 0; k < count; ++k) {
+                    if (k % kGPromote == 0) {
+                        ok = bar_wait(acc_empty, ((k / kGPromote) & 1) ^ 1, gone);
+                        if (!ok) break;
+                    }
+                    ok = bar_wait(full + s, phase, gone);
                     if (!ok) break;
                     tc_fence_after();
-                }
-                ok = bar_wait(full + s, phase, gone);
-                if (!ok) break;
-                tc_fence_after();
-                const uint8_t *at = base + s * kGStageBytes;
-                const uint64_t a0 = umma_desc(at, kGRows * 128, 1024), a1 = umma_desc(at + kGPlane, kGRows * 128, 1024);
-                const uint64_t b = umma_desc(at + 2 * kGPlane, kGRows * 128, 1024);
-                const uint32_t d = tmem + acc * kGN;
+                    const uint64_t b = umma_desc(base + s * kGStageBytes, kGRows * 128, 1024);
+                    const uint32_t a = tmem + kGTerms + s * 32;
 #pragma unroll
-                for (int j = 0; j < kGRows / 16; ++j) {  // sixteen rows: two groups of eight
-                    const uint64_t step = 2048u * j >> 4;
-                    umma(d, a0 + step, b + step, idesc, k % kGPromote > 0 || j > 0);
-                    umma(d, a1 + step, b + step, idesc, true);
+                    for (int j = 0; j < kGRows / 16; ++j) {  // sixteen rows: two groups of eight, eight columns of tensor memory
+                        const uint64_t step = 2048u * j >> 4;
+                        umma_ts(tmem, a + 8 * j, b + step, idesc, k % kGPromote > 0 || j > 0);
+                        umma_ts(tmem, a + 16 + 8 * j, b + step, idesc, true);
+                    }
+                    tc_commit(empty + s);
+                    if (k % kGPromote == kGPromote - 1 || k == count - 1) tc_commit(acc_full);
+                    if (++s == kGStages) s = 0, phase ^= 1;
                 }
-                tc_commit(empty + s);
-                if (k % kGPromote == kGPromote - 1 || k == count - 1) tc_commit(acc_full + acc);
-                if (++s == kGStages) s = 0, phase ^= 1;
+                if (!ok) {
+                    tc_commit(drained);
+                    bar_drain(drained, 0);
+                }
             }
-            if (!ok) {
-                tc_commit(drained);
-                bar_drain(drained, 0);
-            }
+            __syncwarp();
         }
-        __syncwarp();
     } else if (warp < kGKeepers) {
         // ---- the sums ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         const int quarter = warp & 3, half = warp >> 2;  // 32 rows, 128 columns of the results
         float sum[128];
 #pragma unroll
         for (int e = 0; e < 128; ++e) sum[e] = 0.f;
 #pragma unroll 1
         for (int round = 0; round < rounds; ++round) {
-            const int acc = round & 1;
-            if (!bar_wait(acc_full + acc, (round >> 1) & 1, gone)) break;
+            if (!bar_wait(acc_full, round & 1, gone)) break;
             tc_fence_after();
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float v[16];
-                tmem_load16(tmem + acc * kGN + half * 128 + 16 * j + ((uint32_t)quarter << 21), v);
+                tmem_load16(tmem + half * 128 + 16 * j + ((uint32_t)quarter << 21), v);
                 tmem_load_wait();
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sum[16 * j + e] += v[e];
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(acc_empty + acc);
+            if (lane == 0) bar_arrive(acc_empty);
         }
         asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
         const float *share = reinterpret_cast<const float *>(raw);
         const int m = quarter * 32 + lane;
-        float own = 0.f;
-#pragma unroll
-        for (int g = 0; g < kGRows / 2; ++g) own += share[g * kGM + m];
+        const float own = share[m] + share[kGM + m];
         if (m0 + m < c.M) {
             float *o = c.partials + ((int64_t)split * c.M + m0 + m) * c.ld + n0 + half * 128;
 #pragma unroll
@@ -255,35 +230,29 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                     *reinterpret_cast<float4 *>(o + e) = make_float4(sum[e] + own, sum[e + 1] + own, sum[e + 2] + own, sum[e + 3] + own);
             }
         }
-    } else if (warp < kGKeepers + kGWorkers) {
+    } else {
         // ---- conversion ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         const int tid = threadIdx.x - kGKeepers * 32, w = warp - kGKeepers;
-        const int q = tid & 15, ra = tid >> 4;          // of g: eight columns, rows ra and ra + 16
-        const int mq = m0 + q * 8, nq = n0 + lane * 8;  // of the codes: eight columns, rows w, w + 8, ...
-        unsigned long long zero[4] = {};  // sum of g zp over this thread's rows, two columns each
+        const int quarter = w & 3, first_row = (w >> 2) * 16;  // of g: one column, sixteen rows
+        const int m = quarter * 32 + lane, nq = n0 + lane * 8;  // of the codes: eight columns, rows w, w + 8, ...
+        const uint32_t terms = tmem + kGTerms + (first_row >> 1) + ((uint32_t)quarter << 21);
+        float zero = 0.f;  // sum of g zp over this thread's rows
         int s = 0, t = 0;
         unsigned phase = 0, raw_phase = 0;
         // operands of a step that come without TMA, one step ahead
-        float gv[2][8];
+        float gv[16];
         uint2 cv[4];
-        float2 pv[2];
         const auto fetch = [&](int k) {
             const int64_t r0 = (int64_t)(first + k) * kGRows;
             if constexpr (FEED != kFeedBoth) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int64_t r = r0 + ra + 16 * i;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        gv[i][e] = r < c.n && mq + e < c.M ? to_f32<T>(static_cast<const T *>(c.g_ptr)[r * c.ldg + mq + e]) : 0.f;
+                for (int i = 0; i < 16; ++i) {
+                    const int64_t r = r0 + first_row + i;
+                    gv[i] = r < c.n && m0 + m < c.M ? to_f32<T>(static_cast<const T *>(c.g_ptr)[r * c.ldg + m0 + m]) : 0.f;
                 }
             }
             if constexpr (FEED == kFeedNone) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int64_t r = r0 + ra + 16 * i;
-                    pv[i] = r < c.n ? __ldg(c.params + r) : make_float2(0.f, 0.f);
-                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int64_t r = r0 + w + 8 * i;
@@ -302,34 +271,42 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             if (FEED != kFeedNone && !bar_wait(raw_full + s, raw_phase, gone)) break;
             if (!bar_wait(empty + t, phase ^ 1, gone)) break;
             uint8_t *at = base + t * kGStageBytes;
+            uint32_t hi[8], lo[8];
+            float share = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = ra + 16 * i;
-                float v[8];
-                float2 par;
-                if constexpr (FEED == kFeedNone) par = pv[i];
-                else par = *reinterpret_cast<const float2 *>(in + kRawG + kGRows * kGN + r * 8);
+            for (int i = 0; i < 8; ++i) {
+                const int r = first_row + 2 * i;
+                float v0, v1;
+                float4 par;  // (zp, sc) of both rows
                 if constexpr (FEED == kFeedBoth) {
-                    unpack8<T>(reinterpret_cast<const uint4 *>(in + (r * kGM + q * 8) * sizeof(T)), v);
+                    const T *g = reinterpret_cast<const T *>(in) + r * kGM + m;
+                    v0 = to_f32<T>(g[0]), v1 = to_f32<T>(g[kGM]);
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = gv[i][e];
+                    v0 = gv[2 * i], v1 = gv[2 * i + 1];
                 }
-                const unsigned long long zp2 = pk2(par.x, par.x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) zero[e] = fma2(pk2(v[2 * e], v[2 * e + 1]), zp2, zero[e]);
-                uint4 hi, lo;
-                two_terms(v, par.y, hi, lo);
-                uint8_t *o = at + (q >> 3) * (kGRows * 128) + r * 128 + ((q & 7) ^ (r & 7)) * 16;
-                *reinterpret_cast<uint4 *>(o) = hi;
-                *reinterpret_cast<uint4 *>(o + kGPlane) = lo;
+                if constexpr (FEED == kFeedNone) {
+                    const int64_t row = (int64_t)(first + k) * kGRows + r;
+                    const float2 p0 = row < c.n ? __ldg(c.params + row) : make_float2(0.f, 0.f);
+                    const float2 p1 = row + 1 < c.n ? __ldg(c.params + row + 1) : make_float2(0.f, 0.f);
+                    par = make_float4(p0.x, p0.y, p1.x, p1.y);
+                } else {
+                    par = *reinterpret_cast<const float4 *>(in + kRawG + kGRows * kGN + r * 8);
+                }
+                share = __fmaf_rn(v0, par.x, share);
+                share = __fmaf_rn(v1, par.z, share);
+                two_terms(v0, v1, par.y, par.w, hi[i], lo[i]);
             }
+            zero += share;
+            tmem_store8(terms + t * 32, hi);
+            tmem_store8(terms + t * 32 + 16, lo);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = w + 8 * i;
                 const uint2 code = FEED == kFeedNone ? cv[i] : *reinterpret_cast<const uint2 *>(in + kRawG + r * kGN + lane * 8);
-                *reinterpret_cast<uint4 *>(at + 2 * kGPlane + (lane >> 3) * (kGRows * 128) + r * 128 + ((lane & 7) ^ (r & 7)) * 16) = code_values(code);
+                *reinterpret_cast<uint4 *>(at + (lane >> 3) * (kGRows * 128) + r * 128 + ((lane & 7) ^ (r & 7)) * 16) = code_values(code);
             }
+            tmem_store_wait();
+            tc_fence_before();
             if (FEED != kFeedBoth && k + 1 < count) fetch(k + 1);
             async_fence();
             __syncwarp();
@@ -340,11 +317,9 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             if (++t == kGStages) t = 0, phase ^= 1;
             if (++s == kGRaw) s = 0, raw_phase ^= 1;
         }
-        // the zero points' share of every column, [16][128]: every buffer of operands as they come has been read by then
+        // the zero points' share of every column, [2][128]: every buffer of operands as they come has been read by then
         asm volatile("bar.sync 2, %0;" ::"n"(kGWorkers * 32) : "memory");
-        float *share = reinterpret_cast<float *>(raw);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) unpk2(zero[e], share[ra * kGM + q * 8 + 2 * e], share[ra * kGM + q * 8 + 2 * e + 1]);
+        reinterpret_cast<float *>(raw)[(w >> 2) * kGM + m] = zero;
         asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
     }
     tc_fence_before();
