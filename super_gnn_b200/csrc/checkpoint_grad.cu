@@ -9,7 +9,7 @@
 // conversion of g.  The activations are never restored in memory: one byte an element is read.
 //
 // A block owns 128 x 256 results and a range of the rows.  Per 32 rows TMA brings 128 columns of g and 256 of the codes
-// into shared memory as they are (where an operand is not aligned for it, the threads load it themselves); eight warps
+// into shared memory as they are (where an operand is not aligned for it, the threads load it themselves); sixteen warps
 // convert them: the terms of g go to tensor memory, a thread for each of its 128 lanes, the codes back to shared memory as the
 // swizzled "MN-major" operand that keeps the order of their rows; one thread issues the products.  What bounds the kernel is the
 // bandwidth of shared memory (128 bytes a clock: 105 KB a step; 129 KB with the terms of g there as well).
@@ -23,7 +23,8 @@ namespace sgnn {
 
 constexpr int kGM = 128, kGN = 256, kGRows = 32;  // results of a block, rows a step
 constexpr int kGKeepers = 8;                      // warps that hold the sums
-constexpr int kGWorkers = 8;                      // warps that convert
+constexpr int kGWorkers = 16;                     // warps that convert
+constexpr int kGOwn = kGRows * 4 / kGWorkers;       // rows of g a converting thread has in a step
 constexpr int kGThreads = (kGKeepers + kGWorkers + 4) * 32;  // and a group of four: one feeds, one issues the products
 constexpr int kGRaw = 5, kGStages = 4;            // buffers of operands as they come, and converted
 constexpr int kGPromote = 16;                     // steps between two moves into registers
@@ -52,7 +53,7 @@ constexpr int grad_raw_bytes() { return FEED == kFeedNone ? 0 : kGRows * ((FEED 
 template <class T, int FEED>
 constexpr int grad_raw_area()
 {
-    const int ring = kGRaw * grad_raw_bytes<T, FEED>(), share = 2 * kGM * 4;  // the shares of the zero points go there last
+    const int ring = kGRaw * grad_raw_bytes<T, FEED>(), share = 4 * kGM * 4;  // the shares of the zero points go there last
     return ring > share ? ring : share;
 }
 template <class T, int FEED>
@@ -132,9 +133,9 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     tc_fence_after();
     const uint32_t tmem = *slot;
 
-    // Registers follow the work: the 20 warps are launched with 96 each, 8 x 152 + 8 x 64 + 4 x 48 = 20 x 96.
+    // Registers follow the work: the 28 warps are launched with 72 each, 8 x 152 + 16 x 40 + 4 x 40 = 28 x 72.
     if (warp >= kGKeepers + kGWorkers) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == kGKeepers + kGWorkers) {
             // ---- loads ----
             if (FEED != kFeedNone && lane == 0) {
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
         asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
         const float *share = reinterpret_cast<const float *>(raw);
         const int m = quarter * 32 + lane;
-        const float own = share[m] + share[kGM + m];
+        const float own = (share[m] + share[kGM + m]) + (share[2 * kGM + m] + share[3 * kGM + m]);
         if (m0 + m < c.M) {
             float *o = c.partials + ((int64_t)split * c.M + m0 + m) * c.ld + n0 + half * 128;
 #pragma unroll
@@ -232,30 +233,30 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
         }
     } else {
         // ---- conversion ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         const int tid = threadIdx.x - kGKeepers * 32, w = warp - kGKeepers;
-        const int quarter = w & 3, first_row = (w >> 2) * 16;  // of g: one column, sixteen rows
-        const int m = quarter * 32 + lane, nq = n0 + lane * 8;  // of the codes: eight columns, rows w, w + 8, ...
+        const int quarter = w & 3, first_row = (w >> 2) * kGOwn;  // of g: one column, kGOwn rows
+        const int m = quarter * 32 + lane, nq = n0 + lane * 8;  // of the codes: eight columns, rows w, w + kGWorkers, ...
         const uint32_t terms = tmem + kGTerms + (first_row >> 1) + ((uint32_t)quarter << 21);
         float zero = 0.f;  // sum of g zp over this thread's rows
         int s = 0, t = 0;
         unsigned phase = 0, raw_phase = 0;
         // operands of a step that come without TMA, one step ahead
-        float gv[16];
-        uint2 cv[4];
+        float gv[kGOwn];
+        uint2 cv[kGRows / kGWorkers];
         const auto fetch = [&](int k) {
             const int64_t r0 = (int64_t)(first + k) * kGRows;
             if constexpr (FEED != kFeedBoth) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < kGOwn; ++i) {
                     const int64_t r = r0 + first_row + i;
                     gv[i] = r < c.n && m0 + m < c.M ? to_f32<T>(static_cast<const T *>(c.g_ptr)[r * c.ldg + m0 + m]) : 0.f;
                 }
             }
             if constexpr (FEED == kFeedNone) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t r = r0 + w + 8 * i;
+                for (int i = 0; i < kGRows / kGWorkers; ++i) {
+                    const int64_t r = r0 + w + kGWorkers * i;
                     uint8_t b[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) b[e] = r < c.n && nq + e < c.F ? c.code_ptr[r * c.ldc + nq + e] : (uint8_t)0;
@@ -271,10 +272,10 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             if (FEED != kFeedNone && !bar_wait(raw_full + s, raw_phase, gone)) break;
             if (!bar_wait(empty + t, phase ^ 1, gone)) break;
             uint8_t *at = base + t * kGStageBytes;
-            uint32_t hi[8], lo[8];
+            uint32_t hi[kGOwn / 2], lo[kGOwn / 2];
             float share = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < kGOwn / 2; ++i) {
                 const int r = first_row + 2 * i;
                 float v0, v1;
                 float4 par;  // (zp, sc) of both rows
@@ -297,11 +298,11 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                 two_terms(v0, v1, par.y, par.w, hi[i], lo[i]);
             }
             zero += share;
-            tmem_store8(terms + t * 32, hi);
-            tmem_store8(terms + t * 32 + 16, lo);
+            tmem_store4(terms + t * 32, hi);
+            tmem_store4(terms + t * 32 + 16, lo);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = w + 8 * i;
+            for (int i = 0; i < kGRows / kGWorkers; ++i) {
+                const int r = w + kGWorkers * i;
                 const uint2 code = FEED == kFeedNone ? cv[i] : *reinterpret_cast<const uint2 *>(in + kRawG + r * kGN + lane * 8);
                 *reinterpret_cast<uint4 *>(at + (lane >> 3) * (kGRows * 128) + r * 128 + ((lane & 7) ^ (r & 7)) * 16) = code_values(code);
             }
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             if (++t == kGStages) t = 0, phase ^= 1;
             if (++s == kGRaw) s = 0, raw_phase ^= 1;
         }
-        // the zero points' share of every column, [2][128]: every buffer of operands as they come has been read by then
+        // the zero points' share of every column, [4][128]: every buffer of operands as they come has been read by then
         asm volatile("bar.sync 2, %0;" ::"n"(kGWorkers * 32) : "memory");
         reinterpret_cast<float *>(raw)[(w >> 2) * kGM + m] = zero;
         asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
