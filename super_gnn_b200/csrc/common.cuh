@@ -52,16 +52,24 @@ int sm_count();
 // Launch of one of a chain of kernels on a stream: its blocks may start while the kernel before them still runs and have to
 // come to wait_for_kernels_before() ahead of their first access to global memory; let_next_kernel_start() allows the kernel
 // behind the same.  Hides what a small kernel spends on being launched and set up (a microsecond or two).
+// `cluster`: blocks of a cluster.
+template <class... P, class... A>
+cudaError_t launch_clusters(int cluster, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args)
+{
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+    cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 template <class... P, class... A>
 cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args)
 {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
-    cfg.attrs = &attr, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return launch_clusters(1, kernel, grid, threads, smem, stream, args...);
 }
 __device__ __forceinline__ void wait_for_kernels_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -580,16 +580,34 @@ static bool nll_may_direct(int dtype, const void *gw, int64_t ldgw)
     return aligned16(gw) && ldgw * (int64_t)elem_bytes(dtype) % 16 == 0;
 }
 
-template <int KIND, int PLANES>
-static int nll_product(const ProductCall &c, int64_t units, cudaStream_t s)
+template <int KIND, int PLANES, int CTAS>
+static int nll_product_blocks(const ProductCall &c, int64_t units, cudaStream_t s)
 {
-    constexpr int smem = product_shared_bytes<KIND, PLANES>();
+    constexpr int smem = product_shared_bytes<KIND, PLANES, CTAS>();
     static ResidentCache cache;
-    int resident = 0, rc = resident_blocks(nll_product_kernel<KIND, PLANES>, kPThreads, smem, smem, cache, &resident);
+    int resident = 0, rc = resident_blocks(nll_product_kernel<KIND, PLANES, CTAS>, kPThreads, smem, smem, cache, &resident);
     if (rc) return rc;
-    const int64_t grid = units < resident ? units : resident;
-    SGNN_CUDA_OK(launch_chained(nll_product_kernel<KIND, PLANES>, dim3((unsigned)grid), kPThreads, smem, s, c));
+    const int64_t most = resident / CTAS, grid = CTAS * (units < most ? units : most);
+    SGNN_CUDA_OK(launch_clusters(CTAS, nll_product_kernel<KIND, PLANES, CTAS>, dim3((unsigned)grid), kPThreads, smem, s, c));
     return SGNN_OK;
+}
+
+// Two blocks a result?  They need a third less of their operands from L2, which bounds the gradients and the fp32 logits (16k x
+// 64k x 512 bf16: gx 1313 -> 989 us, gw 1490 -> 1259 us; 8k x 16k x 512 fp32: logits 266 -> 241 us); the bf16 logits wait for
+// their exponentials (779 against 789 us), and few rows are better spread over more blocks (300 x 30000 x 256 bf16, all of it: 104
+// against 130 us).
+template <int KIND, int PLANES>
+static bool nll_in_pairs(int64_t row_cap)
+{
+    return row_cap > 1024 && (KIND == kRowGrad || KIND == kWeightGrad || PLANES == 2);
+}
+
+// `rows` of the result at most, `tiles` beside and behind each other (columns of the result, splits)
+template <int KIND, int PLANES>
+static int nll_product(const ProductCall &c, int64_t rows, int64_t tiles, cudaStream_t s)
+{
+    if (nll_in_pairs<KIND, PLANES>(c.row_cap)) return nll_product_blocks<KIND, PLANES, 2>(c, ceil_div(rows, 2 * kPM) * tiles, s);
+    return nll_product_blocks<KIND, PLANES, 1>(c, ceil_div(rows, kPM) * tiles, s);
 }
 
 template <class T, int PLANES>
@@ -638,7 +656,8 @@ static int nll_run(const NllCall &c, const NllPlan &p)
     const void *wp = p.copy_w ? (const void *)ws.row.p : c.w;
     const int64_t wld = p.copy_w ? p.ld : c.ldw, wst = p.copy_w ? ws.row.stride : c.C * c.ldw;
     if ((rc = umma_tensor_map(&lc.a, xs.row.p, !f32, c.K, p.padded, p.ld, PLANES, xs.row.stride, kPM))) return rc;
-    if ((rc = umma_tensor_map(&lc.b, wp, !f32, c.K, c.C, wld, PLANES, wst, kPN))) return rc;
+    const bool pairs = nll_in_pairs<kLogitStats, PLANES>(p.row_cap);  // each of the two reads half of a tile's classes
+    if ((rc = umma_tensor_map(&lc.b, wp, !f32, c.K, c.C, wld, PLANES, wst, pairs ? kPN / 2 : kPN))) return rc;
     lc.total = ints(p.total), lc.failed = ints(p.failed), lc.feats = (int)c.K, lc.splits = 1, lc.bf16 = !f32;
     lc.bias2 = floats(p.bias2), lc.row_scale = xs.row_down, lc.cls_scale = ws.row_down, lc.classes = c.C;
     lc.stats = reinterpret_cast<float2 *>(c.ws + p.stats), lc.row_cap = (int)p.row_cap, lc.lse2 = floats(p.lse2);
@@ -664,13 +683,13 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         }
         if (rc) return rc;
     }
-    const int64_t tiles_k = ceil_div(c.K, kPN), join_blocks = p.row_cap / kJoinRows, tiles_m = p.row_cap / kPM;
+    const int64_t tiles_k = ceil_div(c.K, kPN), join_blocks = p.row_cap / kJoinRows;
     for (int64_t q = 0; q < p.chunks; ++q) {
         const int row0 = (int)(q * p.row_cap);
         for (ProductCall *k : {&lc, &xc, &wc}) k->row0 = row0;
         lc.label = ints(p.label) + row0, lc.picked2 = floats(p.picked2) + row0;
         lc.cls0 = 0, lc.cls_count = (int)c.C;
-        if ((rc = nll_product<kLogitStats, PLANES>(lc, tiles_m * ceil_div(c.C, kPN), s))) return rc;
+        if ((rc = nll_product<kLogitStats, PLANES>(lc, p.row_cap, ceil_div(c.C, kPN), s))) return rc;
         const NllJoin join{lc.stats, (int)(p.cls_padded / 128), row0, (int)p.row_cap, ints(p.rows), ints(p.total), lc.picked2,
                            floats(p.lse2), c.lse, floats(p.loss_part) + q * join_blocks, floats(p.loss_part),
                            (int)(p.chunks * join_blocks), c.inv_count, ints(p.joined), ints(p.failed), c.loss};
@@ -679,11 +698,11 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         for (int64_t first = 0; first < c.C; first += p.piece) {
             const int64_t count = c.C - first < p.piece ? c.C - first : p.piece;
             for (ProductCall *k : {&lc, &xc, &wc}) k->cls0 = (int)first, k->cls_count = (int)count;
-            if ((rc = nll_product<kLogitGrad, PLANES>(lc, tiles_m * ceil_div(count, kPN), s))) return rc;
+            if ((rc = nll_product<kLogitGrad, PLANES>(lc, p.row_cap, ceil_div(count, kPN), s))) return rc;
             xc.add = first > 0;
-            if ((rc = nll_product<kRowGrad, PLANES>(xc, tiles_m * tiles_k * p.row_splits, s))) return rc;
+            if ((rc = nll_product<kRowGrad, PLANES>(xc, p.row_cap, tiles_k * p.row_splits, s))) return rc;
             wc.add = q > 0;
-            if ((rc = nll_product<kWeightGrad, PLANES>(wc, ceil_div(count, kPM) * tiles_k * p.weight_splits, s))) return rc;
+            if ((rc = nll_product<kWeightGrad, PLANES>(wc, count, tiles_k * p.weight_splits, s))) return rc;
             if (c.gb) {
                 char *gb = static_cast<char *>(c.gb) + first * (c.bias.f32 ? 4 : sizeof(T));
                 const bool deal = p.row_cap / 32 > 32;

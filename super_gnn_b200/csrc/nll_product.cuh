@@ -4,9 +4,10 @@
 //     rows     gx[i, k] = sum_c G[i, c] W[c, k]
 //     weights  gw[c, k] = sum_i G[i, c] x[i, k]     and gb[c] = sum_i G[i, c], a product with ones
 //
-// One persistent block an SM.  A warp feeds 128 x 64 and 256 x 64 operand tiles by TMA through a ring of shared memory
-// buffers, a thread issues the tcgen05 products into tensor memory, eight warps turn finished 128 x 256 results into
-// the outputs.  The operands lie as their matrices do: x and W are read along k by the first product and across it by the
+// One persistent block an SM.  A warp feeds operand tiles by TMA through a ring of shared memory buffers, a thread issues
+// the tcgen05 products into tensor memory, eight warps turn finished 128 x 256 results into the outputs.  Two blocks of a
+// cluster share a 256 x 256 result where that is faster (nll_in_pairs in linear_nll.cu): each brings 128 rows of the first operand and half of
+// the second, 32 KB a step of 64 for 128 x 256 results where a block alone needs 48 KB.  The operands lie as their matrices do: x and W are read along k by the first product and across it by the
 // other two, G along the classes by the second and across by the third, so that nothing is ever transposed in memory.
 //
 // fp32 operands come as two fp16 planes (v 2^e = v0 + v1, 22 bits; see linear_nll.cu) and three products
@@ -53,18 +54,18 @@ struct ProductCall {
     int64_t classes;
 };
 
-template <int PLANES>
+template <int PLANES, int CTAS>
 struct ProductShared {
-    static constexpr int kStages = 4 / PLANES;
-    static constexpr int kA = kPM * kPK * 2, kB = kPN * kPK * 2;
+    static constexpr int kStages = (CTAS == 2 ? 6 : 4) / PLANES;
+    static constexpr int kA = kPM * kPK * 2, kB = kPN / CTAS * kPK * 2;
     static constexpr int kStageBytes = PLANES * (kA + kB);
     static constexpr int kBox = 4096;  // result box of a warp: 32 rows of 128 bytes
 };
 
-template <int KIND, int PLANES>
+template <int KIND, int PLANES, int CTAS>
 constexpr int product_shared_bytes()
 {
-    using S = ProductShared<PLANES>;
+    using S = ProductShared<PLANES, CTAS>;
     const int ring = S::kStages * S::kStageBytes;
     if (KIND == kLogitStats) return ring + 2 * kPN * 8 + 256;
     if (KIND == kLogitGrad) return ring + kPEpilogueWarps * S::kBox + kPN * 8 + 256;
@@ -76,7 +77,7 @@ struct ProductUnits {
     int m, n, blocks, per_split, tiles_m, tiles_n, units, rows;
 };
 
-template <int KIND>
+template <int KIND, int CTAS>
 __device__ __forceinline__ ProductUnits product_units(const ProductCall &c)
 {
     ProductUnits u;
@@ -89,7 +90,7 @@ __device__ __forceinline__ ProductUnits product_units(const ProductCall &c)
     else u.m = c.cls_count, u.n = c.feats, red = rows;
     u.blocks = (red + kPK - 1) / kPK;
     u.per_split = (u.blocks + c.splits - 1) / c.splits;
-    u.tiles_m = (u.m + kPM - 1) / kPM;
+    u.tiles_m = (u.m + kPM * CTAS - 1) / (kPM * CTAS);
     u.tiles_n = (u.n + kPN - 1) / kPN;
     u.units = u.tiles_m * u.tiles_n * c.splits;
     return u;
@@ -97,13 +98,14 @@ __device__ __forceinline__ ProductUnits product_units(const ProductCall &c)
 
 // unit -> tile and range of reduction steps; an empty range still writes its zeros
 struct ProductUnit {
-    int m0, n0, split, first, count;
+    int m0, n0, split, first, count;  // m0: this block's first row
 };
-__device__ __forceinline__ ProductUnit product_unit(const ProductUnits &u, int i)
+template <int CTAS>
+__device__ __forceinline__ ProductUnit product_unit(const ProductUnits &u, int i, int rank)
 {
     ProductUnit t;
     const int tm = i % u.tiles_m, rest = i / u.tiles_m;
-    t.m0 = tm * kPM, t.n0 = rest % u.tiles_n * kPN, t.split = rest / u.tiles_n;
+    t.m0 = (tm * CTAS + rank) * kPM, t.n0 = rest % u.tiles_n * kPN, t.split = rest / u.tiles_n;
     t.first = t.split * u.per_split;
     const int end = t.first + u.per_split < u.blocks ? t.first + u.per_split : u.blocks;
     t.count = end > t.first ? end - t.first : 0;
@@ -138,10 +140,10 @@ __device__ __forceinline__ void plane_scale(float largest, float &up, float &dow
 
 constexpr float kGradScale = 32768.0f;  // fp16 planes of G: |G| <= 1 fills the range, 2^-40 is the smallest step
 
-template <int KIND, int PLANES>
+template <int KIND, int PLANES, int CTAS>
 __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_constant__ ProductCall c)
 {
-    using S = ProductShared<PLANES>;
+    using S = ProductShared<PLANES, CTAS>;
     constexpr bool kLogits = KIND == kLogitStats || KIND == kLogitGrad;
     constexpr bool kAmn = KIND == kWeightGrad, kBmn = !kLogits;
     constexpr bool kCross = !kLogits && PLANES == 2;  // cross products have their own sums, in the other half of the tensor memory
@@ -158,6 +160,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     uint32_t *slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int *gone = reinterpret_cast<volatile int *>(slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CTAS == 2 ? (int)cluster_rank() : 0, first_unit = blockIdx.x / CTAS, unit_step = gridDim.x / CTAS;
     let_next_kernel_start();
     if ((smem_addr(base) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
         wait_for_kernels_before();
@@ -167,18 +170,22 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) bar_init(full + s, 1), bar_init(empty + s, 1);
-        for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, kPEpilogueWarps);
+        for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, kPEpilogueWarps * CTAS);
         bar_init(drained, 1);
         *gone = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kPEpilogueWarps + 1) tmem_alloc(slot, kPAccCols);
+    if (warp == kPEpilogueWarps + 1) {
+        if (CTAS == 2) tmem_alloc_pair(slot, kPAccCols);
+        else tmem_alloc(slot, kPAccCols);
+    }
     tc_fence_before();
     __syncthreads();
+    if (CTAS == 2) cluster_sync();  // the barriers of both blocks are there
     tc_fence_after();
     const uint32_t tmem = *slot;
     wait_for_kernels_before();
-    const ProductUnits u = product_units<KIND>(c);
+    const ProductUnits u = product_units<KIND, CTAS>(c);
 
     if (warp == kPEpilogueWarps) {
         // ---- loads ----
@@ -188,30 +195,36 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
             int stage = 0;
             unsigned phase = 0, used = 0;
             bool ok = true;
-            for (int i = blockIdx.x; i < u.units && ok; i += gridDim.x) {
-                const ProductUnit t = product_unit(u, i);
-                const int runs = kBmn ? ((u.n - t.n0 < kPN ? u.n - t.n0 : kPN) + 63) / 64 : 1;
+            for (int i = first_unit; i < u.units && ok; i += unit_step) {
+                const ProductUnit t = product_unit<CTAS>(u, i, rank);
+                const int left = u.n - t.n0, own_n = (left < kPN ? (left + 15) / 16 * 16 : kPN) / CTAS;  // columns of the second operand here
+                const int runs = kBmn ? (own_n + 63) / 64 : 1;
                 const unsigned bytes = PLANES * (S::kA + (kBmn ? runs * 64 * kPK * 2 : S::kB));
                 for (int k = 0; k < t.count; ++k) {
                     ok = bar_wait(empty + stage, phase ^ 1, gone);
                     if (!ok) break;
                     uint8_t *at = base + stage * S::kStageBytes;
-                    bar_expect(full + stage, bytes);
+                    if (rank == 0) bar_expect(full + stage, CTAS * bytes);
+                    const uint32_t lead = CTAS == 2 ? leader_addr(full + stage) : 0u;
+                    const auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int z) {
+                        if (CTAS == 2) tma_load_pair(dst, map, x, y, z, lead);
+                        else tma_load(dst, map, x, y, z, full + stage);
+                    };
                     const int k0 = (t.first + k) * kPK;
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p) {
                         uint8_t *pa = at + p * S::kA, *pb = at + PLANES * S::kA + p * S::kB;
                         if (kAmn) {
-                            tma_load(pa, &c.a, t.m0, k0, p, full + stage);
-                            tma_load(pa + 64 * kPK * 2, &c.a, t.m0 + 64, k0, p, full + stage);
+                            load(pa, &c.a, t.m0, k0, p);
+                            load(pa + 64 * kPK * 2, &c.a, t.m0 + 64, k0, p);
                         } else {
-                            tma_load(pa, &c.a, k0, t.m0 + (kLogits ? c.row0 : 0), p, full + stage);
+                            load(pa, &c.a, k0, t.m0 + (kLogits ? c.row0 : 0), p);
                         }
                         if (kBmn) {
                             const int k1 = k0 + (KIND == kRowGrad ? c.cls0 : c.row0);
-                            for (int r = 0; r < runs; ++r) tma_load(pb + r * 64 * kPK * 2, &c.b, t.n0 + 64 * r, k1, p, full + stage);
+                            for (int r = 0; r < runs; ++r) load(pb + r * 64 * kPK * 2, &c.b, t.n0 + rank * own_n + 64 * r, k1, p);
                         } else {
-                            tma_load(pb, &c.b, k0, t.n0 + c.cls0, p, full + stage);
+                            load(pb, &c.b, k0, t.n0 + c.cls0 + rank * (kPN / CTAS), p);
                         }
                     }
                     ++used;
@@ -219,7 +232,11 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                 }
             }
             if (!ok) {  // copies of this block still under way: their buffers must not be left to another block
-                for (int s = 0; s < S::kStages; ++s) {
+                if (rank != 0) {  // what counts them is the other block's
+                    const uint64_t until = now_ns() + kWaitNs / 8;
+                    while (now_ns() < until) __nanosleep(1000);
+                }
+                for (int s = 0; rank == 0 && s < S::kStages; ++s) {
                     if (used < (unsigned)(s + 1)) continue;
                     const unsigned uses = (used - 1 - s) / S::kStages + 1;  // fills of this buffer so far
                     bar_drain(full + s, (uses - 1) & 1);
@@ -228,16 +245,24 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
         }
         __syncwarp();
     } else if (warp == kPEpilogueWarps + 1) {
-        // ---- products ----
-        if (lane == 0) {
+        // ---- products (of both blocks: the first one's) ----
+        if (lane == 0 && rank == 0) {
             int stage = 0, acc = 0;
             unsigned phase = 0, acc_phase = 0;
             bool ok = true;
-            for (int i = blockIdx.x; i < u.units && ok; i += gridDim.x) {
-                const ProductUnit t = product_unit(u, i);
+            const auto commit = [&](uint64_t *bar) {
+                if (CTAS == 2) tc_commit_pair(bar);
+                else tc_commit(bar);
+            };
+            const auto product = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+                if (CTAS == 2) umma_pair(d, a, b, idesc, add);
+                else umma(d, a, b, idesc, add);
+            };
+            for (int i = first_unit; i < u.units && ok; i += unit_step) {
+                const ProductUnit t = product_unit<CTAS>(u, i, rank);
                 const int left = u.n - t.n0;
                 const int n = kBmn ? (left < kPN ? (left + 15) / 16 * 16 : kPN) : kPN;
-                const uint32_t idesc = umma_idesc(c.bf16, kAmn, kBmn, n);
+                const uint32_t idesc = umma_idesc(c.bf16, kAmn, kBmn, n, kPM * CTAS);
                 ok = bar_wait(acc_empty + acc, acc_phase ^ 1, gone);
                 if (!ok) break;
                 tc_fence_after();
@@ -260,22 +285,22 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         // sixteen steps of the reduction: 32 bytes along a row, or two groups of eight rows
                         const uint64_t sa = (kAmn ? 2048u : 32u) * j >> 4, sb = (kBmn ? 2048u : 32u) * j >> 4;
                         const bool more = k > 0 || j > 0;
-                        umma(d, da[0] + sa, db[0] + sb, idesc, more);
+                        product(d, da[0] + sa, db[0] + sb, idesc, more);
                         if (PLANES == 2) {
                             const uint32_t dx = kCross ? tmem + kPN : d;
-                            umma(dx, da[0] + sa, db[PLANES - 1] + sb, idesc, !kCross || more);
-                            umma(dx, da[PLANES - 1] + sa, db[0] + sb, idesc, true);
+                            product(dx, da[0] + sa, db[PLANES - 1] + sb, idesc, !kCross || more);
+                            product(dx, da[PLANES - 1] + sa, db[0] + sb, idesc, true);
                         }
                     }
-                    tc_commit(empty + stage);
+                    commit(empty + stage);
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
                 }
                 if (!ok) break;
-                tc_commit(acc_full + acc);
+                commit(acc_full + acc);
                 if (++acc == kAcc) acc = 0, acc_phase ^= 1;
             }
             if (!ok) {  // products still under way write tensor memory and read the buffers
-                tc_commit(drained);
+                commit(drained);
                 bar_drain(drained, 0);
             }
         }
@@ -287,8 +312,8 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
         uint8_t *box_row = box + lane * 128;
         int acc = 0;
         unsigned acc_phase = 0;
-        for (int i = blockIdx.x; i < u.units; i += gridDim.x) {
-            const ProductUnit t = product_unit(u, i);
+        for (int i = first_unit; i < u.units; i += unit_step) {
+            const ProductUnit t = product_unit<CTAS>(u, i, rank);
             const int row = t.m0 + quarter * 32 + lane;  // of the product
             float *bias_col = column + (kColumns == 2 ? acc : 0) * 2 * kPN, *scale_col = bias_col + kPN;
             if (kLogits) {
@@ -384,11 +409,11 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         }
                         if (j & 1) {
                             box_done();
-                            if (lane == 0) {
+                            if (lane == 0 && y0 < c.row_cap) {
                                 tma_store(&c.o, box, x0 + 32 * (j - 1), y0, 0);
                                 store_commit();
                             }
-                            if (c.bias_part != nullptr) {  // two columns a lane, down the rows of the box
+                            if (c.bias_part != nullptr && y0 < c.row_cap) {  // two columns a lane, down the rows of the box
                                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                                 for (int r = 0; r < 32; ++r) {
@@ -419,12 +444,12 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                             *reinterpret_cast<uint4 *>(r1 + (q ^ turn) * 16) = w1;
                         }
                         box_done();
-                        if (lane == 0) {
+                        if (lane == 0 && y0 < c.row_cap) {
                             tma_store(&c.o, box, x0 + 32 * j, y0, 0);
                             tma_store(&c.o, box + 2048, x0 + 32 * j, y0, 1);
                             store_commit();
                         }
-                        if (c.bias_part != nullptr) {
+                        if (c.bias_part != nullptr && y0 < c.row_cap) {
                             // 32 rows x 32 columns: every exchange halves the columns a lane carries; lane l ends with column l
 #pragma unroll
                             for (int o = 16; o > 0; o >>= 1) {
@@ -489,7 +514,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         if ((j & 1) == 0 && k0 + 32 < u.n) continue;  // 64 columns a box
                     }
                     box_done();
-                    if (lane == 0 && (KIND != kWeightGrad || y0 < c.classes)) {
+                    if (lane == 0 && y0 < (KIND == kWeightGrad ? (int)c.classes : c.row_cap)) {
                         const int x0 = wide ? t.n0 + half * 128 + 64 * (j >> 1) : k0;
                         if (c.add) tma_add(&c.o, box, x0, y0, t.split);
                         else tma_store(&c.o, box, x0, y0, t.split);
@@ -499,7 +524,10 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(acc_empty + acc);
+            if (lane == 0) {
+                if (CTAS == 2) leader_arrive(acc_empty + acc);
+                else bar_arrive(acc_empty + acc);
+            }
             if (++acc == kAcc) acc = 0, acc_phase ^= 1;
         }
         if (KIND != kLogitStats && lane == 0) store_wait_all();
@@ -507,9 +535,13 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     }
     tc_fence_before();
     __syncthreads();
+    if (CTAS == 2) cluster_sync();  // nothing of the other block is under way to this one any more
     tc_fence_after();
     if (threadIdx.x == 0 && *gone) atomicExch(c.failed, 1);
-    if (warp == kPEpilogueWarps + 1) tmem_free(tmem, kPAccCols);
+    if (warp == kPEpilogueWarps + 1) {
+        if (CTAS == 2) tmem_free_pair(tmem, kPAccCols);
+        else tmem_free(tmem, kPAccCols);
+    }
 }
 
 }  // namespace sgnn

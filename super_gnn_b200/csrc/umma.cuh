@@ -82,6 +82,36 @@ __device__ __forceinline__ void bar_drain(uint64_t *bar, unsigned parity)
         if (bar_try(bar, parity)) return;
 }
 
+// ---- two blocks of a cluster that work on one product (cta_group::2): the first of them leads ----
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// address of the same place in the leading block's shared memory
+__device__ __forceinline__ uint32_t leader_addr(const void *p)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
+    return a;
+}
+__device__ __forceinline__ void leader_arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+}
+// into this block's shared memory, counted by the leader's barrier
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+
 // columns [x, x + 64) of rows [y, y + box rows) of plane z
 __device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar)
 {
@@ -137,6 +167,23 @@ __device__ __forceinline__ void tmem_free(uint32_t base, int cols)
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, int cols)
+{
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t base, int cols)
+{
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
+}
+// the barrier at this place in both blocks
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+
 // arrives on the barrier once every product issued before by this thread has finished
 __device__ __forceinline__ void tc_commit(uint64_t *bar)
 {
@@ -154,17 +201,25 @@ __device__ __forceinline__ uint64_t umma_desc(const void *p, unsigned run_bytes,
            (1ull << 46) | (2ull << 61);
 }
 
-// 128 x n product of 16-bit operands with fp32 sums
-__device__ __forceinline__ uint32_t umma_idesc(bool bf16, bool a_mn, bool b_mn, int n)
+// m x n product of 16-bit operands with fp32 sums: m = 128, or 256 of two blocks
+__device__ __forceinline__ uint32_t umma_idesc(bool bf16, bool a_mn, bool b_mn, int n, int m = 128)
 {
     const uint32_t t = bf16 ? 1u : 0u;
     return (1u << 4) | (t << 7) | (t << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
-           ((128u >> 4) << 24);
+           ((uint32_t)(m >> 4) << 24);
 }
 
 __device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
+                 : "memory");
+}
+
+// The product of two blocks: each has 128 rows of the first operand, half of the second's columns, 128 rows of the result
+__device__ __forceinline__ void umma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
                  "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
                  : "memory");
 }
