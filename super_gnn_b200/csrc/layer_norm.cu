@@ -480,9 +480,10 @@ __device__ __forceinline__ void load_source(const NormSource &src, int64_t r, in
     else load_row<T, E>(static_cast<const T *>(src.x) + r * src.ldx + c, v);
 }
 
-// partials: [gridDim.x, 2, H], per-block column sums of (gy xh, gy)
+// partials: [gridDim.x, 2, H], per-block column sums of (gy xh, gy).  From codes, with a byte an element instead of four to wait
+// for, a fourth block an SM is worth more than registers (600000 x 256 fp32: 270 us against 295; from x 283 against 277).
 template <class T, int E, int NV, bool CK>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, CK && E * NV <= 8 ? 4 : 1)
 norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
                      NormParam par, T *__restrict__ gx, int64_t ldgx, float *__restrict__ partials, int64_t n, int H)
 {

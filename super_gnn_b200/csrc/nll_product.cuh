@@ -100,12 +100,16 @@ __device__ __forceinline__ ProductUnits product_units(const ProductCall &c)
 struct ProductUnit {
     int m0, n0, split, first, count;  // m0: this block's first row
 };
-template <int CTAS>
+// Logits: the row tiles of one tile of classes follow each other (its part of W stays in L2).  Gradients: the column tiles of the
+// same rows, which read the same part of G, the largest operand, at about the same time.
+template <int KIND, int CTAS>
 __device__ __forceinline__ ProductUnit product_unit(const ProductUnits &u, int i, int rank)
 {
+    constexpr bool kRowsFirst = KIND == kLogitStats || KIND == kLogitGrad;
     ProductUnit t;
-    const int tm = i % u.tiles_m, rest = i / u.tiles_m;
-    t.m0 = (tm * CTAS + rank) * kPM, t.n0 = rest % u.tiles_n * kPN, t.split = rest / u.tiles_n;
+    const int tiles = u.tiles_m * u.tiles_n, in = i % tiles;
+    const int tm = kRowsFirst ? in % u.tiles_m : in / u.tiles_n, tn = kRowsFirst ? in / u.tiles_m : in % u.tiles_n;
+    t.m0 = (tm * CTAS + rank) * kPM, t.n0 = tn * kPN, t.split = i / tiles;
     t.first = t.split * u.per_split;
     const int end = t.first + u.per_split < u.blocks ? t.first + u.per_split : u.blocks;
     t.count = end > t.first ? end - t.first : 0;
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
             unsigned phase = 0, used = 0;
             bool ok = true;
             for (int i = first_unit; i < u.units && ok; i += unit_step) {
-                const ProductUnit t = product_unit<CTAS>(u, i, rank);
+                const ProductUnit t = product_unit<KIND, CTAS>(u, i, rank);
                 const int left = u.n - t.n0, own_n = (left < kPN ? (left + 15) / 16 * 16 : kPN) / CTAS;  // columns of the second operand here
                 const int runs = kBmn ? (own_n + 63) / 64 : 1;
                 const unsigned bytes = PLANES * (S::kA + (kBmn ? runs * 64 * kPK * 2 : S::kB));
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                 else umma(d, a, b, idesc, add);
             };
             for (int i = first_unit; i < u.units && ok; i += unit_step) {
-                const ProductUnit t = product_unit<CTAS>(u, i, rank);
+                const ProductUnit t = product_unit<KIND, CTAS>(u, i, rank);
                 const int left = u.n - t.n0;
                 const int n = kBmn ? (left < kPN ? (left + 15) / 16 * 16 : kPN) : kPN;
                 const uint32_t idesc = umma_idesc(c.bf16, kAmn, kBmn, n, kPM * CTAS);
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
         int acc = 0;
         unsigned acc_phase = 0;
         for (int i = first_unit; i < u.units; i += unit_step) {
-            const ProductUnit t = product_unit<CTAS>(u, i, rank);
+            const ProductUnit t = product_unit<KIND, CTAS>(u, i, rank);
             const int row = t.m0 + quarter * 32 + lane;  // of the product
             float *bias_col = column + (kColumns == 2 ? acc : 0) * 2 * kPN, *scale_col = bias_col + kPN;
             if (kLogits) {
