@@ -455,7 +455,8 @@ extern "C" SGNN_API int sgnn_checkpoint_weight_grad(int dtype, const void *d_g, 
     int rc = weight_grad_check(who, dtype, n, M, F);
     if (rc) return rc;
     SGNN_REQUIRE(beta == beta, SGNN_ERR_INVALID_ARGUMENT, "%s: beta is NaN", who);
-    SGNN_REQUIRE(d_out != nullptr && ldo >= F, SGNN_ERR_INVALID_ARGUMENT, "%s: bad output", who);
+    SGNN_REQUIRE(d_out != nullptr && ldo >= F && reinterpret_cast<uintptr_t>(d_out) % 4 == 0, SGNN_ERR_INVALID_ARGUMENT,
+                 "%s: bad output", who);
     cudaStream_t s = (cudaStream_t)stream;
     if (n == 0) {
         const dim3 grid((unsigned)ceil_div(F, 32), (unsigned)(M < 65535 ? M : 65535));

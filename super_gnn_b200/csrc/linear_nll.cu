@@ -779,6 +779,10 @@ extern "C" SGNN_API int sgnn_linear_nll_loss(int dtype, const void *d_x, int64_t
     }
     SGNN_REQUIRE(d_x && d_w && d_labels, SGNN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
     SGNN_REQUIRE((n == 1 || ldx >= K) && (C == 1 || ldw >= K), SGNN_ERR_INVALID_ARGUMENT, "%s: leading dimension shorter than a row", who);
+    const auto on = [](const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; };
+    SGNN_REQUIRE(on(d_x, b) && on(d_w, b) && on(d_gx, b) && on(d_gw, b) && on(d_bias, elem_bytes(bias_dtype)) &&
+                     on(d_gb, elem_bytes(bias_dtype)) && on(d_labels, 8) && on(d_loss, 4) && on(d_lse, 4),
+                 SGNN_ERR_INVALID_ARGUMENT, "%s: pointers must be aligned to their element", who);
     const NllPlan p = nll_plan(dtype, n, K, C, d_gx != nullptr, nll_must_copy_weights(dtype, d_w, ldw, C),
                                nll_may_direct(dtype, d_gw, ldgw));
     SGNN_REQUIRE(d_workspace != nullptr && workspace_bytes >= p.bytes && reinterpret_cast<uintptr_t>(d_workspace) % 256 == 0,

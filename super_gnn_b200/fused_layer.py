@@ -21,6 +21,7 @@ results do not change; an input that the caller holds anyway (the features) is k
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import supergnn_ops as ops
 from .aggregator import _spmm_overwrite, _world, aggregate_backward, aggregate_forward
@@ -467,6 +468,7 @@ class FusedSAGELossManyClasses(torch.autograd.Function):
         return loss.reshape(())
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_loss):
         gax, gw, gb = ctx.saved_tensors
         if not ctx.unit_grad:

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import supergnn_ops as ops
 
@@ -32,6 +33,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy):
         stats, weight, *kept = ctx.saved_tensors
         if ctx.bits == 8:
@@ -55,6 +57,7 @@ class _CheckpointLinear(torch.autograd.Function):
         return F.linear(x, weight)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         weight, codes, params = ctx.saved_tensors
         gx = g @ weight if ctx.needs_input_grad[0] else None
@@ -80,6 +83,7 @@ class _LinearNLL(torch.autograd.Function):
         return loss.reshape(())
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         gx, gw, gb = ctx.saved_tensors
         need = ctx.needs_input_grad

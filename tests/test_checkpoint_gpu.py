@@ -174,3 +174,37 @@ def test_refusals(call):
     x = torch.randn(6, 8, device=DEV)
     with pytest.raises(RuntimeError):
         call(x, *ops.checkpoint_pack_rows(x))
+
+
+def test_weight_grad_over_many_rounds_and_row_ranges():
+    """Rows enough for several moves of the sums into registers in every row range, for both ways operands come in."""
+    n, M, F = 300_007, 40, 96
+    x = torch.relu(rows(n, F, torch.float32, 1))
+    x[::3] = 0  # rows without a range: the zero point alone
+    g = rows(n, M, torch.float32, 2, spread=0.3)
+    codes, params = ops.checkpoint_pack_rows(x)
+    want, worst, typical = grad_bounds(g, codes, params)
+    wide = torch.zeros(n, M + 1, device=DEV)
+    wide[:, 1:] = g  # rows that are not aligned
+    for operand in (g, wide[:, 1:]):
+        off = (ops.checkpoint_weight_grad(operand, codes, params).double() - want).abs()
+        assert (off <= worst).all()
+        # terms of 2^-17, and sums of 512 rows in tensor memory: 64 additions of 2^-24 on average, all towards zero
+        assert off.norm() <= (2 ** -17 + 64 * 2 ** -24) * typical.norm()
+
+
+def test_captured_weight_grad():
+    x, g = rows(700, 96, torch.float32, 1), rows(700, 40, torch.float32, 2)
+    codes, params = ops.checkpoint_pack_rows(x)
+    ops.checkpoint_weight_grad(g, codes, params)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        codes, params = ops.checkpoint_pack_rows(x)
+        got = ops.checkpoint_weight_grad(g, codes, params)
+        back = ops.checkpoint_unpack_rows(codes, params)
+    x.copy_(rows(700, 96, torch.float32, 5))
+    g.copy_(rows(700, 40, torch.float32, 6))
+    graph.replay()
+    torch.cuda.synchronize()
+    want = ops.checkpoint_pack_rows(x)
+    assert torch.equal(got, ops.checkpoint_weight_grad(g, *want)) and torch.equal(back, ops.checkpoint_unpack_rows(*want))

@@ -207,3 +207,45 @@ def test_gradient_against_differences():
 def test_refusals(call):
     with pytest.raises(RuntimeError):
         call(torch.randn(4, 8, device=DEV), torch.ones(8, device=DEV))
+
+
+@pytest.mark.parametrize("n,H,dtype", [(8, 601, torch.float32), (9, 601, torch.bfloat16), (4000, 257, torch.float32),
+                                       (5003, 602, torch.bfloat16), (3001, 1021, torch.float16), (700, 300, torch.float16),
+                                       (6007, 512, torch.bfloat16), (2500, 640, torch.float32), (10_000, 66, torch.bfloat16)])
+def test_packed_rows_through_the_ring(n, H, dtype):
+    """More batches of eight rows than the ring has buffers, a short last batch, and gx over gy."""
+    x, gy, gamma, beta = make(n, H, dtype, torch.float32, seed=n + H)
+    x = x.contiguous()
+    y, stats = ops.layer_norm_forward(x, gamma, beta)
+    ref = Ref(x, gamma, beta, 1e-5)
+    close(y, ref.y, ref.e_y)
+    got = ops.layer_norm_backward(gy, x, stats, gamma)
+    for g, (want, err) in zip(got, ref.backward(gy)):
+        close(g, want, err)
+    own = gy.clone()
+    for a, b in zip(ops.layer_norm_backward(own, x, stats, gamma, in_place=True), got):
+        assert torch.equal(a, b)
+    back = x.clone()  # y over x
+    assert torch.equal(ops.layer_norm_forward(back, gamma, beta, out=back)[0], y)
+
+
+def test_captured_and_on_another_stream():
+    x, gy, gamma, beta = make(900, 300, torch.bfloat16, torch.float32, seed=3)
+    x = x.contiguous()
+    ops.layer_norm_backward(gy, x, ops.layer_norm_forward(x, gamma, beta)[1], gamma)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, stats, codes, params = ops.layer_norm_forward(x, gamma, beta, checkpoint=True)
+        grads = ops.layer_norm_backward_checkpoint(gy, codes, params, stats, gamma)
+    x2, gy2, gamma2, beta2 = make(900, 300, torch.bfloat16, torch.float32, seed=4)
+    for t, v in zip((x, gy, gamma, beta), (x2, gy2, gamma2, beta2)):
+        t.copy_(v)
+    graph.replay()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = ops.layer_norm_forward(x, gamma, beta, checkpoint=True)
+        want_grads = ops.layer_norm_backward_checkpoint(gy, want[2], want[3], want[1], gamma)
+    torch.cuda.synchronize()
+    for a, b in zip((y, stats, codes, params) + grads, want + want_grads):
+        assert torch.equal(a, b)

@@ -266,3 +266,40 @@ def test_gradient_against_differences():
 def test_refusals(call):
     with pytest.raises(RuntimeError):
         call(*make(8, 16, 300, torch.float32, 1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_results_of_two_blocks(dtype):
+    """More than 1024 rows: the gradients (and fp32 logits) come from pairs of blocks, with ragged tiles on every side."""
+    check(*make(1100, 200, 900, dtype, 3), 0.01)
+    check(*make(1025, 40, 257, dtype, 4, on=1.0), 0.01)
+    check(*make(2000, 264, 515, dtype, 5, on=0.1), 0.01)  # far fewer rows in the loss than the tiles allow for
+    x, w, b, labels, mask = make(1500, 40, 300, dtype, 9)
+    loss, gx, gw, gb = ops.linear_nll_loss_grad(x, w, b, labels, torch.zeros_like(mask), 1.0)
+    assert loss.item() == 0 and not gx.any() and not gw.any() and not gb.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_several_chunks_of_rows(dtype):
+    check(*make(20_000, 24, 600, dtype, 3), 0.01)
+    check(*make(17_000, 9, 12_000, dtype, 4, on=0.8), 0.01)
+    x, w, b, labels, mask = make(17_000, 24, 600, dtype, 5)
+    mask[5000:] = False  # the later chunks have no rows in the loss
+    check(x, w, b, labels, mask, 0.01)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_call_of_two_blocks(dtype):
+    x, w, b, labels, mask = make(1300, 72, 900, dtype, 4)
+    ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_nll_loss_grad(x, w, b, labels, mask, 0.1)
+    new = make(1300, 72, 900, dtype, 6)
+    for t, v in zip((x, w, b, labels, mask), new):
+        t.copy_(v)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, c in zip(got, ops.linear_nll_loss_grad(*new, 0.1)):
+        assert torch.equal(a, c)
