@@ -352,93 +352,130 @@ __global__ void __launch_bounds__(1024) nll_join_kernel(const NllJoin a)
     }
 }
 
-// gx of the listed rows of a chunk: the partial sums of the splits, scaled back; NaN when a wait gave up before.  One row
-// and 32 columns a block of 32 x 8 threads with many splits (dealt over the eight), a warp a row otherwise.
-template <class T>
-__global__ void __launch_bounds__(256)
-nll_rows_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_split, int splits, int row0, int row_cap,
-                    const int *__restrict__ rows, const int *__restrict__ total, float scale, const unsigned *__restrict__ largest,
-                    const int *__restrict__ failed, T *__restrict__ gx, int64_t ldgx, int K, float *__restrict__ loss, bool dealt)
+// ---- what is left once the products are done: three independent sums, in one launch ----
+// WARPS warps a block: 8, or 32 for the bias sums of many rows, at 32 registers so that two blocks fit an SM (16k x 64k x 512 bf16:
+// 4.38 ms in all; 4.65 with 8 warps, 4.44 with one block an SM).
+// gx of the listed rows of a chunk: the partial sums of the splits, scaled back; NaN when a wait gave up before.  With many splits
+// (`dealt`) a block has one row and 32 columns, and its warps share the splits; otherwise a warp has a row.
+struct RowsOut {
+    const float *acc;
+    int64_t ld, split;
+    int splits, row0, row_cap, K;
+    const int *rows, *total, *failed;
+    float scale;
+    const unsigned *largest;
+    void *gx;
+    int64_t ldgx;
+    float *loss;
+    bool dealt;
+    int blocks_x, blocks_y;
+};
+// gb of a piece from the sums over 32 rows of a chunk, onto those of the chunks before (acc); the last chunk writes the result.
+// 32 classes a block, the sums dealt over its warps; with few rows (not `dealt`) a thread adds up a class alone.
+struct BiasOut {
+    const float *part;
+    int64_t ld;
+    int row0, row_cap, count;
+    const int *total;
+    float scale;
+    float *acc;
+    bool first, last, f32;
+    void *gb;
+    bool dealt;
+    int blocks;
+};
+// gw from the partial sums of the splits (and of all chunks)
+struct WeightsOut {
+    const float *acc;
+    int64_t ld, split, C, ldgw;
+    int splits, K;
+    float scale;
+    const unsigned *largest;
+    void *gw;
+    int blocks;
+};
+
+template <class T, int WARPS>
+__device__ __forceinline__ void rows_out(const RowsOut &a, int block, float (&red)[WARPS][33])
 {
-    __shared__ float red[8][33];
-    let_next_kernel_start();
-    wait_for_kernels_before();
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const bool bad = *failed != 0;
-    if (bad && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *loss = __int_as_float(0x7fffffff);
-    const int left = *total - row0, count = left < row_cap ? left : row_cap;
-    for (int i = dealt ? blockIdx.x : blockIdx.x * 8 + g; i < count; i += dealt ? gridDim.x : gridDim.x * 8) {
-        T *out = gx + (int64_t)rows[row0 + i] * ldgx;
-        for (int k = (dealt ? blockIdx.y * 32 : 0) + lane; k < K || dealt; k += 32) {
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, bx = block % a.blocks_x, by = block / a.blocks_x;
+    const bool bad = *a.failed != 0;
+    if (bad && block == 0 && threadIdx.x == 0) *a.loss = __int_as_float(0x7fffffff);
+    const int left = *a.total - a.row0, count = left < a.row_cap ? left : a.row_cap;
+    for (int i = a.dealt ? bx : bx * WARPS + g; i < count; i += a.dealt ? a.blocks_x : a.blocks_x * WARPS) {
+        T *out = static_cast<T *>(a.gx) + (int64_t)a.rows[a.row0 + i] * a.ldgx;
+        for (int k = (a.dealt ? by * 32 : 0) + lane; k < a.K || a.dealt; k += 32) {
             float v = 0.f;
-            if (k < K) {
+            if (k < a.K) {
 #pragma unroll 4
-                for (int s = dealt ? g : 0; s < splits; s += dealt ? 8 : 1) v += acc[s * acc_split + (int64_t)i * acc_ld + k];
+                for (int s = a.dealt ? g : 0; s < a.splits; s += a.dealt ? WARPS : 1) v += a.acc[s * a.split + (int64_t)i * a.ld + k];
             }
-            if (dealt) {
+            if (a.dealt) {
                 __syncthreads();
                 red[g][lane] = v;
                 __syncthreads();
-                for (int w = 1; w < 8; ++w) v = (w == 1 ? red[0][lane] : v) + red[w][lane];
+                if (g == 0)
+                    for (int w = 1; w < WARPS; ++w) v += red[w][lane];
             }
             float up, down = 1.f;
-            if (largest != nullptr && k < K) plane_scale(__uint_as_float(largest[k]), up, down);
-            if (k < K && (!dealt || g == 0)) out[k] = from_f32<T>(bad ? __int_as_float(0x7fffffff) : v * scale * down);
-            if (dealt) break;
+            if (a.largest != nullptr && k < a.K) plane_scale(__uint_as_float(a.largest[k]), up, down);
+            if (k < a.K && (!a.dealt || g == 0)) out[k] = from_f32<T>(bad ? __int_as_float(0x7fffffff) : v * a.scale * down);
+            if (a.dealt) break;
         }
     }
 }
 
-// gb of a piece from the sums over 32 rows of a chunk, onto those of the chunks before (acc); the last chunk writes the result.
-// 32 classes a block, the sums dealt over its 32 warps; with few rows a thread adds up a class alone.
-template <class T>
-__global__ void __launch_bounds__(1024)
-nll_bias_out_kernel(const float *__restrict__ part, int64_t ld, int row0, int row_cap, const int *__restrict__ total, int count, float scale,
-                    float *__restrict__ acc, bool first, bool last, bool f32, void *__restrict__ gb, bool dealt)
+template <class T, int WARPS>
+__device__ __forceinline__ void bias_out(const BiasOut &a, int block, float (&red)[WARPS][33])
 {
-    __shared__ float red[32][33];
-    let_next_kernel_start();
-    wait_for_kernels_before();
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = dealt ? blockIdx.x * 32 + lane : blockIdx.x * 1024 + threadIdx.x;
-    int rows = *total - row0;
-    rows = rows < 0 ? 0 : rows < row_cap ? rows : row_cap;
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = a.dealt ? block * 32 + lane : block * WARPS * 32 + threadIdx.x;
+    int rows = *a.total - a.row0;
+    rows = rows < 0 ? 0 : rows < a.row_cap ? rows : a.row_cap;
     const int groups = (rows + kPM - 1) / kPM * (kPM / 32);  // whole tiles have been written
     float s = 0.f;
-    if (c < count) {
-#pragma unroll 4
-        for (int i = dealt ? g : 0; i < groups; i += dealt ? 32 : 1) s += part[(int64_t)i * ld + c];
+    if (c < a.count) {
+#pragma unroll 8
+        for (int i = a.dealt ? g : 0; i < groups; i += a.dealt ? WARPS : 1) s += a.part[(int64_t)i * a.ld + c];
     }
-    if (dealt) {
+    if (a.dealt) {
         red[g][lane] = s;
         __syncthreads();
         if (g != 0) return;
-        for (int w = 1; w < 32; ++w) s += red[w][lane];
+        for (int w = 1; w < WARPS; ++w) s += red[w][lane];
     }
-    if (c >= count) return;
-    if (!first) s += acc[c];
-    if (!last) acc[c] = s;
-    else if (f32) static_cast<float *>(gb)[c] = s * scale;
-    else static_cast<T *>(gb)[c] = from_f32<T>(s * scale);
+    if (c >= a.count) return;
+    if (!a.first) s += a.acc[c];
+    if (!a.last) a.acc[c] = s;
+    else if (a.f32) static_cast<float *>(a.gb)[c] = s * a.scale;
+    else static_cast<T *>(a.gb)[c] = from_f32<T>(s * a.scale);
 }
 
-// gw from the partial sums of the splits (and of all chunks)
-template <class T>
-__global__ void __launch_bounds__(256)
-nll_weight_out_kernel(const float *__restrict__ acc, int64_t acc_ld, int64_t acc_split, int splits, int64_t C, int K, float scale,
-                      const unsigned *__restrict__ largest, T *__restrict__ gw, int64_t ldgw)
+template <class T, int WARPS>
+__device__ __forceinline__ void weights_out(const WeightsOut &a, int block)
 {
-    let_next_kernel_start();
-    wait_for_kernels_before();
     const int lane = threadIdx.x & 31;
-    for (int64_t c = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); c < C; c += (int64_t)gridDim.x * 8) {
+    for (int64_t c = (int64_t)block * WARPS + (threadIdx.x >> 5); c < a.C; c += (int64_t)a.blocks * WARPS) {
 #pragma unroll 4
-        for (int k = lane; k < K; k += 32) {
+        for (int k = lane; k < a.K; k += 32) {
             float v = 0.f, up, down = 1.f;
-            for (int s = 0; s < splits; ++s) v += acc[s * acc_split + c * acc_ld + k];
-            if (largest != nullptr) plane_scale(__uint_as_float(__ldg(largest + k)), up, down);
-            gw[c * ldgw + k] = from_f32<T>(v * scale * down);
+            for (int s = 0; s < a.splits; ++s) v += a.acc[s * a.split + c * a.ld + k];
+            if (a.largest != nullptr) plane_scale(__uint_as_float(__ldg(a.largest + k)), up, down);
+            static_cast<T *>(a.gw)[c * a.ldgw + k] = from_f32<T>(v * a.scale * down);
         }
     }
+}
+
+// The first blocks sum up rows, the next ones the bias, the rest weights; none of a kind whose `blocks` are 0.
+template <class T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 64 / WARPS) nll_out_kernel(const RowsOut r, const BiasOut b, const WeightsOut w)
+{
+    __shared__ float red[WARPS][33];
+    let_next_kernel_start();
+    wait_for_kernels_before();
+    const int rows_blocks = r.blocks_x * r.blocks_y, block = (int)blockIdx.x;
+    if (block < rows_blocks) rows_out<T, WARPS>(r, block, red);
+    else if (block < rows_blocks + b.blocks) bias_out<T, WARPS>(b, block - rows_blocks, red);
+    else weights_out<T, WARPS>(w, block - rows_blocks - b.blocks);
 }
 
 // ---------------------------------------------------------------------------
@@ -473,7 +510,7 @@ struct NllPlan {
     int planes;
     int64_t blocks, padded, row_cap, chunks, cls_padded, piece, ld, acc_ld;
     int row_splits, weight_splits;
-    bool copy_w, direct;
+    bool copy_w, direct, together;
     size_t counts, rows, total, failed, joined, label, picked2, lse2, loss_part, bias2, stats;
     size_t x_row, x_col, w_row, w_col, x_down, w_down, largest;
     size_t grad, acc_x, acc_w, bias_part, bias_acc, bytes;
@@ -505,6 +542,9 @@ static void nll_divide(NllPlan &p, int64_t K, int64_t C, bool may_direct)
         if (best == 0 || ns < best) {
             best = ns;
             p.row_cap = t * kPM, p.chunks = chunks, p.piece = piece * kPN, p.row_splits = rs, p.weight_splits = ws, p.direct = direct;
+            // One launch: 300 x 30000 x 256 bf16 in 97 us instead of 109, 5003 x 20011 x 200 fp32 in 598 instead of 624 (with
+            // the sums in one launch too); 16k x 64k x 512 bf16, where the rule keeps them apart, in 4.65 ms instead of 4.37.
+            p.together = rows_ns + weights_ns < 150e3;
         }
         if (tiles <= 8) break;  // a small call: one chunk, and no search
     }
@@ -581,14 +621,14 @@ static bool nll_may_direct(int dtype, const void *gw, int64_t ldgw)
 }
 
 template <int KIND, int PLANES, int CTAS>
-static int nll_product_blocks(const ProductCall &c, int64_t units, cudaStream_t s)
+static int nll_product_blocks(const ProductCall &c, const ProductCall &c2, int64_t units, cudaStream_t s)
 {
     constexpr int smem = product_shared_bytes<KIND, PLANES, CTAS>();
     static ResidentCache cache;
     int resident = 0, rc = resident_blocks(nll_product_kernel<KIND, PLANES, CTAS>, kPThreads, smem, smem, cache, &resident);
     if (rc) return rc;
     const int64_t most = resident / CTAS, grid = CTAS * (units < most ? units : most);
-    SGNN_CUDA_OK(launch_clusters(CTAS, nll_product_kernel<KIND, PLANES, CTAS>, dim3((unsigned)grid), kPThreads, smem, s, c));
+    SGNN_CUDA_OK(launch_clusters(CTAS, nll_product_kernel<KIND, PLANES, CTAS>, dim3((unsigned)grid), kPThreads, smem, s, c, c2));
     return SGNN_OK;
 }
 
@@ -599,15 +639,16 @@ static int nll_product_blocks(const ProductCall &c, int64_t units, cudaStream_t 
 template <int KIND, int PLANES>
 static bool nll_in_pairs(int64_t row_cap)
 {
-    return row_cap > 1024 && (KIND == kRowGrad || KIND == kWeightGrad || PLANES == 2);
+    return row_cap > 1024 && (PLANES == 2 || (KIND != kLogitStats && KIND != kLogitGrad));
 }
 
-// `rows` of the result at most, `tiles` beside and behind each other (columns of the result, splits)
+// Results of `rows` rows at most and `tiles` beside each other (gradients: and of `rows2` and `tiles2`; splits count as tiles)
 template <int KIND, int PLANES>
-static int nll_product(const ProductCall &c, int64_t rows, int64_t tiles, cudaStream_t s)
+static int nll_product(const ProductCall &c, const ProductCall &c2, int64_t rows, int64_t tiles, int64_t rows2, int64_t tiles2, cudaStream_t s)
 {
-    if (nll_in_pairs<KIND, PLANES>(c.row_cap)) return nll_product_blocks<KIND, PLANES, 2>(c, ceil_div(rows, 2 * kPM) * tiles, s);
-    return nll_product_blocks<KIND, PLANES, 1>(c, ceil_div(rows, kPM) * tiles, s);
+    if (nll_in_pairs<KIND, PLANES>(c.row_cap))
+        return nll_product_blocks<KIND, PLANES, 2>(c, c2, ceil_div(rows, 2 * kPM) * tiles + ceil_div(rows2, 2 * kPM) * tiles2, s);
+    return nll_product_blocks<KIND, PLANES, 1>(c, c2, ceil_div(rows, kPM) * tiles + ceil_div(rows2, kPM) * tiles2, s);
 }
 
 template <class T, int PLANES>
@@ -689,7 +730,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         for (ProductCall *k : {&lc, &xc, &wc}) k->row0 = row0;
         lc.label = ints(p.label) + row0, lc.picked2 = floats(p.picked2) + row0;
         lc.cls0 = 0, lc.cls_count = (int)c.C;
-        if ((rc = nll_product<kLogitStats, PLANES>(lc, p.row_cap, ceil_div(c.C, kPN), s))) return rc;
+        if ((rc = nll_product<kLogitStats, PLANES>(lc, lc, p.row_cap, ceil_div(c.C, kPN), 0, 0, s))) return rc;
         const NllJoin join{lc.stats, (int)(p.cls_padded / 128), row0, (int)p.row_cap, ints(p.rows), ints(p.total), lc.picked2,
                            floats(p.lse2), c.lse, floats(p.loss_part) + q * join_blocks, floats(p.loss_part),
                            (int)(p.chunks * join_blocks), c.inv_count, ints(p.joined), ints(p.failed), c.loss};
@@ -698,29 +739,41 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         for (int64_t first = 0; first < c.C; first += p.piece) {
             const int64_t count = c.C - first < p.piece ? c.C - first : p.piece;
             for (ProductCall *k : {&lc, &xc, &wc}) k->cls0 = (int)first, k->cls_count = (int)count;
-            if ((rc = nll_product<kLogitGrad, PLANES>(lc, p.row_cap, ceil_div(count, kPN), s))) return rc;
-            xc.add = first > 0;
-            if ((rc = nll_product<kRowGrad, PLANES>(xc, p.row_cap, tiles_k * p.row_splits, s))) return rc;
-            wc.add = q > 0;
-            if ((rc = nll_product<kWeightGrad, PLANES>(wc, count, tiles_k * p.weight_splits, s))) return rc;
+            if ((rc = nll_product<kLogitGrad, PLANES>(lc, lc, p.row_cap, ceil_div(count, kPN), 0, 0, s))) return rc;
+            xc.add = first > 0, wc.add = q > 0;
+            if (p.together) {
+                if ((rc = nll_product<kGradients, PLANES>(xc, wc, p.row_cap, tiles_k * p.row_splits, count, tiles_k * p.weight_splits, s))) return rc;
+            } else {
+                if ((rc = nll_product<kRowGrad, PLANES>(xc, xc, p.row_cap, tiles_k * p.row_splits, 0, 0, s))) return rc;
+                if ((rc = nll_product<kWeightGrad, PLANES>(wc, wc, count, tiles_k * p.weight_splits, 0, 0, s))) return rc;
+            }
+            const bool deal = p.row_cap > 256;
+            const int warps = p.row_cap >= 8192 ? 32 : 8;
+            BiasOut bias{};
             if (c.gb) {
                 char *gb = static_cast<char *>(c.gb) + first * (c.bias.f32 ? 4 : sizeof(T));
-                const bool deal = p.row_cap / 32 > 32;
-                SGNN_CUDA_OK(launch_chained(nll_bias_out_kernel<T>, dim3((unsigned)ceil_div(count, deal ? 32 : 1024)), 1024, 0, s,
-                                            lc.bias_part, p.piece, row0, (int)p.row_cap, ints(p.total), (int)count, lc.scale,
-                                            p.chunks > 1 ? floats(p.bias_acc) + first : nullptr, q == 0, q + 1 == p.chunks,
-                                            c.bias.f32, gb, deal));
+                bias = BiasOut{lc.bias_part, p.piece, row0, (int)p.row_cap, (int)count, ints(p.total), lc.scale,
+                               p.chunks > 1 ? floats(p.bias_acc) + first : nullptr, q == 0, q + 1 == p.chunks, c.bias.f32, gb, deal,
+                               (int)ceil_div(count, deal ? 32 : 32 * warps)};
             }
+            const bool last = first + p.piece >= c.C;  // the pieces of this chunk are all in gx
+            RowsOut rows{};
+            if (last) {
+                const bool dealt = p.row_splits >= 8;
+                rows = RowsOut{floats(p.acc_x), p.acc_ld, x_split, p.row_splits, row0, (int)p.row_cap, (int)c.K, ints(p.rows), ints(p.total),
+                               ints(p.failed), lc.scale, cols ? largest + c.K : nullptr, c.gx, c.ldgx, c.loss, dealt,
+                               dealt ? (int)(p.row_cap < wide ? p.row_cap : wide) : (int)ceil_div(p.row_cap, warps),
+                               dealt ? (int)ceil_div(c.K, 32) : 1};
+            }
+            WeightsOut weights{};
+            if (last && q + 1 == p.chunks && !p.direct)
+                weights = WeightsOut{floats(p.acc_w), p.acc_ld, w_split, c.C, c.ldgw, p.weight_splits, (int)c.K, lc.scale, largest, c.gw,
+                                     (int)ceil_div(c.C, 4 * warps)};
+            const int grid = rows.blocks_x * rows.blocks_y + bias.blocks + weights.blocks;
+            if (grid > 0)
+                SGNN_CUDA_OK(launch_chained(warps == 32 ? nll_out_kernel<T, 32> : nll_out_kernel<T, 8>, dim3((unsigned)grid), warps * 32, 0, s,
+                                            rows, bias, weights));
         }
-        const bool dealt = p.row_splits >= 8;
-        const dim3 out_grid = dealt ? dim3((unsigned)(p.row_cap < wide ? p.row_cap : wide), (unsigned)ceil_div(c.K, 32)) : dim3(blocks(p.row_cap));
-        SGNN_CUDA_OK(launch_chained(nll_rows_out_kernel<T>, out_grid, 256, 0, s, floats(p.acc_x), p.acc_ld, x_split, p.row_splits, row0,
-                                    (int)p.row_cap, ints(p.rows), ints(p.total), lc.scale, cols ? largest + c.K : nullptr, ints(p.failed),
-                                    static_cast<T *>(c.gx), c.ldgx, (int)c.K, c.loss, dealt));
-    }
-    if (grad && !p.direct) {
-        SGNN_CUDA_OK(launch_chained(nll_weight_out_kernel<T>, dim3(blocks(c.C)), 256, 0, s, floats(p.acc_w), p.acc_ld, w_split,
-                                    p.weight_splits, c.C, (int)c.K, lc.scale, largest, static_cast<T *>(c.gw), c.ldgw));
     }
     return SGNN_OK;
 }

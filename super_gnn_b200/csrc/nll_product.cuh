@@ -2,7 +2,11 @@
 //
 //     logits   z[i, c]  = sum_k x[i, k] W[c, k]     epilogue: running (max, sum) of a row, or the gradient G
 //     rows     gx[i, k] = sum_c G[i, c] W[c, k]
-//     weights  gw[c, k] = sum_i G[i, c] x[i, k]     and gb[c] = sum_i G[i, c], a product with ones
+//     weights  gw[c, k] = sum_i G[i, c] x[i, k]
+//
+// The two gradients run as one launch where they are short: one tail, and one launch less to wait for.  Long ones run better
+// alone (16k x 64k x 512 bf16: 4.37 ms against 4.65), where which of the two it is is known to the compiler and G has one reader
+// at a time.
 //
 // One persistent block an SM.  A warp feeds operand tiles by TMA through a ring of shared memory buffers, a thread issues
 // the tcgen05 products into tensor memory, eight warps turn finished 128 x 256 results into the outputs.  Two blocks of a
@@ -24,7 +28,7 @@ constexpr int kPEpilogueWarps = 8;
 constexpr int kPThreads = (kPEpilogueWarps + 2) * 32;
 constexpr int kPAccCols = 512;  // all of the tensor memory: two results, or one and its cross products
 
-enum ProductKind { kLogitStats, kLogitGrad, kRowGrad, kWeightGrad };
+enum ProductKind { kLogitStats, kLogitGrad, kGradients, kRowGrad, kWeightGrad };
 
 struct ProductCall {
     CUtensorMap a, b, o;  // operands, result
@@ -77,8 +81,9 @@ struct ProductUnits {
     int m, n, blocks, per_split, tiles_m, tiles_n, units, rows;
 };
 
+// `weights`: of the two gradients the second
 template <int KIND, int CTAS>
-__device__ __forceinline__ ProductUnits product_units(const ProductCall &c)
+__device__ __forceinline__ ProductUnits product_units(const ProductCall &c, bool weights)
 {
     ProductUnits u;
     int rows = *c.total - c.row0;
@@ -86,7 +91,7 @@ __device__ __forceinline__ ProductUnits product_units(const ProductCall &c)
     u.rows = rows;
     int red;
     if (KIND == kLogitStats || KIND == kLogitGrad) u.m = rows, u.n = c.cls_count, red = c.feats;
-    else if (KIND == kRowGrad) u.m = rows, u.n = c.feats, red = c.cls_count;
+    else if (!weights) u.m = rows, u.n = c.feats, red = c.cls_count;
     else u.m = c.cls_count, u.n = c.feats, red = rows;
     u.blocks = (red + kPK - 1) / kPK;
     u.per_split = (u.blocks + c.splits - 1) / c.splits;
@@ -144,12 +149,14 @@ __device__ __forceinline__ void plane_scale(float largest, float &up, float &dow
 
 constexpr float kGradScale = 32768.0f;  // fp16 planes of G: |G| <= 1 fills the range, 2^-40 is the smallest step
 
+// `c`: the logits or the rows' gradient; `c2`: the weights' gradient (a kernel of one kind takes the same for both)
 template <int KIND, int PLANES, int CTAS>
-__global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_constant__ ProductCall c)
+__global__ void __launch_bounds__(kPThreads, 1)
+nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant__ ProductCall c2)
 {
     using S = ProductShared<PLANES, CTAS>;
     constexpr bool kLogits = KIND == kLogitStats || KIND == kLogitGrad;
-    constexpr bool kAmn = KIND == kWeightGrad, kBmn = !kLogits;
+    constexpr bool kBmn = !kLogits;
     constexpr bool kCross = !kLogits && PLANES == 2;  // cross products have their own sums, in the other half of the tensor memory
     constexpr int kAcc = kCross ? 1 : 2;              // results in flight
     extern __shared__ __align__(1024) uint8_t base[];
@@ -189,18 +196,24 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
     tc_fence_after();
     const uint32_t tmem = *slot;
     wait_for_kernels_before();
-    const ProductUnits u = product_units<KIND, CTAS>(c);
+    constexpr bool kBoth = KIND == kGradients;
+    const ProductUnits u1 = product_units<KIND, CTAS>(c, KIND == kWeightGrad), u2 = kBoth ? product_units<KIND, CTAS>(c2, true) : u1;
+    const int units = u1.units + (kBoth ? u2.units : 0);
 
     if (warp == kPEpilogueWarps) {
         // ---- loads ----
         if (lane == 0) {
             tma_prefetch(&c.a);
             tma_prefetch(&c.b);
+            if (kBoth) tma_prefetch(&c2.a), tma_prefetch(&c2.b);
             int stage = 0;
             unsigned phase = 0, used = 0;
             bool ok = true;
-            for (int i = first_unit; i < u.units && ok; i += unit_step) {
-                const ProductUnit t = product_unit<KIND, CTAS>(u, i, rank);
+            for (int i = first_unit; i < units && ok; i += unit_step) {
+                const bool second = kBoth && i >= u1.units, weights = KIND == kWeightGrad || second;
+                const ProductUnits &u = second ? u2 : u1;
+                const CUtensorMap *ma = second ? &c2.a : &c.a, *mb = second ? &c2.b : &c.b;
+                const ProductUnit t = product_unit<KIND, CTAS>(u, second ? i - u1.units : i, rank);
                 const int left = u.n - t.n0, own_n = (left < kPN ? (left + 15) / 16 * 16 : kPN) / CTAS;  // columns of the second operand here
                 const int runs = kBmn ? (own_n + 63) / 64 : 1;
                 const unsigned bytes = PLANES * (S::kA + (kBmn ? runs * 64 * kPK * 2 : S::kB));
@@ -218,17 +231,17 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p) {
                         uint8_t *pa = at + p * S::kA, *pb = at + PLANES * S::kA + p * S::kB;
-                        if (kAmn) {
-                            load(pa, &c.a, t.m0, k0, p);
-                            load(pa + 64 * kPK * 2, &c.a, t.m0 + 64, k0, p);
+                        if (weights) {
+                            load(pa, ma, t.m0, k0, p);
+                            load(pa + 64 * kPK * 2, ma, t.m0 + 64, k0, p);
                         } else {
-                            load(pa, &c.a, k0, t.m0 + (kLogits ? c.row0 : 0), p);
+                            load(pa, ma, k0, t.m0 + (kLogits ? c.row0 : 0), p);
                         }
                         if (kBmn) {
-                            const int k1 = k0 + (KIND == kRowGrad ? c.cls0 : c.row0);
-                            for (int r = 0; r < runs; ++r) load(pb + r * 64 * kPK * 2, &c.b, t.n0 + rank * own_n + 64 * r, k1, p);
+                            const int k1 = k0 + (weights ? c.row0 : c.cls0);
+                            for (int r = 0; r < runs; ++r) load(pb + r * 64 * kPK * 2, mb, t.n0 + rank * own_n + 64 * r, k1, p);
                         } else {
-                            load(pb, &c.b, k0, t.n0 + c.cls0 + rank * (kPN / CTAS), p);
+                            load(pb, mb, k0, t.n0 + c.cls0 + rank * (kPN / CTAS), p);
                         }
                     }
                     ++used;
@@ -262,11 +275,13 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                 if (CTAS == 2) umma_pair(d, a, b, idesc, add);
                 else umma(d, a, b, idesc, add);
             };
-            for (int i = first_unit; i < u.units && ok; i += unit_step) {
-                const ProductUnit t = product_unit<KIND, CTAS>(u, i, rank);
+            for (int i = first_unit; i < units && ok; i += unit_step) {
+                const bool second = kBoth && i >= u1.units, weights = KIND == kWeightGrad || second;
+                const ProductUnits &u = second ? u2 : u1;
+                const ProductUnit t = product_unit<KIND, CTAS>(u, second ? i - u1.units : i, rank);
                 const int left = u.n - t.n0;
                 const int n = kBmn ? (left < kPN ? (left + 15) / 16 * 16 : kPN) : kPN;
-                const uint32_t idesc = umma_idesc(c.bf16, kAmn, kBmn, n, kPM * CTAS);
+                const uint32_t idesc = umma_idesc(c.bf16, weights, kBmn, n, kPM * CTAS);
                 ok = bar_wait(acc_empty + acc, acc_phase ^ 1, gone);
                 if (!ok) break;
                 tc_fence_after();
@@ -277,7 +292,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                     tc_fence_after();
                     const uint8_t *at = base + stage * S::kStageBytes;
                     // eight-row groups 1024 bytes apart; MN-major operands: 64-element runs of kPK rows each
-                    const unsigned a_run = kAmn ? 64 * kPK * 2 : 16, b_run = kBmn ? 64 * kPK * 2 : 16;
+                    const unsigned a_run = weights ? 64 * kPK * 2 : 16, b_run = kBmn ? 64 * kPK * 2 : 16;
                     uint64_t da[PLANES], db[PLANES];
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p) {
@@ -287,7 +302,7 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
 #pragma unroll
                     for (int j = 0; j < kPK / 16; ++j) {
                         // sixteen steps of the reduction: 32 bytes along a row, or two groups of eight rows
-                        const uint64_t sa = (kAmn ? 2048u : 32u) * j >> 4, sb = (kBmn ? 2048u : 32u) * j >> 4;
+                        const uint64_t sa = (weights ? 2048u : 32u) * j >> 4, sb = (kBmn ? 2048u : 32u) * j >> 4;
                         const bool more = k > 0 || j > 0;
                         product(d, da[0] + sa, db[0] + sb, idesc, more);
                         if (PLANES == 2) {
@@ -316,8 +331,10 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
         uint8_t *box_row = box + lane * 128;
         int acc = 0;
         unsigned acc_phase = 0;
-        for (int i = first_unit; i < u.units; i += unit_step) {
-            const ProductUnit t = product_unit<KIND, CTAS>(u, i, rank);
+        for (int i = first_unit; i < units; i += unit_step) {
+            const bool second = kBoth && i >= u1.units, weights = KIND == kWeightGrad || second;
+            const ProductUnits &u = second ? u2 : u1;
+            const ProductUnit t = product_unit<KIND, CTAS>(u, second ? i - u1.units : i, rank);
             const int row = t.m0 + quarter * 32 + lane;  // of the product
             float *bias_col = column + (kColumns == 2 ? acc : 0) * 2 * kPN, *scale_col = bias_col + kPN;
             if (kLogits) {
@@ -469,8 +486,9 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                     }
                 }
             } else {
-                const bool direct = KIND == kWeightGrad && c.direct, wide = direct && c.direct_bf16;
-                const int y0 = t.m0 + quarter * 32 + (KIND == kWeightGrad ? c.cls0 : 0);
+                const bool direct = weights && c2.direct, wide = direct && c2.direct_bf16, add = weights ? c2.add : c.add;
+                const CUtensorMap *mo = second ? &c2.o : &c.o;
+                const int y0 = t.m0 + quarter * 32 + (weights ? c.cls0 : 0), end = weights ? (int)c.classes : c.row_cap;
 #pragma unroll 1
                 for (int j = 0; j < 4; ++j) {
                     const int k0 = t.n0 + half * 128 + 32 * j;
@@ -490,12 +508,12 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                     }
                     if (direct) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] *= c.scale;
+                        for (int e = 0; e < 32; ++e) v[e] *= c2.scale;
                         if (PLANES == 2) {
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
                                 float up, down;
-                                plane_scale(__uint_as_float(k0 + e < u.n ? __ldg(c.col_largest + k0 + e) : 0u), up, down);
+                                plane_scale(__uint_as_float(k0 + e < u.n ? __ldg(c2.col_largest + k0 + e) : 0u), up, down);
                                 v[e] *= down;
                             }
                         }
@@ -518,10 +536,10 @@ __global__ void __launch_bounds__(kPThreads, 1) nll_product_kernel(const __grid_
                         if ((j & 1) == 0 && k0 + 32 < u.n) continue;  // 64 columns a box
                     }
                     box_done();
-                    if (lane == 0 && y0 < (KIND == kWeightGrad ? (int)c.classes : c.row_cap)) {
+                    if (lane == 0 && y0 < end) {
                         const int x0 = wide ? t.n0 + half * 128 + 64 * (j >> 1) : k0;
-                        if (c.add) tma_add(&c.o, box, x0, y0, t.split);
-                        else tma_store(&c.o, box, x0, y0, t.split);
+                        if (add) tma_add(mo, box, x0, y0, t.split);
+                        else tma_store(mo, box, x0, y0, t.split);
                         store_commit();
                     }
                 }
