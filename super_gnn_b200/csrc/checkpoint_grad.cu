@@ -3,18 +3,19 @@
 //     gW[m, k] = sum_r g[r, m] (zp_r + sc_r code[r, k])  (+ beta gW[m, k])
 //              = sum_r (g[r, m] sc_r) code[r, k]  +  sum_r g[r, m] zp_r
 //
-// The first sum runs on the tensor cores: a code is exact in bf16, and g sc is carried as two bf16 terms (16 bits and
-// more of significand, 2^-17 of a value at most, next to codes that are half a step of 255 off), so a tile takes two
-// products where two fp32 operands would take six.  The second does not depend on k: a few fp32 multiply-adds beside the
-// conversion of g.  The activations are never restored in memory: one byte an element is read.
+// The first sum runs on the tensor cores: a code is exact in bf16, and g sc, rounded once, is carried as three bf16 terms, its
+// 24 bits, so a tile takes three products where two fp32 operands would take six.  (Two terms, 2^-17 of a value off, took 570 us
+// instead of 625 for 600k rows of 512 and 256 columns, and left the result 2.6e-6 off instead of 0.7e-6.)  The second sum does
+// not depend on k: a few fp32 multiply-adds beside the conversion of g.  The activations are never restored in memory: one byte
+// an element is read.
 //
 // A block owns 128 x 256 results and a range of the rows.  Per 32 rows TMA brings 128 columns of g and 256 of the codes
 // into shared memory as they are (where an operand is not aligned for it, the threads load it themselves); sixteen warps
 // convert them: the terms of g go to tensor memory, a thread for each of its 128 lanes, the codes back to shared memory as the
 // swizzled "MN-major" operand that keeps the order of their rows; one thread issues the products.  What bounds the kernel is the
-// bandwidth of shared memory (128 bytes a clock: 105 KB a step; 129 KB with the terms of g there as well).
+// bandwidth of shared memory (128 bytes a clock: 121 KB a step; 157 KB with the terms of g there as well).
 // Tensor memory rounds every addition towards zero, which over thousands of rows would shrink the result by 1e-5 of itself, so
-// after 512 rows the sums move on into the fp32 registers of eight other warps.  The partial results of the row ranges are added
+// after 256 rows the sums move on into the fp32 registers of eight other warps.  The partial results of the row ranges are added
 // in a fixed order.
 #include "row_io.cuh"
 #include "umma.cuh"
@@ -27,8 +28,9 @@ constexpr int kGWorkers = 16;                     // warps that convert
 constexpr int kGOwn = kGRows * 4 / kGWorkers;       // rows of g a converting thread has in a step
 constexpr int kGThreads = (kGKeepers + kGWorkers + 4) * 32;  // and a group of four: one feeds, one issues the products
 constexpr int kGRaw = 5, kGStages = 4;            // buffers of operands as they come, and converted
-constexpr int kGPromote = 16;                     // steps between two moves into registers
-constexpr int kGStageBytes = kGN * kGRows * 2;    // the codes of a step; the two terms of g take 32 columns of tensor memory
+constexpr int kGPromote = 8;                      // steps between two moves into registers
+constexpr int kGStageBytes = kGN * kGRows * 2;    // the codes of a step; the terms of g take 48 columns of tensor memory
+constexpr int kGTermColumns = 3 * 16;              // of a step: 32 bf16 values a lane and term
 constexpr int kGTerms = kGN;                      // where those columns begin, behind the sums
 
 struct GradCall {
@@ -83,17 +85,15 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
     return r;
 }
 
-// two values times their scales as two bf16 terms each, hi + lo
-__device__ __forceinline__ void two_terms(float v0, float v1, float sc0, float sc1, uint32_t &hi, uint32_t &lo)
+// two bf16 values, the nearest to x and y, which keep what is left
+__device__ __forceinline__ uint32_t next_term(unsigned long long &xy)
 {
-    const unsigned long long x2 = mul2(pk2(v0, v1), pk2(sc0, sc1));
     float x, y;
-    unpk2(x2, x, y);
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    unpk2(sub2(x2, pk2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u))), x, y);
-    const __nv_bfloat162 l = __floats2bfloat162_rn(x, y);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+    unpk2(xy, x, y);
+    const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
+    const uint32_t bits = *reinterpret_cast<const uint32_t *>(&t);
+    xy = sub2(xy, pk2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xFFFF0000u)));
+    return bits;
 }
 
 template <class T, int FEED>
@@ -178,12 +178,13 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t b = umma_desc(base + s * kGStageBytes, kGRows * 128, 1024);
-                    const uint32_t a = tmem + kGTerms + s * 32;
+                    const uint32_t a = tmem + kGTerms + s * kGTermColumns;
 #pragma unroll
                     for (int j = 0; j < kGRows / 16; ++j) {  // sixteen rows: two groups of eight, eight columns of tensor memory
                         const uint64_t step = 2048u * j >> 4;
                         umma_ts(tmem, a + 8 * j, b + step, idesc, k % kGPromote > 0 || j > 0);
                         umma_ts(tmem, a + 16 + 8 * j, b + step, idesc, true);
+                        umma_ts(tmem, a + 32 + 8 * j, b + step, idesc, true);
                     }
                     tc_commit(empty + s);
                     if (k % kGPromote == kGPromote - 1 || k == count - 1) tc_commit(acc_full);
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     } else {
         // ---- conversion ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        const int tid = threadIdx.x - kGKeepers * 32, w = warp - kGKeepers;
+        const int w = warp - kGKeepers;
         const int quarter = w & 3, first_row = (w >> 2) * kGOwn;  // of g: one column, kGOwn rows
         const int m = quarter * 32 + lane, nq = n0 + lane * 8;  // of the codes: eight columns, rows w, w + kGWorkers, ...
         const uint32_t terms = tmem + kGTerms + (first_row >> 1) + ((uint32_t)quarter << 21);
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             if (FEED != kFeedNone && !bar_wait(raw_full + s, raw_phase, gone)) break;
             if (!bar_wait(empty + t, phase ^ 1, gone)) break;
             uint8_t *at = base + t * kGStageBytes;
-            uint32_t hi[kGOwn / 2], lo[kGOwn / 2];
+            uint32_t term[3][kGOwn / 2];
             float share = 0.f;
 #pragma unroll
             for (int i = 0; i < kGOwn / 2; ++i) {
@@ -295,11 +296,13 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                 }
                 share = __fmaf_rn(v0, par.x, share);
                 share = __fmaf_rn(v1, par.z, share);
-                two_terms(v0, v1, par.y, par.w, hi[i], lo[i]);
+                unsigned long long left = mul2(pk2(v0, v1), pk2(par.y, par.w));
+#pragma unroll
+                for (int e = 0; e < 3; ++e) term[e][i] = next_term(left);
             }
             zero += share;
-            tmem_store4(terms + t * 32, hi);
-            tmem_store4(terms + t * 32 + 16, lo);
+#pragma unroll
+            for (int e = 0; e < 3; ++e) tmem_store4(terms + t * kGTermColumns + 16 * e, term[e]);
 #pragma unroll
             for (int i = 0; i < kGRows / kGWorkers; ++i) {
                 const int r = w + kGWorkers * i;

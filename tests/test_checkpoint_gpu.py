@@ -94,15 +94,15 @@ def test_strided_input_and_codes():
 def grad_bounds(g, codes, params):
     """The product in 64 bits, the worst case of its error and the size its errors have when they are independent.
 
-    g sc is carried with at least 16 bits of significand (2^-17 off), the codes are exact, and every addition of a sum of
-    n terms (of the scaled codes and of the zero points) is off by at most 2^-23 of the sum of the magnitudes."""
+    g sc is rounded once (2^-24) and carried in three terms of eight bits (2^-27 more), the codes are exact, and every addition
+    of a sum of 3 n terms (of the scaled codes; n of the zero points) is off by at most 2^-23 of the sum of the magnitudes."""
     g, c = g.double(), codes.double()
     zp, sc = params[:, :1].double(), params[:, 1:].double()
     n = g.size(0)
     kept = zp + sc * c
     want = g.t() @ kept
     mags = g.abs().t() @ (sc * c + zp.abs())
-    worst = mags * (2 ** -17 + (n + 40) * 2 ** -23)
+    worst = mags * (2 ** -23 + (3 * n + 40) * 2 ** -23)
     typical = (g.square().t() @ (sc * c + zp.abs()).square()).sqrt()
     return want, worst, typical
 
@@ -122,9 +122,9 @@ def test_weight_grad(n, M, F, dtype):
     assert got.dtype == torch.float32 and got.shape == (M, F)
     off = (got.double() - want).abs()
     assert (off <= worst).all(), float((off / worst).max())
-    # errors of random sign: 2^-17 / sqrt(3) of each term for g sc, and 2^-23 of a partial sum (a few times the typical
-    # size) at no more than one addition in sixteen terms
-    assert off.norm() <= (2 ** -17 + 4 * (n / 16) ** 0.5 * 2 ** -23 + 2 ** -22) * typical.norm()
+    # 2^-23 of each value for g sc, and 2^-24 on average of a partial sum (of the typical size) at each of the three additions
+    # for sixteen rows, all towards zero, of 256 rows at most; those sums then add up with errors of random sign
+    assert off.norm() <= (2 ** -23 + (3 * min(n, 256) / 16 + 4 * (n / 256) ** 0.5 + 2) * 2 ** -24) * typical.norm()
     # adding onto an existing gradient: one more rounding
     base = torch.randn(M, F + 3, device=DEV)[:, 1:1 + F]
     out = torch.empty(M, F + 3, device=DEV)[:, 1:1 + F].copy_(base)
@@ -189,8 +189,8 @@ def test_weight_grad_over_many_rounds_and_row_ranges():
     for operand in (g, wide[:, 1:]):
         off = (ops.checkpoint_weight_grad(operand, codes, params).double() - want).abs()
         assert (off <= worst).all()
-        # terms of 2^-17, and sums of 512 rows in tensor memory: 64 additions of 2^-24 on average, all towards zero
-        assert off.norm() <= (2 ** -17 + 64 * 2 ** -24) * typical.norm()
+        # sums of 256 rows in tensor memory: 48 additions of 2^-24 on average, all towards zero, and 2^-23 for g sc and the rest
+        assert off.norm() <= (2 ** -23 + 48 * 2 ** -24 + 4 * (n / 256) ** 0.5 * 2 ** -24) * typical.norm()
 
 
 def test_captured_weight_grad():

@@ -55,7 +55,7 @@ def test_functional_forms_are_the_formulas():
     assert torch.equal(y, F.linear(xf, lw))
     gx, gw = torch.autograd.grad(y, (xf, lw), gl)
     assert torch.equal(gx, gl @ lw)
-    assert near(gw, gl.double().t() @ kept, 2 ** -16)  # g sc in two bf16 terms
+    assert near(gw, gl.double().t() @ kept, 2 ** -19)  # 10 x 3 additions towards zero, 2^-24 each, and g sc
     assert L.linear(xf, lw, checkpoint_bits=8).grad_fn is not None
     for bits in (4, 16, None):
         with pytest.raises(ValueError):
