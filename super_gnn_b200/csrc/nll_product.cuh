@@ -16,8 +16,9 @@
 //
 // fp32 operands come as two fp16 planes (v 2^e = v0 + v1, 22 bits; see linear_nll.cu) and three products
 // v0 w0 + v0 w1 + v1 w0 a tile; bf16 operands as one plane and one product.  Tensor memory rounds every addition towards zero, a
-// relative 2^-25 on average, so in the two gradients, whose reductions are long, the cross products of the planes, 2^-11 of
-// the others, have sums of their own, and the main sums a third of the additions.
+// relative 2^-25 on average, and most of G has one sign: in the two gradients, whose reductions are long, the cross products of the planes, 2^-11 of
+// the others, have sums of their own, and the main sums move on into registers every 512 of the reduction.  A sum over 55k
+// classes would else be 5e-6 of itself too small (0.7e-6 so).
 #pragma once
 #include "umma.cuh"
 
@@ -26,6 +27,7 @@ namespace sgnn {
 constexpr int kPM = 128, kPN = 256, kPK = 64;  // tile of a product, step of its reduction
 constexpr int kPEpilogueWarps = 8;
 constexpr int kPThreads = (kPEpilogueWarps + 2) * 32;
+constexpr int kPWindow = 8;     // fp32 gradients: steps after which the main sums move on into registers
 constexpr int kPAccCols = 512;  // all of the tensor memory: two results, or one and its cross products
 
 enum ProductKind { kLogitStats, kLogitGrad, kGradients, kRowGrad, kWeightGrad };
@@ -290,6 +292,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                     ok = bar_wait(full + stage, phase, gone);
                     if (!ok) break;
                     tc_fence_after();
+                    const bool starts = kCross && k % kPWindow == 0, ends = kCross && k % kPWindow == kPWindow - 1 && k + 1 < t.count;
                     const uint8_t *at = base + stage * S::kStageBytes;
                     // eight-row groups 1024 bytes apart; MN-major operands: 64-element runs of kPK rows each
                     const unsigned a_run = weights ? 64 * kPK * 2 : 16, b_run = kBmn ? 64 * kPK * 2 : 16;
@@ -299,16 +302,34 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                         da[p] = umma_desc(at + p * S::kA, a_run, 1024);
                         db[p] = umma_desc(at + PLANES * S::kA + p * S::kB, b_run, 1024);
                     }
+                    // sixteen steps of the reduction: 32 bytes along a row, or two groups of eight rows
+                    const uint64_t step_a = (weights ? 2048u : 32u) >> 4, step_b = (kBmn ? 2048u : 32u) >> 4;
+                    const auto main = [&](int j) { product(d, da[0] + step_a * j, db[0] + step_b * j, idesc, kCross ? !starts || j > 0 : k > 0 || j > 0); };
+                    const auto cross = [&](int j) {
+                        const uint32_t dx = kCross ? tmem + kPN : d;
+                        product(dx, da[0] + step_a * j, db[PLANES - 1] + step_b * j, idesc, !kCross || k > 0 || j > 0);
+                        product(dx, da[PLANES - 1] + step_a * j, db[0] + step_b * j, idesc, true);
+                    };
+                    if (kCross) {  // the cross products run while the main sums are read
+                        if (starts && k > 0) {
 #pragma unroll
-                    for (int j = 0; j < kPK / 16; ++j) {
-                        // sixteen steps of the reduction: 32 bytes along a row, or two groups of eight rows
-                        const uint64_t sa = (weights ? 2048u : 32u) * j >> 4, sb = (kBmn ? 2048u : 32u) * j >> 4;
-                        const bool more = k > 0 || j > 0;
-                        product(d, da[0] + sa, db[0] + sb, idesc, more);
-                        if (PLANES == 2) {
-                            const uint32_t dx = kCross ? tmem + kPN : d;
-                            product(dx, da[0] + sa, db[PLANES - 1] + sb, idesc, !kCross || more);
-                            product(dx, da[PLANES - 1] + sa, db[0] + sb, idesc, true);
+                            for (int j = 0; j < kPK / 16; ++j) cross(j);
+                            ok = bar_wait(acc_empty, acc_phase ^ 1, gone);
+                            if (!ok) break;
+                            tc_fence_after();
+                        }
+#pragma unroll
+                        for (int j = 0; j < kPK / 16; ++j) main(j);
+                        if (ends) commit(acc_full), acc_phase ^= 1;
+                        if (!starts || k == 0) {
+#pragma unroll
+                            for (int j = 0; j < kPK / 16; ++j) cross(j);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kPK / 16; ++j) {
+                            main(j);
+                            if (PLANES == 2) cross(j);
                         }
                     }
                     commit(empty + stage);
@@ -348,6 +369,34 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
             float scale = 1.4426950408889634f, lse2 = 0.f;
             if (kLogits && PLANES == 2) scale *= __ldg(c.row_scale + c.row0 + (row < u.m ? row : 0));
             if (KIND == kLogitGrad && row < u.m) lse2 = __ldg(c.lse2 + row);
+            float sum[kCross ? 4 : 1][32];  // the main sums of the windows before the last
+            if constexpr (kCross) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) sum[j][e] = 0.f;
+#pragma unroll 1
+                for (int k = kPWindow; k < t.count; k += kPWindow) {
+                    if (!bar_wait(acc_full, acc_phase, gone)) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (t.n0 + half * 128 + 32 * j >= u.n) break;
+                        float x[32];
+                        tmem_load32(tmem + half * 128 + 32 * j + ((uint32_t)quarter << 21), x);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) sum[j][e] += x[e];
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (CTAS == 2) leader_arrive(acc_empty);
+                        else bar_arrive(acc_empty);
+                    }
+                    acc_phase ^= 1;
+                }
+            }
             if (!bar_wait(acc_full + acc, acc_phase, gone)) {  // the others may stand at the barrier above: keep coming to it
                 if (++acc == kAcc) acc = 0, acc_phase ^= 1;
                 continue;
@@ -489,7 +538,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                 const bool direct = weights && c2.direct, wide = direct && c2.direct_bf16, add = weights ? c2.add : c.add;
                 const CUtensorMap *mo = second ? &c2.o : &c.o;
                 const int y0 = t.m0 + quarter * 32 + (weights ? c.cls0 : 0), end = weights ? (int)c.classes : c.row_cap;
-#pragma unroll 1
+#pragma unroll(kCross ? 4 : 1)
                 for (int j = 0; j < 4; ++j) {
                     const int k0 = t.n0 + half * 128 + 32 * j;
                     if (k0 >= u.n) break;
@@ -500,7 +549,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                         tmem_load32(d + kPN + 32 * j, x);
                         tmem_load_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] += x[e];
+                        for (int e = 0; e < 32; ++e) v[e] = (v[e] + sum[j][e]) + x[e];
                     }
                     if (!there) {
 #pragma unroll
