@@ -404,11 +404,14 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
             tc_fence_after();
             const uint32_t d = tmem + acc * kPN + half * 128 + ((uint32_t)quarter << 21);
             const bool there = t.count > 0;  // an empty range of the reduction: zeros
-            float v[32];
-            // logits in units of log2, 32 columns at a time
+            float v[32], ahead[32];
+            if (kLogits) tmem_load32(d, ahead);
+            // logits in units of log2, 32 columns at a time; the next ones come while these are worked on
             const auto logits = [&](int j) {
-                tmem_load32(d + 32 * j, v);
                 tmem_load_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = ahead[e];
+                if (j < 3) tmem_load32(d + 32 * (j + 1), ahead);
                 const float4 *b4 = reinterpret_cast<const float4 *>(bias_col + half * 128 + 32 * j);
                 const float4 *s4 = reinterpret_cast<const float4 *>(scale_col + half * 128 + 32 * j);
 #pragma unroll
@@ -433,7 +436,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
             };
             if constexpr (KIND == kLogitStats) {
                 float mx = -INFINITY, sum = 0.f;
-#pragma unroll 1
+#pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     logits(j);
                     float top = mx;
@@ -452,7 +455,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                                       ? (exp2_fast(__ldg(c.picked2 + row) - lse2) - 1.0f) * (PLANES == 2 ? kGradScale : 1.0f)
                                       : 0.f;  // G of the label's class
                 const int x0 = t.n0 + half * 128, y0 = t.m0 + quarter * 32;
-#pragma unroll 1
+#pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     logits(j);
 #pragma unroll
