@@ -1,7 +1,7 @@
 // Negative log-likelihood of a linear classifier over many classes and its gradients (sm_100a), in pieces of the
 // classes, so that the logits z = x W^T + b, [n, C], are never kept:
 //
-//     lse[r] = log sum_c exp z[r, c]        running maximum and sum over the pieces
+//     lse[r] = log sum_c exp z[r, c]        maximum and sum of every 128 classes, joined in a tree
 //     loss   = inv_count sum_r (lse[r] - z[r, label])
 //     G      = inv_count (exp(z - lse) - onehot)  piece by piece, from logits computed a second time
 //     gx += G W_piece,  gw_piece = G^T x,  gb_piece = sum_r G
@@ -637,17 +637,17 @@ static int nll_product_blocks(const ProductCall &c, const ProductCall &c2, int64
 // their exponentials (779 against 789 us), and few rows are better spread over more blocks (300 x 30000 x 256 bf16, all of it: 104
 // against 130 us).
 template <int KIND, int PLANES>
-static bool nll_in_pairs(int64_t row_cap)
-{
-    return row_cap > 1024 && (PLANES == 2 || (KIND != kLogitStats && KIND != kLogitGrad));
-}
+constexpr bool kNllPairs = PLANES == 2 || (KIND != kLogitStats && KIND != kLogitGrad);
+static bool nll_in_pairs(int64_t row_cap) { return row_cap > 1024; }
 
 // Results of `rows` rows at most and `tiles` beside each other (gradients: and of `rows2` and `tiles2`; splits count as tiles)
 template <int KIND, int PLANES>
 static int nll_product(const ProductCall &c, const ProductCall &c2, int64_t rows, int64_t tiles, int64_t rows2, int64_t tiles2, cudaStream_t s)
 {
-    if (nll_in_pairs<KIND, PLANES>(c.row_cap))
-        return nll_product_blocks<KIND, PLANES, 2>(c, c2, ceil_div(rows, 2 * kPM) * tiles + ceil_div(rows2, 2 * kPM) * tiles2, s);
+    if constexpr (kNllPairs<KIND, PLANES>) {
+        if (nll_in_pairs(c.row_cap))
+            return nll_product_blocks<KIND, PLANES, 2>(c, c2, ceil_div(rows, 2 * kPM) * tiles + ceil_div(rows2, 2 * kPM) * tiles2, s);
+    }
     return nll_product_blocks<KIND, PLANES, 1>(c, c2, ceil_div(rows, kPM) * tiles + ceil_div(rows2, kPM) * tiles2, s);
 }
 
@@ -697,7 +697,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
     const void *wp = p.copy_w ? (const void *)ws.row.p : c.w;
     const int64_t wld = p.copy_w ? p.ld : c.ldw, wst = p.copy_w ? ws.row.stride : c.C * c.ldw;
     if ((rc = umma_tensor_map(&lc.a, xs.row.p, !f32, c.K, p.padded, p.ld, PLANES, xs.row.stride, kPM))) return rc;
-    const bool pairs = nll_in_pairs<kLogitStats, PLANES>(p.row_cap);  // each of the two reads half of a tile's classes
+    const bool pairs = kNllPairs<kLogitStats, PLANES> && nll_in_pairs(p.row_cap);  // each of the two reads half of a tile's classes
     if ((rc = umma_tensor_map(&lc.b, wp, !f32, c.K, c.C, wld, PLANES, wst, pairs ? kPN / 2 : kPN))) return rc;
     lc.total = ints(p.total), lc.failed = ints(p.failed), lc.feats = (int)c.K, lc.splits = 1, lc.bf16 = !f32;
     lc.bias2 = floats(p.bias2), lc.row_scale = xs.row_down, lc.cls_scale = ws.row_down, lc.classes = c.C;
