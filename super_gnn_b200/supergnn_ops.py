@@ -987,7 +987,8 @@ def softmax_nll_loss(logits, bias, labels, mask, inv_count: float, grad=None):
 # layer norm, 8-bit activation checkpoints, many-class loss
 # ---------------------------------------------------------------------------
 # The smallest of these calls take microseconds on the device, so the wrappers below test first and build messages only
-# for what failed, and ask for the device and its stream the cheap way.
+# for what failed, ask for the device and its stream the cheap way, and give torch.empty its sizes one by one (1.6 us; 2.3 us
+# as a tuple).
 _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # torch.cuda.current_stream without the object
 
@@ -1055,8 +1056,8 @@ def _vector(t, name, dtype, width, dev) -> int:
 def _new_codes(n, width, device):
     """Codes and parameters of an 8-bit checkpoint; the rows are padded to 16 bytes."""
     pitch = -(-width // 16) * 16
-    codes = torch.empty((n, pitch), dtype=torch.uint8, device=device)
-    return (codes if pitch == width else codes[:, :width]), torch.empty((n, 2), dtype=torch.float32, device=device)
+    codes = torch.empty(n, pitch, dtype=torch.uint8, device=device)
+    return (codes if pitch == width else codes[:, :width]), torch.empty(n, 2, dtype=torch.float32, device=device)
 
 
 def _pairs(t, name, n, dev):
@@ -1101,10 +1102,10 @@ def layer_norm_forward(x, gamma=None, beta=None, eps: float = 1e-5, checkpoint: 
         raise RuntimeError("gamma and beta must have one type")
     x = _row_major(x)
     if out is None:
-        out = torch.empty_like(x) if x.is_contiguous() else torch.empty((n, H), dtype=dtype, device=dev)
+        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(n, H, dtype=dtype, device=dev)
     else:
         _result(out, "out", n, H, dtype, dev)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=dev)
+    stats = torch.empty(n, 2, dtype=torch.float32, device=dev)
     codes, params = _new_codes(n, H, dev) if checkpoint else (None, None)
     with _on(dev), _Logged("layer_norm_fwd", dev, n=n, H=H):
         rc = _cabi.lib().sgnn_layer_norm_forward(code, x.data_ptr(), x.stride(0), pcode, _ptr(gamma), _ptr(beta), eps,
@@ -1126,7 +1127,7 @@ def _layer_norm_backward(gy, x, codes, params, stats, gamma, in_place):
     rows = _row_major(gy)
     _need(not in_place or rows is gy, "in_place needs gy with contiguous rows")
     gy = rows
-    gx = gy if in_place else torch.empty_like(gy) if gy.is_contiguous() else torch.empty((n, H), dtype=dtype, device=dev)
+    gx = gy if in_place else torch.empty_like(gy) if gy.is_contiguous() else torch.empty(n, H, dtype=dtype, device=dev)
     g_gamma = torch.empty(H, dtype=torch.float32, device=dev) if gamma is None else torch.empty_like(gamma)
     g_beta = torch.empty_like(g_gamma)
     lib = _cabi.lib()
@@ -1184,7 +1185,7 @@ def checkpoint_unpack_rows(codes, params, dtype=torch.float32):
         raise RuntimeError(f"dtype must be one of {', '.join(str(a) for a in _ELEMENT)}, got {dtype}")
     n, F = codes.shape
     dev = codes.device
-    out = torch.empty((n, F), dtype=dtype, device=dev)
+    out = torch.empty(n, F, dtype=dtype, device=dev)
     with _on(dev), _Logged("checkpoint_unpack", dev, n=n, F=F):
         rc = _cabi.lib().sgnn_checkpoint_unpack_rows(codes.data_ptr(), codes.stride(0), params.data_ptr(), code,
                                                      out.data_ptr(), out.stride(0), n, F, _stream_on(dev))
@@ -1205,7 +1206,7 @@ def checkpoint_weight_grad(g, codes, params, out=None, beta: float = 0.0):
         _need(False, "all tensors must be on the same CUDA device")
     if out is None:
         _need(beta == 0.0, "checkpoint_weight_grad: beta needs an existing out")
-        out = torch.empty((M, F), dtype=torch.float32, device=dev)
+        out = torch.empty(M, F, dtype=torch.float32, device=dev)
     else:
         _result(out, "out", M, F, torch.float32, dev)
     g = _row_major(g)
@@ -1247,8 +1248,8 @@ def _linear_nll(x, weight, bias, labels, mask, inv_count, with_grad: bool):
     loss = torch.empty(1, dtype=torch.float32, device=dev)
     lse = gx = gw = gb = None
     if with_grad:
-        gx = torch.empty((n, K), dtype=dtype, device=dev)
-        gw = torch.empty((C, K), dtype=dtype, device=dev)
+        gx = torch.empty(n, K, dtype=dtype, device=dev)
+        gw = torch.empty(C, K, dtype=dtype, device=dev)
         gb = torch.empty(C, dtype=bias.dtype, device=dev) if bias is not None else None
     else:
         lse = torch.empty(n, dtype=torch.float32, device=dev)
@@ -1282,7 +1283,7 @@ def linear_nll_loss_grad(x, weight, bias, labels, mask, inv_count: float):
 
 def dropout_mask(seed: int, p: float, n: int, H: int, device) -> torch.Tensor:
     """The scaled keep mask the counter-based dropout applies for ``(seed, p)``."""
-    out = torch.empty((n, H), dtype=torch.float32, device=device)
+    out = torch.empty(n, H, dtype=torch.float32, device=device)
     with torch.cuda.device(out.device):
         rc = _cabi.lib().sgnn_dropout_mask(int(seed), float(p), n, H, _ptr(out), _stream(out))
     _cabi.check(rc, "dropout_mask")
