@@ -5,7 +5,7 @@
 //
 // The first sum runs on the tensor cores: a code is exact in bf16, and g sc, rounded once, is carried as three bf16 terms, its
 // 24 bits, so a tile takes three products where two fp32 operands would take six.  (Two terms, 2^-17 of a value off, took 570 us
-// instead of 625 for 600k rows of 512 and 256 columns, and left the result 2.6e-6 off instead of 0.7e-6.)  The second sum does
+// instead of 625 for 600k rows of 512 and 256 columns with the pack, and left the result 2.6e-6 off instead of 0.7e-6.)  The second sum does
 // not depend on k: a few fp32 multiply-adds beside the conversion of g.  The activations are never restored in memory: one byte
 // an element is read.
 //
@@ -25,7 +25,7 @@ namespace sgnn {
 constexpr int kGM = 128, kGN = 256, kGRows = 32;  // results of a block, rows a step
 constexpr int kGKeepers = 8;                      // warps that hold the sums
 constexpr int kGWorkers = 16;                     // warps that convert
-constexpr int kGOwn = kGRows * 4 / kGWorkers;       // rows of g a converting thread has in a step
+constexpr int kGOwn = kGRows * 4 / kGWorkers;     // rows of g a converting thread works on at a time
 constexpr int kGThreads = (kGKeepers + kGWorkers + 4) * 32;  // and a group of four: one feeds, one issues the products
 constexpr int kGRaw = 5, kGStages = 4;            // buffers of operands as they come, and converted
 constexpr int kGPromote = 8;                      // steps between two moves into registers
@@ -50,12 +50,16 @@ struct GradCall {
 
 // What TMA brings: neither g nor the codes (and parameters), the codes, both.  The threads load the rest themselves.
 enum GradFeed { kFeedNone, kFeedCodes, kFeedBoth };
+// Where TMA brings everything, two groups of eight converting warps take every other step each, twice the work at once: what a
+// step waits for (barriers, tensor memory, the fence) then counts half (600k rows of 512 and 256 columns: 620 -> 600 us with the pack).
+template <int FEED>
+constexpr int kGGroups = FEED == kFeedBoth ? 2 : 1;
 template <class T, int FEED>
 constexpr int grad_raw_bytes() { return FEED == kFeedNone ? 0 : kGRows * ((FEED == kFeedBoth ? kGM * (int)sizeof(T) : 0) + kGN + 8); }
 template <class T, int FEED>
 constexpr int grad_raw_area()
 {
-    const int ring = kGRaw * grad_raw_bytes<T, FEED>(), share = 4 * kGM * 4;  // the shares of the zero points go there last
+    const int ring = kGRaw * grad_raw_bytes<T, FEED>(), share = 8 * kGM * 4;  // the shares of the zero points go there last
     return ring > share ? ring : share;
 }
 template <class T, int FEED>
@@ -102,6 +106,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *raw = base + kGStages * kGStageBytes;
     constexpr int kRawBytes = grad_raw_bytes<T, FEED>(), kRawArea = grad_raw_area<T, FEED>();
+    constexpr int kGroups = kGGroups<FEED>, kOwnWarps = kGWorkers / kGroups;
     constexpr int kRawG = FEED == kFeedBoth ? kGRows * kGM * (int)sizeof(T) : 0;  // g first, then the codes, then the parameters
     uint64_t *raw_full = reinterpret_cast<uint64_t *>(raw + kRawArea), *raw_empty = raw_full + kGRaw;
     uint64_t *full = raw_empty + kGRaw, *empty = full + kGStages, *acc_full = empty + kGStages, *acc_empty = acc_full + 1;
@@ -120,8 +125,8 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     const int rounds = (count + kGPromote - 1) / kGPromote;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kGRaw; ++s) bar_init(raw_full + s, 1), bar_init(raw_empty + s, kGWorkers);
-        for (int s = 0; s < kGStages; ++s) bar_init(full + s, kGWorkers), bar_init(empty + s, 1);
+        for (int s = 0; s < kGRaw; ++s) bar_init(raw_full + s, 1), bar_init(raw_empty + s, kOwnWarps);
+        for (int s = 0; s < kGStages; ++s) bar_init(full + s, kOwnWarps), bar_init(empty + s, 1);
         bar_init(acc_full, 1), bar_init(acc_empty, kGKeepers);
         bar_init(drained, 1);
         *gone = 0;
@@ -223,7 +228,9 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
         asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
         const float *share = reinterpret_cast<const float *>(raw);
         const int m = quarter * 32 + lane;
-        const float own = (share[m] + share[kGM + m]) + (share[2 * kGM + m] + share[3 * kGM + m]);
+        float own = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) own += share[e * kGM + m] + share[(4 + e) * kGM + m];
         if (m0 + m < c.M) {
             float *o = c.partials + ((int64_t)split * c.M + m0 + m) * c.ld + n0 + half * 128;
 #pragma unroll
@@ -235,16 +242,17 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     } else {
         // ---- conversion ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        const int w = warp - kGKeepers;
-        const int quarter = w & 3, first_row = (w >> 2) * kGOwn;  // of g: one column, kGOwn rows
-        const int m = quarter * 32 + lane, nq = n0 + lane * 8;  // of the codes: eight columns, rows w, w + kGWorkers, ...
+        const int w = warp - kGKeepers, group = w / kOwnWarps, own = w % kOwnWarps;
+        const int quarter = w & 3, first_row = (own >> 2) * kGOwn * kGroups;  // of g: one column, kGOwn rows, kGroups times
+        const int m = quarter * 32 + lane, nq = n0 + lane * 8;  // of the codes: eight columns, rows own, own + kOwnWarps, ...
         const uint32_t terms = tmem + kGTerms + (first_row >> 1) + ((uint32_t)quarter << 21);
-        float zero = 0.f;  // sum of g zp over this thread's rows
-        int s = 0, t = 0;
+        // sums of g zp: over even and odd steps and over every eight rows of them, whoever has them, for one result whatever FEED is
+        float zero[2] = {0.f, 0.f};
+        int s = group, t = group;
         unsigned phase = 0, raw_phase = 0;
         // operands of a step that come without TMA, one step ahead
         float gv[kGOwn];
-        uint2 cv[kGRows / kGWorkers];
+        uint2 cv[kGRows / kOwnWarps];
         const auto fetch = [&](int k) {
             const int64_t r0 = (int64_t)(first + k) * kGRows;
             if constexpr (FEED != kFeedBoth) {
@@ -256,8 +264,8 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             }
             if constexpr (FEED == kFeedNone) {
 #pragma unroll
-                for (int i = 0; i < kGRows / kGWorkers; ++i) {
-                    const int64_t r = r0 + w + kGWorkers * i;
+                for (int i = 0; i < kGRows / kOwnWarps; ++i) {
+                    const int64_t r = r0 + own + kOwnWarps * i;
                     uint8_t b[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) b[e] = r < c.n && nq + e < c.F ? c.code_ptr[r * c.ldc + nq + e] : (uint8_t)0;
@@ -268,62 +276,69 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
         };
         fetch(0);
 #pragma unroll 1
-        for (int k = 0; k < count; ++k) {
+        for (int k = group; k < count; k += kGroups) {
             const uint8_t *in = raw + s * kRawBytes;
             if (FEED != kFeedNone && !bar_wait(raw_full + s, raw_phase, gone)) break;
             if (!bar_wait(empty + t, phase ^ 1, gone)) break;
             uint8_t *at = base + t * kGStageBytes;
-            uint32_t term[3][kGOwn / 2];
-            float share = 0.f;
 #pragma unroll
-            for (int i = 0; i < kGOwn / 2; ++i) {
-                const int r = first_row + 2 * i;
-                float v0, v1;
-                float4 par;  // (zp, sc) of both rows
-                if constexpr (FEED == kFeedBoth) {
-                    const T *g = reinterpret_cast<const T *>(in) + r * kGM + m;
-                    v0 = to_f32<T>(g[0]), v1 = to_f32<T>(g[kGM]);
-                } else {
-                    v0 = gv[2 * i], v1 = gv[2 * i + 1];
-                }
-                if constexpr (FEED == kFeedNone) {
-                    const int64_t row = (int64_t)(first + k) * kGRows + r;
-                    const float2 p0 = row < c.n ? __ldg(c.params + row) : make_float2(0.f, 0.f);
-                    const float2 p1 = row + 1 < c.n ? __ldg(c.params + row + 1) : make_float2(0.f, 0.f);
-                    par = make_float4(p0.x, p0.y, p1.x, p1.y);
-                } else {
-                    par = *reinterpret_cast<const float4 *>(in + kRawG + kGRows * kGN + r * 8);
-                }
-                share = __fmaf_rn(v0, par.x, share);
-                share = __fmaf_rn(v1, par.z, share);
-                unsigned long long left = mul2(pk2(v0, v1), pk2(par.y, par.w));
+            for (int p = 0; p < kGroups; ++p) {
+                float share = 0.f;
+                uint32_t term[3][kGOwn / 2];
 #pragma unroll
-                for (int e = 0; e < 3; ++e) term[e][i] = next_term(left);
+                for (int i = 0; i < kGOwn / 2; ++i) {
+                    const int r = first_row + p * kGOwn + 2 * i;
+                    float v0, v1;
+                    float4 par;  // (zp, sc) of both rows
+                    if constexpr (FEED == kFeedBoth) {
+                        const T *g = reinterpret_cast<const T *>(in) + r * kGM + m;
+                        v0 = to_f32<T>(g[0]), v1 = to_f32<T>(g[kGM]);
+                    } else {
+                        v0 = gv[2 * i], v1 = gv[2 * i + 1];
+                    }
+                    if constexpr (FEED == kFeedNone) {
+                        const int64_t row = (int64_t)(first + k) * kGRows + r;
+                        const float2 p0 = row < c.n ? __ldg(c.params + row) : make_float2(0.f, 0.f);
+                        const float2 p1 = row + 1 < c.n ? __ldg(c.params + row + 1) : make_float2(0.f, 0.f);
+                        par = make_float4(p0.x, p0.y, p1.x, p1.y);
+                    } else {
+                        par = *reinterpret_cast<const float4 *>(in + kRawG + kGRows * kGN + r * 8);
+                    }
+                    share = __fmaf_rn(v0, par.x, share);
+                    share = __fmaf_rn(v1, par.z, share);
+                    unsigned long long left = mul2(pk2(v0, v1), pk2(par.y, par.w));
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) term[e][i] = next_term(left);
+                }
+#pragma unroll
+                for (int e = 0; e < 3; ++e) tmem_store4(terms + t * kGTermColumns + 16 * e + p * (kGOwn / 2), term[e]);
+                zero[kGroups == 2 ? p : k & 1] += share;
             }
-            zero += share;
 #pragma unroll
-            for (int e = 0; e < 3; ++e) tmem_store4(terms + t * kGTermColumns + 16 * e, term[e]);
-#pragma unroll
-            for (int i = 0; i < kGRows / kGWorkers; ++i) {
-                const int r = w + kGWorkers * i;
+            for (int i = 0; i < kGRows / kOwnWarps; ++i) {
+                const int r = own + kOwnWarps * i;
                 const uint2 code = FEED == kFeedNone ? cv[i] : *reinterpret_cast<const uint2 *>(in + kRawG + r * kGN + lane * 8);
                 *reinterpret_cast<uint4 *>(at + (lane >> 3) * (kGRows * 128) + r * 128 + ((lane & 7) ^ (r & 7)) * 16) = code_values(code);
             }
             tmem_store_wait();
             tc_fence_before();
-            if (FEED != kFeedBoth && k + 1 < count) fetch(k + 1);
+            if (FEED != kFeedBoth && k + kGroups < count) fetch(k + kGroups);
             async_fence();
             __syncwarp();
             if (lane == 0) {
                 bar_arrive(full + t);
                 if (FEED != kFeedNone) bar_arrive(raw_empty + s);
             }
-            if (++t == kGStages) t = 0, phase ^= 1;
-            if (++s == kGRaw) s = 0, raw_phase ^= 1;
+            if ((t += kGroups) >= kGStages) t -= kGStages, phase ^= 1;
+            if ((s += kGroups) >= kGRaw) s -= kGRaw, raw_phase ^= 1;
         }
-        // the zero points' share of every column, [4][128]: every buffer of operands as they come has been read by then
+        // the zero points' shares of every column, [2][4][128]: every buffer of operands as they come has been read by then
         asm volatile("bar.sync 2, %0;" ::"n"(kGWorkers * 32) : "memory");
-        reinterpret_cast<float *>(raw)[(w >> 2) * kGM + m] = zero;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int place = kGroups == 2 ? group * 4 + (own >> 2) * 2 + p : p * 4 + (own >> 2);
+            reinterpret_cast<float *>(raw)[place * kGM + m] = zero[p];
+        }
         asm volatile("bar.sync 1, %0;" ::"n"((kGKeepers + kGWorkers) * 32) : "memory");
     }
     tc_fence_before();
