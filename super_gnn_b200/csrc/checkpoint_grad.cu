@@ -48,14 +48,19 @@ struct GradCall {
     int *failed;
 };
 
-// What TMA brings: neither g nor the codes (and parameters), the codes, both.  The threads load the rest themselves.
-enum GradFeed { kFeedNone, kFeedCodes, kFeedBoth };
-// Where TMA brings everything, two groups of eight converting warps take every other step each, twice the work at once: what a
+// What TMA brings: neither g nor the codes (and parameters), the codes, both; the threads load the rest themselves.  Rows of g
+// that follow each other without a gap, whatever their width, come as one run of bytes a step: 32 rows always begin at a
+// multiple of 16 bytes (the rows of a last step that is not whole, the threads load).
+enum GradFeed { kFeedNone, kFeedCodes, kFeedRows, kFeedBoth };
+constexpr int kGRowBytes = 512;  // the longest such row
+// Where everything is brought, two groups of eight converting warps take every other step each, twice the work at once: what a
 // step waits for (barriers, tensor memory, the fence) then counts half (600k rows of 512 and 256 columns: 620 -> 600 us with the pack).
 template <int FEED>
-constexpr int kGGroups = FEED == kFeedBoth ? 2 : 1;
+constexpr int kGGroups = FEED >= kFeedRows ? 2 : 1;
 template <class T, int FEED>
-constexpr int grad_raw_bytes() { return FEED == kFeedNone ? 0 : kGRows * ((FEED == kFeedBoth ? kGM * (int)sizeof(T) : 0) + kGN + 8); }
+constexpr int grad_raw_g() { return FEED == kFeedBoth ? kGRows * kGM * (int)sizeof(T) : FEED == kFeedRows ? kGRows * kGRowBytes : 0; }
+template <class T, int FEED>
+constexpr int grad_raw_bytes() { return FEED == kFeedNone ? 0 : grad_raw_g<T, FEED>() + kGRows * (kGN + 8); }
 template <class T, int FEED>
 constexpr int grad_raw_area()
 {
@@ -107,7 +112,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
     uint8_t *raw = base + kGStages * kGStageBytes;
     constexpr int kRawBytes = grad_raw_bytes<T, FEED>(), kRawArea = grad_raw_area<T, FEED>();
     constexpr int kGroups = kGGroups<FEED>, kOwnWarps = kGWorkers / kGroups;
-    constexpr int kRawG = FEED == kFeedBoth ? kGRows * kGM * (int)sizeof(T) : 0;  // g first, then the codes, then the parameters
+    constexpr int kRawG = grad_raw_g<T, FEED>();  // g first, then the codes, then the parameters
     uint64_t *raw_full = reinterpret_cast<uint64_t *>(raw + kRawArea), *raw_empty = raw_full + kGRaw;
     uint64_t *full = raw_empty + kGRaw, *empty = full + kGStages, *acc_full = empty + kGStages, *acc_empty = acc_full + 1;
     uint64_t *drained = acc_empty + 1;
@@ -154,7 +159,9 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                     if (!bar_wait(raw_empty + s, phase ^ 1, gone)) break;
                     uint8_t *at = raw + s * kRawBytes;
                     const int r0 = (first + done) * kGRows;
-                    bar_expect(raw_full + s, kRawBytes);
+                    const unsigned g_bytes = FEED == kFeedRows && r0 + kGRows <= c.n ? kGRows * c.M * (unsigned)sizeof(T) : 0u;
+                    bar_expect(raw_full + s, FEED == kFeedRows ? kRawBytes - kRawG + g_bytes : kRawBytes);
+                    if (g_bytes) bulk_load(at, static_cast<const T *>(c.g_ptr) + (int64_t)r0 * c.M, g_bytes, raw_full + s);
                     if (FEED == kFeedBoth) tma_load(at, &c.g, m0, r0, 0, raw_full + s);
                     tma_load(at + kRawG, &c.codes, n0, r0, 0, raw_full + s);
                     tma_load(at + kRawG + kGRows * kGN, &c.zs, 2 * r0, 0, 0, raw_full + s);
@@ -245,6 +252,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
         const int w = warp - kGKeepers, group = w / kOwnWarps, own = w % kOwnWarps;
         const int quarter = w & 3, first_row = (own >> 2) * kGOwn * kGroups;  // of g: one column, kGOwn rows, kGroups times
         const int m = quarter * 32 + lane, nq = n0 + lane * 8;  // of the codes: eight columns, rows own, own + kOwnWarps, ...
+        const int column = m0 + m < c.M ? m0 + m : 0;  // kFeedRows: lanes beyond the last column work for nothing
         const uint32_t terms = tmem + kGTerms + (first_row >> 1) + ((uint32_t)quarter << 21);
         // sums of g zp: over even and odd steps and over every eight rows of them, whoever has them, for one result whatever FEED is
         float zero[2] = {0.f, 0.f};
@@ -255,7 +263,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
         uint2 cv[kGRows / kOwnWarps];
         const auto fetch = [&](int k) {
             const int64_t r0 = (int64_t)(first + k) * kGRows;
-            if constexpr (FEED != kFeedBoth) {
+            if constexpr (FEED < kFeedRows) {
 #pragma unroll
                 for (int i = 0; i < kGOwn; ++i) {
                     const int64_t r = r0 + first_row + i;
@@ -281,6 +289,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             if (FEED != kFeedNone && !bar_wait(raw_full + s, raw_phase, gone)) break;
             if (!bar_wait(empty + t, phase ^ 1, gone)) break;
             uint8_t *at = base + t * kGStageBytes;
+            const bool whole = (int64_t)(first + k + 1) * kGRows <= c.n;
 #pragma unroll
             for (int p = 0; p < kGroups; ++p) {
                 float share = 0.f;
@@ -293,6 +302,15 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                     if constexpr (FEED == kFeedBoth) {
                         const T *g = reinterpret_cast<const T *>(in) + r * kGM + m;
                         v0 = to_f32<T>(g[0]), v1 = to_f32<T>(g[kGM]);
+                    } else if constexpr (FEED == kFeedRows) {
+                        if (whole) {
+                            const T *g = reinterpret_cast<const T *>(in) + r * c.M + column;
+                            v0 = to_f32<T>(g[0]), v1 = to_f32<T>(g[c.M]);
+                        } else {
+                            const int64_t row = (int64_t)(first + k) * kGRows + r;
+                            const T *g = static_cast<const T *>(c.g_ptr) + row * c.M + column;
+                            v0 = row < c.n ? to_f32<T>(g[0]) : 0.f, v1 = row + 1 < c.n ? to_f32<T>(g[c.M]) : 0.f;
+                        }
                     } else {
                         v0 = gv[2 * i], v1 = gv[2 * i + 1];
                     }
@@ -322,7 +340,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             }
             tmem_store_wait();
             tc_fence_before();
-            if (FEED != kFeedBoth && k + kGroups < count) fetch(k + kGroups);
+            if (FEED < kFeedRows && k + kGroups < count) fetch(k + kGroups);
             async_fence();
             __syncwarp();
             if (lane == 0) {
@@ -430,6 +448,8 @@ static int weight_grad_run(const void *g, int64_t ldg, const uint8_t *codes, int
     if (g_fed) {
         if ((rc = raw_tensor_map(&c.g, g, sizeof(T), M, n, ldg, kGM, kGRows))) return rc;
         rc = weight_grad_launch<T, kFeedBoth>(c, p, s);
+    } else if (codes_fed && aligned16(g) && ldg == M && M * (int)sizeof(T) <= kGRowBytes) {
+        rc = weight_grad_launch<T, kFeedRows>(c, p, s);
     } else if (codes_fed) {
         rc = weight_grad_launch<T, kFeedCodes>(c, p, s);
     } else {
