@@ -5,7 +5,7 @@
 //
 // The quantiser is the boundary exchange's (8 bits, min-max a row), for rows of any width, strided, in fp32, bf16 or
 // fp16.  See row_io.cuh for rows without a range and for NaN and infinities.  Both kernels are bound by memory: the row
-// is read once (rows of up to 1024 elements stay in a warp's registers, longer ones are read a second time from
+// is read once (rows of up to 1024 elements stay in a warp's registers, several narrow ones at a time, longer ones are read a second time from
 // L1 / L2 by the block that owns them).
 #include "row_io.cuh"
 
@@ -14,35 +14,38 @@ namespace sgnn {
 constexpr int kCkptThreads = 256;
 constexpr int kCkptWarps = kCkptThreads / 32;
 
-template <class T, int E, int NV>
+template <class T, int E, int NV, int LANES>
 __global__ void __launch_bounds__(kCkptThreads)
 checkpoint_pack_warp_kernel(const T *__restrict__ x, int64_t ldx, uint8_t *__restrict__ codes, int64_t ldc,
                             float2 *__restrict__ params, int64_t n, int F)
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t step = (int64_t)gridDim.x * kCkptWarps;
-    for (int64_t r = (int64_t)blockIdx.x * kCkptWarps + (threadIdx.x >> 5); r < n; r += step) {
+    constexpr int kRows = 32 / LANES;  // of a warp at a time
+    const int lane = threadIdx.x % LANES, sub = (threadIdx.x & 31) / LANES;
+    const int64_t step = (int64_t)gridDim.x * kCkptWarps * kRows;
+    for (int64_t r0 = ((int64_t)blockIdx.x * kCkptWarps + (threadIdx.x >> 5)) * kRows; r0 < n; r0 += step) {
+        const int64_t r = r0 + sub;
+        const int width = r < n ? F : 0;
         float v[NV][E];
         float mn = INFINITY, mx = -INFINITY, poison = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
-            if (c < F) load_row<T, E>(x + r * ldx + c, v[i]);
+            const int c = (lane + LANES * i) * E;
+            if (c < width) load_row<T, E>(x + r * ldx + c, v[i]);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if ((lane + 32 * i) * E < F) {
+            if ((lane + LANES * i) * E < width) {
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     mn = fminf(mn, v[i][e]), mx = fmaxf(mx, v[i][e]), poison = __fmaf_rn(v[i][e], 0.f, poison);
             }
         }
-        const RowQ q = row_quantiser(redux_min(mn), redux_max(mx), all_sum(poison));
-        if (lane == 0) params[r] = make_float2(q.mn, q.sc);
+        const RowQ q = row_quantiser(row_min<LANES>(mn), row_max<LANES>(mx), row_sum<LANES>(poison));
+        if (lane == 0 && r < n) params[r] = make_float2(q.mn, q.sc);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
-            if (c < F) store_codes<E>(codes + r * ldc + c, v[i], q);
+            const int c = (lane + LANES * i) * E;
+            if (c < width) store_codes<E>(codes + r * ldc + c, v[i], q);
         }
     }
 }
@@ -78,16 +81,17 @@ checkpoint_pack_block_kernel(const T *__restrict__ x, int64_t ldx, uint8_t *__re
     }
 }
 
-template <class T, int E>
+template <class T, int E, int LANES>
 __global__ void __launch_bounds__(kCkptThreads)
 checkpoint_unpack_kernel(const uint8_t *__restrict__ codes, int64_t ldc, const float2 *__restrict__ params,
                          T *__restrict__ out, int64_t ldo, int64_t n, int F)
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t step = (int64_t)gridDim.x * kCkptWarps;
-    for (int64_t r = (int64_t)blockIdx.x * kCkptWarps + (threadIdx.x >> 5); r < n; r += step) {
+    constexpr int kRows = kCkptThreads / LANES;  // of a block at a time
+    const int lane = threadIdx.x % LANES;
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES; r < n; r += step) {
         const float2 p = __ldg(params + r);
-        for (int c = lane * E; c < F; c += 32 * E) {
+        for (int c = lane * E; c < F; c += LANES * E) {
             float v[E];
             load_codes<E>(codes + r * ldc + c, v);
 #pragma unroll
@@ -119,14 +123,14 @@ static int ckpt_grid(K kernel, int64_t n, int rows_per_block, ResidentCache &cac
     return rc;
 }
 
-template <class T, int E, int NV>
+template <class T, int E, int NV, int LANES>
 static int pack_launch(const CkptCall &c)
 {
     static ResidentCache cache;
     int grid = 0, rc;
     if constexpr (NV > 0) {
-        if ((rc = ckpt_grid(checkpoint_pack_warp_kernel<T, E, NV>, c.n, kCkptWarps, cache, &grid))) return rc;
-        checkpoint_pack_warp_kernel<T, E, NV><<<grid, kCkptThreads, 0, c.stream>>>(static_cast<const T *>(c.x), c.ldx,
+        if ((rc = ckpt_grid(checkpoint_pack_warp_kernel<T, E, NV, LANES>, c.n, kCkptThreads / LANES, cache, &grid))) return rc;
+        checkpoint_pack_warp_kernel<T, E, NV, LANES><<<grid, kCkptThreads, 0, c.stream>>>(static_cast<const T *>(c.x), c.ldx,
                                                                                    c.codes, c.ldc, c.params, c.n, c.F);
     } else {
         if ((rc = ckpt_grid(checkpoint_pack_block_kernel<T, E>, c.n, 1, cache, &grid))) return rc;
@@ -140,32 +144,39 @@ static int pack_launch(const CkptCall &c)
 template <class T, int E>
 static int pack_width(const CkptCall &c)
 {
-    const int need = (int)ceil_div(c.F, 32 * E);
+    const int lanes = row_lanes(c.F), need = (int)ceil_div(c.F, 32 * E);
+    if (lanes == 4) return pack_launch<T, E, 8 / E, 4>(c);
+    if (lanes == 8) return pack_launch<T, E, 8 / E, 8>(c);
+    if (lanes == 16) return pack_launch<T, E, 8 / E, 16>(c);
+    if (need <= 8 / E) return pack_launch<T, E, 8 / E, 32>(c);
     if constexpr (E >= 4) {
-        if (need <= 1) return pack_launch<T, E, 1>(c);
-        if (need <= 2) return pack_launch<T, E, 2>(c);
-        if (need <= 4) return pack_launch<T, E, 4>(c);
-        if constexpr (E == 4) {
-            if (need <= 8) return pack_launch<T, E, 8>(c);
-        }
-    } else {
-        if (need <= 8 / E) return pack_launch<T, E, 8 / E>(c);
-        if (need <= 32 / E) return pack_launch<T, E, 32 / E>(c);
+        if (need <= 16 / E) return pack_launch<T, E, 16 / E, 32>(c);
     }
-    return pack_launch<T, E, 0>(c);
+    if (need <= 32 / E) return pack_launch<T, E, 32 / E, 32>(c);
+    return pack_launch<T, E, 0, 32>(c);
 }
 
-template <class T, int E>
+template <class T, int E, int LANES>
 static int unpack_launch(const CkptCall &c)
 {
     static ResidentCache cache;
     int grid = 0;
-    int rc = ckpt_grid(checkpoint_unpack_kernel<T, E>, c.n, kCkptWarps, cache, &grid);
+    int rc = ckpt_grid(checkpoint_unpack_kernel<T, E, LANES>, c.n, kCkptThreads / LANES, cache, &grid);
     if (rc) return rc;
-    checkpoint_unpack_kernel<T, E><<<grid, kCkptThreads, 0, c.stream>>>(c.codes, c.ldc, c.params, static_cast<T *>(c.x),
+    checkpoint_unpack_kernel<T, E, LANES><<<grid, kCkptThreads, 0, c.stream>>>(c.codes, c.ldc, c.params, static_cast<T *>(c.x),
                                                                         c.ldx, c.n, c.F);
     SGNN_LAUNCH_OK("checkpoint_unpack_rows");
     return SGNN_OK;
+}
+
+template <class T, int E>
+static int unpack_width(const CkptCall &c)
+{
+    const int lanes = row_lanes(c.F);
+    if (lanes == 4) return unpack_launch<T, E, 4>(c);
+    if (lanes == 8) return unpack_launch<T, E, 8>(c);
+    if (lanes == 16) return unpack_launch<T, E, 16>(c);
+    return unpack_launch<T, E, 32>(c);
 }
 
 template <class T, bool PACK>
@@ -179,9 +190,9 @@ static int ckpt_step(const CkptCall &c)
         if (e == 2) return pack_width<T, 2>(c);
         return pack_width<T, 1>(c);
     } else {
-        if (e == W) return unpack_launch<T, W>(c);
-        if (e == 2) return unpack_launch<T, 2>(c);
-        return unpack_launch<T, 1>(c);
+        if (e == W) return unpack_width<T, W>(c);
+        if (e == 2) return unpack_width<T, 2>(c);
+        return unpack_width<T, 1>(c);
     }
 }
 

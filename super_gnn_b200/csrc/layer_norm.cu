@@ -10,7 +10,7 @@
 // x: one byte an element kept between the two instead of four.
 //
 // Everything is bound by memory: the forward moves x and y once, the backward gy, x (or its codes) and gx once.  Rows
-// of up to 1024 elements belong to a warp, which holds them in registers between the reductions and the
+// of up to 1024 elements belong to a warp (narrow ones to 4, 8 or 16 of its lanes), which holds them in registers between the reductions and the
 // outputs; longer rows to a block, which reads them again (from L1 / L2) for every step.  All sums are fp32: the variance
 // from the differences to the mean, the column sums per warp, then per block, then over the blocks, in a fixed order.
 #include "row_io.cuh"
@@ -31,38 +31,41 @@ struct NormParam {
 // forward
 // ---------------------------------------------------------------------------
 // CK: also write the 8-bit codes of x and their (zero point, scale)
-template <class T, int E, int NV, bool CK>
+template <class T, int E, int NV, bool CK, int LANES>
 __global__ void __launch_bounds__(kNormThreads)
 norm_fwd_warp_kernel(const T *__restrict__ x, int64_t ldx, NormParam par, float eps, T *__restrict__ y, int64_t ldy,
                      float2 *__restrict__ stats, uint8_t *__restrict__ codes, int64_t ldc, float2 *__restrict__ params,
                      int64_t n, int H)
 {
     constexpr bool kHold = E * NV <= 8;  // gamma and beta in registers; from L1 every row where they would not fit
-    const int lane = threadIdx.x & 31;
+    constexpr int kRows = 32 / LANES;  // of a warp at a time
+    const int lane = threadIdx.x % LANES, sub = (threadIdx.x & 31) / LANES;
     const float invH = 1.0f / (float)H;
     float ga[kHold ? NV : 1][E], be[kHold ? NV : 1][E];
     if constexpr (kHold) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
+            const int c = (lane + LANES * i) * E;
             if (c < H) {
                 load_param<T, E>(par.gamma, par.f32, c, 1.f, ga[i]);
                 load_param<T, E>(par.beta, par.f32, c, 0.f, be[i]);
             }
         }
     }
-    const int64_t step = (int64_t)gridDim.x * kNormWarps;
-    for (int64_t r = (int64_t)blockIdx.x * kNormWarps + (threadIdx.x >> 5); r < n; r += step) {
+    const int64_t step = (int64_t)gridDim.x * kNormWarps * kRows;
+    for (int64_t r0 = ((int64_t)blockIdx.x * kNormWarps + (threadIdx.x >> 5)) * kRows; r0 < n; r0 += step) {
+        const int64_t r = r0 + sub;
+        const int width = r < n ? H : 0;
         float v[NV][E];
         float s = 0.f, mn = INFINITY, mx = -INFINITY, poison = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
-            if (c < H) load_row<T, E>(x + r * ldx + c, v[i]);
+            const int c = (lane + LANES * i) * E;
+            if (c < width) load_row<T, E>(x + r * ldx + c, v[i]);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if ((lane + 32 * i) * E < H) {
+            if ((lane + LANES * i) * E < width) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     s += v[i][e];
@@ -74,11 +77,11 @@ norm_fwd_warp_kernel(const T *__restrict__ x, int64_t ldx, NormParam par, float 
                 }
             }
         }
-        const float mean = all_sum(s) * invH;
+        const float mean = row_sum<LANES>(s) * invH;
         float q = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if ((lane + 32 * i) * E < H) {
+            if ((lane + LANES * i) * E < width) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float d = v[i][e] - mean;
@@ -86,17 +89,17 @@ norm_fwd_warp_kernel(const T *__restrict__ x, int64_t ldx, NormParam par, float 
                 }
             }
         }
-        const float rstd = __frsqrt_rn(all_sum(q) * invH + eps);
-        if (lane == 0) stats[r] = make_float2(mean, rstd);
+        const float rstd = __frsqrt_rn(row_sum<LANES>(q) * invH + eps);
+        if (lane == 0 && r < n) stats[r] = make_float2(mean, rstd);
         RowQ rq;
         if (CK) {
-            rq = row_quantiser(redux_min(mn), redux_max(mx), all_sum(poison));
-            if (lane == 0) params[r] = make_float2(rq.mn, rq.sc);
+            rq = row_quantiser(row_min<LANES>(mn), row_max<LANES>(mx), row_sum<LANES>(poison));
+            if (lane == 0 && r < n) params[r] = make_float2(rq.mn, rq.sc);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
-            if (c < H) {
+            const int c = (lane + LANES * i) * E;
+            if (c < width) {
                 if (CK) store_codes<E>(codes + r * ldc + c, v[i], rq);
                 float g[E], b[E];
                 if constexpr (!kHold) {
@@ -482,20 +485,21 @@ __device__ __forceinline__ void load_source(const NormSource &src, int64_t r, in
 
 // partials: [gridDim.x, 2, H], per-block column sums of (gy xh, gy).  From codes, with a byte an element instead of four to wait
 // for, a fourth block an SM is worth more than registers (600000 x 256 fp32: 270 us against 295; from x 283 against 277).
-template <class T, int E, int NV, bool CK>
+template <class T, int E, int NV, bool CK, int LANES>
 __global__ void __launch_bounds__(kNormThreads, CK && E * NV <= 8 ? 4 : 1)
 norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
                      NormParam par, T *__restrict__ gx, int64_t ldgx, float *__restrict__ partials, int64_t n, int H)
 {
     extern __shared__ float sums[];  // [warps, 2, H]: every lane touches its own columns only until the last step
     constexpr bool kHold = E * NV <= 8;  // the column sums of longer rows live in shared memory
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kRows = 32 / LANES;  // of a warp at a time
+    const int lane = threadIdx.x % LANES, sub = (threadIdx.x & 31) / LANES, warp = threadIdx.x >> 5;
     float *mine = sums + (size_t)warp * 2 * H;
     const float invH = 1.0f / (float)H;
     float ga[kHold ? NV : 1][E], sg[kHold ? NV : 1][E], sb[kHold ? NV : 1][E];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (lane + 32 * i) * E;
+        const int c = (lane + LANES * i) * E;
         if constexpr (kHold) {
             if (c < H) load_param<T, E>(par.gamma, par.f32, c, 1.f, ga[i]);
 #pragma unroll
@@ -505,24 +509,27 @@ norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, cons
             for (int e = 0; e < E; ++e) mine[c + e] = mine[H + c + e] = 0.f;
         }
     }
-    const int64_t step = (int64_t)gridDim.x * kNormWarps;
-    for (int64_t r = (int64_t)blockIdx.x * kNormWarps + warp; r < n; r += step) {
+    const int64_t step = (int64_t)gridDim.x * kNormWarps * kRows;
+    for (int64_t r0 = ((int64_t)blockIdx.x * kNormWarps + warp) * kRows; r0 < n; r0 += step) {
+        const int64_t r = r0 + sub;
+        const int width = r < n ? H : 0;
         float a[NV][E], xh[NV][E];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
-            if (c < H) {
+            const int c = (lane + LANES * i) * E;
+            if (c < width) {
                 load_row<T, E>(gy + r * ldg + c, a[i]);
                 load_source<T, E, CK>(src, r, c, xh[i]);
             }
         }
-        const float2 st = __ldg(stats + r);
-        const NormAffine f = norm_affine<CK>(src, r, st);
+        const int64_t known = r < n ? r : 0;
+        const float2 st = __ldg(stats + known);
+        const NormAffine f = norm_affine<CK>(src, known, st);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
-            if (c < H) {
+            const int c = (lane + LANES * i) * E;
+            if (c < width) {
                 float g[E];
                 if constexpr (!kHold) load_param<T, E>(par.gamma, par.f32, c, 1.f, g);
 #pragma unroll
@@ -541,11 +548,11 @@ norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, cons
                 }
             }
         }
-        const float m1 = all_sum(s1) * invH, m2 = all_sum(s2) * invH;
+        const float m1 = row_sum<LANES>(s1) * invH, m2 = row_sum<LANES>(s2) * invH;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
-            if (c < H) {
+            const int c = (lane + LANES * i) * E;
+            if (c < width) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) a[i][e] = st.y * (a[i][e] - m1 - xh[i][e] * m2);
                 store_row<T, E>(gx + r * ldgx + c, a[i]);
@@ -554,11 +561,21 @@ norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, cons
     }
     if constexpr (kHold) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + 32 * i) * E;
+        for (int i = 0; i < NV; ++i) {  // the rows of a warp together
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+#pragma unroll
+                for (int o = 16; o >= LANES; o >>= 1) {
+                    sg[i][e] += __shfl_xor_sync(FULL, sg[i][e], o);
+                    sb[i][e] += __shfl_xor_sync(FULL, sb[i][e], o);
+                }
+            }
+            const int c = (lane + LANES * i) * E;
             if (c < H) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) mine[c + e] = sg[i][e], mine[H + c + e] = sb[i][e];
+                for (int e = 0; e < E; ++e) {
+                    if (sub == 0) mine[c + e] = sg[i][e], mine[H + c + e] = sb[i][e];
+                }
             }
         }
     }
@@ -683,15 +700,15 @@ static int norm_grid(K kernel, int64_t n, int rows_per_block, size_t smem, size_
     return SGNN_OK;
 }
 
-template <class T, int E, int NV, bool CK>
+template <class T, int E, int NV, bool CK, int LANES>
 static int norm_fwd_launch(const NormCall &c)
 {
     static ResidentCache cache;
     int grid = 0;
     if constexpr (NV > 0) {
-        int rc = norm_grid(norm_fwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, 0, 0, cache, &grid);
+        int rc = norm_grid(norm_fwd_warp_kernel<T, E, NV, CK, LANES>, c.n, kNormThreads / LANES, 0, 0, cache, &grid);
         if (rc) return rc;
-        norm_fwd_warp_kernel<T, E, NV, CK><<<grid, kNormThreads, 0, c.stream>>>(
+        norm_fwd_warp_kernel<T, E, NV, CK, LANES><<<grid, kNormThreads, 0, c.stream>>>(
             static_cast<const T *>(c.x), c.ldx, c.par, c.eps, static_cast<T *>(c.y), c.ldy, c.stats, c.codes, c.ldc,
             c.params, c.n, c.H);
     } else {
@@ -705,18 +722,18 @@ static int norm_fwd_launch(const NormCall &c)
     return SGNN_OK;
 }
 
-template <class T, int E, int NV, bool CK>
+template <class T, int E, int NV, bool CK, int LANES>
 static int norm_bwd_launch(const NormCall &c, int *blocks)
 {
     static ResidentCache cache;
     const NormSource src{c.x, c.ldx, c.codes, c.ldc, c.params};
     if constexpr (NV > 0) {
         // room for the widest row of this kernel, whatever the row: the answer about residency then stays the same
-        constexpr size_t most = (size_t)kNormWarps * 2 * 32 * E * NV * sizeof(float);
+        constexpr size_t most = (size_t)kNormWarps * 2 * LANES * E * NV * sizeof(float);
         const size_t smem = (size_t)kNormWarps * 2 * c.H * sizeof(float);
-        int rc = norm_grid(norm_bwd_warp_kernel<T, E, NV, CK>, c.n, kNormWarps, E * NV <= 8 ? most : smem, most, cache, blocks);
+        int rc = norm_grid(norm_bwd_warp_kernel<T, E, NV, CK, LANES>, c.n, kNormThreads / LANES, E * NV <= 8 ? most : smem, most, cache, blocks);
         if (rc) return rc;
-        norm_bwd_warp_kernel<T, E, NV, CK><<<*blocks, kNormThreads, smem, c.stream>>>(
+        norm_bwd_warp_kernel<T, E, NV, CK, LANES><<<*blocks, kNormThreads, smem, c.stream>>>(
             static_cast<const T *>(c.gy), c.ldg, src, c.stats, c.par, static_cast<T *>(c.gx), c.ldgx, c.partials, c.n,
             c.H);
     } else {
@@ -731,13 +748,14 @@ static int norm_bwd_launch(const NormCall &c, int *blocks)
     return SGNN_OK;
 }
 
-// Staged rows: packed operands on 16-byte boundaries, rows of a warp's length; where narrow accesses were the alternative.
+// Staged rows: packed operands on 16-byte boundaries, rows of a whole warp's length (narrower ones share a warp: 600000 x 99 fp32
+// 399 us staged, 263 so; 300000 x 201 239 us staged, 260 not); where narrow accesses were the alternative.
 // The ring has as many buffers as leave room for two blocks an SM, at least two, at most four.
 static bool norm_can_stage(const NormCall &c, size_t bytes)
 {
     const bool fwd = c.y != nullptr;
     const auto packed = [&](const void *p, int64_t ld) { return ld == c.H && aligned16(p); };
-    return c.n >= kNormWarps && c.H <= 1024 && c.H * bytes >= 128 && packed(c.x, c.ldx) &&
+    return c.n >= kNormWarps && c.H <= 1024 && c.H > 128 && packed(c.x, c.ldx) &&
            (fwd ? packed(c.y, c.ldy) : packed(c.gy, c.ldg) && packed(c.gx, c.ldgx));
 }
 struct NormStage {
@@ -803,22 +821,19 @@ static int norm_bwd_staged(const NormCall &c, int *blocks)
         return fn<T, 1, 32>(c, ##__VA_ARGS__);                                                                          \
     } while (0)
 
-// fn<T, E, NV, CK>(c, ...) with the accesses a lane needs for a row (NV = 0: the block kernel)
+// fn<T, E, NV, CK, LANES>(c, ...) with the lanes of a row and the accesses a lane needs for it (NV = 0: the block kernel)
 #define SGNN_NORM_NV(T, E, fn, ...)                                                                                     \
     do {                                                                                                                \
-        const int need = (int)ceil_div(c.H, 32 * E);                                                                    \
+        const int lanes = row_lanes(c.H), need = (int)ceil_div(c.H, 32 * E);                                            \
+        if (lanes == 4) return fn<T, E, 8 / E, CK, 4>(__VA_ARGS__);                                                     \
+        if (lanes == 8) return fn<T, E, 8 / E, CK, 8>(__VA_ARGS__);                                                     \
+        if (lanes == 16) return fn<T, E, 8 / E, CK, 16>(__VA_ARGS__);                                                   \
+        if (need <= 8 / E) return fn<T, E, 8 / E, CK, 32>(__VA_ARGS__);                                                 \
         if constexpr (E >= 4) {                                                                                         \
-            if (need <= 1) return fn<T, E, 1, CK>(__VA_ARGS__);                                                         \
-            if (need <= 2) return fn<T, E, 2, CK>(__VA_ARGS__);                                                         \
-            if (need <= 4) return fn<T, E, 4, CK>(__VA_ARGS__);                                                         \
-            if constexpr (E == 4) {                                                                                     \
-                if (need <= 8) return fn<T, E, 8, CK>(__VA_ARGS__);                                                     \
-            }                                                                                                           \
-        } else {                                                                                                        \
-            if (need <= 8 / E) return fn<T, E, 8 / E, CK>(__VA_ARGS__);                                                 \
-            if (need <= 32 / E) return fn<T, E, 32 / E, CK>(__VA_ARGS__);                                               \
+            if (need <= 16 / E) return fn<T, E, 16 / E, CK, 32>(__VA_ARGS__);                                           \
         }                                                                                                               \
-        return fn<T, E, 0, CK>(__VA_ARGS__);                                                                            \
+        if (need <= 32 / E) return fn<T, E, 32 / E, CK, 32>(__VA_ARGS__);                                               \
+        return fn<T, E, 0, CK, 32>(__VA_ARGS__);                                                                        \
     } while (0)
 
 template <bool CK>

@@ -186,5 +186,41 @@ __device__ __forceinline__ float all_sum(float v)
     return v;
 }
 
+// The same over the LANES lanes that share a row, where a warp has several rows
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v)
+{
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float row_min(float v)
+{
+    if constexpr (LANES == 32) {
+        v = redux_min(v);
+    } else {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(FULL, v, o));
+    }
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float row_max(float v)
+{
+    if constexpr (LANES == 32) {
+        v = redux_max(v);
+    } else {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+    }
+    return v;
+}
+
+// Lanes for a row of H elements, at most eight elements a lane up to 256: narrow rows share a warp.  600000 rows of 16 fp32, layer
+// norm in both directions: 53 us with four lanes a row, 78 with eight, 189 with 32; 64 in bf16 96 us against 298, 128 fp32 246
+// against 275; checkpoint and back, 16 fp32: 28, 45 and 132 us.
+inline int row_lanes(int64_t H) { return H <= 32 ? 4 : H <= 64 ? 8 : H <= 128 ? 16 : 32; }
+
 #endif  // __CUDACC__
 }  // namespace sgnn
