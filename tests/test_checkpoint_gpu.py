@@ -48,6 +48,17 @@ def test_pack_is_bit_exact_and_unpack_is_one_rounding(n, F, dtype):
     assert ((kept - x.cpu().double()).abs() <= step * (0.5 + 2 ** -14) + 4 * U * x.cpu().double().abs()).all()
 
 
+@pytest.mark.parametrize("n,F", [(150_001, 3), (150_006, 32), (90_007, 63), (60_001, 100)])
+def test_narrow_rows_that_share_a_warp(n, F):
+    x = rows(n, F, torch.float32, n)
+    codes, params = ops.checkpoint_pack_rows(x)
+    want_codes, want_params = expected(x)
+    assert torch.equal(params.cpu(), want_params) and torch.equal(codes.cpu(), want_codes)
+    kept = want_params[:, :1].double() + want_params[:, 1:].double() * want_codes.double()
+    off = (ops.checkpoint_unpack_rows(codes, params).cpu().double() - kept).abs()
+    assert (off <= kept.abs() * 2 * U + torch.finfo(torch.float32).smallest_normal * 2 * U).all()  # one fused multiply-add
+
+
 def test_values_next_to_a_border_between_two_codes():
     """Quotients on and next to k + 1/2: the codes are those of the IEEE quotient, to nearest even."""
     base = torch.arange(0, 255, device=DEV, dtype=torch.float32) + 0.5

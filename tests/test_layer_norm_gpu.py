@@ -16,7 +16,7 @@ def half_step(t, dtype):
 
 def depth(H):
     """Additions behind one fp32 row sum: at most H / 32 a lane of a warp (H / 256 a thread of a block), the shuffle
-    tree, the eight warps of a block."""
+    tree, the eight warps of a block; or eight a lane and at most four shuffles where narrow rows share a warp."""
     return H / 32 + 5 + 8
 
 
@@ -106,6 +106,14 @@ def test_forward_and_backward(n, H, dtype, pdtype, checkpoint):
     close(y, ref.y, ref.e_y)
     for g, (want, err) in zip(got, ref.backward(gy)):
         close(g, want, err)
+
+
+@pytest.mark.parametrize("n,H", [(150_001, 2), (150_007, 20), (90_002, 61), (60_003, 64), (60_005, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_narrow_rows_that_share_a_warp(n, H, dtype, checkpoint):
+    """More rows than the resident warps take at once, and a last group that is not whole."""
+    test_forward_and_backward(n, H, dtype, torch.float32, checkpoint)
 
 
 @pytest.mark.parametrize("pad,offset", [(4, 0), (1, 0), (0, 1), (3, 2), (12, 4)])
