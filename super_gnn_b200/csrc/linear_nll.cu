@@ -455,9 +455,10 @@ __device__ __forceinline__ void weights_out(const WeightsOut &a, int block)
 {
     const int lane = threadIdx.x & 31;
     for (int64_t c = (int64_t)block * WARPS + (threadIdx.x >> 5); c < a.C; c += (int64_t)a.blocks * WARPS) {
-#pragma unroll 4
+#pragma unroll 2
         for (int k = lane; k < a.K; k += 32) {
             float v = 0.f, up, down = 1.f;
+#pragma unroll 8
             for (int s = 0; s < a.splits; ++s) v += a.acc[s * a.split + c * a.ld + k];
             if (a.largest != nullptr) plane_scale(__uint_as_float(__ldg(a.largest + k)), up, down);
             static_cast<T *>(a.gw)[c * a.ldgw + k] = from_f32<T>(v * a.scale * down);
@@ -768,7 +769,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
             WeightsOut weights{};
             if (last && q + 1 == p.chunks && !p.direct)
                 weights = WeightsOut{floats(p.acc_w), p.acc_ld, w_split, c.C, c.ldgw, p.weight_splits, (int)c.K, lc.scale, largest, c.gw,
-                                     (int)ceil_div(c.C, 4 * warps)};
+                                     (int)(ceil_div(c.C, warps) < wide ? ceil_div(c.C, warps) : wide)};
             const int grid = rows.blocks_x * rows.blocks_y + bias.blocks + weights.blocks;
             if (grid > 0)
                 SGNN_CUDA_OK(launch_chained(warps == 32 ? nll_out_kernel<T, 32> : nll_out_kernel<T, 8>, dim3((unsigned)grid), warps * 32, 0, s,
