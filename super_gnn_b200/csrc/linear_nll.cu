@@ -395,33 +395,57 @@ struct WeightsOut {
     int blocks;
 };
 
+// One row of a result by a warp, from the partial sums of the splits; four columns a lane at a time, loads of several splits
+// on their way together.
+template <class T>
+__device__ __forceinline__ void sum_splits(const float *acc, int64_t split, int splits, int K, float scale, const unsigned *largest, bool bad, T *out)
+{
+    for (int k0 = threadIdx.x & 31; k0 < K; k0 += 128) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += k0 + 32 * j < K ? acc[s * split + k0 + 32 * j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = k0 + 32 * j;
+            if (k >= K) break;
+            float up, down = 1.f;
+            if (largest != nullptr) plane_scale(__uint_as_float(__ldg(largest + k)), up, down);
+            out[k] = from_f32<T>(bad ? __int_as_float(0x7fffffff) : v[j] * scale * down);
+        }
+    }
+}
+
 template <class T, int WARPS>
 __device__ __forceinline__ void rows_out(const RowsOut &a, int block, float (&red)[WARPS][33])
 {
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, bx = block % a.blocks_x, by = block / a.blocks_x;
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, bx = block % a.blocks_x;
     const bool bad = *a.failed != 0;
     if (bad && block == 0 && threadIdx.x == 0) *a.loss = __int_as_float(0x7fffffff);
     const int left = *a.total - a.row0, count = left < a.row_cap ? left : a.row_cap;
-    for (int i = a.dealt ? bx : bx * WARPS + g; i < count; i += a.dealt ? a.blocks_x : a.blocks_x * WARPS) {
-        T *out = static_cast<T *>(a.gx) + (int64_t)a.rows[a.row0 + i] * a.ldgx;
-        for (int k = (a.dealt ? by * 32 : 0) + lane; k < a.K || a.dealt; k += 32) {
-            float v = 0.f;
-            if (k < a.K) {
+    if (!a.dealt) {
+        for (int i = bx * WARPS + g; i < count; i += a.blocks_x * WARPS)
+            sum_splits<T>(a.acc + (int64_t)i * a.ld, a.split, a.splits, a.K, a.scale, a.largest, bad,
+                          static_cast<T *>(a.gx) + (int64_t)a.rows[a.row0 + i] * a.ldgx);
+        return;
+    }
+    const int k = block / a.blocks_x * 32 + lane;
+    for (int i = bx; i < count; i += a.blocks_x) {
+        float v = 0.f;
+        if (k < a.K) {
 #pragma unroll 4
-                for (int s = a.dealt ? g : 0; s < a.splits; s += a.dealt ? WARPS : 1) v += a.acc[s * a.split + (int64_t)i * a.ld + k];
-            }
-            if (a.dealt) {
-                __syncthreads();
-                red[g][lane] = v;
-                __syncthreads();
-                if (g == 0)
-                    for (int w = 1; w < WARPS; ++w) v += red[w][lane];
-            }
-            float up, down = 1.f;
-            if (a.largest != nullptr && k < a.K) plane_scale(__uint_as_float(a.largest[k]), up, down);
-            if (k < a.K && (!a.dealt || g == 0)) out[k] = from_f32<T>(bad ? __int_as_float(0x7fffffff) : v * a.scale * down);
-            if (a.dealt) break;
+            for (int s = g; s < a.splits; s += WARPS) v += a.acc[s * a.split + (int64_t)i * a.ld + k];
         }
+        __syncthreads();
+        red[g][lane] = v;
+        __syncthreads();
+        if (g != 0 || k >= a.K) continue;
+        for (int w = 1; w < WARPS; ++w) v += red[w][lane];
+        float up, down = 1.f;
+        if (a.largest != nullptr) plane_scale(__uint_as_float(__ldg(a.largest + k)), up, down);
+        static_cast<T *>(a.gx)[(int64_t)a.rows[a.row0 + i] * a.ldgx + k] = from_f32<T>(bad ? __int_as_float(0x7fffffff) : v * a.scale * down);
     }
 }
 
@@ -453,17 +477,8 @@ __device__ __forceinline__ void bias_out(const BiasOut &a, int block, float (&re
 template <class T, int WARPS>
 __device__ __forceinline__ void weights_out(const WeightsOut &a, int block)
 {
-    const int lane = threadIdx.x & 31;
-    for (int64_t c = (int64_t)block * WARPS + (threadIdx.x >> 5); c < a.C; c += (int64_t)a.blocks * WARPS) {
-#pragma unroll 2
-        for (int k = lane; k < a.K; k += 32) {
-            float v = 0.f, up, down = 1.f;
-#pragma unroll 8
-            for (int s = 0; s < a.splits; ++s) v += a.acc[s * a.split + c * a.ld + k];
-            if (a.largest != nullptr) plane_scale(__uint_as_float(__ldg(a.largest + k)), up, down);
-            static_cast<T *>(a.gw)[c * a.ldgw + k] = from_f32<T>(v * a.scale * down);
-        }
-    }
+    for (int64_t c = (int64_t)block * WARPS + (threadIdx.x >> 5); c < a.C; c += (int64_t)a.blocks * WARPS)
+        sum_splits<T>(a.acc + c * a.ld, a.split, a.splits, a.K, a.scale, a.largest, false, static_cast<T *>(a.gw) + c * a.ldgw);
 }
 
 // The first blocks sum up rows, the next ones the bias, the rest weights; none of a kind whose `blocks` are 0.
