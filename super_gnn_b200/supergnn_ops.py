@@ -1021,6 +1021,12 @@ def _workspace_bytes(query: str, device: int, *sizes) -> int:
     return need.value
 
 
+@functools.lru_cache(maxsize=64)
+def _layer_norm_blocks(device: int) -> int:
+    """Rows of partial column sums a layer norm backward may need on this device."""
+    return _cabi.lib().sgnn_layer_norm_blocks()
+
+
 def _matrix(t, name, allowed=_ELEMENT) -> int:
     """Checks a 2-d CUDA tensor with at least one column; its element code."""
     code = allowed.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 else None
@@ -1029,6 +1035,13 @@ def _matrix(t, name, allowed=_ELEMENT) -> int:
         _need(t.dtype in allowed, f"{name} must be one of {', '.join(str(a) for a in allowed)}, got {t.dtype}")
         _need(False, f"{name} must have at least one column")
     return code
+
+
+def _tensor(t, name, dtype, dim, dev) -> None:
+    """Checks a CUDA tensor of ``dtype`` and ``dim`` dimensions on ``dev``."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == dim and t.device == dev):
+        _cuda(t, name, dtype, dim)
+        _need(False, "all tensors must be on the same CUDA device")
 
 
 def _row_major(t):
@@ -1122,7 +1135,7 @@ def _layer_norm_backward(gy, x, codes, params, stats, gamma, in_place):
     dev, dtype = gy.device, gy.dtype
     pcode = _vector(gamma, "gamma", dtype, H, dev)
     _pairs(stats, "stats", n, dev)
-    if (codes if x is None else x).device != dev:
+    if x is None and codes.device != dev:
         raise RuntimeError("all tensors must be on the same CUDA device")
     rows = _row_major(gy)
     _need(not in_place or rows is gy, "in_place needs gy with contiguous rows")
@@ -1132,7 +1145,7 @@ def _layer_norm_backward(gy, x, codes, params, stats, gamma, in_place):
     g_beta = torch.empty_like(g_gamma)
     lib = _cabi.lib()
     with _on(dev), _Logged("layer_norm_bwd", dev, n=n, H=H):
-        partials = torch.empty(lib.sgnn_layer_norm_blocks() * 2 * H, dtype=torch.float32, device=dev)
+        partials = torch.empty(_layer_norm_blocks(dev.index) * 2 * H, dtype=torch.float32, device=dev)
         rc = lib.sgnn_layer_norm_backward(code, gy.data_ptr(), gy.stride(0), _ptr(x), x.stride(0) if x is not None else 0,
                                           _ptr(codes), codes.stride(0) if codes is not None else 0, _ptr(params),
                                           stats.data_ptr(), pcode, _ptr(gamma), gx.data_ptr(), gx.stride(0),
@@ -1147,7 +1160,7 @@ def layer_norm_backward(gy, x, stats, gamma=None, in_place: bool = False):
     """Gradients of :func:`layer_norm_forward` from the same ``x`` and its ``stats``: ``(gx, g_gamma, g_beta)``, the
     last two in gamma's type.  ``in_place``: ``gx`` overwrites ``gy``."""
     _matrix(gy, "gy")
-    _cuda(x, "x", gy.dtype, 2)
+    _tensor(x, "x", gy.dtype, 2, gy.device)
     _need(gy.shape == x.shape, "gy and x must have the same shape")
     return _layer_norm_backward(gy, _row_major(x), None, None, stats, gamma, in_place)
 
@@ -1229,21 +1242,20 @@ def _linear_nll(x, weight, bias, labels, mask, inv_count, with_grad: bool):
     code = _matrix(x, "x", _NLL_ELEMENT)
     n, K = x.shape
     dev, dtype = x.device, x.dtype
-    _cuda(weight, "weight", dtype, 2)
+    _tensor(weight, "weight", dtype, 2, dev)
     C = weight.size(0)
-    if C == 0 or weight.size(1) != K or weight.device != dev:
-        _need(weight.device == dev, "all tensors must be on the same CUDA device")
-        _need(False, f"weight must be [C, {K}] like x")
+    if C == 0 or weight.size(1) != K:
+        raise RuntimeError(f"weight must be [C, {K}] like x")
     bcode = _vector(bias, "bias", dtype, C, dev)
-    _cuda(labels, "labels", torch.int64, 1)
-    if labels.numel() != n or not labels.is_contiguous() or labels.device != dev:
-        _need(labels.device == dev, "all tensors must be on the same CUDA device")
-        _need(False, "labels must be a contiguous int64 [n] tensor")
-    if mask is not None:
+    _tensor(labels, "labels", torch.int64, 1, dev)
+    if labels.numel() != n or not labels.is_contiguous():
+        raise RuntimeError("labels must be a contiguous int64 [n] tensor")
+    if mask is not None and not (isinstance(mask, torch.Tensor) and mask.is_cuda and mask.dim() == 1 and mask.device == dev
+                                 and (mask.dtype == torch.bool or mask.dtype == torch.uint8) and mask.numel() == n
+                                 and mask.is_contiguous()):
         _cuda(mask, "mask", None, 1)
-        if mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != n or not mask.is_contiguous() or mask.device != dev:
-            _need(mask.device == dev, "all tensors must be on the same CUDA device")
-            _need(False, "mask must be a contiguous bool / uint8 [n] tensor")
+        _need(mask.device == dev, "all tensors must be on the same CUDA device")
+        _need(False, "mask must be a contiguous bool / uint8 [n] tensor")
     x, weight = _row_major(x), _row_major(weight)
     loss = torch.empty(1, dtype=torch.float32, device=dev)
     lse = gx = gw = gb = None
