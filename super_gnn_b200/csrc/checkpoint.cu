@@ -153,6 +153,9 @@ static int pack_width(const CkptCall &c)
         if (need <= 16 / E) return pack_launch<T, E, 16 / E, 32>(c);
     }
     if (need <= 32 / E) return pack_launch<T, E, 32 / E, 32>(c);
+    if constexpr (E >= 4) {
+        if (need <= 64 / E) return pack_launch<T, E, 64 / E, 32>(c);
+    }
     return pack_launch<T, E, 0, 32>(c);
 }
 

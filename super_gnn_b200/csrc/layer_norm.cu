@@ -755,7 +755,7 @@ static bool norm_can_stage(const NormCall &c, size_t bytes)
 {
     const bool fwd = c.y != nullptr;
     const auto packed = [&](const void *p, int64_t ld) { return ld == c.H && aligned16(p); };
-    return c.n >= kNormWarps && c.H <= 1024 && c.H > 128 && packed(c.x, c.ldx) &&
+    return c.n >= kNormWarps && c.H <= (fwd ? 2048 : 1024) && c.H > 128 && packed(c.x, c.ldx) &&
            (fwd ? packed(c.y, c.ldy) : packed(c.gy, c.ldg) && packed(c.gx, c.ldgx));
 }
 struct NormStage {
@@ -805,24 +805,26 @@ static int norm_bwd_staged(const NormCall &c, int *blocks)
     return SGNN_OK;
 }
 // 8, 12, 20 or 32 elements a lane, two at a time where 16-bit rows of even length allow it
-#define SGNN_NORM_STAGED(T, fn, ...)                                                                                    \
+#define SGNN_NORM_STAGED(FWD, T, fn, ...)                                                                                    \
     do {                                                                                                                \
         if constexpr (sizeof(T) == 2) {                                                                                 \
             if (c.H % 2 == 0) {                                                                                         \
                 if (c.H <= 256) return fn<T, 2, 4>(c, ##__VA_ARGS__);                                                   \
                 if (c.H <= 384) return fn<T, 2, 6>(c, ##__VA_ARGS__);                                                   \
                 if (c.H <= 640) return fn<T, 2, 10>(c, ##__VA_ARGS__);                                                  \
-                return fn<T, 2, 16>(c, ##__VA_ARGS__);                                                                  \
+                if (c.H <= 1024) return fn<T, 2, 16>(c, ##__VA_ARGS__);                                                 \
+                return fn<T, 2, FWD ? 32 : 16>(c, ##__VA_ARGS__);                                                       \
             }                                                                                                           \
         }                                                                                                               \
         if (c.H <= 256) return fn<T, 1, 8>(c, ##__VA_ARGS__);                                                           \
         if (c.H <= 384) return fn<T, 1, 12>(c, ##__VA_ARGS__);                                                          \
         if (c.H <= 640) return fn<T, 1, 20>(c, ##__VA_ARGS__);                                                          \
-        return fn<T, 1, 32>(c, ##__VA_ARGS__);                                                                          \
+        if (c.H <= 1024) return fn<T, 1, 32>(c, ##__VA_ARGS__);                                                         \
+        return fn<T, 1, FWD ? 64 : 32>(c, ##__VA_ARGS__);                                                               \
     } while (0)
 
 // fn<T, E, NV, CK, LANES>(c, ...) with the lanes of a row and the accesses a lane needs for it (NV = 0: the block kernel)
-#define SGNN_NORM_NV(T, E, fn, ...)                                                                                     \
+#define SGNN_NORM_NV(FWD, T, E, fn, ...)                                                                                     \
     do {                                                                                                                \
         const int lanes = row_lanes(c.H), need = (int)ceil_div(c.H, 32 * E);                                            \
         if (lanes == 4) return fn<T, E, 8 / E, CK, 4>(__VA_ARGS__);                                                     \
@@ -833,6 +835,7 @@ static int norm_bwd_staged(const NormCall &c, int *blocks)
             if (need <= 16 / E) return fn<T, E, 16 / E, CK, 32>(__VA_ARGS__);                                           \
         }                                                                                                               \
         if (need <= 32 / E) return fn<T, E, 32 / E, CK, 32>(__VA_ARGS__);                                               \
+        if (FWD && E >= 4 && need <= 64 / E) return fn<T, E, FWD && E >= 4 ? 64 / E : 0, CK, 32>(__VA_ARGS__);          \
         return fn<T, E, 0, CK, 32>(__VA_ARGS__);                                                                        \
     } while (0)
 
@@ -846,23 +849,23 @@ static int norm_fwd_dispatch(const NormCall &c)
                               {CK ? c.codes : nullptr, c.ldc, 1}};
     const int e = row_step(c.H, wide, ops);
     if (!CK && e != wide && norm_can_stage(c, b)) {
-        if (c.dtype == SGNN_F32) SGNN_NORM_STAGED(float, norm_fwd_staged);
-        if (c.dtype == SGNN_BF16) SGNN_NORM_STAGED(__nv_bfloat16, norm_fwd_staged);
-        SGNN_NORM_STAGED(__half, norm_fwd_staged);
+        if (c.dtype == SGNN_F32) SGNN_NORM_STAGED(true, float, norm_fwd_staged);
+        if (c.dtype == SGNN_BF16) SGNN_NORM_STAGED(true, __nv_bfloat16, norm_fwd_staged);
+        SGNN_NORM_STAGED(true, __half, norm_fwd_staged);
     }
     if (c.dtype == SGNN_F32) {
-        if (e == 4) SGNN_NORM_NV(float, 4, norm_fwd_launch, c);
-        if (e == 2) SGNN_NORM_NV(float, 2, norm_fwd_launch, c);
-        SGNN_NORM_NV(float, 1, norm_fwd_launch, c);
+        if (e == 4) SGNN_NORM_NV(true, float, 4, norm_fwd_launch, c);
+        if (e == 2) SGNN_NORM_NV(true, float, 2, norm_fwd_launch, c);
+        SGNN_NORM_NV(true, float, 1, norm_fwd_launch, c);
     }
     if (c.dtype == SGNN_BF16) {
-        if (e == 8) SGNN_NORM_NV(__nv_bfloat16, 8, norm_fwd_launch, c);
-        if (e == 2) SGNN_NORM_NV(__nv_bfloat16, 2, norm_fwd_launch, c);
-        SGNN_NORM_NV(__nv_bfloat16, 1, norm_fwd_launch, c);
+        if (e == 8) SGNN_NORM_NV(true, __nv_bfloat16, 8, norm_fwd_launch, c);
+        if (e == 2) SGNN_NORM_NV(true, __nv_bfloat16, 2, norm_fwd_launch, c);
+        SGNN_NORM_NV(true, __nv_bfloat16, 1, norm_fwd_launch, c);
     }
-    if (e == 8) SGNN_NORM_NV(__half, 8, norm_fwd_launch, c);
-    if (e == 2) SGNN_NORM_NV(__half, 2, norm_fwd_launch, c);
-    SGNN_NORM_NV(__half, 1, norm_fwd_launch, c);
+    if (e == 8) SGNN_NORM_NV(true, __half, 8, norm_fwd_launch, c);
+    if (e == 2) SGNN_NORM_NV(true, __half, 2, norm_fwd_launch, c);
+    SGNN_NORM_NV(true, __half, 1, norm_fwd_launch, c);
 }
 
 template <bool CK>
@@ -877,23 +880,23 @@ static int norm_bwd_dispatch(const NormCall &c, int *blocks)
     // (600000 x 512 bf16: 464 us against 1254, 300000 x 512 fp32: 298 against 392), but for 32 fp32 elements a lane (150000 x 1024:
     // 607 us against 449).
     if (!CK && norm_can_stage(c, b) && (e != wide || (c.H > 256 && (b == 2 || c.H <= 640)))) {
-        if (c.dtype == SGNN_F32) SGNN_NORM_STAGED(float, norm_bwd_staged, blocks);
-        if (c.dtype == SGNN_BF16) SGNN_NORM_STAGED(__nv_bfloat16, norm_bwd_staged, blocks);
-        SGNN_NORM_STAGED(__half, norm_bwd_staged, blocks);
+        if (c.dtype == SGNN_F32) SGNN_NORM_STAGED(false, float, norm_bwd_staged, blocks);
+        if (c.dtype == SGNN_BF16) SGNN_NORM_STAGED(false, __nv_bfloat16, norm_bwd_staged, blocks);
+        SGNN_NORM_STAGED(false, __half, norm_bwd_staged, blocks);
     }
     if (c.dtype == SGNN_F32) {
-        if (e == 4) SGNN_NORM_NV(float, 4, norm_bwd_launch, c, blocks);
-        if (e == 2) SGNN_NORM_NV(float, 2, norm_bwd_launch, c, blocks);
-        SGNN_NORM_NV(float, 1, norm_bwd_launch, c, blocks);
+        if (e == 4) SGNN_NORM_NV(false, float, 4, norm_bwd_launch, c, blocks);
+        if (e == 2) SGNN_NORM_NV(false, float, 2, norm_bwd_launch, c, blocks);
+        SGNN_NORM_NV(false, float, 1, norm_bwd_launch, c, blocks);
     }
     if (c.dtype == SGNN_BF16) {
-        if (e == 8) SGNN_NORM_NV(__nv_bfloat16, 8, norm_bwd_launch, c, blocks);
-        if (e == 2) SGNN_NORM_NV(__nv_bfloat16, 2, norm_bwd_launch, c, blocks);
-        SGNN_NORM_NV(__nv_bfloat16, 1, norm_bwd_launch, c, blocks);
+        if (e == 8) SGNN_NORM_NV(false, __nv_bfloat16, 8, norm_bwd_launch, c, blocks);
+        if (e == 2) SGNN_NORM_NV(false, __nv_bfloat16, 2, norm_bwd_launch, c, blocks);
+        SGNN_NORM_NV(false, __nv_bfloat16, 1, norm_bwd_launch, c, blocks);
     }
-    if (e == 8) SGNN_NORM_NV(__half, 8, norm_bwd_launch, c, blocks);
-    if (e == 2) SGNN_NORM_NV(__half, 2, norm_bwd_launch, c, blocks);
-    SGNN_NORM_NV(__half, 1, norm_bwd_launch, c, blocks);
+    if (e == 8) SGNN_NORM_NV(false, __half, 8, norm_bwd_launch, c, blocks);
+    if (e == 2) SGNN_NORM_NV(false, __half, 2, norm_bwd_launch, c, blocks);
+    SGNN_NORM_NV(false, __half, 1, norm_bwd_launch, c, blocks);
 }
 #undef SGNN_NORM_NV
 #undef SGNN_NORM_STAGED
