@@ -588,6 +588,82 @@ norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, cons
     }
 }
 
+// Rows of 1025 to 2048 elements by a block: eight columns a thread, whose sums stay in registers; the row is read once, and the
+// blocks of an SM wait for each other's barriers (one a row).
+constexpr int kNormWide = 8 * kNormThreads;
+template <class T, int E, bool CK>
+__global__ void __launch_bounds__(kNormThreads, 3)
+norm_bwd_wide_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
+                     NormParam par, T *__restrict__ gx, int64_t ldgx, float *__restrict__ partials, int64_t n, int H)
+{
+    constexpr int NV = 8 / E;
+    __shared__ float2 red[2][kNormWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float invH = 1.0f / (float)H;
+    float ga[NV][E], sg[NV][E], sb[NV][E];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (threadIdx.x + kNormThreads * i) * E;
+        if (c < H) load_param<T, E>(par.gamma, par.f32, c, 1.f, ga[i]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sg[i][e] = sb[i][e] = 0.f;
+    }
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < n; r += gridDim.x, turn ^= 1) {
+        float a[NV][E], xh[NV][E];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + kNormThreads * i) * E;
+            if (c < H) {
+                load_row<T, E>(gy + r * ldg + c, a[i]);
+                load_source<T, E, CK>(src, r, c, xh[i]);
+            }
+        }
+        const float2 st = __ldg(stats + r);
+        const NormAffine f = norm_affine<CK>(src, r, st);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((threadIdx.x + kNormThreads * i) * E < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    xh[i][e] = norm_hat<CK>(xh[i][e], f);
+                    sg[i][e] += a[i][e] * xh[i][e];
+                    sb[i][e] += a[i][e];
+                    a[i][e] *= ga[i][e];
+                    s1 += a[i][e];
+                    s2 += a[i][e] * xh[i][e];
+                }
+            }
+        }
+        s1 = all_sum(s1), s2 = all_sum(s2);
+        if (lane == 0) red[turn][warp] = make_float2(s1, s2);
+        __syncthreads();  // whoever comes back to this half of red has passed the next row's barrier
+        float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+        for (int w = 0; w < kNormWarps; ++w) m1 += red[turn][w].x, m2 += red[turn][w].y;
+        m1 *= invH, m2 *= invH;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + kNormThreads * i) * E;
+            if (c < H) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) a[i][e] = st.y * (a[i][e] - m1 - xh[i][e] * m2);
+                store_row<T, E>(gx + r * ldgx + c, a[i]);
+            }
+        }
+    }
+    float *out = partials + (size_t)blockIdx.x * 2 * H;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (threadIdx.x + kNormThreads * i) * E;
+        if (c < H) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) out[c + e] = sg[i][e], out[H + c + e] = sb[i][e];
+        }
+    }
+}
+
 template <class T, int E, bool CK>
 __global__ void __launch_bounds__(kNormThreads)
 norm_bwd_block_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
@@ -736,6 +812,12 @@ static int norm_bwd_launch(const NormCall &c, int *blocks)
         norm_bwd_warp_kernel<T, E, NV, CK, LANES><<<*blocks, kNormThreads, smem, c.stream>>>(
             static_cast<const T *>(c.gy), c.ldg, src, c.stats, c.par, static_cast<T *>(c.gx), c.ldgx, c.partials, c.n,
             c.H);
+    } else if constexpr (NV < 0) {
+        int rc = norm_grid(norm_bwd_wide_kernel<T, E, CK>, c.n, 1, 0, 0, cache, blocks);
+        if (rc) return rc;
+        norm_bwd_wide_kernel<T, E, CK><<<*blocks, kNormThreads, 0, c.stream>>>(
+            static_cast<const T *>(c.gy), c.ldg, src, c.stats, c.par, static_cast<T *>(c.gx), c.ldgx, c.partials, c.n,
+            c.H);
     } else {
         const size_t smem = (size_t)2 * c.H * sizeof(float);
         int rc = norm_grid(norm_bwd_block_kernel<T, E, CK>, c.n, 1, smem, 2 * kNormMaxWidth * sizeof(float), cache, blocks);
@@ -823,7 +905,8 @@ static int norm_bwd_staged(const NormCall &c, int *blocks)
         return fn<T, 1, FWD ? 64 : 32>(c, ##__VA_ARGS__);                                                               \
     } while (0)
 
-// fn<T, E, NV, CK, LANES>(c, ...) with the lanes of a row and the accesses a lane needs for it (NV = 0: the block kernel)
+// fn<T, E, NV, CK, LANES>(c, ...) with the lanes of a row and the accesses a lane needs for it (NV = 0: the block kernel, -1:
+// the backward's for rows up to kNormWide)
 #define SGNN_NORM_NV(FWD, T, E, fn, ...)                                                                                     \
     do {                                                                                                                \
         const int lanes = row_lanes(c.H), need = (int)ceil_div(c.H, 32 * E);                                            \
@@ -836,6 +919,7 @@ static int norm_bwd_staged(const NormCall &c, int *blocks)
         }                                                                                                               \
         if (need <= 32 / E) return fn<T, E, 32 / E, CK, 32>(__VA_ARGS__);                                               \
         if (FWD && E >= 4 && need <= 64 / E) return fn<T, E, FWD && E >= 4 ? 64 / E : 0, CK, 32>(__VA_ARGS__);          \
+        if (!FWD && c.H <= kNormWide) return fn<T, E, FWD ? 0 : -1, CK, 32>(__VA_ARGS__);                               \
         return fn<T, E, 0, CK, 32>(__VA_ARGS__);                                                                        \
     } while (0)
 
