@@ -588,9 +588,11 @@ norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, cons
     }
 }
 
-// Rows of 1025 to 2048 elements by a block: eight columns a thread, whose sums stay in registers; the row is read once, and the
-// blocks of an SM wait for each other's barriers (one a row).
-constexpr int kNormWide = 8 * kNormThreads;
+// Rows of up to 2048 elements by a block: eight columns a thread, whose sums stay in registers; the row is read once, with one
+// barrier.  For rows of more than kNormSplit elements, and from codes, unless fp32 rows lie on boundaries, of more than 512
+// (both directions, 100000 rows: 1023 fp32 449 us, 553 through the ring; 1024 fp32 422, 452 by a warp; 800 fp32 379, 370; from
+// codes 1024 bf16 403, 605 by a warp; 576 bf16 365, 433; 640 fp32 347, 296).
+constexpr int kNormWide = 8 * kNormThreads, kNormSplit = 832;
 template <class T, int E, bool CK>
 __global__ void __launch_bounds__(kNormThreads, 3)
 norm_bwd_wide_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
@@ -837,7 +839,7 @@ static bool norm_can_stage(const NormCall &c, size_t bytes)
 {
     const bool fwd = c.y != nullptr;
     const auto packed = [&](const void *p, int64_t ld) { return ld == c.H && aligned16(p); };
-    return c.n >= kNormWarps && c.H <= (fwd ? 2048 : 1024) && c.H > 128 && packed(c.x, c.ldx) &&
+    return c.n >= kNormWarps && c.H <= (fwd ? 2048 : bytes == 4 ? kNormSplit : 1024) && c.H > 128 && packed(c.x, c.ldx) &&
            (fwd ? packed(c.y, c.ldy) : packed(c.gy, c.ldg) && packed(c.gx, c.ldgx));
 }
 struct NormStage {
@@ -917,9 +919,9 @@ static int norm_bwd_staged(const NormCall &c, int *blocks)
         if constexpr (E >= 4) {                                                                                         \
             if (need <= 16 / E) return fn<T, E, 16 / E, CK, 32>(__VA_ARGS__);                                           \
         }                                                                                                               \
+        if (!FWD && c.H > (CK && E != 4 ? 512 : kNormSplit) && c.H <= kNormWide) return fn<T, E, FWD ? 0 : -1, CK, 32>(__VA_ARGS__); \
         if (need <= 32 / E) return fn<T, E, 32 / E, CK, 32>(__VA_ARGS__);                                               \
         if (FWD && E >= 4 && need <= 64 / E) return fn<T, E, FWD && E >= 4 ? 64 / E : 0, CK, 32>(__VA_ARGS__);          \
-        if (!FWD && c.H <= kNormWide) return fn<T, E, FWD ? 0 : -1, CK, 32>(__VA_ARGS__);                               \
         return fn<T, E, 0, CK, 32>(__VA_ARGS__);                                                                        \
     } while (0)
 
