@@ -116,6 +116,13 @@ def test_narrow_rows_that_share_a_warp(n, H, dtype, checkpoint):
     test_forward_and_backward(n, H, dtype, torch.float32, checkpoint)
 
 
+@pytest.mark.parametrize("n,H", [(1501, 544), (1502, 840), (2003, 1026), (1501, 1301), (1999, 2048)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_long_rows_several_a_block(n, H, dtype, checkpoint):
+    test_forward_and_backward(n, H, dtype, torch.float32, checkpoint)
+
+
 @pytest.mark.parametrize("pad,offset", [(4, 0), (1, 0), (0, 1), (3, 2), (12, 4)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strided_and_misaligned_rows(pad, offset, dtype):
