@@ -4,10 +4,10 @@
 //              = sum_r (g[r, m] sc_r) code[r, k]  +  sum_r g[r, m] zp_r
 //
 // The first sum runs on the tensor cores: a code is exact in bf16, and g sc, rounded once, is carried as three bf16 terms, its
-// 24 bits, so a tile takes three products where two fp32 operands would take six.  (Two terms, 2^-17 of a value off, took 570 us
-// instead of 625 for 600k rows of 512 and 256 columns with the pack, and left the result 2.6e-6 off instead of 0.7e-6.)  The second sum does
-// not depend on k: a few fp32 multiply-adds beside the conversion of g.  The activations are never restored in memory: one byte
-// an element is read.
+// 24 bits, so a tile takes three products where two fp32 operands would take six.  (Two terms, 2^-17 of a value off, took
+// 570 us instead of 625 for 600k rows of 512 and 256 columns with the pack, and left the result 2.6e-6 off instead of
+// 0.7e-6.)  The second sum does not depend on k: a few fp32 multiply-adds beside the conversion of g.  The activations are
+// never restored in memory: one byte an element is read.
 //
 // A block owns 128 x 256 results and a range of the rows.  Per 32 rows TMA brings 128 columns of g and 256 of the codes
 // into shared memory as they are (where an operand is not aligned for it, the threads load it themselves); sixteen warps

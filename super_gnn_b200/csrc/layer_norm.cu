@@ -10,9 +10,10 @@
 // x: one byte an element kept between the two instead of four.
 //
 // Everything is bound by memory: the forward moves x and y once, the backward gy, x (or its codes) and gx once.  Rows
-// of up to 1024 elements belong to a warp (narrow ones to 4, 8 or 16 of its lanes), which holds them in registers between the reductions and the
-// outputs; longer rows to a block, which reads them again (from L1 / L2) for every step.  All sums are fp32: the variance
-// from the differences to the mean, the column sums per warp, then per block, then over the blocks, in a fixed order.
+// of up to 1024 elements (2048 forward) belong to a warp, narrow ones to 4, 8 or 16 of its lanes, which hold them in
+// registers between the reductions and the outputs; up to 2048 backward to a block that does the same; longer rows to a
+// block that reads them again (from L1 / L2) for every step.  All sums are fp32: the variance from the differences to
+// the mean, the column sums per warp, then per block, then over the blocks, in a fixed order.
 #include "row_io.cuh"
 #include "umma.cuh"
 
@@ -920,7 +921,9 @@ static int norm_bwd_staged(const NormCall &c, int *blocks)
             if (need <= 16 / E) return fn<T, E, 16 / E, CK, 32>(__VA_ARGS__);                                           \
         }                                                                                                               \
         if (!FWD && c.H > (CK && E != 4 ? 512 : kNormSplit) && c.H <= kNormWide) return fn<T, E, FWD ? 0 : -1, CK, 32>(__VA_ARGS__); \
-        if (need <= 32 / E) return fn<T, E, 32 / E, CK, 32>(__VA_ARGS__);                                               \
+        if constexpr (FWD || !CK || E != 8) {                                                                           \
+            if (need <= 32 / E) return fn<T, E, 32 / E, CK, 32>(__VA_ARGS__);                                           \
+        }                                                                                                               \
         if (FWD && E >= 4 && need <= 64 / E) return fn<T, E, FWD && E >= 4 ? 64 / E : 0, CK, 32>(__VA_ARGS__);          \
         return fn<T, E, 0, CK, 32>(__VA_ARGS__);                                                                        \
     } while (0)

@@ -10,15 +10,16 @@
 //
 // One persistent block an SM.  A warp feeds operand tiles by TMA through a ring of shared memory buffers, a thread issues
 // the tcgen05 products into tensor memory, eight warps turn finished 128 x 256 results into the outputs.  Two blocks of a
-// cluster share a 256 x 256 result where that is faster (nll_in_pairs in linear_nll.cu): each brings 128 rows of the first operand and half of
-// the second, 32 KB a step of 64 for 128 x 256 results where a block alone needs 48 KB.  The operands lie as their matrices do: x and W are read along k by the first product and across it by the
-// other two, G along the classes by the second and across by the third, so that nothing is ever transposed in memory.
+// cluster share a 256 x 256 result where that is faster (nll_in_pairs in linear_nll.cu): each brings 128 rows of the
+// first operand and half of the second, 32 KB a step of 64 for 128 x 256 results where a block alone needs 48 KB.  The
+// operands lie as their matrices do: x and W are read along k by the first product and across it by the other two, G along
+// the classes by the second and across by the third, so that nothing is ever transposed in memory.
 //
 // fp32 operands come as two fp16 planes (v 2^e = v0 + v1, 22 bits; see linear_nll.cu) and three products
-// v0 w0 + v0 w1 + v1 w0 a tile; bf16 operands as one plane and one product.  Tensor memory rounds every addition towards zero, a
-// relative 2^-25 on average, and most of G has one sign: in the two gradients, whose reductions are long, the cross products of the planes, 2^-11 of
-// the others, have sums of their own, and the main sums move on into registers every 512 of the reduction.  A sum over 55k
-// classes would else be 5e-6 of itself too small (0.7e-6 so).
+// v0 w0 + v0 w1 + v1 w0 a tile; bf16 operands as one plane and one product.  Tensor memory rounds every addition towards
+// zero, a relative 2^-25 on average, and most of G has one sign: in the two gradients, whose reductions are long, the
+// cross products of the planes, 2^-11 of the others, have sums of their own, and the main sums move on into registers every
+// 512 of the reduction.  A sum over 55k classes would else be 5e-6 of itself too small (0.7e-6 so).
 #pragma once
 #include "umma.cuh"
 
