@@ -208,6 +208,10 @@ __device__ __forceinline__ void staged_walk(const StagedRing &ring, const T *p, 
         if (b < full) {
             bar_wait(full_bar + s, phase, gone);
         } else {
+            // ordinary stores by every thread into a buffer whose result of an earlier batch left it by a bulk store of thread 0's:
+            // it has to have been read (with two buffers no barrier since thread 0's last wait says so)
+            if (threadIdx.x == 0) store_wait_read();
+            __syncthreads();
             staged_copy_in(data, p, b, n, H);
             if (q) staged_copy_in(other, q, b, n, H);
             __syncthreads();

@@ -244,6 +244,29 @@ def test_packed_rows_through_the_ring(n, H, dtype):
     assert torch.equal(ops.layer_norm_forward(back, gamma, beta, out=back)[0], y)
 
 
+@pytest.mark.parametrize("n,H,dtype,backward", [
+    (20_003, 602, torch.float32, True), (10_003, 600, torch.float32, True), (40_005, 831, torch.float32, True),
+    (10_003, 1301, torch.float32, False), (10_007, 2047, torch.float32, False), (10_005, 2038, torch.float16, False)])
+def test_short_last_batch_in_a_ring_of_two_buffers(n, H, dtype, backward):
+    """Rows so long that the ring has two buffers, at least three batches a block, and a last batch that is not whole: its
+    rows are written over a buffer that a result has just left from.  (The rows before it are the ones that would suffer.)"""
+    x, gy, gamma, beta = make(n, H, dtype, torch.float32, seed=n + H)
+    x = x.contiguous()
+    y, stats = ops.layer_norm_forward(x, gamma, beta)
+    ref = Ref(x, gamma, beta, 1e-5)
+    close(y, ref.y, ref.e_y)
+    if not backward:
+        for _ in range(4):
+            assert torch.equal(ops.layer_norm_forward(x, gamma, beta)[0], y)
+        return
+    got = ops.layer_norm_backward(gy, x, stats, gamma)
+    for g, (want, err) in zip(got, ref.backward(gy)):
+        close(g, want, err)
+    for _ in range(4):
+        for a, b in zip(ops.layer_norm_backward(gy, x, stats, gamma), got):
+            assert torch.equal(a, b)
+
+
 def test_captured_and_on_another_stream():
     x, gy, gamma, beta = make(900, 300, torch.bfloat16, torch.float32, seed=3)
     x = x.contiguous()
