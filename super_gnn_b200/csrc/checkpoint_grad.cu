@@ -167,9 +167,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
                     tma_load(at + kRawG + kGRows * kGN, &c.zs, 2 * r0, 0, 0, raw_full + s);
                     if (++s == kGRaw) s = 0, phase ^= 1;
                 }
-                if (done < count) {
-                    for (int b = 0; b < kGRaw && b < done; ++b) bar_drain(raw_full + b, ((done - 1 - b) / kGRaw) & 1);
-                }
+                if (done < count) ring_drain(raw_full, done, kGRaw);
             }
             __syncwarp();
         } else if (warp == kGKeepers + kGWorkers + 1) {

@@ -133,13 +133,14 @@ struct StagedRing {
     int depth;
 };
 
-// 8 H sizeof(T) bytes from each of one or two operands into buffer s; the last batch of a matrix may be short and is copied
-// by the threads.
+// 8 H sizeof(T) bytes from each of one or two operands into buffer s, one fill more; the last batch of a matrix may be short and is
+// copied by the threads.
 template <class T>
 __device__ __forceinline__ void staged_load(const StagedRing &ring, int s, const T *p, const T *q, int64_t batch, int64_t full, int64_t n,
-                                            int H, uint64_t *bar)
+                                            int H, uint64_t *bar, unsigned &used)
 {
     if (batch >= full || threadIdx.x != 0) return;
+    ++used;
     const unsigned bytes = (unsigned)(kNormWarps * H * sizeof(T));
     uint8_t *at = ring.base + s * ring.stride;
     bar_expect(bar, q ? 2 * bytes : bytes);
@@ -197,9 +198,10 @@ __device__ __forceinline__ void staged_walk(const StagedRing &ring, const T *p, 
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    unsigned used = 0;  // fills by thread 0: buffer 0, 1, ..., 0, 1, ...
     for (int s = 0; s < ring.depth; ++s)
         if ((int64_t)blockIdx.x + (int64_t)s * gridDim.x < batches)
-            staged_load(ring, s, p, q, (int64_t)blockIdx.x + (int64_t)s * gridDim.x, full, n, H, full_bar + s);
+            staged_load(ring, s, p, q, (int64_t)blockIdx.x + (int64_t)s * gridDim.x, full, n, H, full_bar + s, used);
     int s = 0;
     unsigned phase = 0;
     for (int64_t b = blockIdx.x; b < batches; b += gridDim.x) {
@@ -232,14 +234,13 @@ __device__ __forceinline__ void staged_walk(const StagedRing &ring, const T *p, 
         if (b != blockIdx.x && next < batches) {
             const int before = s == 0 ? ring.depth - 1 : s - 1;
             if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-            staged_load(ring, before, p, q, next, full, n, H, full_bar + before);
+            staged_load(ring, before, p, q, next, full, n, H, full_bar + before, used);
         }
         if (++s == ring.depth) s = 0, phase ^= 1;
     }
     if (threadIdx.x == 0) {
         store_wait_all();
-        if (*gone)
-            for (int i = 0; i < ring.depth; ++i) bar_drain(full_bar + i, phase);
+        if (*gone) ring_drain(full_bar, used, ring.depth);
     }
 }
 

@@ -256,11 +256,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                     const uint64_t until = now_ns() + kWaitNs / 8;
                     while (now_ns() < until) __nanosleep(1000);
                 }
-                for (int s = 0; rank == 0 && s < S::kStages; ++s) {
-                    if (used < (unsigned)(s + 1)) continue;
-                    const unsigned uses = (used - 1 - s) / S::kStages + 1;  // fills of this buffer so far
-                    bar_drain(full + s, (uses - 1) & 1);
-                }
+                if (rank == 0) ring_drain(full, used, S::kStages);
             }
         }
         __syncwarp();

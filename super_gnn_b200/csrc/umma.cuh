@@ -74,12 +74,28 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, unsigned parity, volatil
     return false;
 }
 
+// Fills that buffer s of a ring has had once `used` of them have been dealt over the buffers in turn; the last one of them completes
+// the phase of parity (fills - 1) & 1 of the buffer's barrier
+__host__ __device__ constexpr unsigned ring_fills(unsigned used, unsigned s, unsigned buffers)
+{
+    return used > s ? (used - 1 - s) / buffers + 1 : 0;
+}
+
 // Waits for what is in flight after a role gave up: the bound alone, whatever the others say.
 __device__ __forceinline__ void bar_drain(uint64_t *bar, unsigned parity)
 {
     const uint64_t until = now_ns() + kWaitNs / 8;
     for (int i = 0; i < (1 << 28) && now_ns() < until; ++i)
         if (bar_try(bar, parity)) return;
+}
+
+// The same for every buffer of a ring that copies may still be on their way to; one that was never filled is not waited for
+__device__ __forceinline__ void ring_drain(uint64_t *bars, unsigned used, int buffers)
+{
+    for (int s = 0; s < buffers; ++s) {
+        const unsigned fills = ring_fills(used, s, buffers);
+        if (fills > 0) bar_drain(bars + s, (fills - 1) & 1);
+    }
 }
 
 // ---- two blocks of a cluster that work on one product (cta_group::2): the first of them leads ----
