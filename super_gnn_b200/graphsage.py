@@ -99,6 +99,7 @@ class DistSAGE(torch.nn.Module):
         nodes times ``loss_inv_count`` is returned instead, computed together with the last layer."""
         chunked = (self.chunked_loss and loss_mask is not None and loss_inv_count is not None
                    and self.can_fuse_loss(nodes_feats, graph))
+        bits = self.checkpoint_bits if torch.is_grad_enabled() else 32  # without a backward pass nothing is kept
         if self._fused_ok(nodes_feats):
             reset_layer_buffers()
             for i, conv in enumerate(self.convs[:-1]):
@@ -116,7 +117,7 @@ class DistSAGE(torch.nn.Module):
                                                    float(norm.eps), seed, mask,
                                                    (i + 1 < len(self.convs) - 1
                                                     and self._layer_fusable(self.convs[i + 1], hidden=True))
-                                                   or (i + 1 == len(self.convs) - 1 and chunked), self.checkpoint_bits)
+                                                   or (i + 1 == len(self.convs) - 1 and chunked), bits)
             last = self.convs[-1]
             if chunked:
                 return self._chunked_loss(graph, nodes_feats, labels, loss_mask, loss_inv_count, loss_unit_grad)
@@ -128,11 +129,11 @@ class DistSAGE(torch.nn.Module):
                 return node.apply(nodes_feats, last.lin_neigh.weight,
                                   last.lin_self.weight, last.bias, graph, len(self.convs) - 1,
                                   last.num_bits, last.is_pre_delay, self.training, labels,
-                                  loss_mask, float(loss_inv_count), bool(loss_unit_grad), self.checkpoint_bits)
+                                  loss_mask, float(loss_inv_count), bool(loss_unit_grad), bits)
             node = FusedSAGEOutputLayerProjectFirst if self._project_first(last) else FusedSAGEOutputLayer
             nodes_feats = node.apply(nodes_feats, last.lin_neigh.weight,
                                      last.lin_self.weight, last.bias, graph, len(self.convs) - 1,
-                                     last.num_bits, last.is_pre_delay, self.training, self.checkpoint_bits)
+                                     last.num_bits, last.is_pre_delay, self.training, bits)
             return F.log_softmax(nodes_feats, dim=1)
         for i in range(len(self.convs) - 1):
             nodes_feats = self._unfused_hidden(graph, nodes_feats, i)

@@ -3,7 +3,8 @@ layer norm whose input is kept in 8 bits for the backward pass, and the loss of 
 
 ``checkpoint_bits``: 32 keeps the input itself (as the reference's autograd graph does), 8 its 8-bit checkpoint
 (``supergnn_ops.checkpoint_pack_rows``): the forward results are the same, the gradients are those of the restored
-input where the formula asks for it.
+input where the formula asks for it.  Nothing is kept, and no gradient computed with a loss, where no backward pass can
+follow (under ``torch.no_grad()``, or when no argument requires a gradient).
 """
 from __future__ import annotations
 
@@ -18,6 +19,11 @@ def check_bits(checkpoint_bits) -> int:
     if checkpoint_bits not in (8, 32):
         raise ValueError(f"checkpoint_bits must be 8 or 32, got {checkpoint_bits}")
     return int(checkpoint_bits)
+
+
+def _backward_can_follow(*tensors) -> bool:
+    """Asked before ``apply``: a parameter's ``needs_input_grad`` stays true inside it when gradients are off."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -46,7 +52,11 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, checkpoint_bits: int = 32):
     """Layer norm over the last dimension of a CUDA tensor (fp32, bf16 or fp16); weight and bias fp32 or of x's type,
     or None."""
-    y = _LayerNorm.apply(x.reshape(-1, x.size(-1)), weight, bias, float(eps), check_bits(checkpoint_bits))
+    bits, rows = check_bits(checkpoint_bits), x.reshape(-1, x.size(-1))
+    if _backward_can_follow(x, weight, bias):
+        y = _LayerNorm.apply(rows, weight, bias, float(eps), bits)
+    else:
+        y = ops.layer_norm_forward(rows, weight, bias, float(eps))[0]
     return y.reshape(x.shape)
 
 
@@ -68,7 +78,7 @@ class _CheckpointLinear(torch.autograd.Function):
 def linear(x, weight, checkpoint_bits: int = 32):
     """``x @ weight.T`` for ``x`` [n, K]; with ``checkpoint_bits=8`` the weight gradient is taken from the 8-bit
     checkpoint of ``x``, and ``x`` itself is not kept."""
-    if check_bits(checkpoint_bits) == 32:
+    if check_bits(checkpoint_bits) == 32 or not _backward_can_follow(x, weight):
         return F.linear(x, weight)
     return _CheckpointLinear.apply(x, weight)
 
@@ -76,8 +86,6 @@ def linear(x, weight, checkpoint_bits: int = 32):
 class _LinearNLL(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, labels, mask, inv_count):
-        if not any(ctx.needs_input_grad):
-            return ops.linear_nll_loss(x, weight, bias, labels, mask, inv_count)[0].reshape(())
         loss, gx, gw, gb = ops.linear_nll_loss_grad(x, weight, bias, labels, mask, inv_count)
         ctx.save_for_backward(gx, gw, gb)
         return loss.reshape(())
@@ -94,4 +102,6 @@ class _LinearNLL(torch.autograd.Function):
 def linear_nll_loss(x, weight, bias, labels, mask, inv_count: float):
     """``-sum_{mask} log_softmax(x @ weight.T + bias)[r, labels[r]] * inv_count`` as a differentiable scalar, without the
     logits in memory (``supergnn_ops.linear_nll_loss_grad``); the gradients are computed with the loss."""
+    if not _backward_can_follow(x, weight, bias):
+        return ops.linear_nll_loss(x, weight, bias, labels, mask, float(inv_count))[0].reshape(())
     return _LinearNLL.apply(x, weight, bias, labels, mask, float(inv_count))

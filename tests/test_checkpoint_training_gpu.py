@@ -238,3 +238,76 @@ def test_second_backward_pass_of_the_chunked_loss():
         again = torch.autograd.grad(loss, (h, conv.lin_self.weight))
         for a, c in zip(first, again):
             assert torch.equal(a, c)
+
+
+def kinds_of(call):
+    """Entry points that a call launched."""
+    ops.LAUNCH_LOG = []
+    try:
+        call()
+        return {entry[0] for entry in ops.LAUNCH_LOG}
+    finally:
+        ops.LAUNCH_LOG = None
+
+
+@pytest.mark.parametrize("fused,hid", [(True, 64), (True, 50), (False, 64)])
+def test_an_evaluation_packs_nothing_and_computes_no_gradients(fused, hid):
+    n, fin, ncls = 2000, 30, 300
+    graph = graph_of(n, 20_000, hid)
+    _, model = models(fin, hid, ncls, checkpoint_bits=8, chunked_loss=True)
+    _, plain = models(fin, hid, ncls)
+    model.fused = plain.fused = fused
+    x, labels = torch.randn(n, fin, device=DEV), torch.randint(0, ncls, (n,), device=DEV)
+    mask = torch.rand(n, device=DEV) < 0.3
+    args, kw = (graph, x, labels, None), dict(loss_mask=mask, loss_inv_count=0.01)
+    model.eval(), plain.eval()
+    got = {}
+
+    def evaluate():
+        with torch.no_grad():
+            got["loss"], got["out"] = model(*args, **kw), model(graph, x)
+
+    assert kinds_of(evaluate).isdisjoint({"checkpoint_pack", "linear_nll_grad"})
+    assert {"checkpoint_pack", "linear_nll_grad"} <= kinds_of(lambda: model(*args, **kw))
+    with torch.no_grad():
+        out = plain(graph, x)
+    # the same forward through other kernels: sums of up to a few hundred neighbours in another order, 2^-24 each, in three layers
+    assert float((got["out"] - out).abs().max()) <= 1e-4 * float(out.abs().max())
+    want = F.nll_loss(out[mask], labels[mask], reduction="sum") * 0.01
+    assert abs(float(got["loss"]) - float(want)) <= 1e-5 * float(want)
+
+
+def test_functional_forms_without_a_backward_pass(monkeypatch):
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(70, 36, generator=gen, device=DEV)
+    w, lw = torch.nn.Parameter(torch.rand(36, device=DEV)), torch.nn.Parameter(torch.rand(300, 36, device=DEV))
+    labels = torch.randint(0, 300, (70,), device=DEV)
+    packed = []
+    forward = ops.layer_norm_forward
+    monkeypatch.setattr(ops, "layer_norm_forward",
+                        lambda *a, **k: (packed.append(k.get("checkpoint", False)), forward(*a, **k))[1])
+
+    def calls(weight, last):
+        return (L.layer_norm(x, weight, checkpoint_bits=8), L.linear(x, last, checkpoint_bits=8),
+                L.linear_nll_loss(x, last, None, labels, None, 0.1))
+
+    want = calls(w, lw)
+    assert packed == [True] and all(y.requires_grad for y in want)
+
+    def quiet():
+        with torch.no_grad():
+            return calls(w, lw)
+
+    for run in (quiet, lambda: calls(w.detach(), lw.detach())):
+        packed.clear()
+        got = []
+        assert kinds_of(lambda: got.extend(run())) == {"layer_norm_fwd", "linear_nll"} and packed == [False]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b) and not a.requires_grad
+    # memory: neither gradients nor codes beside the result
+    big = torch.randn(20_000, 36, device=DEV)
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        before = torch.cuda.memory_allocated()
+        y = L.layer_norm(big, w, checkpoint_bits=8)
+        assert torch.cuda.memory_allocated() - before <= y.numel() * 4 + 1024
