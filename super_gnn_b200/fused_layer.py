@@ -499,7 +499,7 @@ def _many_classes_input(x, w_neigh, w_self, graph, layer, num_bits, is_pre_delay
     return actx, ax, torch.cat([w_neigh, w_self], dim=1)
 
 
-def many_classes_loss(x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, labels, mask, inv_count):
-    """The loss of :class:`FusedSAGELossManyClasses` alone, for validation: nothing is kept for a backward pass."""
-    _, ax, w_cat = _many_classes_input(x, w_neigh, w_self, graph, layer, num_bits, is_pre_delay, False)
+def many_classes_loss(x, w_neigh, w_self, bias, graph, layer, num_bits, is_pre_delay, training, labels, mask, inv_count):
+    """The loss of :class:`FusedSAGELossManyClasses` alone, the same number: nothing is kept for a backward pass."""
+    _, ax, w_cat = _many_classes_input(x, w_neigh, w_self, graph, layer, num_bits, is_pre_delay, training)
     return ops.linear_nll_loss(ax, w_cat, bias, labels, mask, inv_count)[0].reshape(())

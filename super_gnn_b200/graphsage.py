@@ -160,10 +160,11 @@ class DistSAGE(torch.nn.Module):
 
     def _chunked_loss(self, graph, x, labels, mask, inv_count, unit_grad):
         last, layer = self.convs[-1], len(self.convs) - 1
-        args = (x, last.lin_neigh.weight, last.lin_self.weight, last.bias, graph, layer, last.num_bits, last.is_pre_delay)
+        args = (x, last.lin_neigh.weight, last.lin_self.weight, last.bias, graph, layer, last.num_bits, last.is_pre_delay,
+                self.training, labels, mask, float(inv_count))
         if not torch.is_grad_enabled():
-            return many_classes_loss(*args, labels, mask, float(inv_count))
-        return FusedSAGELossManyClasses.apply(*args, self.training, labels, mask, float(inv_count), bool(unit_grad))
+            return many_classes_loss(*args)
+        return FusedSAGELossManyClasses.apply(*args, bool(unit_grad))
 
 
 def allreduce_hook(process_group, bucket):

@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from super_gnn_b200 import graphsage, supergnn_ops as ops, synthetic
+from super_gnn_b200 import fused_layer, graphsage, supergnn_ops as ops, synthetic
 from super_gnn_b200.data_manager import build_distributed_graph
 from super_gnn_b200.layers import functional as L
 
@@ -311,3 +311,47 @@ def test_functional_forms_without_a_backward_pass(monkeypatch):
         before = torch.cuda.memory_allocated()
         y = L.layer_norm(big, w, checkpoint_bits=8)
         assert torch.cuda.memory_allocated() - before <= y.numel() * 4 + 1024
+
+
+def test_the_loss_alone_takes_the_exchange_of_the_mode(monkeypatch):
+    """A model in training mode quantises the rows it exchanges, whether or not gradients are on."""
+    n, fin, hid, ncls = 500, 20, 32, 300
+    graph = graph_of(n, 5000, hid)
+    _, model = models(fin, hid, ncls, chunked_loss=True)
+    x, labels = torch.randn(n, fin, device=DEV), torch.randint(0, ncls, (n,), device=DEV)
+    mask = torch.ones(n, dtype=torch.bool, device=DEV)
+    seen = []
+    inner = fused_layer.aggregate_forward
+
+    def forward(ctx, graph, x, layer, num_bits, is_pre_delay, is_training, **kw):
+        seen.append((layer, is_training))
+        return inner(ctx, graph, x, layer, num_bits, is_pre_delay, is_training, **kw)
+
+    monkeypatch.setattr(fused_layer, "aggregate_forward", forward)
+    for training in (True, False):
+        model.train(training)
+        for grad in (True, False):
+            seen.clear()
+            with torch.set_grad_enabled(grad):
+                model(graph, x, labels, None, loss_mask=mask, loss_inv_count=0.01)
+            assert seen == [(0, training), (1, training), (2, training)], (training, grad, seen)
+
+
+@pytest.mark.parametrize("unit", [True, False])
+def test_gradients_of_several_backward_passes_add_up(unit):
+    """What the loss keeps for its backward pass is not handed out as somebody's gradient to add to."""
+    n, hid, ncls = 600, 32, 300
+    graph = graph_of(n, 6000, hid)
+    _, model = models(20, hid, ncls, chunked_loss=True)
+    labels = torch.randint(0, ncls, (n,), device=DEV)
+    conv = model.convs[-1]
+    h = torch.randn(n, hid, device=DEV, requires_grad=True)
+    loss = graphsage.FusedSAGELossManyClasses.apply(h, conv.lin_neigh.weight, conv.lin_self.weight, conv.bias, graph, 2, 32,
+                                                    False, True, labels, None, 0.01, unit)
+    leaves = (h, conv.lin_neigh.weight, conv.lin_self.weight, conv.bias)
+    first = [g.clone() for g in torch.autograd.grad(loss, leaves, retain_graph=True)]
+    for turn in range(1, 5):
+        loss.backward(retain_graph=True)
+        for leaf, g in zip(leaves, first):
+            # sums of equal fp32 numbers: up to three roundings; h: an SpMM whose atomic adds come in any order
+            assert near(leaf.grad, turn * g, 1e-5)
