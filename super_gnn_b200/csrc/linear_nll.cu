@@ -2,7 +2,7 @@
 // classes, so that the logits z = x W^T + b, [n, C], are never kept:
 //
 //     lse[r] = log sum_c exp z[r, c]        maximum and sum of every 128 classes, joined in a tree
-//     loss   = inv_count sum_r (lse[r] - z[r, label])
+//     loss   = inv_count sum_r (lse[r] - z[r, label])   both from the same sums: a row that is certain of its label adds 0
 //     G      = inv_count (exp(z - lse) - onehot)  piece by piece, from logits computed a second time
 //     gx += G W_piece,  gw_piece = G^T x,  gb_piece = sum_r G
 //
@@ -160,14 +160,10 @@ struct Planes {
     int64_t ld, stride;
 };
 
-// The label's logit of the listed rows, in units of log2, from the operands as they are given
+// The labels of the listed rows
 struct Picked {
     const int64_t *labels;
-    const void *w;
-    int64_t ldw;
-    NllBias bias;
     int *label;
-    float *picked2;
 };
 
 __device__ __forceinline__ void store_split(const Planes &pl, int64_t at, float v, float up)
@@ -227,17 +223,7 @@ __global__ void __launch_bounds__(256) nll_take_kernel(const TakeSide xs, const 
         const bool there = i < n;
         const int64_t r = there ? source_row(s, i) : 0;
         const T *x = static_cast<const T *>(s.src) + r * s.ld;
-        if (is_x && there) {
-            const int64_t label = pick.labels[r];
-            const T *w = static_cast<const T *>(pick.w) + label * pick.ldw;
-            float z = 0.f;
-            for (int k = lane; k < s.K; k += 32) z = __fmaf_rn(to_f32<T>(x[k]), to_f32<T>(w[k]), z);
-            z = all_sum(z);
-            if (lane == 0) {
-                pick.label[i] = (int)label;
-                pick.picked2[i] = (z + bias_at<T>(pick.bias, label)) * kLog2e;
-            }
-        }
+        if (is_x && there && lane == 0) pick.label[i] = (int)pick.labels[r];
         float up = 1.f, down = 1.f;
         if (SPLIT) {
             float largest = 0.f, poison = 0.f;
@@ -706,7 +692,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         SGNN_CUDA_OK(launch_chained(nll_column_max_kernel, dim3((unsigned)ceil_div(c.K, 32), (unsigned)tall, 2), 256, 0, s, xs.src, ws.src, largest));
     }
     SGNN_CUDA_OK(launch_chained(nll_take_kernel<T, f32>, dim3((unsigned)(xs.blocks + ws.blocks)), 256, 0, s, xs, ws,
-                                Picked{c.labels, c.w, c.ldw, c.bias, ints(p.label), floats(p.picked2)}));
+                                Picked{c.labels, ints(p.label)}));
 
     // tensor maps: x and W along k (rows of a tile at once) and across it (64 steps of the reduction at once), G likewise
     ProductCall lc{}, xc{}, wc{};

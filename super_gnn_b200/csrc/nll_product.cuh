@@ -48,7 +48,7 @@ struct ProductCall {
     const float *cls_scale;
     float2 *stats;           // [2 x class tiles, row_cap]: (maximum, sum of 2^(t - maximum)), in units of log2
     const float *lse2;       // [row_cap]
-    const float *picked2;    // [row_cap] the label's logit
+    float *picked2;          // [row_cap] the label's logit, from the same sums as the others
     const int *label;        // [row_cap]
     float *bias_part;        // [row_cap / 32, grad_ld]: sums of G over 32 rows, or nullptr
     int64_t grad_ld;
@@ -433,9 +433,17 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
             };
             if constexpr (KIND == kLogitStats) {
                 float mx = -INFINITY, sum = 0.f;
+                const int label = row < u.m ? c.label[row] - c.cls0 - t.n0 - half * 128 : -1;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     logits(j);
+                    const int at = label - 32 * j;
+                    if (at >= 0 && at < 32) {  // in these columns
+                        float z = v[0];
+#pragma unroll
+                        for (int e = 1; e < 32; ++e) z = e == at ? v[e] : z;
+                        c.picked2[row] = z;
+                    }
                     float top = mx;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) top = fmaxf(top, v[e]);
@@ -448,9 +456,9 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                 if (row < u.m) c.stats[(int64_t)(t.n0 / 128 + half) * c.row_cap + row] = make_float2(mx, sum);
             } else if constexpr (KIND == kLogitGrad) {
                 const int label = row < u.m ? c.label[row] - c.cls0 - t.n0 - half * 128 : -1;
-                const float own = label >= 0 && label < 128
-                                      ? (exp2_fast(__ldg(c.picked2 + row) - lse2) - 1.0f) * (PLANES == 2 ? kGradScale : 1.0f)
-                                      : 0.f;  // G of the label's class
+                const float own = label >= 0 && label < 128  // G of the label's class, p - 1, without the cancellation of a p next to 1
+                                      ? expm1f((__ldg(c.picked2 + row) - lse2) * 0.6931471805599453f) * (PLANES == 2 ? kGradScale : 1.0f)
+                                      : 0.f;
                 const int x0 = t.n0 + half * 128, y0 = t.m0 + quarter * 32;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {

@@ -303,3 +303,34 @@ def test_captured_call_of_two_blocks(dtype):
     torch.cuda.synchronize()
     for a, c in zip(got, ops.linear_nll_loss_grad(*new, 0.1)):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [64, 200])
+def test_rows_that_are_certain_of_their_label(dtype, K):
+    """The largest logit is the label's and all others are far below: lse and that logit come from the same sums, so that their
+    difference is off by the rounding of lse alone (and is never negative), not by the error of a dot product."""
+    gen = torch.Generator(device=DEV).manual_seed(K)
+    n, C = 150, 700
+    w = torch.randn(C, K, generator=gen, device=DEV).to(dtype)
+    labels = torch.randint(0, C, (n,), generator=gen, device=DEV)
+    # the label's logit 90, the others' deviation 90 / sqrt(K) <= 12
+    x = (w[labels].double() * (90 / w[labels].double().square().sum(1, keepdim=True))).to(dtype)
+    z = x.double() @ w.double().t()
+    lse = torch.logsumexp(z, 1)
+    terms = lse - z[torch.arange(n, device=DEV), labels]
+    assert float(terms.max()) < 1e-3 and float(terms.min()) >= 0
+    # a step of lse in its units of log2, each way, and what moves the terms: the other classes' share p = terms, off by
+    # p (2 e_z), e_z = (K + 16) 2^-23 sum |x w|
+    e_z = (K + 16) * STEP * (x.double().abs() @ w.double().abs().t()).amax(1)
+    bound = 2 * STEP * lse + 2.1 * terms * e_z
+    assert float((e_z * terms).max()) < float(bound.min())
+    loss, got_lse = ops.linear_nll_loss(x, w, None, labels, None, 1.0)
+    assert float(loss) >= 0 and abs(float(loss) - float(terms.sum())) <= float(bound.sum())
+    for r in range(0, n, 7):
+        mask = torch.zeros(n, dtype=torch.bool, device=DEV)
+        mask[r] = True
+        one, gx, gw, gb = ops.linear_nll_loss_grad(x, w, torch.zeros(C, device=DEV), labels, mask, 1.0)
+        assert float(one) >= 0 and abs(float(one) - float(terms[r])) <= float(bound[r])
+        # p - 1 of the label: of the size of what the others have, or a step of lse
+        assert float(gb[labels[r]]) <= 0 and abs(float(gb[labels[r]]) + float(-torch.expm1(-terms[r]))) <= float(bound[r])
