@@ -13,10 +13,10 @@
 //
 // bf16 operands enter the products as they are; G is rounded to bf16, as it is between two bf16 layers.  fp32 operands are
 // split into two fp16 planes, v 2^e = v0 + v1 with 2^e bringing the largest value of the row below 2^15: 22 bits of every
-// value that is not 2^-16 of the largest, an absolute 2^-39 of the largest below that.  A product of two such operands
-// takes three products of planes (v1 w1 is below 2^-22).  The scale belongs to a row for the logits, where rows of x meet
-// rows of W, and to a column for the gradients, where columns come out: two sets of planes of each.  bf16 terms would need
-// no scale but six products for the same accuracy.
+// value that is not below 2^-16 of the largest, an absolute 2^-39 of the largest below that (in the gradients 2^-27 and 2^-50, see
+// kSecondPlane).  A product of two such operands takes three products of planes (v1 w1 is below 2^-22).  The scale belongs to a row
+// for the logits, where rows of x meet rows of W, and to a column for the gradients, where columns come out: two sets of
+// planes of each.  bf16 terms would need no scale but six products for the same accuracy.
 #include "nll_product.cuh"
 #include "row_io.cuh"
 
@@ -166,12 +166,13 @@ struct Picked {
     int *label;
 };
 
-__device__ __forceinline__ void store_split(const Planes &pl, int64_t at, float v, float up)
+// `second`: what the second plane is scaled by beyond the first
+__device__ __forceinline__ void store_split(const Planes &pl, int64_t at, float v, float up, float second)
 {
     const float s = v * up;
     const __half h = __float2half_rn(s);
     reinterpret_cast<__half *>(pl.p)[at] = h;
-    reinterpret_cast<__half *>(pl.p)[at + pl.stride] = __float2half_rn(s - __half2float(h));
+    reinterpret_cast<__half *>(pl.p)[at + pl.stride] = __float2half_rn((s - __half2float(h)) * second);
 }
 
 // largest |value| of every column of x (z = 0) and W (z = 1), as bits: a NaN or an infinity stays above every number
@@ -241,11 +242,11 @@ __global__ void __launch_bounds__(256) nll_take_kernel(const TakeSide xs, const 
             const int64_t at = i * t.row.ld + k;
             if (SPLIT) {
                 const float v = in ? to_f32<T>(x[k]) : 0.f;
-                store_split(t.row, at, v, up);
+                store_split(t.row, at, v, up, 1.0f);
                 if (t.col.p) {
                     float cup = 1.f, cdown;
                     if (k < s.K) plane_scale(__uint_as_float(__ldg(t.largest + k)), cup, cdown);
-                    store_split(t.col, at, v, cup);
+                    store_split(t.col, at, v, cup, kSecondPlane);
                 }
             } else {
                 t.row.p[at] = in ? reinterpret_cast<const uint16_t *>(x)[k] : (uint16_t)0;

@@ -150,7 +150,14 @@ __device__ __forceinline__ void plane_scale(float largest, float &up, float &dow
     down = __uint_as_float((unsigned)(127 - e) << 23);
 }
 
-constexpr float kGradScale = 32768.0f;  // fp16 planes of G: |G| <= 1 fills the range, 2^-40 is the smallest step
+constexpr float kGradScale = 32768.0f;  // fp16 planes of G: |G| <= 1 fills the range
+// What the first plane of an operand of the gradients leaves, at most half of its last step, goes into the second one 2^11 times as
+// large; the sums of the cross products are scaled back once.  Two planes then keep 22 bits of every value that is not below 2^-27
+// of the largest (G, where 1 is known to be the largest: 2^-28), and are an absolute 2^-50 of the largest (2^-51) off below that.
+// Unscaled these are 2^-16 and 2^-39 (2^-17 and 2^-40): a class of probability 2^-30 would keep 9 bits of its weights' gradient.
+// The logits add both kinds of products into one sum and stay unscaled; there the scale is a row's own, and what is that small
+// beside the row's largest value moves no logit.
+constexpr float kSecondPlane = 2048.0f;
 
 // `c`: the logits or the rows' gradient; `c2`: the weights' gradient (a kernel of one kind takes the same for both)
 template <int KIND, int PLANES, int CTAS>
@@ -516,7 +523,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                                 const float g0 = v[8 * q + 2 * e], g1 = v[8 * q + 2 * e + 1];
                                 p0[e] = pack16<__half>(g0, g1);
                                 const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(p0 + e));
-                                p1[e] = pack16<__half>(g0 - r.x, g1 - r.y);
+                                p1[e] = pack16<__half>((g0 - r.x) * kSecondPlane, (g1 - r.y) * kSecondPlane);
                             }
                             *reinterpret_cast<uint4 *>(r0 + (q ^ turn) * 16) = w0;
                             *reinterpret_cast<uint4 *>(r1 + (q ^ turn) * 16) = w1;
@@ -557,7 +564,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                         tmem_load32(d + kPN + 32 * j, x);
                         tmem_load_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = (v[e] + sum[j][e]) + x[e];
+                        for (int e = 0; e < 32; ++e) v[e] = __fmaf_rn(x[e], 1.0f / kSecondPlane, v[e] + sum[j][e]);
                     }
                     if (!there) {
 #pragma unroll

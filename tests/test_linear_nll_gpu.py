@@ -334,3 +334,31 @@ def test_rows_that_are_certain_of_their_label(dtype, K):
         assert float(one) >= 0 and abs(float(one) - float(terms[r])) <= float(bound[r])
         # p - 1 of the label: of the size of what the others have, or a step of lse
         assert float(gb[labels[r]]) <= 0 and abs(float(gb[labels[r]]) + float(-torch.expm1(-terms[r]))) <= float(bound[r])
+
+
+@pytest.mark.parametrize("n,K", [(150, 24), (1200, 40)])
+def test_weight_gradients_of_very_rare_classes(n, K):
+    """Classes of probability 2^-30 to 2^-50 that no row has as its label: their gradients keep their own accuracy.  G is carried in
+    22 bits down to 2^-28 and is 2^-51 off below, an operand's value likewise beside the largest of its column."""
+    x, w, b, labels, mask = make(n, K, 300, torch.float32, n)
+    labels = labels % 200
+    b[200:225] -= 14.0
+    b[225:250] -= 21.0
+    b[250:] -= 27.0
+    ref = Ref(x, w, b, labels, mask, 1.0)
+    _, _, gw, gb = ops.linear_nll_loss_grad(x, w, b, labels, mask, 1.0)
+    # the bound of a class's gradients from its own probabilities: p (e_z + e_lse) as in Ref, 2^-21 of G for its two planes and as
+    # much for x's, sums of m terms
+    xr = x[ref.rows].double()
+    z = xr @ w.double().t() + b.double()
+    p = (z - torch.logsumexp(z, 1, keepdim=True)).exp()[:, 200:]
+    e_z = (K + 16) * STEP * (xr.abs() @ w.double().abs().t() + b.double().abs())
+    e_p = p * (e_z[:, 200:] + ref.e_lse[ref.rows][:, None] + 8 * STEP) * 1.01
+    m = len(ref.rows)
+    e_w = (e_p + p * 2.0 ** -20 + 2.0 ** -50).t() @ xr.abs() + (m + 16) * STEP * (p.t() @ xr.abs())
+    e_b = e_p.sum(0) + (m + 16) * STEP * p.sum(0)
+    close(gw[200:], p.t() @ xr, e_w)
+    close(gb[200:], p.sum(0), e_b)
+    # How sharp that bound is (a statement about the reference alone): lse is about log 300 + 2 = 7.7, so classes 21 below are of
+    # probability e^-28.7 = 2^-41, of which the absolute 2^-50 is 2^-9; the logits' share, 2 e_z, is below 2^-11
+    assert float(p[:, 25:50].max()) < 2.0 ** -25 and float((e_w / (p.t() @ xr.abs()))[25:50].max()) < 2.0 ** -8
