@@ -640,7 +640,7 @@ static int nll_product_blocks(const ProductCall &c, const ProductCall &c2, int64
 // their exponentials (779 against 789 us), and few rows are better spread over more blocks (300 x 30000 x 256 bf16, all of it: 104
 // against 130 us).
 template <int KIND, int PLANES>
-constexpr bool kNllPairs = PLANES == 2 || (KIND != kLogitStats && KIND != kLogitGrad);
+constexpr bool kNllPairs = PLANES == 2 || !nll_is_logits(KIND);
 static bool nll_in_pairs(int64_t row_cap) { return row_cap > 1024; }
 
 // Results of `rows` rows at most and `tiles` beside each other (gradients: and of `rows2` and `tiles2`; splits count as tiles)
@@ -652,6 +652,23 @@ static int nll_product(const ProductCall &c, const ProductCall &c2, int64_t rows
             return nll_product_blocks<KIND, PLANES, 2>(c, c2, ceil_div(rows, 2 * kPM) * tiles + ceil_div(rows2, 2 * kPM) * tiles2, s);
     }
     return nll_product_blocks<KIND, PLANES, 1>(c, c2, ceil_div(rows, kPM) * tiles + ceil_div(rows2, kPM) * tiles2, s);
+}
+
+// fp32 logits over more features than this: sums of their own for the cross products of the planes, and the main sums move on into
+// registers every 512.  Every addition in tensor memory rounds towards zero, and with all three products in one sum a logit over
+// 512 features has 96 of them, 32 so: gradients over 16 to 300 classes come out 0.4e-6 to 0.8e-6 off instead of 1.0e-6 to 1.4e-6
+// (and over 256 features 0.7e-6 either way).  One result in tensor memory at a time is the price: 5003 x 512 x 20011 with gradients
+// 1.42 ms against 1.26, the loss alone 327 us against 268; 100 x 2048 x 30000, with several windows, 0.76 ms against 0.79.
+constexpr int64_t kNllShortFeatures = 256;
+static bool nll_logits_long(int64_t K) { return K > kNllShortFeatures; }
+
+template <int SHORT, int LONG, int PLANES>
+static int nll_logits(const ProductCall &c, int64_t rows, int64_t tiles, cudaStream_t s)
+{
+    if constexpr (PLANES == 2) {
+        if (nll_logits_long(c.feats)) return nll_product<LONG, PLANES>(c, c, rows, tiles, 0, 0, s);
+    }
+    return nll_product<SHORT, PLANES>(c, c, rows, tiles, 0, 0, s);
 }
 
 template <class T, int PLANES>
@@ -733,7 +750,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         for (ProductCall *k : {&lc, &xc, &wc}) k->row0 = row0;
         lc.label = ints(p.label) + row0, lc.picked2 = floats(p.picked2) + row0;
         lc.cls0 = 0, lc.cls_count = (int)c.C;
-        if ((rc = nll_product<kLogitStats, PLANES>(lc, lc, p.row_cap, ceil_div(c.C, kPN), 0, 0, s))) return rc;
+        if ((rc = nll_logits<kLogitStats, kLongStats, PLANES>(lc, p.row_cap, ceil_div(c.C, kPN), s))) return rc;
         const NllJoin join{lc.stats, (int)(p.cls_padded / 128), row0, (int)p.row_cap, ints(p.rows), ints(p.total), lc.picked2,
                            floats(p.lse2), c.lse, floats(p.loss_part) + q * join_blocks, floats(p.loss_part),
                            (int)(p.chunks * join_blocks), c.inv_count, ints(p.joined), ints(p.failed), c.loss};
@@ -742,7 +759,7 @@ static int nll_run(const NllCall &c, const NllPlan &p)
         for (int64_t first = 0; first < c.C; first += p.piece) {
             const int64_t count = c.C - first < p.piece ? c.C - first : p.piece;
             for (ProductCall *k : {&lc, &xc, &wc}) k->cls0 = (int)first, k->cls_count = (int)count;
-            if ((rc = nll_product<kLogitGrad, PLANES>(lc, lc, p.row_cap, ceil_div(count, kPN), 0, 0, s))) return rc;
+            if ((rc = nll_logits<kLogitGrad, kLongGrad, PLANES>(lc, p.row_cap, ceil_div(count, kPN), s))) return rc;
             xc.add = first > 0, wc.add = q > 0;
             if (p.together) {
                 if ((rc = nll_product<kGradients, PLANES>(xc, wc, p.row_cap, tiles_k * p.row_splits, count, tiles_k * p.weight_splits, s))) return rc;

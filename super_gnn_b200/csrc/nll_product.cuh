@@ -31,7 +31,12 @@ constexpr int kPThreads = (kPEpilogueWarps + 2) * 32;
 constexpr int kPWindow = 8;     // fp32 gradients: steps after which the main sums move on into registers
 constexpr int kPAccCols = 512;  // all of the tensor memory: two results, or one and its cross products
 
-enum ProductKind { kLogitStats, kLogitGrad, kGradients, kRowGrad, kWeightGrad };
+// kLong...: the logits of fp32 operands over many features, with sums of their own for the cross products (see nll_logits_long)
+enum ProductKind { kLogitStats, kLogitGrad, kGradients, kRowGrad, kWeightGrad, kLongStats, kLongGrad };
+constexpr bool nll_is_stats(int kind) { return kind == kLogitStats || kind == kLongStats; }
+constexpr bool nll_is_grad(int kind) { return kind == kLogitGrad || kind == kLongGrad; }
+constexpr bool nll_is_logits(int kind) { return nll_is_stats(kind) || nll_is_grad(kind); }
+constexpr bool nll_is_long(int kind) { return kind == kLongStats || kind == kLongGrad; }
 
 struct ProductCall {
     CUtensorMap a, b, o;  // operands, result
@@ -74,8 +79,8 @@ constexpr int product_shared_bytes()
 {
     using S = ProductShared<PLANES, CTAS>;
     const int ring = S::kStages * S::kStageBytes;
-    if (KIND == kLogitStats) return ring + 2 * kPN * 8 + 256;
-    if (KIND == kLogitGrad) return ring + kPEpilogueWarps * S::kBox + kPN * 8 + 256;
+    if (nll_is_stats(KIND)) return ring + 2 * kPN * 8 + 256;
+    if (nll_is_grad(KIND)) return ring + kPEpilogueWarps * S::kBox + kPN * 8 + 256;
     return ring + kPEpilogueWarps * S::kBox + 256;
 }
 
@@ -93,7 +98,7 @@ __device__ __forceinline__ ProductUnits product_units(const ProductCall &c, bool
     rows = rows < 0 ? 0 : rows < c.row_cap ? rows : c.row_cap;
     u.rows = rows;
     int red;
-    if (KIND == kLogitStats || KIND == kLogitGrad) u.m = rows, u.n = c.cls_count, red = c.feats;
+    if (nll_is_logits(KIND)) u.m = rows, u.n = c.cls_count, red = c.feats;
     else if (!weights) u.m = rows, u.n = c.feats, red = c.cls_count;
     else u.m = c.cls_count, u.n = c.feats, red = rows;
     u.blocks = (red + kPK - 1) / kPK;
@@ -113,7 +118,7 @@ struct ProductUnit {
 template <int KIND, int CTAS>
 __device__ __forceinline__ ProductUnit product_unit(const ProductUnits &u, int i, int rank)
 {
-    constexpr bool kRowsFirst = KIND == kLogitStats || KIND == kLogitGrad;
+    constexpr bool kRowsFirst = nll_is_logits(KIND);
     ProductUnit t;
     const int tiles = u.tiles_m * u.tiles_n, in = i % tiles;
     const int tm = kRowsFirst ? in % u.tiles_m : in / u.tiles_n, tn = kRowsFirst ? in / u.tiles_m : in % u.tiles_n;
@@ -165,15 +170,15 @@ __global__ void __launch_bounds__(kPThreads, 1)
 nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant__ ProductCall c2)
 {
     using S = ProductShared<PLANES, CTAS>;
-    constexpr bool kLogits = KIND == kLogitStats || KIND == kLogitGrad;
+    constexpr bool kLogits = nll_is_logits(KIND), kStats = nll_is_stats(KIND);
     constexpr bool kBmn = !kLogits;
-    constexpr bool kCross = !kLogits && PLANES == 2;  // cross products have their own sums, in the other half of the tensor memory
+    constexpr bool kCross = (!kLogits || nll_is_long(KIND)) && PLANES == 2;  // cross products have their own sums, in the other half of the tensor memory
     constexpr int kAcc = kCross ? 1 : 2;              // results in flight
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *boxes = base + S::kStages * S::kStageBytes;
-    uint8_t *after = boxes + (KIND == kLogitStats ? 0 : kPEpilogueWarps * S::kBox);
+    uint8_t *after = boxes + (kStats ? 0 : kPEpilogueWarps * S::kBox);
     float *column = reinterpret_cast<float *>(after);  // logits: bias, then scale, of the classes of a tile
-    constexpr int kColumns = KIND == kLogitStats ? 2 : 1;  // tiles whose classes are held at once
+    constexpr int kColumns = kStats && kAcc == 2 ? 2 : 1;  // tiles whose classes are held at once
     uint8_t *behind = after + (kLogits ? kColumns * kPN * 8 : 0);
     uint64_t *full = reinterpret_cast<uint64_t *>(behind);
     uint64_t *empty = full + S::kStages, *acc_full = empty + S::kStages, *acc_empty = acc_full + 2;
@@ -372,7 +377,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
             }
             float scale = 1.4426950408889634f, lse2 = 0.f;
             if (kLogits && PLANES == 2) scale *= __ldg(c.row_scale + c.row0 + (row < u.m ? row : 0));
-            if (KIND == kLogitGrad && row < u.m) lse2 = __ldg(c.lse2 + row);
+            if (nll_is_grad(KIND) && row < u.m) lse2 = __ldg(c.lse2 + row);
             float sum[kCross ? 4 : 1][32];  // the main sums of the windows before the last
             if constexpr (kCross) {
 #pragma unroll
@@ -409,13 +414,22 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
             const uint32_t d = tmem + acc * kPN + half * 128 + ((uint32_t)quarter << 21);
             const bool there = t.count > 0;  // an empty range of the reduction: zeros
             float v[32], ahead[32];
-            if (kLogits) tmem_load32(d, ahead);
-            // logits in units of log2, 32 columns at a time; the next ones come while these are worked on
+            if (kLogits && !kCross) tmem_load32(d, ahead);
+            // logits in units of log2, 32 columns at a time; the next ones come while these are worked on (not beside the sums of the
+            // windows before, which fill the registers)
             const auto logits = [&](int j) {
-                tmem_load_wait();
+                if constexpr (kCross) {
+                    tmem_load32(d + 32 * j, v);
+                    tmem_load32(d + kPN + 32 * j, ahead);
+                    tmem_load_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = ahead[e];
-                if (j < 3) tmem_load32(d + 32 * (j + 1), ahead);
+                    for (int e = 0; e < 32; ++e) v[e] = (v[e] + sum[j][e]) + ahead[e];
+                } else {
+                    tmem_load_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = ahead[e];
+                    if (j < 3) tmem_load32(d + 32 * (j + 1), ahead);
+                }
                 const float4 *b4 = reinterpret_cast<const float4 *>(bias_col + half * 128 + 32 * j);
                 const float4 *s4 = reinterpret_cast<const float4 *>(scale_col + half * 128 + 32 * j);
 #pragma unroll
@@ -438,8 +452,8 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                 async_fence();
                 __syncwarp();
             };
-            if constexpr (KIND == kLogitStats) {
-                float mx = -INFINITY, sum = 0.f;
+            if constexpr (kStats) {
+                float mx = -INFINITY, total = 0.f;
                 const int label = row < u.m ? c.label[row] - c.cls0 - t.n0 - half * 128 : -1;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -455,13 +469,13 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 32; ++e) top = fmaxf(top, v[e]);
                     const float ref = top == -INFINITY ? 0.f : top;
-                    sum *= exp2_fast(mx - ref);
+                    total *= exp2_fast(mx - ref);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) sum += exp2_fast(v[e] - ref);
+                    for (int e = 0; e < 32; ++e) total += exp2_fast(v[e] - ref);
                     mx = top;
                 }
-                if (row < u.m) c.stats[(int64_t)(t.n0 / 128 + half) * c.row_cap + row] = make_float2(mx, sum);
-            } else if constexpr (KIND == kLogitGrad) {
+                if (row < u.m) c.stats[(int64_t)(t.n0 / 128 + half) * c.row_cap + row] = make_float2(mx, total);
+            } else if constexpr (nll_is_grad(KIND)) {
                 const int label = row < u.m ? c.label[row] - c.cls0 - t.n0 - half * 128 : -1;
                 const float own = label >= 0 && label < 128  // G of the label's class, p - 1, without the cancellation of a p next to 1
                                       ? expm1f((__ldg(c.picked2 + row) - lse2) * 0.6931471805599453f) * (PLANES == 2 ? kGradScale : 1.0f)
@@ -616,7 +630,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
             }
             if (++acc == kAcc) acc = 0, acc_phase ^= 1;
         }
-        if (KIND != kLogitStats && lane == 0) store_wait_all();
+        if (!kStats && lane == 0) store_wait_all();
         __syncwarp();
     }
     tc_fence_before();

@@ -362,3 +362,16 @@ def test_weight_gradients_of_very_rare_classes(n, K):
     # How sharp that bound is (a statement about the reference alone): lse is about log 300 + 2 = 7.7, so classes 21 below are of
     # probability e^-28.7 = 2^-41, of which the absolute 2^-50 is 2^-9; the logits' share, 2 e_z, is below 2^-11
     assert float(p[:, 25:50].max()) < 2.0 ** -25 and float((e_w / (p.t() @ xr.abs()))[25:50].max()) < 2.0 ** -8
+
+
+@pytest.mark.parametrize("n,K,C", [(5000, 512, 16), (700, 512, 46), (2500, 400, 300), (3000, 1100, 100)])
+def test_fp32_gradients_over_many_features(n, K, C):
+    """As exact as fp32 sums: a logit takes at most 32 additions that round towards zero before its sums move on, half a step of
+    2^-23 each on average, of partial sums that grow like a random walk (two thirds of the whole): 32 x 2^-24 x 2/3 = 2^-20.6 of
+    it at most, and a gradient is off by about what its logits are."""
+    x, w, b, labels, mask = make(n, K, C, torch.float32, n + K + C)
+    ref = Ref(x, w, b, labels, mask, 1.0 / n)
+    _, *grads = ops.linear_nll_loss_grad(x, w, b, labels, mask, 1.0 / n)
+    for got, want in zip(grads, (ref.gx, ref.gw, ref.gb)):
+        assert float((got.double() - want).norm()) <= 2.0 ** -20 * float(want.norm())
+    assert float((ops.linear_nll_loss(x, w, b, labels, mask, 1.0 / n)[0].double() - ref.loss).abs()) <= 2.0 ** -20 * float(ref.loss)
