@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kGThreads, 1) weight_grad_kernel(const __grid_
             for (int j = 0; j < 8; ++j) {
                 float v[16];
                 tmem_load16(tmem + half * 128 + 16 * j + ((uint32_t)quarter << 21), v);
-                tmem_load_wait();
+                tmem_load_wait(v);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sum[16 * j + e] += v[e];
             }

@@ -393,7 +393,7 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                         if (t.n0 + half * 128 + 32 * j >= u.n) break;
                         float x[32];
                         tmem_load32(tmem + half * 128 + 32 * j + ((uint32_t)quarter << 21), x);
-                        tmem_load_wait();
+                        tmem_load_wait(x);
 #pragma unroll
                         for (int e = 0; e < 32; ++e) sum[j][e] += x[e];
                     }
@@ -421,11 +421,12 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                 if constexpr (kCross) {
                     tmem_load32(d + 32 * j, v);
                     tmem_load32(d + kPN + 32 * j, ahead);
-                    tmem_load_wait();
+                    tmem_load_wait(v);
+                    tmem_load_wait(ahead);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] = (v[e] + sum[j][e]) + ahead[e];
                 } else {
-                    tmem_load_wait();
+                    tmem_load_wait(ahead);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] = ahead[e];
                     if (j < 3) tmem_load32(d + 32 * (j + 1), ahead);
@@ -572,11 +573,11 @@ nll_product_kernel(const __grid_constant__ ProductCall c, const __grid_constant_
                     const int k0 = t.n0 + half * 128 + 32 * j;
                     if (k0 >= u.n) break;
                     tmem_load32(d + 32 * j, v);
-                    tmem_load_wait();
+                    tmem_load_wait(v);
                     if (kCross) {
                         float x[32];
                         tmem_load32(d + kPN + 32 * j, x);
-                        tmem_load_wait();
+                        tmem_load_wait(x);
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = __fmaf_rn(x[e], 1.0f / kSecondPlane, v[e] + sum[j][e]);
                     }
