@@ -219,3 +219,11 @@ def test_captured_weight_grad():
     torch.cuda.synchronize()
     want = ops.checkpoint_pack_rows(x)
     assert torch.equal(got, ops.checkpoint_weight_grad(g, *want)) and torch.equal(back, ops.checkpoint_unpack_rows(*want))
+
+
+@pytest.mark.parametrize("n,M,F,dtype", [(1000, 127, 96, torch.float32), (1003, 255, 300, torch.bfloat16), (999, 255, 64, torch.float16),
+                                         (700, 129, 40, torch.float32), (90, 5000, 33, torch.float32), (70, 9, 5001, torch.bfloat16),
+                                         (33, 65536, 1, torch.float16), (31, 1, 65536, torch.float32)])
+def test_weight_grad_of_packed_odd_rows_and_many_columns(n, M, F, dtype):
+    """Rows of g that come as one run of bytes, the widest of them and one more, and results of many tiles."""
+    test_weight_grad(n, M, F, dtype)

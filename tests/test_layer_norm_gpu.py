@@ -287,3 +287,25 @@ def test_captured_and_on_another_stream():
     torch.cuda.synchronize()
     for a, b in zip((y, stats, codes, params) + grads, want + want_grads):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n,H", [(700, 2049), (500, 5003), (333, 9000), (301, 16384)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_rows_read_again_several_a_block(n, H, dtype, checkpoint):
+    """Rows beyond what a block holds in registers, up to the limit, more of them than blocks."""
+    test_forward_and_backward(n, H, dtype, torch.float32, checkpoint)
+
+
+@pytest.mark.parametrize("n,H,dtype", [(8 * 296 * 3 + 5, 300, torch.bfloat16), (8 * 592 * 2 + 1, 201, torch.float32),
+                                       (10_001, 129, torch.float16), (2377, 1024, torch.bfloat16)])
+def test_short_last_batch_in_longer_rings(n, H, dtype):
+    """Three and four buffers, where the short batch comes first, second or later in its block."""
+    x, gy, gamma, beta = make(n, H, dtype, torch.float32, seed=n + H)
+    for rows in (n, n - 1, 8, 9, 15):
+        a, g = x[:rows].contiguous(), gy[:rows].contiguous()
+        y, stats = ops.layer_norm_forward(a, gamma, beta)
+        ref = Ref(a, gamma, beta, 1e-5)
+        close(y, ref.y, ref.e_y)
+        for got, (want, err) in zip(ops.layer_norm_backward(g, a, stats, gamma), ref.backward(g)):
+            close(got, want, err)

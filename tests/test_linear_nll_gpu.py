@@ -375,3 +375,28 @@ def test_fp32_gradients_over_many_features(n, K, C):
     for got, want in zip(grads, (ref.gx, ref.gw, ref.gb)):
         assert float((got.double() - want).norm()) <= 2.0 ** -20 * float(want.norm())
     assert float((ops.linear_nll_loss(x, w, b, labels, mask, 1.0 / n)[0].double() - ref.loss).abs()) <= 2.0 ** -20 * float(ref.loss)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_most_features(dtype):
+    check(*make(33, 16384, 40, dtype, 3), 0.1)
+    check(*make(1100, 1500, 300, dtype, 4), 0.1)  # pairs of blocks, three windows
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_large_calls_at_once(dtype):
+    """Calls whose kernels want all of an SM's tensor memory, on two streams."""
+    a, b = make(1500, 300, 2000, dtype, 4), make(1300, 520, 1500, dtype, 5)
+    want_a, want_b = ops.linear_nll_loss_grad(*a, 0.1), ops.linear_nll_loss_grad(*b, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got_a, got_b = [], []
+    for _ in range(4):
+        got_a.append(ops.linear_nll_loss_grad(*a, 0.1))
+        with torch.cuda.stream(side):
+            got_b.append(ops.linear_nll_loss_grad(*b, 0.1))
+    torch.cuda.synchronize()
+    for got, want in ((got_a, want_a), (got_b, want_b)):
+        for one in got:
+            for u, v in zip(one, want):
+                assert torch.equal(u, v)

@@ -73,3 +73,48 @@ def test_many_class_loss_with_weights_beyond_2_31_elements():
     # G and the result in bf16
     assert float((gw[at].double() - rows).abs().max()) <= 2 ** -6 * float(rows.abs().max())
     assert not gx[7].any()
+
+
+def test_weight_gradient_of_rows_beyond_2_31_elements_keeps_all_terms():
+    """22 rows at both ends have a gradient: against the formula in 64 bits, at the accuracy of three terms of g sc."""
+    _need_memory(20)
+    n, F, M = (1 << 22) + 5, 520, 12
+    x = torch.empty(n, F, dtype=torch.bfloat16, device=DEV)
+    x.normal_()
+    ends = torch.cat([torch.arange(9), torch.arange(n - 13, n)]).to(DEV)
+    codes, params = ops.checkpoint_pack_rows(x)
+    del x
+    g = torch.zeros(n, M, device=DEV)
+    g[ends] = torch.randn(len(ends), M, device=DEV)
+    got = ops.checkpoint_weight_grad(g, codes, params)
+    zp, sc, c = params[ends, :1].double(), params[ends, 1:].double(), codes[ends].double()
+    ge = g[ends].double()
+    want = ge.t() @ (zp + sc * c)
+    typical = (ge.square().t() @ (sc * c + zp.abs()).square()).sqrt()
+    # 2^-23 of each value for g sc in three terms (two would leave 2^-18), 2^-24 on average at each of the three additions for
+    # sixteen rows, of which there are at most four at the ends; the rows between add zeros, which is exact; joining two row
+    # ranges and adding the zero points' share a few roundings more
+    assert (got.double() - want).norm() <= (2 ** -23 + (3 * 4 + 6) * 2 ** -24) * typical.norm()
+
+
+def test_many_class_loss_of_a_whole_partition():
+    """A few rows of very many are in the loss, as a model has it that hands over all of its nodes: what the same rows give alone."""
+    _need_memory(20)
+    n, K, C = 400_000, 256, 1000
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    x = torch.randn(n, K, generator=gen, device=DEV)
+    w = torch.randn(C, K, generator=gen, device=DEV) * (2 / K ** 0.5)
+    b = torch.randn(C, generator=gen, device=DEV)
+    labels = torch.randint(0, C, (n,), generator=gen, device=DEV)
+    mask = torch.rand(n, generator=gen, device=DEV) < 0.08
+    rows = mask.nonzero()[:, 0]
+    inv = 1.0 / len(rows)
+    loss, gx, gw, gb = ops.linear_nll_loss_grad(x, w, b, labels, mask, inv)
+    want = ops.linear_nll_loss_grad(x[rows], w, b, labels[rows], None, inv)
+    # the same products in other chunks of rows: each side is within 2^-20 of the formula
+    for a, c in ((loss, want[0]), (gx[rows], want[1]), (gw, want[2]), (gb, want[3])):
+        assert float((a - c).norm()) <= 2 * 2.0 ** -20 * float(c.norm())
+    gx[rows] = 0
+    assert not gx.any()
+    value, lse = ops.linear_nll_loss(x, w, b, labels, mask, inv)
+    assert torch.equal(value, loss) and not lse[~mask].any()
