@@ -51,7 +51,9 @@ class DistSAGEConvGrad(torch.nn.Module):
                 out += self.lin_self(local_nodes_feat)
             else:
                 out = linear(out, self.lin_neigh.weight, self.checkpoint_bits)
-                out += linear(local_nodes_feat, self.lin_self.weight, self.checkpoint_bits)
+                # features without a gradient stay with the caller anyway
+                bits = self.checkpoint_bits if local_nodes_feat.requires_grad else 32
+                out += linear(local_nodes_feat, self.lin_self.weight, bits)
         with TimeRecorder.ctx.time_block("add_bias", is_record=False):
             if self.bias is not None:
                 out += self.bias

@@ -355,3 +355,24 @@ def test_gradients_of_several_backward_passes_add_up(unit):
         for leaf, g in zip(leaves, first):
             # sums of equal fp32 numbers: up to three roundings; h: an SpMM whose atomic adds come in any order
             assert near(leaf.grad, turn * g, 1e-5)
+
+
+def test_features_are_not_packed_where_layers_are_not_fused():
+    """The first layer's own input stays with the caller; everything between the layers is kept in 8 bits."""
+    n, fin, hid, ncls = 1500, 30, 50, 6
+    graph = graph_of(n, 9000, hid)
+    base, small = models(fin, hid, ncls, checkpoint_bits=8)
+    base.fused = small.fused = False
+    base.dropout = small.dropout = 0.0
+    x = torch.randn(n, fin, device=DEV)
+    ops.LAUNCH_LOG = []
+    try:
+        out = small(graph, x)
+        packs = [entry[1]["F"] for entry in ops.LAUNCH_LOG if entry[0] == "checkpoint_pack"]
+    finally:
+        ops.LAUNCH_LOG = None
+    assert packs == [fin, hid, hid, hid, hid]  # aggregated features; (aggregated | own) of the two layers behind
+    out.square().sum().backward()
+    base(graph, x).square().sum().backward()
+    for (k, a), b in zip(small.named_parameters(), base.parameters()):
+        assert float((a.grad - b.grad).norm()) <= 0.15 * float(b.grad.norm()), k  # as in test_model_with_8_bit_checkpoints
