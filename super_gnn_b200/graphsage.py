@@ -41,6 +41,11 @@ class DistSAGE(torch.nn.Module):
         # the training loss of the last layer in pieces of the classes, without the logits in memory (any number of
         # classes; the boundary exchange stays the reference's)
         self.chunked_loss = bool(chunked_loss)
+        # what the kernels behind these options take, asked here and not in the first backward pass
+        if self.checkpoint_bits == 8 and (max(dims) > 32768 or (num_layers > 1 and norm_type is not None and hidden_channels > 16384)):
+            raise ValueError("checkpoint_bits=8: at most 32768 channels a layer, and 16384 hidden channels with a LayerNorm")
+        if self.chunked_loss and dims[-2] > 8192:
+            raise ValueError("chunked_loss: at most 8192 channels into the last layer")
         # optional fixed dropout masks (one per hidden layer) for runs that must be
         # reproducible against a CPU reference; None = native dropout
         self.dropout_masks = None
