@@ -476,7 +476,8 @@ int sgnn_layer_norm_backward(int dtype, const void *d_gy, int64_t ldg, const voi
  *   d_codes uint8[n, ldc], d_params fp32[n, 2] = (zp, sc).
  * sgnn_checkpoint_weight_grad: the weight gradient of y = x W^T from the codes of x,
  *     out[m, k] = sum_r g[r, m] (zp_r + sc_r code[r, k]) + beta out[m, k]     fp32[M, ldo]
- *   with g[n, M] of `dtype`; g sc is carried in 16 bits of significand or more, sums in fp32 and in a fixed order.
+ *   with g[n, M] of `dtype`; g sc is rounded to fp32 once and carried in its 24 bits, sums in fp32 and in a fixed order.
+ *   A g that is not finite, or a g sc beyond the largest bf16 (3.39e38), makes its row of the result NaN.
  *   d_workspace: the bytes ..._workspace_bytes reports; not to be shared by calls that can run concurrently.
  *   n < 2^31, M, F <= 65536.
  * ------------------------------------------------------------------------- */
@@ -502,6 +503,10 @@ int sgnn_checkpoint_weight_grad(int dtype, const void *d_g, int64_t ldg, const u
  *   [0, C); the others are not read: their lse is 0 and their gx rows are zero, whatever x holds there.
  *   d_loss fp32[1], d_lse fp32[n] (may be NULL); d_gx, d_gw, d_gb all NULL (loss only) or d_gx and d_gw not NULL.
  *   Sums in a fixed order.  n, C <= 2^30, K <= 16384.
+ *   bf16 operands are exact, and G is rounded to bf16 before gx and gw (and, for a gb of any type, before gb).  fp32
+ *   operands are carried in 22 bits beside the largest value of their row (logits) or column (gradients), G in 22 bits
+ *   down to 2^-28 and 2^-51 off below that: gradients were within 2^-20 of their size
+ *   for up to 1100 features.
  *   A kernel whose wait was not answered within two seconds gives up; the loss and gx are then NaN.
  *   d_workspace: the bytes ..._workspace_bytes reports; not to be shared by calls that can run concurrently.
  * ------------------------------------------------------------------------- */

@@ -5,8 +5,8 @@
 //
 // The quantiser is the boundary exchange's (8 bits, min-max a row), for rows of any width, strided, in fp32, bf16 or
 // fp16.  See row_io.cuh for rows without a range and for NaN and infinities.  Both kernels are bound by memory: the row
-// is read once (rows of up to 1024 elements stay in a warp's registers, several narrow ones at a time, longer ones are read a second time from
-// L1 / L2 by the block that owns them).
+// is read once (rows of up to 2048 elements, 1024 where they allow no accesses of 16 bytes, stay in a warp's registers, several narrow
+// ones at a time; longer ones are read a second time from L1 / L2 by the block that owns them).
 #include "row_io.cuh"
 
 namespace sgnn {

@@ -10,9 +10,11 @@
 // x: one byte an element kept between the two instead of four.
 //
 // Everything is bound by memory: the forward moves x and y once, the backward gy, x (or its codes) and gx once.  Rows
-// of up to 1024 elements (2048 forward) belong to a warp, narrow ones to 4, 8 or 16 of its lanes, which hold them in
-// registers between the reductions and the outputs; up to 2048 backward to a block that does the same; longer rows to a
-// block that reads them again (from L1 / L2) for every step.  All sums are fp32: the variance from the differences to
+// belong to a warp, narrow ones to 4, 8 or 16 of its lanes, which hold them in registers between the reductions and the
+// outputs: forward up to 2048 elements where accesses of 16 bytes or the ring of bulk copies apply and 1024 elsewhere;
+// backward up to 832 (kNormSplit), 16-bit rows through the ring up to 1024, from codes up to 512 unless fp32 rows lie on
+// boundaries.  Backward up to 2048 they belong to a block that does the same; longer rows to a block that reads them again
+// (from L1 / L2) for every step: 30000 x 4096 fp32 220 us forward of 150 that the bytes take, 528 of 226 backward.  All sums are fp32: the variance from the differences to
 // the mean, the column sums per warp, then per block, then over the blocks, in a fixed order.
 #include "row_io.cuh"
 #include "umma.cuh"
@@ -125,7 +127,10 @@ norm_fwd_warp_kernel(const T *__restrict__ x, int64_t ldx, NormParam par, float 
 // 100003 x 602 in bf16 took 117 us forward and 303 us backward (too few bytes on their way, and 146 registers).
 // ---------------------------------------------------------------------------
 constexpr int kStagedMax = 4;             // buffers of the ring
-constexpr size_t kStagedCap = 160 * 1024;  // shared memory of a block: two buffers of two operands of 1024 floats are 131 KB
+constexpr size_t kStagedCap = 160 * 1024;  // shared memory of a block
+constexpr int kStagedForward = 2048;       // longest rows of the forward; of the backward 1024 of 16 bits, kNormSplit of fp32
+// two buffers of eight such fp32 rows and gamma and beta (147 KB), two of two operands and gamma (110 KB)
+static_assert(2 * kNormWarps * kStagedForward * 4 + 2 * kStagedForward * 4 <= kStagedCap);
 
 struct StagedRing {
     uint8_t *base;  // buffer s at base + s * stride; the second operand of the backward `second` bytes behind
@@ -599,6 +604,7 @@ norm_bwd_warp_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, cons
 // (both directions, 100000 rows: 1023 fp32 449 us, 553 through the ring; 1024 fp32 422, 452 by a warp; 800 fp32 379, 370; from
 // codes 1024 bf16 403, 605 by a warp; 576 bf16 365, 433; 640 fp32 347, 296).
 constexpr int kNormWide = 8 * kNormThreads, kNormSplit = 832;
+static_assert(2 * 2 * kNormWarps * kNormSplit * 4 + kNormSplit * 4 <= kStagedCap && 2 * 2 * kNormWarps * 1024 * 2 + 1024 * 4 <= kStagedCap);
 template <class T, int E, bool CK>
 __global__ void __launch_bounds__(kNormThreads, 3)
 norm_bwd_wide_kernel(const T *__restrict__ gy, int64_t ldg, NormSource src, const float2 *__restrict__ stats,
@@ -845,7 +851,7 @@ static bool norm_can_stage(const NormCall &c, size_t bytes)
 {
     const bool fwd = c.y != nullptr;
     const auto packed = [&](const void *p, int64_t ld) { return ld == c.H && aligned16(p); };
-    return c.n >= kNormWarps && c.H <= (fwd ? 2048 : bytes == 4 ? kNormSplit : 1024) && c.H > 128 && packed(c.x, c.ldx) &&
+    return c.n >= kNormWarps && c.H <= (fwd ? kStagedForward : bytes == 4 ? kNormSplit : 1024) && c.H > 128 && packed(c.x, c.ldx) &&
            (fwd ? packed(c.y, c.ldy) : packed(c.gy, c.ldg) && packed(c.gx, c.ldgx));
 }
 struct NormStage {

@@ -1209,7 +1209,8 @@ def checkpoint_unpack_rows(codes, params, dtype=torch.float32):
 
 def checkpoint_weight_grad(g, codes, params, out=None, beta: float = 0.0):
     """``out = g.T @ x (+ beta * out)`` with ``x`` [n, F] given by its 8-bit checkpoint and ``g`` [n, M] in fp32, bf16
-    or fp16: the weight gradient of a linear map, fp32 [M, F], straight from the codes."""
+    or fp16: the weight gradient of a linear map, fp32 [M, F], straight from the codes.  A value of ``g`` that is not finite
+    makes its row of the result NaN."""
     code = _matrix(g, "g")
     codes = _checkpoint_args(codes, params)
     n, F = codes.shape
@@ -1288,7 +1289,9 @@ def linear_nll_loss(x, weight, bias, labels, mask, inv_count: float):
 
 def linear_nll_loss_grad(x, weight, bias, labels, mask, inv_count: float):
     """The loss of :func:`linear_nll_loss` and its gradients in one call: ``(loss [1], gx, gw, gb)``, in the types of
-    ``x``, ``weight`` and ``bias`` (``gb`` is None without a bias).  ``gx`` is zero in the rows outside the loss."""
+    ``x``, ``weight`` and ``bias`` (``gb`` is None without a bias).  ``gx`` is zero in the rows outside the loss.  With bf16
+    operands the gradient of the logits is rounded to bf16 on its way to all three; fp32 operands are carried in 22 bits
+    (24 in a plain fp32 product) and the gradients come out within 2^-20 of their size."""
     loss, _, gx, gw, gb = _linear_nll(x, weight, bias, labels, mask, inv_count, True)
     return loss, gx, gw, gb
 

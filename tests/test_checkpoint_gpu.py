@@ -227,3 +227,16 @@ def test_captured_weight_grad():
 def test_weight_grad_of_packed_odd_rows_and_many_columns(n, M, F, dtype):
     """Rows of g that come as one run of bytes, the widest of them and one more, and results of many tiles."""
     test_weight_grad(n, M, F, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weight_grad_of_a_gradient_that_is_not_finite(dtype):
+    """Its row of the result says so; the others do not change."""
+    x, g = rows(300, 40, torch.float32, 1), rows(300, 20, dtype, 2)
+    kept = ops.checkpoint_pack_rows(x)
+    want = ops.checkpoint_weight_grad(g, *kept)
+    g[77, 3], g[299, 11] = float("inf"), float("nan")
+    got = ops.checkpoint_weight_grad(g, *kept)
+    assert torch.isnan(got[[3, 11]]).all()
+    got[[3, 11]] = want[[3, 11]]
+    assert torch.equal(got, want)
