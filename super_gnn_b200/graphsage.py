@@ -15,6 +15,7 @@ from torch.nn import LayerNorm
 from .fused_layer import (FusedSAGELayer, FusedSAGELossManyClasses, FusedSAGELossNarrowLocal, FusedSAGELossProjectFirst,
                           FusedSAGEOutputLayer, FusedSAGEOutputLayerProjectFirst, many_classes_loss, narrow_local_applies,
                           reset_layer_buffers)
+from . import supergnn_ops as ops
 from .layers import DistSAGEConvGrad
 from .layers.functional import check_bits, layer_norm
 
@@ -41,11 +42,6 @@ class DistSAGE(torch.nn.Module):
         # the training loss of the last layer in pieces of the classes, without the logits in memory (any number of
         # classes; the boundary exchange stays the reference's)
         self.chunked_loss = bool(chunked_loss)
-        # what the kernels behind these options take, asked here and not in the first backward pass
-        if self.checkpoint_bits == 8 and (max(dims) > 32768 or (num_layers > 1 and norm_type is not None and hidden_channels > 16384)):
-            raise ValueError("checkpoint_bits=8: at most 32768 channels a layer, and 16384 hidden channels with a LayerNorm")
-        if self.chunked_loss and dims[-2] > 8192:
-            raise ValueError("chunked_loss: at most 8192 channels into the last layer")
         # optional fixed dropout masks (one per hidden layer) for runs that must be
         # reproducible against a CPU reference; None = native dropout
         self.dropout_masks = None
@@ -88,10 +84,12 @@ class DistSAGE(torch.nn.Module):
     def can_fuse_loss(self, nodes_feats, graph=None) -> bool:
         """True when ``forward(..., loss_mask=, loss_inv_count=)`` returns the training loss from a fused node: fused
         CUDA path, at most 256 classes, and a last layer that either projects before it aggregates or (given the
-        graph) aggregates only the remote edges at the input width; or ``chunked_loss``, for any number of classes."""
+        graph) aggregates only the remote edges at the input width; or ``chunked_loss``, for any number of classes and at most
+        8192 channels into the last layer."""
         last = self.convs[-1]
         if self.chunked_loss:
-            return nodes_feats.is_cuda and nodes_feats.dtype == torch.float32 and last.normalize
+            return (nodes_feats.is_cuda and nodes_feats.dtype == torch.float32 and last.normalize
+                    and 2 * last.in_channels <= ops.LONGEST_ROW)
         if not (self._fused_ok(nodes_feats) and self._layer_fusable(last, hidden=False) and last.out_channels <= 256):
             return False
         return self._project_first(last) or (fuse_loss_narrow_local and graph is not None
@@ -157,7 +155,7 @@ class DistSAGE(torch.nn.Module):
             nodes_feats = F.dropout(nodes_feats, p=self.dropout, training=self.training)
         if self.norm_type is not None:
             norm = self.norms[i]
-            if self.checkpoint_bits == 8 and nodes_feats.is_cuda:
+            if self.checkpoint_bits == 8 and nodes_feats.is_cuda and nodes_feats.size(1) <= ops.LONGEST_ROW:
                 nodes_feats = layer_norm(nodes_feats, norm.weight, norm.bias, norm.eps, self.checkpoint_bits)
             else:
                 nodes_feats = norm(nodes_feats)

@@ -990,6 +990,8 @@ def softmax_nll_loss(logits, bias, labels, mask, inv_count: float, grad=None):
 # for what failed, ask for the device and its stream the cheap way, and give torch.empty its sizes one by one (1.6 us; 2.3 us
 # as a tuple).
 _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LONGEST_ROW = 16384  # of the layer norm; most features of the many-class loss
+_MOST_COLUMNS = 65536  # of either operand of one weight gradient
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # torch.cuda.current_stream without the object
 
 
@@ -1224,6 +1226,12 @@ def checkpoint_weight_grad(g, codes, params, out=None, beta: float = 0.0):
     else:
         _result(out, "out", M, F, torch.float32, dev)
     g = _row_major(g)
+    if M > _MOST_COLUMNS or F > _MOST_COLUMNS:
+        for m in range(0, M, _MOST_COLUMNS):
+            for f in range(0, F, _MOST_COLUMNS):
+                checkpoint_weight_grad(g[:, m:m + _MOST_COLUMNS], codes[:, f:f + _MOST_COLUMNS], params,
+                                       out=out[m:m + _MOST_COLUMNS, f:f + _MOST_COLUMNS], beta=beta)
+        return out
     lib = _cabi.lib()
     with _on(dev), _Logged("checkpoint_weight_grad", dev, n=n, M=M, F=F):
         need = _workspace_bytes("sgnn_checkpoint_weight_grad_workspace_bytes", dev.index, code, n, M, F)

@@ -240,3 +240,8 @@ def test_weight_grad_of_a_gradient_that_is_not_finite(dtype):
     assert torch.isnan(got[[3, 11]]).all()
     got[[3, 11]] = want[[3, 11]]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M,F", [(70_001, 3), (5, 70_001), (65_537, 1)])
+def test_weight_grad_of_more_columns_than_one_call_takes(M, F):
+    test_weight_grad(25, M, F, torch.bfloat16)

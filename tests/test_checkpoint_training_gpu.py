@@ -376,3 +376,37 @@ def test_features_are_not_packed_where_layers_are_not_fused():
     base(graph, x).square().sum().backward()
     for (k, a), b in zip(small.named_parameters(), base.parameters()):
         assert float((a.grad - b.grad).norm()) <= 0.15 * float(b.grad.norm()), k  # as in test_model_with_8_bit_checkpoints
+
+
+def test_layers_wider_than_the_kernels_take():
+    """Beyond 65536 columns a weight gradient is taken in parts; a layer norm beyond 16384 keeps its input; the loss in pieces is
+    not offered beyond 8192 channels into the last layer.  None of them fails, at the first backward pass least of all."""
+    n = 40
+    graph = graph_of(n, 300, 16400)
+    for fin, hid, ncls in ((70_000, 8, 3), (10, 16_400, 3), (10, 8, 70_001)):
+        base, small = models(fin, hid, ncls, checkpoint_bits=8, chunked_loss=True)
+        base.dropout = small.dropout = 0.0
+        assert small.can_fuse_loss(torch.empty(n, fin, device=DEV), graph) == (hid <= 8192)
+        x = torch.randn(n, fin, device=DEV)
+        labels, mask = torch.randint(0, ncls, (n,), device=DEV), torch.ones(n, dtype=torch.bool, device=DEV)
+        loss, grads = step(base, graph, x, labels, mask, None)
+        loss8, grads8 = step(small, graph, x, labels, mask, None)
+        assert abs(float(loss) - float(loss8)) <= 1e-4 * abs(float(loss))
+        # With 40 nodes a few of the hundreds of units change sides at a relu (one in a hundred does), and each of them is a visible
+        # part of the gradients before it, bias sums above all: no bound there but that they are numbers.  Between the loss
+        # and the last layer's weights lies nothing but the quantisation of its input, as in test_model_with_8_bit_checkpoints.
+        assert all(torch.isfinite(g).all() for g in grads8.values())
+        for k in ("convs.2.lin_neigh.weight", "convs.2.lin_self.weight"):
+            assert float((grads8[k] - grads[k]).norm()) <= 0.01 * float(grads[k].norm()), (fin, hid, ncls, k)
+
+
+def test_weight_gradients_in_parts_are_those_in_one(monkeypatch):
+    x, g = torch.randn(900, 500, device=DEV), torch.randn(900, 300, device=DEV)
+    kept = ops.checkpoint_pack_rows(x)
+    whole = ops.checkpoint_weight_grad(g, *kept)
+    out = torch.randn(300, 507, device=DEV)[:, 3:503]
+    want = whole + 0.5 * out
+    monkeypatch.setattr(ops, "_MOST_COLUMNS", 64)
+    # other row ranges: sums of 900 rows in another order
+    assert near(ops.checkpoint_weight_grad(g, *kept), whole, 2 ** -19)
+    assert ops.checkpoint_weight_grad(g, *kept, out=out, beta=0.5) is out and near(out, want, 2 ** -19)

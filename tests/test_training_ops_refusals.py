@@ -108,33 +108,3 @@ def test_workspace_queries():
 def test_host_tensors_are_refused(call):
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         call(torch.zeros(4, 8))
-
-
-@pytest.mark.parametrize("channels,kw", [
-    ((32769, 16, 4), dict(checkpoint_bits=8)), ((8, 16, 32769), dict(checkpoint_bits=8)), ((8, 16385, 4), dict(checkpoint_bits=8)),
-    ((8, 32769, 4), dict(checkpoint_bits=8, norm_type=None)), ((8, 8193, 4), dict(chunked_loss=True)),
-    ((8193, 16, 4), dict(chunked_loss=True, num_layers=1)), ((8, 16, 4), dict(checkpoint_bits=16)),
-])
-def test_models_beyond_what_the_kernels_take_are_refused_at_once(channels, kw):
-    """Not in the first backward pass."""
-    from super_gnn_b200.graphsage import DistSAGE
-
-    with pytest.raises(ValueError, match="checkpoint_bits|chunked_loss"), torch.device("meta"):
-        DistSAGE(*channels, **{"num_layers": 2, **kw})
-
-
-@pytest.mark.parametrize("channels,kw", [((32768, 16, 4), dict(checkpoint_bits=8)), ((8, 16384, 4), dict(checkpoint_bits=8)),
-                                         ((40000, 16, 40000), dict(chunked_loss=True)), ((8, 8192, 4), dict(chunked_loss=True))])
-def test_models_at_those_limits_are_built(channels, kw):
-    from super_gnn_b200.graphsage import DistSAGE
-
-    with torch.device("meta"):
-        DistSAGE(*channels, num_layers=2, **kw)
-
-
-def test_a_linear_map_whose_gradient_could_not_be_taken_is_refused():
-    from super_gnn_b200.layers import functional as L
-
-    weight = torch.empty(2, 65537, device="meta", requires_grad=True)
-    with pytest.raises(RuntimeError, match="65536"):
-        L.linear(torch.empty(3, 65537, device="meta"), weight, checkpoint_bits=8)
