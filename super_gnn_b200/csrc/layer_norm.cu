@@ -14,8 +14,9 @@
 // outputs: forward up to 2048 elements where accesses of 16 bytes or the ring of bulk copies apply and 1024 elsewhere;
 // backward up to 832 (kNormSplit), 16-bit rows through the ring up to 1024, from codes up to 512 unless fp32 rows lie on
 // boundaries.  Backward up to 2048 they belong to a block that does the same; longer rows to a block that reads them again
-// (from L1 / L2) for every step: 30000 x 4096 fp32 220 us forward of 150 that the bytes take, 528 of 226 backward.  All sums are fp32: the variance from the differences to
-// the mean, the column sums per warp, then per block, then over the blocks, in a fixed order.
+// (from L1 / L2) for every step: 30000 x 4096 fp32 220 us forward of 150 that the bytes take, 528 of 226 backward.  All sums
+// are fp32: the variance from the differences to the mean, the column sums per warp, then per block, then over the blocks,
+// in a fixed order.
 #include "row_io.cuh"
 #include "umma.cuh"
 
